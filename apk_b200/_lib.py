@@ -25,6 +25,8 @@ APK_DISC_DRAIN, APK_DISC_POISON = 0, 2
 APK_SET_DEVICE, APK_SET_HOST_MAPPED, APK_SET_HOST_MEMCPY = 0, 1, 2
 APK_MEM_HOST, APK_MEM_DEVICE = 0, 1
 APK_SCHED_QUEUE, APK_SCHED_CLC = 0, 1
+APK_ACT_NONE, APK_ACT_RELU, APK_ACT_GELU, APK_ACT_GELU_TANH, APK_ACT_SILU = range(5)
+APK_W_KN, APK_W_NK = 0, 1
 APK_TASKS_UNBOUNDED = 0xFFFFFFFFFFFFFFFF
 
 
@@ -86,6 +88,24 @@ class VisibilityResult(ctypes.Structure):
                 ("device_status", c_int)]
 
 
+class LinearConfig(ctypes.Structure):
+    _fields_ = [("device", c_int), ("in_features", c_int), ("out_features", c_int), ("w_layout", c_int),
+                ("act", c_int), ("bias_dtype", c_int), ("W", c_void_p), ("ldw", c_ll), ("bias", c_void_p),
+                ("sms", c_int), ("wait_limit_ns", c_ll)]
+
+
+class LinearIO(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("ldx", c_ll), ("rows", c_int), ("residual_dtype", c_int),
+                ("residual", c_void_p), ("ld_residual", c_ll), ("y", c_void_p), ("ldy", c_ll), ("y_dtype", c_int),
+                ("preact", c_void_p), ("ld_preact", c_ll), ("stream", c_void_p)]
+
+
+class LinearGrads(ctypes.Structure):
+    _fields_ = [("dy", c_void_p), ("ld_dy", c_ll), ("x", c_void_p), ("ldx", c_ll), ("preact", c_void_p),
+                ("ld_preact", c_ll), ("rows", c_int), ("dw_dtype", c_int), ("dx", c_void_p), ("ld_dx", c_ll),
+                ("dw", c_void_p), ("ld_dw", c_ll), ("db", c_void_p), ("stream", c_void_p)]
+
+
 P = c_void_p
 # name -> (restype, argtypes); every symbol include/apk.h declares
 SIGNATURES = {
@@ -125,6 +145,12 @@ SIGNATURES = {
     "apk_gen_tasks": (c_ll, [c_ull, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                              c_int, P]),
     "apk_shard_tasks": (c_int, [P, c_int, c_int, c_int, P]),
+    "apk_linear_create": (c_int, [ctypes.POINTER(LinearConfig), ctypes.POINTER(P)]),
+    "apk_linear_destroy": (c_int, [P]),
+    "apk_linear_last_error": (c_char_p, [P]),
+    "apk_linear_forward": (c_int, [P, ctypes.POINTER(LinearIO)]),
+    "apk_linear_backward": (c_int, [P, ctypes.POINTER(LinearGrads)]),
+    "apk_linear_status": (c_int, [P, P, ctypes.POINTER(c_int)]),
     "apk_sgemm_f32_noalloc": (c_int, [P, P, P, c_int, c_int, c_int, c_int, P]),
     "apk_sgemm_f32_noalloc_status": (c_int, [P, ctypes.POINTER(c_int)]),
     "apk_sgemm_f32_noalloc_selftest": (c_int, [c_ll, P]),

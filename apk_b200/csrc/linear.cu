@@ -1,0 +1,492 @@
+// A linear layer, y = act(x W + b) + r, and its gradients (apk_linear_* of
+// include/apk.h): argument checks, scratch, and the two memory-bound kernels
+// around the products of linear_gemm.cu.  No reference counterpart: the
+// reference multiplies bare matrices (src/tcyield.cu:91-356).
+#include <algorithm>
+#include <mutex>
+#include <new>
+
+#include "act.cuh"
+#include "common.cuh"
+#include "linear.h"
+
+namespace apk {
+
+apk_status cu_status(cudaError_t e, const char* what, Err* err) {
+  if (e == cudaSuccess) return APK_OK;
+  return err->fail(e == cudaErrorMemoryAllocation ? APK_ENOMEM : APK_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+apk_status Scratch::begin(size_t bytes, size_t zeroed, cudaStream_t stream, Err* err) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  apk_status st = cu_status(cudaStreamIsCapturing(stream, &cap), "cudaStreamIsCapturing", err);
+  if (st != APK_OK) return st;
+  capturing_ = cap != cudaStreamCaptureStatusNone;
+  if (bytes > bytes_) {
+    if (capturing_)
+      return err->fail(APK_ESTATE, "the scratch has to grow to %zu bytes: make one call of this size before the capture",
+                       bytes);
+    if (ev_ && used_ && (st = cu_status(cudaEventSynchronize(ev_), "waiting for the scratch", err)) != APK_OK) return st;
+    used_ = false;
+    if (p_) cudaFree(p_);
+    p_ = nullptr;
+    bytes_ = 0;
+    void* q = nullptr;
+    if ((st = cu_status(cudaMalloc(&q, bytes), "cudaMalloc(scratch)", err)) != APK_OK) return st;
+    p_ = static_cast<uint8_t*>(q);
+    if ((st = cu_status(cudaMemset(p_, 0, zeroed), "cudaMemset", err)) != APK_OK) return st;
+    // the memset of the legacy stream is not ordered before a non-blocking stream's work
+    if ((st = cu_status(cudaStreamSynchronize(nullptr), "cudaStreamSynchronize", err)) != APK_OK) return st;
+    bytes_ = bytes;
+  }
+  if (!capturing_ && used_ && last_ != stream)
+    return cu_status(cudaStreamWaitEvent(stream, ev_, 0), "cudaStreamWaitEvent", err);
+  return APK_OK;
+}
+
+apk_status Scratch::end(cudaStream_t stream, Err* err) {
+  if (capturing_) return APK_OK;
+  apk_status st = APK_OK;
+  if (!ev_ && (st = cu_status(cudaEventCreateWithFlags(&ev_, cudaEventDisableTiming), "cudaEventCreate", err)) != APK_OK)
+    return st;
+  if ((st = cu_status(cudaEventRecord(ev_, stream), "cudaEventRecord", err)) != APK_OK) return st;
+  last_ = stream;
+  used_ = true;
+  return APK_OK;
+}
+
+void Scratch::release() {
+  if (p_) cudaFree(p_);  // waits for the device
+  if (ev_) cudaEventDestroy(ev_);
+  p_ = nullptr;
+  ev_ = nullptr;
+  bytes_ = 0;
+  used_ = false;
+}
+
+namespace lin {
+
+__device__ __forceinline__ float bf2f(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+__device__ __forceinline__ uint16_t f2bf(float v) {
+  uint16_t r;
+  asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
+  return r;
+}
+
+// Copies an operand whose base or row stride is not a multiple of 16 bytes
+// (TMA cannot address it) to rows of ld elements, ld a multiple of 8.  One
+// thread per 8 elements, 2-byte loads along a warp.
+__global__ void __launch_bounds__(256) repack(const uint16_t* src, long long lds, int rows, int cols, uint16_t* dst,
+                                              int ld) {
+  const int chunks = ld / 8;
+  const long long n = (long long)rows * chunks;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long r = i / chunks;
+    const int c = (int)(i % chunks) * 8;
+    union {
+      uint16_t h[8];
+      uint4 v;
+    } u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u.h[j] = c + j < cols ? src[r * lds + c + j] : (uint16_t)0;
+    *reinterpret_cast<uint4*>(dst + r * ld + c) = u.v;
+  }
+}
+
+struct DzParams {
+  const uint16_t* dy;
+  const uint16_t* z;  // null: no activation
+  uint16_t* dz;       // null: not wanted (it is dy)
+  void* db;           // null: no bias
+  float* part;        // [row blocks][cols] partial column sums
+  unsigned* count;    // one per column block, zero between launches
+  long long ld_dy, ld_z, ld_dz;
+  int rows, cols, rows_per_block, act, db_f32;
+};
+
+constexpr int DZ_COLS = 256;  // columns of a block: 8 per lane
+
+// dz = dy * act'(z), rounded to bf16 (the products' operand type), and the
+// column sums of the unrounded dz.  One pass over dy and z.  A block sums its
+// rows in registers and shared memory; the last block of a column range adds
+// the row blocks' sums in their order, so db does not depend on the order of
+// arrival.  VEC: rows of 16-byte aligned 8-element chunks.
+template <bool VEC>
+__global__ void __launch_bounds__(256) dz_kernel(const DzParams p) {
+  __shared__ float sum[8][DZ_COLS];
+  __shared__ bool last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c0 = (int)blockIdx.x * DZ_COLS;
+  const long long r1 = min((long long)p.rows, (long long)(blockIdx.y + 1) * p.rows_per_block);
+  float acc[8] = {};
+  auto colof = [&](int i) { return VEC ? lane * 8 + i : lane + 32 * i; };
+  with_act(p.z ? p.act : APK_ACT_NONE, [&](auto tag) {
+    constexpr int ACT = decltype(tag)::value;
+#pragma unroll 2
+    for (long long r = (long long)blockIdx.y * p.rows_per_block + warp; r < r1; r += 8) {
+      union {
+        uint16_t h[8];
+        uint4 v;
+      } y, z;
+      z.v = make_uint4(0, 0, 0, 0);
+      if constexpr (VEC) {
+        if (c0 + lane * 8 >= p.cols) continue;
+        y.v = *reinterpret_cast<const uint4*>(p.dy + r * p.ld_dy + c0 + lane * 8);
+        if (ACT != APK_ACT_NONE) z.v = *reinterpret_cast<const uint4*>(p.z + r * p.ld_z + c0 + lane * 8);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool in = c0 + colof(i) < p.cols;
+          y.h[i] = in ? p.dy[r * p.ld_dy + c0 + colof(i)] : (uint16_t)0;
+          if (ACT != APK_ACT_NONE) z.h[i] = in ? p.z[r * p.ld_z + c0 + colof(i)] : (uint16_t)0;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = bf2f(y.h[i]) * act_grad_f<ACT>(bf2f(z.h[i]));
+        acc[i] += d;
+        y.h[i] = f2bf(d);
+      }
+      if (p.dz) {
+        if constexpr (VEC) {
+          *reinterpret_cast<uint4*>(p.dz + r * p.ld_dz + c0 + lane * 8) = y.v;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (c0 + colof(i) < p.cols) p.dz[r * p.ld_dz + c0 + colof(i)] = y.h[i];
+        }
+      }
+    }
+  });
+  if (!p.db) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum[warp][colof(i)] = acc[i];
+  __syncthreads();
+  const int c = c0 + (int)threadIdx.x;
+  float s = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) s += sum[w][threadIdx.x];
+  if (gridDim.y > 1) {
+    if (c < p.cols) p.part[(long long)blockIdx.y * p.cols + c] = s;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      last = atomicAdd(&p.count[blockIdx.x], 1u) == gridDim.y - 1;
+      if (last) p.count[blockIdx.x] = 0;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    s = 0.f;
+    if (c < p.cols)
+      for (unsigned b = 0; b < gridDim.y; ++b) s += __ldcg(p.part + (long long)b * p.cols + c);
+  }
+  if (c < p.cols) {
+    if (p.db_f32) static_cast<float*>(p.db)[c] = s;
+    else static_cast<uint16_t*>(p.db)[c] = f2bf(s);
+  }
+}
+
+}  // namespace lin
+}  // namespace apk
+
+using namespace apk;
+
+struct apk_linear {
+  apk_linear_config cfg{};
+  Err err;
+  int sms = 0;
+  int* status = nullptr;  // device word
+  Scratch scratch;
+  std::mutex mu;  // calls from several host threads are taken one at a time
+};
+
+namespace {
+
+bool tma_ok(const void* p, long long ld, int outer) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld % 8 == 0 || outer == 1);
+}
+int up8(int n) { return (n + 7) / 8 * 8; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// an operand as TMA can address it; one row needs no stride
+lin::Operand operand(const void* p, long long ld, int outer, int inner, bool mn) {
+  return {p, outer == 1 ? (long long)up8(inner) : ld, outer, inner, mn};
+}
+apk_status launch_repack(const void* src, long long lds, int rows, int cols, void* dst, cudaStream_t s, Err* err) {
+  const int ld = up8(cols);
+  const long long n = (long long)rows * (ld / 8);
+  const int grid = (int)std::min<long long>((n + 255) / 256, 148 * 16);
+  lin::repack<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(src), lds, rows, cols, static_cast<uint16_t*>(dst), ld);
+  return cu_status(cudaGetLastError(), "launching the repack kernel", err);
+}
+
+#define APK_TRY(x)                    \
+  do {                                \
+    const apk_status st_ = (x);       \
+    if (st_ != APK_OK) return st_;    \
+  } while (0)
+
+bool valid_dtype(int d) { return d == APK_F32 || d == APK_BF16; }
+const size_t esize[2] = {4, 2};  // APK_F32, APK_BF16
+bool aligned_to(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % esize[dtype] == 0; }
+
+apk_status forward(apk_linear* h, const apk_linear_io* io) {
+  const apk_linear_config& c = h->cfg;
+  const int K = c.in_features, N = c.out_features, M = io->rows;
+  const cudaStream_t s = static_cast<cudaStream_t>(io->stream);
+  if (M < 0) return h->err.fail(APK_EINVAL, "rows is %d", M);
+  if (M == 0) return APK_OK;
+  if (!io->x || !io->y) return h->err.fail(APK_EINVAL, "x or y is NULL");
+  if (!valid_dtype(io->y_dtype)) return h->err.fail(APK_EINVAL, "y_dtype %d", io->y_dtype);
+  if (io->residual && !valid_dtype(io->residual_dtype))
+    return h->err.fail(APK_EINVAL, "residual_dtype %d", io->residual_dtype);
+  if (io->ldx < K || io->ldy < N || (io->residual && io->ld_residual < N) || (io->preact && io->ld_preact < N))
+    return h->err.fail(APK_EINVAL, "a row stride is below its row: ldx %lld, ldy %lld, ld_residual %lld, ld_preact %lld",
+                       io->ldx, io->ldy, io->ld_residual, io->ld_preact);
+  if (!aligned_to(io->x, APK_BF16) || !aligned_to(io->y, io->y_dtype) ||
+      (io->residual && !aligned_to(io->residual, io->residual_dtype)) || !aligned_to(io->preact, APK_BF16))
+    return h->err.fail(APK_EINVAL, "a pointer is not aligned to its element");
+  DeviceGuard guard(c.device);
+  const int w_outer = c.w_layout == APK_W_KN ? K : N, w_inner = c.w_layout == APK_W_KN ? N : K;
+  const void* x = io->x;
+  const void* w = c.W;
+  long long ldx = io->ldx, ldw = c.ldw;
+  const bool px = !tma_ok(x, ldx, M), pw = !tma_ok(w, ldw, w_outer);
+  if (px || pw) {
+    const size_t bx = px ? up256((size_t)M * up8(K) * 2) : 0, bw = pw ? up256((size_t)w_outer * up8(w_inner) * 2) : 0;
+    const size_t zeroed = up256((size_t)(N + lin::DZ_COLS - 1) / lin::DZ_COLS * 4);
+    APK_TRY(h->scratch.begin(zeroed + bx + bw, zeroed, s, &h->err));
+    if (px) {
+      APK_TRY(launch_repack(x, ldx, M, K, h->scratch.data() + zeroed, s, &h->err));
+      x = h->scratch.data() + zeroed;
+      ldx = up8(K);
+    }
+    if (pw) {
+      APK_TRY(launch_repack(w, ldw, w_outer, w_inner, h->scratch.data() + zeroed + bx, s, &h->err));
+      w = h->scratch.data() + zeroed + bx;
+      ldw = up8(w_inner);
+    }
+  }
+  lin::Product p{};
+  p.P = operand(w, ldw, w_outer, w_inner, c.w_layout == APK_W_KN);
+  p.Q = operand(x, ldx, M, K, false);
+  p.rows = M;
+  p.cols = N;
+  p.k = K;
+  p.epi = {c.bias, io->residual, io->y, io->preact, io->ld_residual, io->ldy, io->ld_preact,
+           c.bias_dtype == APK_F32, io->residual_dtype == APK_F32, io->y_dtype == APK_F32, c.act};
+  APK_TRY(lin::run_products(&p, 1, h->sms, h->status, c.wait_limit_ns, s, &h->err.text));
+  if (px || pw) APK_TRY(h->scratch.end(s, &h->err));
+  return APK_OK;
+}
+
+apk_status backward(apk_linear* h, const apk_linear_grads* g) {
+  const apk_linear_config& c = h->cfg;
+  const int K = c.in_features, N = c.out_features, M = g->rows;
+  const cudaStream_t s = static_cast<cudaStream_t>(g->stream);
+  const bool kn = c.w_layout == APK_W_KN;
+  const int w_outer = kn ? K : N, w_inner = kn ? N : K;
+  if (M < 0) return h->err.fail(APK_EINVAL, "rows is %d", M);
+  if (!g->dx && !g->dw && !g->db) return h->err.fail(APK_EINVAL, "no gradient is asked for");
+  if (g->db && !c.bias) return h->err.fail(APK_EINVAL, "db of a layer without a bias");
+  if (g->dw && !valid_dtype(g->dw_dtype)) return h->err.fail(APK_EINVAL, "dw_dtype %d", g->dw_dtype);
+  if (M > 0 && (!g->dy || (g->dw && !g->x) || (c.act != APK_ACT_NONE && !g->preact)))
+    return h->err.fail(APK_EINVAL, "dy, x (for dw) or preact (with an activation) is NULL");
+  if (g->ld_dy < N || (g->dw && (g->ldx < K || g->ld_dw < w_inner)) || (g->dx && g->ld_dx < K) ||
+      (c.act != APK_ACT_NONE && g->ld_preact < N))
+    return h->err.fail(APK_EINVAL, "a row stride is below its row: ldx %lld, ld_dy %lld, ld_preact %lld, ld_dx %lld, ld_dw %lld",
+                       g->ldx, g->ld_dy, g->ld_preact, g->ld_dx, g->ld_dw);
+  if (!aligned_to(g->dy, APK_BF16) || !aligned_to(g->x, APK_BF16) || !aligned_to(g->preact, APK_BF16) ||
+      !aligned_to(g->dx, APK_BF16) || (g->dw && !aligned_to(g->dw, g->dw_dtype)) ||
+      (g->db && !aligned_to(g->db, c.bias_dtype)))
+    return h->err.fail(APK_EINVAL, "a pointer is not aligned to its element");
+  DeviceGuard guard(c.device);
+  if (M == 0) {  // sums over no rows
+    if (g->dw)
+      APK_TRY(cu_status(cudaMemset2DAsync(g->dw, (size_t)g->ld_dw * esize[g->dw_dtype], 0,
+                                          (size_t)w_inner * esize[g->dw_dtype], w_outer, s),
+                        "clearing dw", &h->err));
+    if (g->db) APK_TRY(cu_status(cudaMemsetAsync(g->db, 0, (size_t)N * esize[c.bias_dtype], s), "clearing db", &h->err));
+    return APK_OK;
+  }
+  const bool act = c.act != APK_ACT_NONE;
+  const bool products = g->dx || g->dw;
+  const bool own_dz = products && (act || !tma_ok(g->dy, g->ld_dy, M));
+  const bool px = g->dw && !tma_ok(g->x, g->ldx, M), pw = g->dx && !tma_ok(c.W, c.ldw, w_outer);
+  // blocks of the elementwise pass: about four per SM, at least 16 rows each
+  const int cblocks = (N + lin::DZ_COLS - 1) / lin::DZ_COLS;
+  int rblocks = std::max(1, std::min((M + 15) / 16, (4 * h->sms + cblocks - 1) / cblocks));
+  const int per = ((M + rblocks - 1) / rblocks + 7) / 8 * 8;
+  rblocks = (M + per - 1) / per;
+  const size_t zeroed = up256((size_t)cblocks * 4);
+  const size_t bpart = g->db ? up256((size_t)rblocks * N * 4) : 0;
+  const size_t bdz = own_dz ? up256((size_t)M * up8(N) * 2) : 0;
+  const size_t bx = px ? up256((size_t)M * up8(K) * 2) : 0, bw = pw ? up256((size_t)w_outer * up8(w_inner) * 2) : 0;
+  const bool scratch = g->db || own_dz || px || pw;
+  if (scratch) APK_TRY(h->scratch.begin(zeroed + bpart + bdz + bx + bw, zeroed, s, &h->err));
+  uint8_t* base = h->scratch.data();
+  const void* dz = g->dy;
+  long long ld_dz = g->ld_dy;
+  if (g->db || own_dz) {
+    lin::DzParams d{};
+    d.dy = static_cast<const uint16_t*>(g->dy);
+    d.z = act ? static_cast<const uint16_t*>(g->preact) : nullptr;
+    d.ld_dy = g->ld_dy;
+    d.ld_z = g->ld_preact;
+    if (own_dz) {
+      d.dz = reinterpret_cast<uint16_t*>(base + zeroed + bpart);
+      d.ld_dz = ld_dz = up8(N);
+      dz = d.dz;
+    }
+    d.db = g->db;
+    d.db_f32 = c.bias_dtype == APK_F32;
+    d.part = reinterpret_cast<float*>(base + zeroed);
+    d.count = reinterpret_cast<unsigned*>(base);
+    d.rows = M;
+    d.cols = N;
+    d.rows_per_block = per;
+    d.act = c.act;
+    // (the last chunk of a row may reach past N: only within an 8-multiple row)
+    const bool vec = N % 8 == 0 && tma_ok(g->dy, g->ld_dy, M) && (!act || tma_ok(g->preact, g->ld_preact, M));
+    if (rblocks > 65535) return h->err.fail(APK_EINVAL, "%d rows", M);
+    if (vec) lin::dz_kernel<true><<<dim3(cblocks, rblocks), 256, 0, s>>>(d);
+    else lin::dz_kernel<false><<<dim3(cblocks, rblocks), 256, 0, s>>>(d);
+    APK_TRY(cu_status(cudaGetLastError(), "launching the dz kernel", &h->err));
+  }
+  const void* x = g->x;
+  const void* w = c.W;
+  long long ldx = g->ldx, ldw = c.ldw;
+  if (px) {
+    void* q = base + zeroed + bpart + bdz;
+    APK_TRY(launch_repack(x, ldx, M, K, q, s, &h->err));
+    x = q;
+    ldx = up8(K);
+  }
+  if (pw) {
+    void* q = base + zeroed + bpart + bdz + bx;
+    APK_TRY(launch_repack(w, ldw, w_outer, w_inner, q, s, &h->err));
+    w = q;
+    ldw = up8(w_inner);
+  }
+  lin::Product p[2] = {};
+  int n = 0;
+  if (g->dx) {  // dx[m][k] = sum_n dz[m][n] W[k][n]
+    lin::Product& a = p[n++];
+    a.P = operand(w, ldw, w_outer, w_inner, !kn);
+    a.Q = operand(dz, ld_dz, M, N, false);
+    a.rows = M;
+    a.cols = K;
+    a.k = N;
+    a.epi = {nullptr, nullptr, g->dx, nullptr, 0, g->ld_dx, 0, 0, 0, 0, APK_ACT_NONE};
+  }
+  if (g->dw) {  // dW in W's layout: rows of x^T by columns of dz, or the reverse
+    lin::Product& a = p[n++];
+    const lin::Operand ox = operand(x, ldx, M, K, true), oz = operand(dz, ld_dz, M, N, true);
+    a.P = kn ? oz : ox;
+    a.Q = kn ? ox : oz;
+    a.rows = w_outer;
+    a.cols = w_inner;
+    a.k = M;
+    a.epi = {nullptr, nullptr, g->dw, nullptr, 0, g->ld_dw, 0, 0, 0, g->dw_dtype == APK_F32, APK_ACT_NONE};
+  }
+  if (n) APK_TRY(lin::run_products(p, n, h->sms, h->status, c.wait_limit_ns, s, &h->err.text));
+  if (scratch) APK_TRY(h->scratch.end(s, &h->err));
+  return APK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+apk_status apk_linear_create(const apk_linear_config* cfg, apk_linear** out) {
+  if (!out) return APK_EINVAL;
+  *out = nullptr;
+  apk_linear* h = new (std::nothrow) apk_linear;
+  if (!h) return APK_ENOMEM;
+  *out = h;  // also on failure: apk_linear_last_error says why, apk_linear_destroy frees it
+  if (!cfg) return h->err.fail(APK_EINVAL, "cfg is NULL");
+  h->cfg = *cfg;
+  const apk_linear_config& c = h->cfg;
+  if (c.in_features < 1 || c.out_features < 1)
+    return h->err.fail(APK_EINVAL, "in_features %d, out_features %d", c.in_features, c.out_features);
+  if (c.w_layout != APK_W_KN && c.w_layout != APK_W_NK) return h->err.fail(APK_EINVAL, "w_layout %d", (int)c.w_layout);
+  if (c.act < APK_ACT_NONE || c.act > APK_ACT_SILU) return h->err.fail(APK_EINVAL, "act %d", (int)c.act);
+  if (!c.W) return h->err.fail(APK_EINVAL, "W is NULL");
+  if (c.ldw < (c.w_layout == APK_W_KN ? c.out_features : c.in_features))
+    return h->err.fail(APK_EINVAL, "ldw %lld is below W's row", c.ldw);
+  if (c.bias && !valid_dtype(c.bias_dtype)) return h->err.fail(APK_EINVAL, "bias_dtype %d", (int)c.bias_dtype);
+  if (!aligned_to(c.W, APK_BF16) || (c.bias && !aligned_to(c.bias, c.bias_dtype)))
+    return h->err.fail(APK_EINVAL, "W or bias is not aligned to its element");
+  if (c.wait_limit_ns < 0) return h->err.fail(APK_EINVAL, "wait_limit_ns is negative");
+  if (c.wait_limit_ns == 0) h->cfg.wait_limit_ns = 2000000000ll;
+  int ndev = 0;
+  if (cudaGetDeviceCount(&ndev) != cudaSuccess || c.device < 0 || c.device >= ndev) {
+    cudaGetLastError();
+    return h->err.fail(APK_ECUDA, "no CUDA device %d", c.device);
+  }
+  DeviceGuard guard(c.device);
+  int major = 0, sms = 0, pairs = 0;
+  APK_TRY(cu_status(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, c.device), "device query", &h->err));
+  APK_TRY(cu_status(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device), "device query", &h->err));
+  if (major != 10) return h->err.fail(APK_EUNSUPPORTED, "the kernels are built for sm_100a");
+  APK_TRY(cu_status(lin::prepare(&pairs), "preparing the linear kernels", &h->err));
+  h->sms = sms;
+  if (c.sms < 0 || c.sms > sms) return h->err.fail(APK_EINVAL, "sms %d of %d", c.sms, sms);
+  if (c.sms > 0) h->sms = c.sms;
+  void* st = nullptr;
+  APK_TRY(cu_status(cudaMalloc(&st, 256), "cudaMalloc", &h->err));
+  h->status = static_cast<int*>(st);
+  APK_TRY(cu_status(cudaMemset(st, 0, 256), "cudaMemset", &h->err));
+  return cu_status(cudaStreamSynchronize(nullptr), "cudaStreamSynchronize", &h->err);
+}
+
+apk_status apk_linear_destroy(apk_linear* h) {
+  if (!h) return APK_OK;
+  if (h->status) {
+    DeviceGuard guard(h->cfg.device);
+    h->scratch.release();
+    cudaFree(h->status);
+  }
+  delete h;
+  return APK_OK;
+}
+
+const char* apk_linear_last_error(const apk_linear* h) { return h ? h->err.text.c_str() : "NULL handle"; }
+
+apk_status apk_linear_forward(apk_linear* h, const apk_linear_io* io) {
+  if (!h || !h->status || !io) return APK_EINVAL;
+  try {
+    std::lock_guard<std::mutex> lock(h->mu);
+    return forward(h, io);
+  } catch (...) {
+    return APK_ENOMEM;
+  }
+}
+
+apk_status apk_linear_backward(apk_linear* h, const apk_linear_grads* g) {
+  if (!h || !h->status || !g) return APK_EINVAL;
+  try {
+    std::lock_guard<std::mutex> lock(h->mu);
+    return backward(h, g);
+  } catch (...) {
+    return APK_ENOMEM;
+  }
+}
+
+apk_status apk_linear_status(apk_linear* h, void* stream, int* device_status) {
+  if (!h || !h->status || !device_status) return APK_EINVAL;
+  try {
+    std::lock_guard<std::mutex> lock(h->mu);
+    DeviceGuard guard(h->cfg.device);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    APK_TRY(cu_status(cudaMemcpyAsync(device_status, h->status, sizeof(int), cudaMemcpyDeviceToHost, s), "status copy",
+                      &h->err));
+    APK_TRY(cu_status(cudaMemsetAsync(h->status, 0, sizeof(int), s), "status clear", &h->err));
+    return cu_status(cudaStreamSynchronize(s), "cudaStreamSynchronize", &h->err);
+  } catch (...) {
+    return APK_ENOMEM;
+  }
+}
+
+}  // extern "C"

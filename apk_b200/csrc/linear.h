@@ -1,0 +1,120 @@
+// Shared by the layer operators (linear_gemm.cu, linear.cu, moe.cu): the
+// GEMM problem the epilogue kernel runs, and host helpers.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <cstdarg>
+#include <cstdio>
+#include <string>
+
+#include "../../include/apk.h"
+
+namespace apk {
+namespace lin {
+
+// One product out[r][c] = act(sum_k Q(r,k) P(k,c) + bias[c]) + res[r][c].
+// P is the operand of the output's columns, Q that of its rows; either is
+// K-major (k contiguous) or MN-major (its columns / rows contiguous).
+struct Epilogue {
+  const void* bias;
+  const void* res;
+  void* out;
+  void* pre;  // bf16 pre-activation, or null
+  long long ld_res, ld_out, ld_pre;
+  int bias_f32, res_f32, out_f32, act;
+};
+struct alignas(64) Problem {
+  CUtensorMap tmP, tmQ;
+  Epilogue epi;
+  int rows, cols, nkb;
+  int tiles_r, tiles_c;
+  int p_mn, q_mn;
+  uint32_t idesc;
+};
+struct GemmParams {
+  Problem pr[2];
+  int nprob;
+  int tiles0, tiles;  // tiles of problem 0 / of all
+  int split;          // CTAs of a cluster that share one tile's K range (1: none)
+  int* status;
+  long long limit;
+};
+
+// An operand as the caller holds it: [outer][inner] bf16, `inner` contiguous.
+struct Operand {
+  const void* p;
+  long long ld;
+  int outer, inner;
+  bool mn;  // the contiguous axis is the output's (MN-major), not k
+};
+struct Product {
+  Operand P, Q;
+  int rows, cols, k;
+  Epilogue epi;
+};
+
+// Launches one or two products (one launch). sms: the SMs it may fill.
+// `why` receives a message on failure.
+apk_status run_products(const Product* pr, int n, int sms, int* status, long long limit, cudaStream_t stream,
+                        std::string* why);
+// The first use on a device sets the kernels' shared-memory attributes.
+cudaError_t prepare(int* pairs);
+
+}  // namespace lin
+
+// ---- host helpers -----------------------------------------------------------
+struct Err {
+  std::string text;
+  apk_status fail(apk_status st, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    text = buf;
+    return st;
+  }
+};
+
+// The calling thread's device is put back when a call returns.
+class DeviceGuard {
+ public:
+  explicit DeviceGuard(int dev) {
+    cudaGetDevice(&old_);
+    if (old_ != dev) cudaSetDevice(dev);
+    else old_ = -1;
+  }
+  ~DeviceGuard() {
+    if (old_ >= 0) cudaSetDevice(old_);
+  }
+
+ private:
+  int old_ = -1;
+};
+
+// Device scratch of one handle.  Calls on one handle may come from different
+// streams: a call that uses the scratch waits for the last one that did.  In
+// a stream capture the events are left out (the order of a graph's launches
+// and of other calls is the caller's), and the scratch may not grow.
+class Scratch {
+ public:
+  // At least `bytes` of scratch, the first `zeroed` of them zero when it was
+  // allocated and left so by every kernel that uses them.
+  apk_status begin(size_t bytes, size_t zeroed, cudaStream_t stream, Err* err);
+  apk_status end(cudaStream_t stream, Err* err);
+  uint8_t* data() const { return p_; }
+  void release();
+
+ private:
+  uint8_t* p_ = nullptr;
+  size_t bytes_ = 0;
+  cudaEvent_t ev_ = nullptr;
+  cudaStream_t last_ = nullptr;
+  bool used_ = false, capturing_ = false;
+};
+
+apk_status cu_status(cudaError_t e, const char* what, Err* err);
+
+}  // namespace apk

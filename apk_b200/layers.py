@@ -1,0 +1,218 @@
+"""Layer operators over torch tensors: Linear (forward, backward) and MoE.
+
+Thin classes over the C ABI's apk_linear_* and apk_moe_* (include/apk.h):
+they check shapes, types and strides, allocate outputs with torch, and run
+on torch's current stream of the weights' device.  torch is used for memory
+and streams only; the arithmetic is libapk's.  No counterpart in the
+reference, which multiplies bare matrices (src/tcyield.cu:91-356).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib as L
+from .runtime import ApkError
+
+_ACT = {"none": L.APK_ACT_NONE, "relu": L.APK_ACT_RELU, "gelu": L.APK_ACT_GELU,
+        "gelu_tanh": L.APK_ACT_GELU_TANH, "silu": L.APK_ACT_SILU}
+_LAYOUT = {"kn": L.APK_W_KN, "nk": L.APK_W_NK}
+_TORCH = {"f32": torch.float32, "bf16": torch.bfloat16}
+_CODE = {torch.float32: L.APK_F32, torch.bfloat16: L.APK_BF16}
+_DEFAULT_WAIT_NS = 2_000_000_000
+
+
+def _pick(table, value, what):
+    try:
+        return table[value]
+    except (KeyError, TypeError):
+        raise ValueError(f"{what} is {value!r}: one of {', '.join(table)}") from None
+
+
+def _tensor(t, what, device=None, dtypes=(torch.bfloat16,), dim=None):
+    """t itself, or a ValueError that says what is wrong with it."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{what} is not a torch tensor")
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise ValueError(f"{what} is on {t.device}, not on {device or 'a CUDA device'}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{what} is {t.dtype}: one of {', '.join(str(d) for d in dtypes)}")
+    if dim is not None and t.dim() != dim:
+        raise ValueError(f"{what} has {t.dim()} axes, not {dim}")
+    return t
+
+
+def _rows(t, what, device, width, dtypes=(torch.bfloat16,)):
+    """(2-D view, row stride) of a [..., width] tensor; the last axis has to be contiguous."""
+    _tensor(t, what, device, dtypes)
+    if t.dim() < 1 or t.shape[-1] != width:
+        raise ValueError(f"{what} is {tuple(t.shape)}: its last axis has to be {width}")
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    s0, s1 = t.stride()
+    if s1 != 1 and width > 1:
+        raise ValueError(f"{what}: its last axis has stride {s1}, not 1")
+    return t, (s0 if t.shape[0] > 1 else width)
+
+
+class _Handle:
+    """Owner of one native handle; subclasses name its functions."""
+    _create = _destroy = _error = _status = ""
+
+    def _open(self, cfg):
+        self._lib = L.load()
+        self._h = ctypes.c_void_p()
+        st = getattr(self._lib, self._create)(ctypes.byref(cfg), ctypes.byref(self._h))
+        if st != L.APK_OK:
+            message = self._message()
+            self.close()
+            raise ApkError(st, message)
+
+    def _message(self):
+        return getattr(self._lib, self._error)(self._h).decode()
+
+    def _check(self, st):
+        if st != L.APK_OK:
+            raise ApkError(st, self._message())
+
+    def status(self) -> int:
+        """The first device error since the last query (0: none); waits for the current stream."""
+        st = ctypes.c_int()
+        self._check(getattr(self._lib, self._status)(self._h, self._stream(), ctypes.byref(st)))
+        return st.value
+
+    def _stream(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def close(self):
+        if getattr(self, "_h", None) is not None and self._h.value:
+            getattr(self._lib, self._destroy)(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Linear(_Handle):
+    """y = act(x W + b) + r with bf16 weights, and its gradients.
+
+    weight: [in, out] for layout "kn" (the GEMM runtime's row-major B) or
+    [out, in] for "nk", bf16, rows of any stride.  bias: [out] fp32 or bf16.
+    act: none, relu, gelu, gelu_tanh or silu.  The layer keeps a reference to
+    the tensors, not a copy: an optimizer may update them in place."""
+    _create, _destroy = "apk_linear_create", "apk_linear_destroy"
+    _error, _status = "apk_linear_last_error", "apk_linear_status"
+
+    def __init__(self, weight, bias=None, act: str = "none", layout: str = "kn", out_dtype: str = "bf16",
+                 sms: int = 0, wait_limit_ns: int = _DEFAULT_WAIT_NS):
+        _tensor(weight, "weight", dim=2)
+        kn = _pick(_LAYOUT, layout, "layout") == L.APK_W_KN
+        self.device = weight.device
+        self.in_features, self.out_features = weight.shape if kn else weight.shape[::-1]
+        w, ldw = _rows(weight, "weight", self.device, weight.shape[1])
+        if bias is not None:
+            _tensor(bias, "bias", self.device, tuple(_CODE), 1)
+            if bias.shape[0] != self.out_features or (bias.shape[0] > 1 and bias.stride(0) != 1):
+                raise ValueError(f"bias is {tuple(bias.shape)} with strides {bias.stride()}: "
+                                 f"{self.out_features} contiguous values are wanted")
+        self.weight, self.bias, self.act, self.layout = weight, bias, act, layout
+        self.out_dtype = _pick(_TORCH, out_dtype, "out_dtype")
+        self._act = _pick(_ACT, act, "act")
+        self._open(L.LinearConfig(self.device.index, self.in_features, self.out_features, _LAYOUT[layout], self._act,
+                                  _CODE[bias.dtype] if bias is not None else L.APK_F32, w.data_ptr(), ldw,
+                                  bias.data_ptr() if bias is not None else None, sms, wait_limit_ns))
+        self._io, self._grads = L.LinearIO(), L.LinearGrads()
+        self._io_ref, self._grads_ref = ctypes.byref(self._io), ctypes.byref(self._grads)
+
+    def forward(self, x, residual=None, save_preact: bool = False, out=None):
+        """act(x W + b) + residual for x [..., in]; with save_preact also
+        x W + b in bf16, as backward() takes it.  out: the output's tensor;
+        it may be the residual."""
+        io, n = self._io, self.out_features
+        x2, io.ldx = _rows(x, "x", self.device, self.in_features)
+        m = x2.shape[0]
+        shape = (*x.shape[:-1], n)
+        if out is None:
+            y = torch.empty(shape, dtype=self.out_dtype, device=self.device)
+            y_ptr, io.ldy = y.data_ptr(), n
+        else:
+            y = out
+            if y.shape != shape:
+                raise ValueError(f"out is {tuple(y.shape)}, not {shape}")
+            y2, io.ldy = _rows(y, "out", self.device, n, (self.out_dtype,))
+            y_ptr = y2.data_ptr()
+            if y_ptr != y.data_ptr():
+                raise ValueError("out cannot be written as rows of one stride")
+        if residual is None:
+            io.residual = None
+        else:
+            if residual.shape != shape:
+                raise ValueError(f"residual is {tuple(residual.shape)}, not {shape}")
+            r2, io.ld_residual = _rows(residual, "residual", self.device, n, tuple(_CODE))
+            io.residual, io.residual_dtype = r2.data_ptr(), _CODE[residual.dtype]
+        z = None
+        if save_preact:
+            z = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            io.preact, io.ld_preact = z.data_ptr(), n
+        else:
+            io.preact = None
+        io.x, io.y, io.rows, io.y_dtype, io.stream = x2.data_ptr(), y_ptr, m, _CODE[self.out_dtype], self._stream()
+        st = self._lib.apk_linear_forward(self._h, self._io_ref)
+        if st:
+            self._check(st)
+        return (y, z) if save_preact else y
+
+    __call__ = forward
+
+    def backward(self, dy, x, preact=None, need_dx: bool = True, need_dw: bool = True, need_db: bool = True,
+                 dw_dtype: str = "bf16"):
+        """(dx, dw, db) for the output gradient dy (the residual's is dy
+        itself); None where one is not needed or the layer has no bias.
+        preact: what forward(save_preact=True) returned, for a layer with an
+        activation."""
+        g, n, k = self._grads, self.out_features, self.in_features
+        dy2, g.ld_dy = _rows(dy, "dy", self.device, n)
+        m = dy2.shape[0]
+        if dy.shape[:-1] != x.shape[:-1]:
+            raise ValueError(f"dy is {tuple(dy.shape)} and x {tuple(x.shape)}")
+        x2, g.ldx = _rows(x, "x", self.device, k)
+        if self._act != L.APK_ACT_NONE:
+            if preact is None or preact.shape != dy.shape:
+                raise ValueError("preact: the pre-activation that forward(save_preact=True) returned is wanted")
+            z2, g.ld_preact = _rows(preact, "preact", self.device, n)
+            g.preact = z2.data_ptr()
+        else:
+            g.preact = None
+        dx = dw = db = None
+        if need_dx:
+            dx = torch.empty(x.shape, dtype=torch.bfloat16, device=self.device)
+            g.dx, g.ld_dx = dx.data_ptr(), k
+        else:
+            g.dx = None
+        if need_dw:
+            dt = _pick(_TORCH, dw_dtype, "dw_dtype")
+            dw = torch.empty(self.weight.shape, dtype=dt, device=self.device)
+            g.dw, g.ld_dw, g.dw_dtype = dw.data_ptr(), self.weight.shape[1], _CODE[dt]
+        else:
+            g.dw = None
+        if need_db and self.bias is not None:
+            db = torch.empty_like(self.bias)
+            g.db = db.data_ptr()
+        else:
+            g.db = None
+        g.dy, g.x, g.rows, g.stream = dy2.data_ptr(), x2.data_ptr(), m, self._stream()
+        if dx is not None or dw is not None or db is not None:
+            st = self._lib.apk_linear_backward(self._h, self._grads_ref)
+            if st:
+                self._check(st)
+        return dx, dw, db

@@ -484,6 +484,106 @@ long long apk_gen_tasks(unsigned long long seed, int n, int mn_lo, int mn_hi, in
  * count.  Deterministic, disjoint, and the ranks' union is every task. */
 int apk_shard_tasks(const apk_task* tasks, int n, int world, int rank, int* idx);
 
+/* ---- layers: the feed-forward half of a transformer ---------------------- */
+
+/* A linear layer with a fused epilogue, its gradients, and a routed
+ * mixture-of-experts layer for a few tokens.  Unlike the contexts above these
+ * take any size, stride and alignment that their comments do not exclude,
+ * run as ordinary kernels on the caller's stream, and hold no operands of
+ * their own: a handle keeps the caller's weight pointers, which may be
+ * updated in place between calls.  All pointers are device memory; strides
+ * count elements; the last axis is contiguous.  No counterpart in the
+ * reference, which multiplies bare matrices (src/tcyield.cu:91-356).
+ *
+ * Calls are asynchronous on `stream` (a cudaStream_t).  A handle may be used
+ * from several streams: calls that need its scratch are ordered among
+ * themselves.  Scratch grows on first use of a size (which allocates, and is
+ * refused with APK_ESTATE inside a stream capture); the order of captured
+ * calls and others is the caller's.  Device waits are bounded by
+ * wait_limit_ns (0: 2 s); one that runs out leaves the outputs incomplete and
+ * shows in apk_linear_status / apk_moe_status. */
+typedef enum apk_act {
+  APK_ACT_NONE = 0,
+  APK_ACT_RELU = 1,         /* a NaN stays one                                */
+  APK_ACT_GELU = 2,         /* x Phi(x)                                       */
+  APK_ACT_GELU_TANH = 3,    /* its tanh form                                  */
+  APK_ACT_SILU = 4          /* x / (1 + exp(-x))                              */
+} apk_act;
+
+/* KN: W [in_features][out_features], the row-major B of the GEMMs above.
+ * NK: W [out_features][in_features]. */
+typedef enum apk_w_layout { APK_W_KN = 0, APK_W_NK = 1 } apk_w_layout;
+
+typedef struct apk_linear_config {
+  int device;
+  int in_features, out_features;  /* at least 1, no other limit               */
+  apk_w_layout w_layout;
+  apk_act act;
+  apk_dtype bias_dtype;
+  const void* W;            /* bf16                                           */
+  long long ldw;
+  const void* bias;         /* out_features values, or NULL                   */
+  int sms;                  /* SMs the products may fill; 0 = all             */
+  long long wait_limit_ns;
+} apk_linear_config;
+typedef struct apk_linear apk_linear;
+
+/* On failure *out is still set (unless memory ran out) so that
+ * apk_linear_last_error can be asked; destroy it in either case. */
+apk_status apk_linear_create(const apk_linear_config* cfg, apk_linear** out);
+apk_status apk_linear_destroy(apk_linear* h);
+const char* apk_linear_last_error(const apk_linear* h);
+
+/* y = act(x W + bias) + residual; preact, if given, receives x W + bias
+ * rounded to bf16 for the backward pass.  Sums, bias, activation and residual
+ * are taken in fp32 and rounded once to y_dtype.  x must not overlap an
+ * output; residual may be y itself.  rows = 0 does nothing.  Rows or a base
+ * that TMA cannot address (not a multiple of 16 bytes) cost a copy of that
+ * operand. */
+typedef struct apk_linear_io {
+  const void* x;            /* bf16 [rows][in_features]                       */
+  long long ldx;
+  int rows;
+  apk_dtype residual_dtype;
+  const void* residual;     /* [rows][out_features] or NULL                   */
+  long long ld_residual;
+  void* y;                  /* [rows][out_features]                           */
+  long long ldy;
+  apk_dtype y_dtype;
+  void* preact;             /* bf16 [rows][out_features] or NULL              */
+  long long ld_preact;
+  void* stream;
+} apk_linear_io;
+apk_status apk_linear_forward(apk_linear* h, const apk_linear_io* io);
+
+/* Gradients of a forward call whose output gradient is dy (the residual's
+ * gradient is dy itself):  dz = dy * act'(preact),  dx = dz W^T,
+ * dw = x^T dz in W's layout,  db = the sum of dz's rows.  An output that is
+ * NULL is not computed.  dz is rounded to bf16 as the products' operand; db
+ * sums it unrounded.  With rows = 0, dw and db are cleared. */
+typedef struct apk_linear_grads {
+  const void* dy;           /* bf16 [rows][out_features]                      */
+  long long ld_dy;
+  const void* x;            /* bf16 [rows][in_features], for dw               */
+  long long ldx;
+  const void* preact;       /* bf16 [rows][out_features]; with APK_ACT_NONE unused */
+  long long ld_preact;
+  int rows;
+  apk_dtype dw_dtype;
+  void* dx;                 /* bf16 [rows][in_features] or NULL               */
+  long long ld_dx;
+  void* dw;                 /* W's shape or NULL                              */
+  long long ld_dw;
+  void* db;                 /* out_features of bias_dtype, or NULL            */
+  void* stream;
+} apk_linear_grads;
+apk_status apk_linear_backward(apk_linear* h, const apk_linear_grads* g);
+
+/* The first device error since the last query (0: none; 1, 2: a pipeline
+ * wait ran out): copies and clears the status word on `stream` and
+ * synchronizes it. */
+apk_status apk_linear_status(apk_linear* h, void* stream, int* device_status);
+
 /* ---- allocation-free entry point --------------------------------------- */
 
 /* C = A * B (fp32, row-major, device pointers, 16-byte aligned; M and N
