@@ -106,6 +106,17 @@ class LinearGrads(ctypes.Structure):
                 ("dw", c_void_p), ("ld_dw", c_ll), ("db", c_void_p), ("stream", c_void_p)]
 
 
+class MoeConfig(ctypes.Structure):
+    _fields_ = [("device", c_int), ("experts", c_int), ("top_k", c_int), ("d_model", c_int), ("d_ff", c_int),
+                ("act", c_int), ("gated", c_int), ("renormalize", c_int), ("router", c_void_p), ("w_in", c_void_p),
+                ("w_out", c_void_p), ("sms", c_int), ("wait_limit_ns", c_ll)]
+
+
+class MoeIO(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("ldx", c_ll), ("tokens", c_int), ("y_dtype", c_int), ("y", c_void_p),
+                ("ldy", c_ll), ("ids", c_void_p), ("probs", c_void_p), ("stream", c_void_p)]
+
+
 P = c_void_p
 # name -> (restype, argtypes); every symbol include/apk.h declares
 SIGNATURES = {
@@ -151,6 +162,11 @@ SIGNATURES = {
     "apk_linear_forward": (c_int, [P, ctypes.POINTER(LinearIO)]),
     "apk_linear_backward": (c_int, [P, ctypes.POINTER(LinearGrads)]),
     "apk_linear_status": (c_int, [P, P, ctypes.POINTER(c_int)]),
+    "apk_moe_create": (c_int, [ctypes.POINTER(MoeConfig), ctypes.POINTER(P)]),
+    "apk_moe_destroy": (c_int, [P]),
+    "apk_moe_last_error": (c_char_p, [P]),
+    "apk_moe_forward": (c_int, [P, ctypes.POINTER(MoeIO)]),
+    "apk_moe_status": (c_int, [P, P, ctypes.POINTER(c_int)]),
     "apk_sgemm_f32_noalloc": (c_int, [P, P, P, c_int, c_int, c_int, c_int, P]),
     "apk_sgemm_f32_noalloc_status": (c_int, [P, ctypes.POINTER(c_int)]),
     "apk_sgemm_f32_noalloc_selftest": (c_int, [c_ll, P]),

@@ -182,6 +182,15 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, in
       : "memory");
 }
 
+// ---- programmatic dependent launch ------------------------------------------
+// A kernel launched with the stream-serialization attribute may start while
+// its predecessor runs.  pdl_wait() returns once the predecessor has completed
+// and its writes are visible: everything before it must touch neither memory
+// that another kernel writes nor memory that one reads.  pdl_launch() lets the
+// successor start, as soon as every CTA of this grid has called it or exited.
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- streamed operands ------------------------------------------------------
 // Wait (bounded) until both readiness words are nonzero; the copies they
 // announce were written by a copy engine, so order this thread's later

@@ -80,6 +80,8 @@ __global__ void __launch_bounds__(256) repack(const uint16_t* src, long long lds
                                               int ld) {
   const int chunks = ld / 8;
   const long long n = (long long)rows * chunks;
+  pdl_launch();
+  pdl_wait();
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
     const long long r = i / chunks;
     const int c = (int)(i % chunks) * 8;
@@ -119,6 +121,8 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzParams p) {
   const int c0 = (int)blockIdx.x * DZ_COLS;
   const long long r1 = min((long long)p.rows, (long long)(blockIdx.y + 1) * p.rows_per_block);
   float acc[8] = {};
+  pdl_launch();
+  pdl_wait();
   auto colof = [&](int i) { return VEC ? lane * 8 + i : lane + 32 * i; };
   with_act(p.z ? p.act : APK_ACT_NONE, [&](auto tag) {
     constexpr int ACT = decltype(tag)::value;
@@ -217,8 +221,10 @@ apk_status launch_repack(const void* src, long long lds, int rows, int cols, voi
   const int ld = up8(cols);
   const long long n = (long long)rows * (ld / 8);
   const int grid = (int)std::min<long long>((n + 255) / 256, 148 * 16);
-  lin::repack<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(src), lds, rows, cols, static_cast<uint16_t*>(dst), ld);
-  return cu_status(cudaGetLastError(), "launching the repack kernel", err);
+  Launch l(dim3(grid), 256, 0, s);
+  return cu_status(cudaLaunchKernelEx(&l.cfg, lin::repack, static_cast<const uint16_t*>(src), lds, rows, cols,
+                                      static_cast<uint16_t*>(dst), ld),
+                   "launching the repack kernel", err);
 }
 
 #define APK_TRY(x)                    \
@@ -249,6 +255,11 @@ apk_status forward(apk_linear* h, const apk_linear_io* io) {
     return h->err.fail(APK_EINVAL, "a pointer is not aligned to its element");
   DeviceGuard guard(c.device);
   const int w_outer = c.w_layout == APK_W_KN ? K : N, w_inner = c.w_layout == APK_W_KN ? N : K;
+  const lin::Epilogue epi = {c.bias, io->residual, io->y, io->preact, io->ld_residual, io->ldy, io->ld_preact,
+                             c.bias_dtype == APK_F32, io->residual_dtype == APK_F32, io->y_dtype == APK_F32, c.act};
+  if (M <= lin::STREAM_ROWS)
+    return cu_status(lin::run_stream(io->x, io->ldx, c.W, c.ldw, c.w_layout == APK_W_NK, M, N, K, epi, h->sms, s),
+                     "launching the streaming kernel", &h->err);
   const void* x = io->x;
   const void* w = c.W;
   long long ldx = io->ldx, ldw = c.ldw;
@@ -274,8 +285,7 @@ apk_status forward(apk_linear* h, const apk_linear_io* io) {
   p.rows = M;
   p.cols = N;
   p.k = K;
-  p.epi = {c.bias, io->residual, io->y, io->preact, io->ld_residual, io->ldy, io->ld_preact,
-           c.bias_dtype == APK_F32, io->residual_dtype == APK_F32, io->y_dtype == APK_F32, c.act};
+  p.epi = epi;
   APK_TRY(lin::run_products(&p, 1, h->sms, h->status, c.wait_limit_ns, s, &h->err.text));
   if (px || pw) APK_TRY(h->scratch.end(s, &h->err));
   return APK_OK;
@@ -350,9 +360,9 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
     // (the last chunk of a row may reach past N: only within an 8-multiple row)
     const bool vec = N % 8 == 0 && tma_ok(g->dy, g->ld_dy, M) && (!act || tma_ok(g->preact, g->ld_preact, M));
     if (rblocks > 65535) return h->err.fail(APK_EINVAL, "%d rows", M);
-    if (vec) lin::dz_kernel<true><<<dim3(cblocks, rblocks), 256, 0, s>>>(d);
-    else lin::dz_kernel<false><<<dim3(cblocks, rblocks), 256, 0, s>>>(d);
-    APK_TRY(cu_status(cudaGetLastError(), "launching the dz kernel", &h->err));
+    Launch l(dim3(cblocks, rblocks), 256, 0, s);
+    APK_TRY(cu_status(cudaLaunchKernelEx(&l.cfg, vec ? lin::dz_kernel<true> : lin::dz_kernel<false>, d),
+                      "launching the dz kernel", &h->err));
   }
   const void* x = g->x;
   const void* w = c.W;

@@ -59,6 +59,11 @@ struct Product {
 // `why` receives a message on failure.
 apk_status run_products(const Product* pr, int n, int sms, int* status, long long limit, cudaStream_t stream,
                         std::string* why);
+// A product of at most STREAM_ROWS rows with weights [n][k] (nk) or [k][n] of
+// any stride and alignment.
+constexpr int STREAM_ROWS = 16;
+cudaError_t run_stream(const void* x, long long ldx, const void* w, long long ldw, bool nk, int rows, int n, int k,
+                       const Epilogue& epi, int sms, cudaStream_t stream);
 // The first use on a device sets the kernels' shared-memory attributes.
 cudaError_t prepare(int* pairs);
 
@@ -113,6 +118,30 @@ class Scratch {
   cudaEvent_t ev_ = nullptr;
   cudaStream_t last_ = nullptr;
   bool used_ = false, capturing_ = false;
+};
+
+// Launch configuration with a cluster size and programmatic stream
+// serialization (every kernel launched with it calls pdl_wait first thing).
+struct Launch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[3];
+  Launch(dim3 grid, int threads, size_t smem, cudaStream_t stream, int cluster = 1) {
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = at;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    if (cluster > 1) {
+      at[1].id = cudaLaunchAttributeClusterDimension;
+      at[1].val.clusterDim.x = cluster;
+      at[1].val.clusterDim.y = 1;
+      at[1].val.clusterDim.z = 1;
+      cfg.numAttrs = 2;
+    }
+  }
 };
 
 apk_status cu_status(cudaError_t e, const char* what, Err* err);

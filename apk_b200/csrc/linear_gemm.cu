@@ -155,17 +155,54 @@ __device__ __forceinline__ void store_elem(void* p, long long i, float v, int f3
   else static_cast<uint16_t*>(p)[i] = to_bf16(v);
 }
 
-// W rows from r of the column c: bias, pre-activation, activation, residual.
-template <int ACT, int W>
-__device__ __forceinline__ void finish_rows(const Epilogue& e, const uint32_t (&v)[W], const float (&res)[W],
-                                            float bias, int r, int rows, long long c) {
+// W rows of one output column: bias, pre-activation, activation, residual,
+// stores.  out and pre point at the first row's element.  The types and the
+// presence of the pre-activation are fixed per call of this function: with
+// run-time flags in the element loop and an address product per element the
+// epilogue took 51 instructions a row and twice the time of the MMAs of 2048 k.
+template <int ACT, bool PRE, bool F32, int W>
+__device__ __forceinline__ void finish_full(const Epilogue& e, const uint32_t (&v)[W], const float (&res)[W],
+                                            float bias, uint8_t* out, uint8_t* pre) {
+  const long long so = e.ld_out * (F32 ? 4 : 2), sp = e.ld_pre * 2;
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    if (r + i < rows) {
-      const float z = __uint_as_float(v[i]) + bias;
-      if (e.pre) store_elem(e.pre, (long long)(r + i) * e.ld_pre + c, z, 0);
-      store_elem(e.out, (long long)(r + i) * e.ld_out + c, act_f<ACT>(z) + res[i], e.out_f32);
+    const float z = __uint_as_float(v[i]) + bias;
+    if (PRE) {
+      *reinterpret_cast<uint16_t*>(pre) = to_bf16(z);
+      pre += sp;
     }
+    const float y = act_f<ACT>(z) + res[i];
+    if (F32) *reinterpret_cast<float*>(out) = y;
+    else *reinterpret_cast<uint16_t*>(out) = to_bf16(y);
+    out += so;
+  }
+}
+// The same for a block that reaches past the last row.
+template <int ACT, int W>
+__device__ __forceinline__ void finish_part(const Epilogue& e, const uint32_t (&v)[W], const float (&res)[W],
+                                            float bias, uint8_t* out, uint8_t* pre, int n) {
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    if (i < n) {
+      const float z = __uint_as_float(v[i]) + bias;
+      if (e.pre) store_elem(pre, i * e.ld_pre, z, 0);
+      store_elem(out, i * e.ld_out, act_f<ACT>(z) + res[i], e.out_f32);
+    }
+  }
+}
+template <int W>
+__device__ __forceinline__ void load_residual(const Epilogue& e, float (&res)[W], int r, int n, long long c) {
+  if (e.res_f32) {
+    const float* p = static_cast<const float*>(e.res) + r * e.ld_res + c;
+#pragma unroll
+    for (int i = 0; i < W; ++i, p += e.ld_res) res[i] = i < n ? *p : 0.f;
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(e.res) + r * e.ld_res + c;
+    uint16_t h[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i, p += e.ld_res) h[i] = i < n ? *p : (uint16_t)0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) res[i] = __uint_as_float((uint32_t)h[i] << 16);
   }
 }
 
@@ -225,6 +262,8 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
   __syncthreads();
   if constexpr (CG == 2 || SPLIT) cluster_sync();
   tc::fence_after_sync();
+  pdl_launch();
+  pdl_wait();
   const uint32_t tbase = sh.tmem_base;
 
   // The tiles of this CTA (pair, cluster): t0, t0 + step, ...
@@ -369,15 +408,26 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
           uint32_t v[W];
           float res[W];
           tc::ld_32x32b<W>(ta + b * W, v);
+          const int n = pr.rows - r;
+          if (e.res && in) {
+            load_residual<W>(e, res, r, n, c);
+          } else {
 #pragma unroll
-          for (int i = 0; i < W; ++i)
-            res[i] = (e.res && in && r + i < pr.rows) ? load_elem(e.res, (long long)(r + i) * e.ld_res + c, e.res_f32)
-                                                      : 0.f;
+            for (int i = 0; i < W; ++i) res[i] = 0.f;
+          }
           tc::wait_ld();
-          if (in)
+          if (in) {
+            uint8_t* out = static_cast<uint8_t*>(e.out) + (r * e.ld_out + c) * (e.out_f32 ? 4 : 2);
+            uint8_t* pre = static_cast<uint8_t*>(e.pre) + (r * e.ld_pre + c) * 2;
             with_act(e.act, [&](auto a) {
-              finish_rows<decltype(a)::value, W>(e, v, res, bias, r, pr.rows, c);
+              constexpr int ACT = decltype(a)::value;
+              if (n < W) finish_part<ACT, W>(e, v, res, bias, out, pre, n);
+              else if (e.out_f32 && e.pre) finish_full<ACT, true, true, W>(e, v, res, bias, out, pre);
+              else if (e.out_f32) finish_full<ACT, false, true, W>(e, v, res, bias, out, pre);
+              else if (e.pre) finish_full<ACT, true, false, W>(e, v, res, bias, out, pre);
+              else finish_full<ACT, false, false, W>(e, v, res, bias, out, pre);
             });
+          }
           __syncwarp();
         }
         tc::fence_before_sync();
@@ -591,22 +641,11 @@ apk_status run_products(const Product* pr, int n, int sms, int* status, long lon
     p.tiles += q.tiles_r * q.tiles_c;
     if (j == 0) p.tiles0 = p.tiles;
   }
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
   const int cl = v.split ? ch.split : v.cg;
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cl;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
   const int groups = v.split ? p.tiles : std::min(p.tiles, std::max(1, sms / v.cg));
-  cfg.gridDim = dim3(groups * cl);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = v.smem;
-  cfg.stream = stream;
-  cfg.attrs = at;
-  cfg.numAttrs = cl > 1 ? 1 : 0;
+  Launch l(dim3(groups * cl), THREADS, v.smem, stream, cl);
   void* args[] = {&p};
-  const cudaError_t e = cudaLaunchKernelExC(&cfg, v.fn, args);
+  const cudaError_t e = cudaLaunchKernelExC(&l.cfg, v.fn, args);
   if (e != cudaSuccess) {
     *why = std::string("launching the linear kernel: ") + cudaGetErrorString(e);
     return APK_ECUDA;

@@ -20,6 +20,9 @@ _ACT = {"none": L.APK_ACT_NONE, "relu": L.APK_ACT_RELU, "gelu": L.APK_ACT_GELU,
 _LAYOUT = {"kn": L.APK_W_KN, "nk": L.APK_W_NK}
 _TORCH = {"f32": torch.float32, "bf16": torch.bfloat16}
 _CODE = {torch.float32: L.APK_F32, torch.bfloat16: L.APK_BF16}
+# the current stream's handle; building a torch.cuda.Stream for it costs 2 us a call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 _DEFAULT_WAIT_NS = 2_000_000_000
 
 
@@ -83,7 +86,7 @@ class _Handle:
         return st.value
 
     def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return _raw_stream(self.device.index)
 
     def close(self):
         if getattr(self, "_h", None) is not None and self._h.value:
@@ -216,3 +219,61 @@ class Linear(_Handle):
             if st:
                 self._check(st)
         return dx, dw, db
+
+
+class MoE(_Handle):
+    """A mixture-of-experts layer for at most 64 tokens at a time.
+
+    router [E, D], w_in [E, 2F, D] (gate rows, then up rows; [E, F, D] when
+    not gated) and w_out [E, D, F], bf16 and contiguous.  Each token goes to
+    its top_k experts, weighted by their softmax probabilities over all
+    experts, divided by the chosen ones' sum if renormalize."""
+    _create, _destroy = "apk_moe_create", "apk_moe_destroy"
+    _error, _status = "apk_moe_last_error", "apk_moe_status"
+
+    def __init__(self, router, w_in, w_out, top_k: int, act: str = "silu", gated: bool = True,
+                 renormalize: bool = True, out_dtype: str = "bf16", sms: int = 0,
+                 wait_limit_ns: int = _DEFAULT_WAIT_NS):
+        _tensor(router, "router", dim=2)
+        self.device = router.device
+        self.experts, self.d_model = router.shape
+        _tensor(w_in, "w_in", self.device, dim=3)
+        _tensor(w_out, "w_out", self.device, dim=3)
+        self.d_ff = w_out.shape[2]
+        want_in = (self.experts, 2 * self.d_ff if gated else self.d_ff, self.d_model)
+        if tuple(w_in.shape) != want_in or tuple(w_out.shape) != (self.experts, self.d_model, self.d_ff):
+            raise ValueError(f"router is {tuple(router.shape)}, w_in {tuple(w_in.shape)}, w_out {tuple(w_out.shape)}: "
+                             "[E, D], [E, 2F or F, D] and [E, D, F] are wanted")
+        for t, what in ((router, "router"), (w_in, "w_in"), (w_out, "w_out")):
+            if not t.is_contiguous():
+                raise ValueError(f"{what} is not contiguous")
+        self.router, self.w_in, self.w_out, self.top_k = router, w_in, w_out, top_k
+        self.out_dtype = _pick(_TORCH, out_dtype, "out_dtype")
+        self._open(L.MoeConfig(self.device.index, self.experts, top_k, self.d_model, self.d_ff, _pick(_ACT, act, "act"),
+                               int(gated), int(renormalize), router.data_ptr(), w_in.data_ptr(), w_out.data_ptr(),
+                               sms, wait_limit_ns))
+        self._io = L.MoeIO()
+        self._io_ref = ctypes.byref(self._io)
+
+    def forward(self, x, return_routing: bool = False):
+        """The layer's output for x [..., D]; with return_routing also the
+        chosen experts (int32 [..., top_k]) and their weights (fp32)."""
+        io = self._io
+        x2, io.ldx = _rows(x, "x", self.device, self.d_model)
+        y = torch.empty(x.shape, dtype=self.out_dtype, device=self.device)
+        ids = probs = None
+        if return_routing:
+            shape = (*x.shape[:-1], self.top_k)
+            ids = torch.empty(shape, dtype=torch.int32, device=self.device)
+            probs = torch.empty(shape, dtype=torch.float32, device=self.device)
+            io.ids, io.probs = ids.data_ptr(), probs.data_ptr()
+        else:
+            io.ids = io.probs = None
+        io.x, io.tokens, io.y, io.ldy = x2.data_ptr(), x2.shape[0], y.data_ptr(), self.d_model
+        io.y_dtype, io.stream = _CODE[self.out_dtype], self._stream()
+        st = self._lib.apk_moe_forward(self._h, self._io_ref)
+        if st:
+            self._check(st)
+        return (y, ids, probs) if return_routing else y
+
+    __call__ = forward

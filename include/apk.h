@@ -584,6 +584,52 @@ apk_status apk_linear_backward(apk_linear* h, const apk_linear_grads* g);
  * synchronizes it. */
 apk_status apk_linear_status(apk_linear* h, void* stream, int* device_status);
 
+/* A mixture-of-experts layer for a few tokens (at most 64), router included,
+ * in one cooperative kernel.  For each token:
+ *   logits = x router^T; the top_k largest (ties to the lowest index; a NaN
+ *   counts as the largest) with their softmax probabilities over all experts,
+ *   divided by their sum if renormalize;
+ *   hidden = act(x gate^T) * (x up^T), or act(x w_in^T) if not gated;
+ *   y = the sum over the chosen experts of p * (hidden w_out^T).
+ * The hidden values are rounded to bf16, everything else is fp32 until y.
+ * Weights are bf16, contiguous, 16-byte aligned; d_model and d_ff are
+ * multiples of 8. */
+typedef struct apk_moe_config {
+  int device;
+  int experts, top_k;       /* up to 512; up to 16 and experts                */
+  int d_model, d_ff;
+  apk_act act;
+  int gated;                /* w_in holds gate rows, then up rows             */
+  int renormalize;
+  const void* router;       /* [experts][d_model]                             */
+  const void* w_in;         /* [experts][gated ? 2 d_ff : d_ff][d_model]      */
+  const void* w_out;        /* [experts][d_model][d_ff]                       */
+  int sms;                  /* SMs the kernel takes (one CTA each); 0 = all   */
+  long long wait_limit_ns;
+} apk_moe_config;
+typedef struct apk_moe apk_moe;
+
+apk_status apk_moe_create(const apk_moe_config* cfg, apk_moe** out); /* as apk_linear_create */
+apk_status apk_moe_destroy(apk_moe* h);
+const char* apk_moe_last_error(const apk_moe* h);
+
+typedef struct apk_moe_io {
+  const void* x;            /* bf16 [tokens][d_model], rows on 16 bytes       */
+  long long ldx;
+  int tokens;               /* 0 does nothing                                 */
+  apk_dtype y_dtype;
+  void* y;                  /* [tokens][d_model]; not x                       */
+  long long ldy;
+  int* ids;                 /* [tokens][top_k] chosen experts, or NULL        */
+  float* probs;             /* [tokens][top_k] their weights, or NULL         */
+  void* stream;
+} apk_moe_io;
+apk_status apk_moe_forward(apk_moe* h, const apk_moe_io* io);
+
+/* As apk_linear_status (3: a grid barrier ran out); also makes the handle
+ * usable again after an error.  Call it with no other call in flight. */
+apk_status apk_moe_status(apk_moe* h, void* stream, int* device_status);
+
 /* ---- allocation-free entry point --------------------------------------- */
 
 /* C = A * B (fp32, row-major, device pointers, 16-byte aligned; M and N
