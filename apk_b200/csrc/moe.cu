@@ -9,11 +9,11 @@
 // layer is one persistent cooperative kernel, one CTA of 16 warps per SM, whose
 // phases meet at grid barriers instead of kernel boundaries:
 //   0  partial router logits: 16 experts x a slice of d_model per item
-//   1  every CTA picks the experts of all tokens for itself (T x E logits are
-//      cheaper to read 148 times from L2 than to pass through another
-//      barrier), then hidden = act(gate) * up, 8 gate and 8 up rows per item,
+//   1  the tokens' experts (up to 16 tokens: every CTA picks them for itself,
+//      which is cheaper than passing them through another barrier), then hidden = act(gate) * up, 8 gate and 8 up rows per item,
 //      so both halves of a product sit in one thread's accumulator
-//   2  each (token, choice) pair's output row in fp32
+//   2  each (token, choice) pair's output row in fp32 (one token: its output,
+//      and no phase 3)
 //   3  y[t] = sum over the choices, in their order, of p * row
 // An item's rows are read by 1-16 warps of a CTA that split k: many when
 // there are few items (a token or two), one when there are many.  Sums across
@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <mutex>
 #include <new>
+#include <type_traits>
 
 #include "act.cuh"
 #include "common.cuh"
@@ -37,6 +38,7 @@ namespace moe {
 
 constexpr int WARPS = 16, THREADS = 32 * WARPS;
 constexpr int MAX_TOKENS = 64, MAX_EXPERTS = 512, MAX_TOPK = 16;
+constexpr int LOCAL_LOGITS = 2048, LOCAL_BYTES = 96 << 10;
 constexpr int ROUND = 128;  // k of one warp's round: 8 16-byte weight loads a lane
 
 struct Params {
@@ -51,10 +53,12 @@ struct Params {
   int tokens, experts, top_k, d, f, act, gated, renorm, y_f32;
   int red_stride;  // floats of a warp's place in the shared sums
   int rsplit;    // slices of d_model in phase 0
+  int local;     // every CTA computes all logits itself
   unsigned* barrier;  // {arrived, generation}
   int* status;
   long long limit;
   float* logits;  // [rsplit][tokens][experts]
+  float2* choice; // [tokens][top_k] expert (as bits), weight
   uint16_t* hid;  // [tokens * top_k][f], rows grouped by expert
   float* out;     // [tokens * top_k][d]
 };
@@ -63,41 +67,58 @@ struct Shared {
   unsigned long long mask[MAX_EXPERTS];  // the tokens that chose an expert
   short active[MAX_EXPERTS];             // experts with tokens, ascending
   short base[MAX_EXPERTS];               // an active expert's first row
-  short sel[MAX_TOKENS * MAX_TOPK];      // expert, then row, of (token, choice)
+  short sel[MAX_TOKENS * MAX_TOPK];      // expert of (token, choice)
+  short row[MAX_TOKENS * MAX_TOPK];      // and its row
   float prob[MAX_TOKENS * MAX_TOPK];
   unsigned char tok[MAX_TOKENS * MAX_TOPK];  // token of a row
+  float logits[LOCAL_LOGITS];            // p.local: all of them
   int warp_n[WARPS], warp_rows[WARPS];
   int n_active;
   int abort;
 };
 
-// Every CTA of the grid has arrived (and its earlier writes are visible).
-// The last to arrive clears the count and advances the generation, so the
-// words need no reset between launches.
-__device__ __forceinline__ bool grid_barrier(const Params& p, Shared& sh) {
+// A grid barrier in two halves, so that loads which do not depend on it can
+// be issued between them (issued before the first, they would delay its
+// fence).  After the second every CTA has arrived, and what it wrote before
+// is visible.  The last to arrive clears the count and advances the
+// generation (on another line, which the others poll), so the words need no
+// reset between launches.
+struct Ticket {
+  unsigned gen;
+  bool last;
+};
+__device__ __forceinline__ Ticket grid_arrive(const Params& p) {
+  Ticket k = {0, false};
   __syncthreads();
   if (threadIdx.x == 0) {
-    unsigned gen, old;
-    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(gen) : "l"(p.barrier + 1) : "memory");
+    unsigned old;
+    unsigned* const word = p.barrier + 32;
+    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(k.gen) : "l"(word) : "memory");
     __threadfence();
-    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(p.barrier) : "memory");
-    if (old == gridDim.x - 1) {
+    asm volatile("atom.relaxed.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(p.barrier) : "memory");
+    k.last = old == gridDim.x - 1;
+    if (k.last) {
       asm volatile("st.relaxed.gpu.global.u32 [%0], 0;" ::"l"(p.barrier) : "memory");
-      asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p.barrier + 1), "r"(gen + 1) : "memory");
-    } else {
-      const long long t0 = globaltimer_ns();
-      int n = 0;
-      while (true) {
-        unsigned now;
-        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(p.barrier + 1) : "memory");
-        if (now != gen) break;
-        if (++n == 64) {
-          n = 0;
-          if (globaltimer_ns() - t0 > p.limit) {
-            report_status(p.status, DEV_WAIT_TIMEOUT_SPIN, nullptr);
-            sh.abort = 1;
-            break;
-          }
+      __threadfence();
+      asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(word), "r"(k.gen + 1) : "memory");
+    }
+  }
+  return k;
+}
+__device__ __forceinline__ bool grid_wait(const Params& p, Shared& sh, const Ticket k) {
+  if (threadIdx.x == 0) {
+    long long t0 = 0;
+    for (int n = 1; !k.last; ++n) {
+      unsigned now;
+      asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(p.barrier + 32) : "memory");
+      if (now != k.gen) break;
+      if ((n & 63) == 0) {
+        const long long t = globaltimer_ns();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > p.limit) {
+          report_status(p.status, DEV_WAIT_TIMEOUT_SPIN, nullptr);
+          sh.abort = 1;
+          break;
         }
       }
     }
@@ -106,36 +127,42 @@ __device__ __forceinline__ bool grid_barrier(const Params& p, Shared& sh) {
   __syncthreads();
   return sh.abort == 0;
 }
+__device__ __forceinline__ bool grid_barrier(const Params& p, Shared& sh) { return grid_wait(p, sh, grid_arrive(p)); }
 
 struct Frag {
   uint4 a[4], b[4];
 };
 // One round of weight rows w0 (MMA rows g) and w1 (g + 8) at k0 + 32 u + 8 t.
+template <bool BOTH = true>
 __device__ __forceinline__ void load_round(Frag& f, const uint16_t* w0, const uint16_t* w1, int k0, int t, int k) {
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int at = k0 + 32 * u + 8 * t;
     const bool in = at < k;
     f.a[u] = in ? stream::ld_weights(w0 + at) : make_uint4(0, 0, 0, 0);
-    f.b[u] = in ? stream::ld_weights(w1 + at) : make_uint4(0, 0, 0, 0);
+    f.b[u] = BOTH && in ? stream::ld_weights(w1 + at) : make_uint4(0, 0, 0, 0);
   }
 }
-// acc += rows (w0 | w1) times the NT8 x 8 token rows xr, over the rounds
-// first, first + step, ... of k.  The next round's weights are in flight while
-// one is multiplied.
-// `Load` reads 16 bytes of a token row.
+// The two weight rows of a lane (MMA rows g and g + 8); null: none.
+struct Rows {
+  const uint16_t* w0;
+  const uint16_t* w1;
+};
+// acc += `w` rows times the NT8 x 8 token rows xr, over the rounds first,
+// first + step, ... of k.  On entry f holds round `first`; the next round's
+// weights are in flight while one is multiplied, and at the end the first
+// round of the next item's rows, so that the loads do not pause between items.
+// Load reads 16 bytes of a token row.
 template <int NT8, class Load>
-__device__ __forceinline__ void stream_rows(float (&acc)[NT8][4], const uint16_t* w0, const uint16_t* w1,
+__device__ __forceinline__ void stream_rows(float (&acc)[NT8][4], Frag& f, const Rows w, const Rows next_item,
                                             const uint16_t* const (&xr)[NT8], int k, int first, int step, int t,
                                             Load ld) {
-  int k0 = first * ROUND;
-  if (k0 >= k) return;
-  Frag f;
-  load_round(f, w0, w1, k0, t, k);
-  while (true) {
+  const int begin = first * ROUND;
+#pragma unroll 1
+  for (int k0 = begin; k0 < k; k0 += step * ROUND) {
     const int next = k0 + step * ROUND;
     Frag n;
-    if (NT8 <= 2) load_round(n, w0, w1, next, t, k);  // (past the end: zero, nothing read)
+    if (NT8 <= 2) load_round(n, w.w0, w.w1, next, t, k);  // (past the end: zero, nothing read)
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int at = k0 + 32 * u + 8 * t;
@@ -148,11 +175,10 @@ __device__ __forceinline__ void stream_rows(float (&acc)[NT8][4], const uint16_t
         stream::mma_bf16(acc[i], f.a[u].z, f.b[u].z, f.a[u].w, f.b[u].w, c[i].z, c[i].w);
       }
     }
-    k0 = next;
-    if (k0 >= k) break;
     if (NT8 <= 2) f = n;
-    else load_round(f, w0, w1, k0, t, k);
+    else if (next < k) load_round(f, w.w0, w.w1, next, t, k);
   }
+  if (next_item.w0) load_round(f, next_item.w0, next_item.w1, begin, t, k);
 }
 
 struct LdConst {  // the layer's input: not written during the kernel
@@ -184,28 +210,82 @@ __device__ __forceinline__ void join_warps(float (&acc)[NT8][4], float* red, int
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(32 * ws) : "memory");  // red is free again
 }
 
-// Warps that share an item: enough that every warp of the grid has one,
-// within the rounds that k has.
+// Warps that share an item: 1, 2, ... 16, by the least time of a warp in
+// rounds: its items times the rounds of one and about three more for the join
+// and what the loads lose at an item's end.
 __device__ __forceinline__ int warps_per_item(long long items, int k) {
-  int ws = 1;
-  while (ws < WARPS && items * ws < (long long)gridDim.x * WARPS && ws * ROUND < k) ws *= 2;
-  return ws;
+  int best = 1;
+  long long least = 1ll << 60;
+  const int rounds = (k + ROUND - 1) / ROUND;
+  for (int ws = 1; ws <= WARPS; ws *= 2) {
+    const int slots = gridDim.x * (WARPS / ws);
+    const long long cost = (items + slots - 1) / slots * ((rounds + ws - 1) / ws + 3);
+    if (cost < least) {
+      least = cost;
+      best = ws;
+    }
+  }
+  return best;
+}
+
+// A phase's items in two parts: full sweeps of one item per warp, then the
+// rest, shared by more warps each.
+struct Walk {
+  struct Part {
+    int ws, first, end, step;
+  };
+  int bulk, items, ws;
+  __device__ Walk(int n, int k) : items(n) {
+    const int warps = gridDim.x * WARPS;
+    ws = warps_per_item(n, k);
+    bulk = 0;
+    if (n > warps && ws == 1) {
+      bulk = n / warps * warps;
+      ws = warps_per_item(n - bulk, k);
+    }
+  }
+  __device__ Part part(int i, int warp) const {
+    if (i == 0) return {1, warp * (int)gridDim.x + (int)blockIdx.x, bulk, (int)gridDim.x * WARPS};
+    return {ws, bulk + warp / ws * (int)gridDim.x + (int)blockIdx.x, items, (int)gridDim.x * (WARPS / ws)};
+  }
+};
+
+// Starts bringing a warp's first rows into L2, past the round that is loaded
+// already: while a barrier is waited for, memory would be idle.  A kilobyte a
+// row keeps it busy for about that time (38 MB over the chip).
+__device__ __forceinline__ void prefetch_rows(const Rows w, int t, int k, int ws) {
+  constexpr int LEAD = 512;
+  if (ws != 1 || t > 1) return;
+  const uint16_t* r = t ? w.w1 : w.w0;
+  const int n = min(k - ROUND, LEAD);
+  if (n > 0)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(r + ROUND), "r"((n & ~7) * 2) : "memory");
+}
+
+// Rows of expert a's tile in the first product.  Gated: MMA row g is gate
+// f0 + g and row g + 8 its up; else features f0 + g and f0 + g + 8.
+__device__ __forceinline__ Rows rows_in(const Params& p, const Shared& sh, int a, int tile, int g) {
+  const uint16_t* w = p.w_in + (long long)sh.active[a] * (p.gated ? 2 * p.f : p.f) * p.d;
+  const int f0 = tile * (p.gated ? 8 : 16);
+  const int r0 = min(f0 + g, p.f - 1), r1 = p.gated ? p.f + r0 : min(f0 + g + 8, p.f - 1);
+  return {w + (long long)r0 * p.d, w + (long long)r1 * p.d};
+}
+__device__ __forceinline__ Rows rows_out(const Params& p, const Shared& sh, int a, int tile, int g) {
+  const uint16_t* w = p.w_out + (long long)sh.active[a] * p.d * p.f;
+  const int d0 = tile * 16;
+  return {w + (long long)min(d0 + g, p.d - 1) * p.f, w + (long long)min(d0 + g + 8, p.d - 1) * p.f};
 }
 
 template <int NT8>
-__device__ __forceinline__ void item_in(const Params& p, const Shared& sh, float* red, int a, int tile, int n, int ws) {
+__device__ __forceinline__ void item_in(const Params& p, const Shared& sh, float* red, Frag& f, Rows w, Rows next, int a,
+                                        int tile, int n, int ws) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int e = sh.active[a], base = sh.base[a];
-  const int rows_e = p.gated ? 2 * p.f : p.f;
-  const int f0 = tile * (p.gated ? 8 : 16);
-  const uint16_t* w = p.w_in + (long long)e * rows_e * p.d;
-  // gated: MMA row g is gate f0 + g, row g + 8 its up; else features f0 + g and f0 + g + 8
-  const int r0 = min(f0 + g, p.f - 1), r1 = p.gated ? p.f + r0 : min(f0 + g + 8, p.f - 1);
+  const int base = sh.base[a], f0 = tile * (p.gated ? 8 : 16);
   const uint16_t* xr[NT8];
 #pragma unroll
   for (int i = 0; i < NT8; ++i) xr[i] = p.x + sh.tok[base + min(8 * i + g, n - 1)] * p.ldx;
   float acc[NT8][4] = {};
-  stream_rows<NT8>(acc, w + (long long)r0 * p.d, w + (long long)r1 * p.d, xr, p.d, warp & (ws - 1), ws, t, LdConst());
+  stream_rows<NT8>(acc, f, w, next, xr, p.d, warp & (ws - 1), ws, t, LdConst());
   join_warps<NT8>(acc, red, p.red_stride, ws, warp, lane);
   if (warp & (ws - 1)) return;
   with_act(p.act, [&](auto tag) {
@@ -217,10 +297,10 @@ __device__ __forceinline__ void item_in(const Params& p, const Shared& sh, float
         const int col = 8 * i + 2 * t + c;
         if (col >= n) continue;
         uint16_t* h = p.hid + (long long)(base + col) * p.f;
-        auto put = [&](int f, float v) {
+        auto put = [&](int at, float v) {
           uint16_t r;
           asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
-          if (f < p.f) h[f] = r;
+          if (at < p.f) h[at] = r;
         };
         if (p.gated) {
           put(f0 + g, act_f<ACT>(acc[i][c]) * acc[i][c + 2]);
@@ -233,16 +313,15 @@ __device__ __forceinline__ void item_in(const Params& p, const Shared& sh, float
 }
 
 template <int NT8>
-__device__ __forceinline__ void item_out(const Params& p, const Shared& sh, float* red, int a, int tile, int n, int ws) {
+__device__ __forceinline__ void item_out(const Params& p, const Shared& sh, float* red, Frag& f, Rows w, Rows next,
+                                         int a, int tile, int n, int ws) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int e = sh.active[a], base = sh.base[a], d0 = tile * 16;
-  const uint16_t* w = p.w_out + (long long)e * p.d * p.f;
+  const int base = sh.base[a], d0 = tile * 16;
   const uint16_t* xr[NT8];
 #pragma unroll
   for (int i = 0; i < NT8; ++i) xr[i] = p.hid + (long long)(base + min(8 * i + g, n - 1)) * p.f;
   float acc[NT8][4] = {};
-  stream_rows<NT8>(acc, w + (long long)min(d0 + g, p.d - 1) * p.f, w + (long long)min(d0 + g + 8, p.d - 1) * p.f, xr, p.f,
-                   warp & (ws - 1), ws, t, LdWritten());
+  stream_rows<NT8>(acc, f, w, next, xr, p.f, warp & (ws - 1), ws, t, LdWritten());
   join_warps<NT8>(acc, red, p.red_stride, ws, warp, lane);
   if (warp & (ws - 1)) return;
 #pragma unroll
@@ -254,27 +333,39 @@ __device__ __forceinline__ void item_out(const Params& p, const Shared& sh, floa
     }
 }
 
-// Partial logits of 16 experts for all tokens, 64 at a time in NT8 = 8 tiles.
-template <int NT8>
-__device__ __forceinline__ void item_router(const Params& p, float* red, int tile, int slice) {
+// Partial logits of 16 experts for the 16 tokens from t0, into dst[token][experts].
+__device__ __forceinline__ void item_router(const Params& p, float* red, int tile, int slice, int slices, int t0,
+                                            float* dst) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int e0 = tile * 16;
-  const uint16_t* xr[NT8];
+  const uint16_t* xr[2];
 #pragma unroll
-  for (int i = 0; i < NT8; ++i) xr[i] = p.x + min(8 * i + g, p.tokens - 1) * p.ldx;
-  float acc[NT8][4] = {};
-  stream_rows<NT8>(acc, p.router + (long long)min(e0 + g, p.experts - 1) * p.d,
-                   p.router + (long long)min(e0 + g + 8, p.experts - 1) * p.d, xr, p.d, slice * WARPS + warp,
-                   p.rsplit * WARPS, t, LdConst());
-  join_warps<NT8>(acc, red, p.red_stride, WARPS, warp, lane);
+  for (int i = 0; i < 2; ++i) xr[i] = p.x + min(t0 + 8 * i + g, p.tokens - 1) * p.ldx;
+  float acc[2][4] = {};
+  const Rows w = {p.router + (long long)min(e0 + g, p.experts - 1) * p.d,
+                  p.router + (long long)min(e0 + g + 8, p.experts - 1) * p.d};
+  Frag f;
+  load_round(f, w.w0, w.w1, (slice * WARPS + warp) * ROUND, t, p.d);
+  stream_rows<2>(acc, f, w, Rows{}, xr, p.d, slice * WARPS + warp, slices * WARPS, t, LdConst());
+  join_warps<2>(acc, red, p.red_stride, WARPS, warp, lane);
   if (warp) return;
 #pragma unroll
-  for (int i = 0; i < NT8; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const int tok = 8 * i + 2 * t + (c & 1), e = e0 + g + 8 * (c >> 1);
-      if (tok < p.tokens && e < p.experts) p.logits[((long long)slice * p.tokens + tok) * p.experts + e] = acc[i][c];
+      const int tok = t0 + 8 * i + 2 * t + (c & 1), e = e0 + g + 8 * (c >> 1);
+      if (tok < p.tokens && e < p.experts) dst[tok * p.experts + e] = acc[i][c];
     }
+}
+
+__device__ __forceinline__ void put_y(const Params& p, long long at, float v) {
+  if (p.y_f32) {
+    static_cast<float*>(p.y)[at] = v;
+  } else {
+    uint16_t r;
+    asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
+    static_cast<uint16_t*>(p.y)[at] = r;
+  }
 }
 
 // Order of the logits as unsigned integers; a NaN comes first, as in a
@@ -286,87 +377,189 @@ __device__ __forceinline__ unsigned order_key(float v) {
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-// One warp picks a token's experts: top_k rounds of "largest key, lowest
-// index", then their softmax over all experts.
-__device__ __forceinline__ void route_token(const Params& p, Shared& sh, int tok) {
+// One warp picks a token's experts from its logits: top_k rounds of "largest
+// key, lowest index", then their softmax over all experts.  Lane j of the
+// first top_k gets the j-th choice and its weight.  PER experts a lane.
+template <int PER, class Load>
+__device__ __forceinline__ void route_token(const Params& p, Load logit, int& my_e, float& my_p) {
   const int lane = threadIdx.x & 31;
-  constexpr int PER = MAX_EXPERTS / 32;
   float v[PER];
   unsigned key[PER];
-  float best = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = lane + 32 * i;
-    v[i] = 0.f;
-    key[i] = 0;  // below every logit's key: -inf has key 0x007FFFFF
-    if (e < p.experts) {
-      for (int s = 0; s < p.rsplit; ++s) v[i] += __ldcg(p.logits + ((long long)s * p.tokens + tok) * p.experts + e);
-      key[i] = order_key(v[i]);
-      best = v[i] != v[i] ? v[i] : fmaxf(best, v[i]);
+  for (int i = 0; i < PER; ++i) v[i] = lane + 32 * i < p.experts ? logit(lane + 32 * i) : 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) key[i] = lane + 32 * i < p.experts ? order_key(v[i]) : 0;  // 0: below any logit's key
+  float my_v = 0.f;
+  my_e = 0;
+  for (int j = 0; j < p.top_k; ++j) {
+    unsigned k = key[0];
+    int i0 = 0;
+#pragma unroll
+    for (int i = 1; i < PER; ++i)
+      if (key[i] > k) {
+        k = key[i];
+        i0 = i;
+      }
+    const unsigned top = __reduce_max_sync(~0u, k);
+    const int at = (int)__reduce_min_sync(~0u, k == top ? (unsigned)(lane + 32 * i0) : ~0u);
+    float mine = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (at == lane + 32 * i) {
+        key[i] = 0;
+        mine = v[i];
+      }
+    mine = __shfl_sync(~0u, mine, at & 31);
+    if (lane == j) {
+      my_e = at;
+      my_v = mine;
     }
   }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const float other = __shfl_xor_sync(~0u, best, o);
-    best = (best != best || other != other) ? NAN : fmaxf(best, other);
-  }
+  // the first choice has the largest logit (or is a NaN, as every probability then is)
+  const float best = __shfl_sync(~0u, my_v, 0);
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i)
     if (lane + 32 * i < p.experts) sum += __expf(v[i] - best);
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  float chosen = 0.f;
-  for (int j = 0; j < p.top_k; ++j) {
-    unsigned k = 0;
+  my_p = lane < p.top_k ? __fdividef(__expf(my_v - best), sum) : 0.f;
+  if (p.renorm) {
+    float chosen = my_p;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) k = max(k, key[i]);
-    k = __reduce_max_sync(~0u, k);
-    int at = MAX_EXPERTS;
-#pragma unroll
-    for (int i = PER - 1; i >= 0; --i)
-      if (key[i] == k && lane + 32 * i < p.experts) at = lane + 32 * i;
-    at = __reduce_min_sync(~0u, at);
-    float pj = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (at == lane + 32 * i) {
-        key[i] = 0;
-        pj = __fdividef(__expf(v[i] - best), sum);
-      }
-    pj = __shfl_sync(~0u, pj, at & 31);
-    chosen += pj;
-    if (lane == 0) {
-      sh.sel[tok * p.top_k + j] = (short)at;
-      sh.prob[tok * p.top_k + j] = pj;
-      atomicOr(&sh.mask[at], 1ull << tok);
-    }
+    for (int o = MAX_TOPK / 2; o; o >>= 1) chosen += __shfl_xor_sync(~0u, chosen, o);
+    my_p = __fdividef(my_p, chosen);
   }
-  __syncwarp();
-  if (p.renorm && lane < p.top_k)
-    sh.prob[tok * p.top_k + lane] = __fdividef(sh.prob[tok * p.top_k + lane], chosen);
+}
+template <class Load>
+__device__ __forceinline__ void route_token(const Params& p, Load logit, int& my_e, float& my_p) {
+  if (p.experts <= 32) route_token<1>(p, logit, my_e, my_p);
+  else if (p.experts <= 64) route_token<2>(p, logit, my_e, my_p);
+  else if (p.experts <= 128) route_token<4>(p, logit, my_e, my_p);
+  else if (p.experts <= 256) route_token<8>(p, logit, my_e, my_p);
+  else route_token<16>(p, logit, my_e, my_p);
+}
+
+// One token: the output without the sum's barrier.  A CTA takes `ROWS` (8 or
+// 16) of the output's rows over all chosen experts, its warps splitting the
+// (expert, round) pairs; the probabilities are applied per expert.
+template <int ROWS>
+__device__ __forceinline__ bool one_token_out(const Params& p, Shared& sh, float* red) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int rounds = (p.f + ROUND - 1) / ROUND, units = p.top_k * rounds;
+  auto load = [&](Frag& f, int tile, int u) {
+    const long long r0 = min(tile * ROWS + g, p.d - 1), r1 = min(tile * ROWS + g + 8, p.d - 1);
+    const int j = u / rounds;
+    const uint16_t* w = p.w_out + (long long)sh.sel[j] * p.d * p.f;
+    load_round<ROWS == 16>(f, w + r0 * p.f, w + r1 * p.f, (u - j * rounds) * ROUND, t, p.f);
+  };
+  Frag f;
+  const Ticket ticket = grid_arrive(p);
+  if (warp < units && (int)blockIdx.x * ROWS < p.d) load(f, blockIdx.x, warp);
+  if (!grid_wait(p, sh, ticket)) return false;
+  for (int tile = blockIdx.x; tile * ROWS < p.d; tile += gridDim.x) {
+    float s0 = 0.f, s1 = 0.f;
+    for (int u = warp; u < units; u += WARPS) {
+      const int j = u / rounds, k0 = (u - j * rounds) * ROUND;
+      const uint16_t* h = p.hid + sh.row[j] * p.f;
+      Frag n;  // the next unit, of this tile or the next one
+      if (u + WARPS < units) load(n, tile, u + WARPS);
+      else if ((tile + (int)gridDim.x) * ROWS < p.d) load(n, tile + gridDim.x, warp);
+      float acc[4] = {};
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int at = k0 + 32 * v + 8 * t;
+        const uint4 c = at < p.f ? LdWritten()(h + at) : make_uint4(0, 0, 0, 0);
+        stream::mma_bf16(acc, f.a[v].x, f.b[v].x, f.a[v].y, f.b[v].y, c.x, c.y);
+        stream::mma_bf16(acc, f.a[v].z, f.b[v].z, f.a[v].w, f.b[v].w, c.z, c.w);
+      }
+      s0 += sh.prob[j] * acc[0];
+      s1 += sh.prob[j] * acc[2];
+      f = n;
+    }
+    // every column holds the same token: column 0 is lane 4g's
+    if (t == 0) {
+      red[warp * 16 + g] = s0;
+      red[warp * 16 + g + 8] = s1;
+    }
+    __syncthreads();
+    const int d = tile * ROWS + (int)threadIdx.x;
+    if (threadIdx.x < ROWS && d < p.d) {
+      float y = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) y += red[w * 16 + threadIdx.x];
+      put_y(p, d, y);
+    }
+    __syncthreads();
+  }
+  return true;
 }
 
 __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ Params p) {
   extern __shared__ float red[];
   __shared__ Shared sh;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   if (tid == 0) sh.abort = 0;
-
-  // -------- 0: partial logits --------
-  const int etiles = (p.experts + 15) / 16;
-  for (int it = blockIdx.x; it < etiles * p.rsplit; it += gridDim.x) {
-    const int tile = it % etiles, slice = it / etiles;
-    if (p.tokens <= 8) item_router<1>(p, red, tile, slice);
-    else if (p.tokens <= 16) item_router<2>(p, red, tile, slice);
-    else if (p.tokens <= 32) item_router<4>(p, red, tile, slice);
-    else item_router<8>(p, red, tile, slice);
-  }
   for (int e = tid; e < p.experts; e += THREADS) sh.mask[e] = 0;
-  if (!grid_barrier(p, sh)) return;
+
+  // -------- 0: logits --------
+  const int etiles = (p.experts + 15) / 16;
+  if (p.local) {
+    for (int tile = 0; tile < etiles; ++tile) item_router(p, red, tile, 0, 1, 0, sh.logits);
+    __syncthreads();
+  } else {
+    const int tgroups = (p.tokens + 15) / 16;
+    for (int it = blockIdx.x; it < etiles * p.rsplit * tgroups; it += gridDim.x) {
+      const int slice = it / etiles % p.rsplit;
+      item_router(p, red, it % etiles, slice, p.rsplit, it / (etiles * p.rsplit) * 16,
+                  p.logits + (long long)slice * p.tokens * p.experts);
+    }
+    if (!grid_barrier(p, sh)) return;
+  }
 
   // -------- 1: routing (by every CTA), then the hidden values --------
-  for (int tok = warp; tok < p.tokens; tok += WARPS) route_token(p, sh, tok);
+  // A logit is the sum of its slices.  Up to 16 tokens: warp w of every CTA
+  // routes token w.  More: warp 0 of CTA b routes token b for all, and another
+  // barrier passes the choices on (64 tokens of 128 experts took every CTA 13 us).
+  const bool shared_out = p.tokens > WARPS;
+  auto each_token = [&](int tok) {
+    int my_e;
+    float my_p;
+    route_token(
+        p,
+        [&](int e) {
+          if (p.local) return sh.logits[tok * p.experts + e];
+          float v[8];
+#pragma unroll
+          for (int s = 0; s < 8; ++s)
+            v[s] = s < p.rsplit ? __ldcg(p.logits + ((long long)s * p.tokens + tok) * p.experts + e) : 0.f;
+          return ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        },
+        my_e, my_p);
+    if (lane < p.top_k) {
+      if (shared_out) {
+        p.choice[tok * p.top_k + lane] = make_float2(__int_as_float(my_e), my_p);
+      } else {
+        sh.sel[tok * p.top_k + lane] = (short)my_e;
+        sh.prob[tok * p.top_k + lane] = my_p;
+        atomicOr(&sh.mask[my_e], 1ull << tok);
+      }
+    }
+  };
+  if (shared_out) {
+    if (warp == 0)
+      for (int tok = blockIdx.x; tok < p.tokens; tok += gridDim.x) each_token(tok);
+    if (!grid_barrier(p, sh)) return;
+    for (int i = tid; i < p.tokens * p.top_k; i += THREADS) {
+      const float2 c = __ldcg(p.choice + i);
+      const int e = __float_as_int(c.x);
+      sh.sel[i] = (short)e;
+      sh.prob[i] = c.y;
+      atomicOr(&sh.mask[e], 1ull << (i / p.top_k));
+    }
+  } else if (warp < p.tokens) {
+    each_token(warp);
+  }
   __syncthreads();
   {
     // thread e: rank of expert e among those with tokens, and its first row
@@ -392,7 +585,12 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
       sh.active[a] = (short)tid;
       sh.base[a] = (short)r;
       unsigned long long m = sh.mask[tid];
-      for (int i = 0; m; ++i, m &= m - 1) sh.tok[r + i] = (unsigned char)(__ffsll((long long)m) - 1);
+      for (int i = 0; m; ++i, m &= m - 1) {
+        const int tok = __ffsll((long long)m) - 1;
+        sh.tok[r + i] = (unsigned char)tok;
+        for (int j = 0; j < p.top_k; ++j)
+          if (sh.sel[tok * p.top_k + j] == tid) sh.row[tok * p.top_k + j] = (short)(r + i);
+      }
     }
     if (tid == THREADS - 1) sh.n_active = a + (n > 0);
   }
@@ -404,42 +602,63 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
       if (p.probs) p.probs[i] = sh.prob[i];
     }
   }
-  // f(a, tile, columns): an item of active expert a's `tiles` row tiles, by warps_per_item warps
-  auto for_items = [&](int tiles, int k, auto f) {
-    const long long items = (long long)n_active * tiles;
-    const int ws = warps_per_item(items, k), slots = gridDim.x * (WARPS / ws);
-    for (long long it = (long long)(warp / ws) * gridDim.x + blockIdx.x; it < items; it += slots) {
-      const int a = (int)(it / tiles);
-      f(a, (int)(it - (long long)a * tiles), __popcll(sh.mask[sh.active[a]]), ws);
-    }
+  // the tokens of a warp's item, as the MMA's N axis
+  auto by_columns = [&](int n, auto f) {
+    if (n <= 8) f(std::integral_constant<int, 1>());
+    else if (n <= 16) f(std::integral_constant<int, 2>());
+    else if (n <= 32) f(std::integral_constant<int, 4>());
+    else f(std::integral_constant<int, 8>());
   };
-  for_items((p.f + (p.gated ? 7 : 15)) / (p.gated ? 8 : 16), p.d, [&](int a, int tile, int n, int ws) {
-    if (n <= 8) item_in<1>(p, sh, red, a, tile, n, ws);
-    else if (n <= 16) item_in<2>(p, sh, red, a, tile, n, ws);
-    else if (n <= 32) item_in<4>(p, sh, red, a, tile, n, ws);
-    else item_in<8>(p, sh, red, a, tile, n, ws);
-  });
-  if (!grid_barrier(p, sh)) return;
+  Frag frag;
+  {
+    const int tiles = (p.f + (p.gated ? 7 : 15)) / (p.gated ? 8 : 16);
+    const Walk walk(n_active * tiles, p.d);
+    for (int part = walk.bulk ? 0 : 1; part < 2; ++part) {
+      const Walk::Part q = walk.part(part, warp);
+      Rows w = {};
+      if (q.first < q.end) {
+        w = rows_in(p, sh, q.first / tiles, q.first % tiles, g);
+        load_round(frag, w.w0, w.w1, (warp & (q.ws - 1)) * ROUND, t, p.d);
+      }
+      for (int it = q.first; it < q.end; it += q.step) {
+        const int a = it / tiles, next = it + q.step;
+        const Rows wn = next < q.end ? rows_in(p, sh, next / tiles, next % tiles, g) : Rows{};
+        const int n = __popcll(sh.mask[sh.active[a]]);
+        by_columns(n, [&](auto c) { item_in<decltype(c)::value>(p, sh, red, frag, w, wn, a, it % tiles, n, q.ws); });
+        w = wn;
+      }
+      __syncthreads();  // the second part's groups are others
+    }
+  }
 
   // -------- 2: output rows of the pairs --------
-  for_items((p.d + 15) / 16, p.f, [&](int a, int tile, int n, int ws) {
-    if (n <= 8) item_out<1>(p, sh, red, a, tile, n, ws);
-    else if (n <= 16) item_out<2>(p, sh, red, a, tile, n, ws);
-    else if (n <= 32) item_out<4>(p, sh, red, a, tile, n, ws);
-    else item_out<8>(p, sh, red, a, tile, n, ws);
-  });
-  // the row of each (token, choice), in place of its expert
-  __syncthreads();
-  for (int a = tid; a < n_active; a += THREADS) {
-    const int e = sh.active[a];
-    unsigned long long m = sh.mask[e];
-    for (int i = 0; m; ++i, m &= m - 1) {
-      const int tok = __ffsll((long long)m) - 1;
-      for (int j = 0; j < p.top_k; ++j)
-        if (sh.sel[tok * p.top_k + j] == e) {
-          sh.sel[tok * p.top_k + j] = (short)(-1 - (sh.base[a] + i));  // (negative: not an expert)
-          break;
-        }
+  if (p.tokens == 1) {
+    if ((p.d + 7) / 8 <= 2 * (int)gridDim.x) one_token_out<8>(p, sh, red);
+    else one_token_out<16>(p, sh, red);
+    return;
+  }
+  {
+    const int tiles = (p.d + 15) / 16;
+    const Walk walk(n_active * tiles, p.f);
+    const int start = walk.bulk ? 0 : 1;
+    const Ticket ticket = grid_arrive(p);
+    for (int part = start; part < 2; ++part) {
+      const Walk::Part q = walk.part(part, warp);
+      Rows w = {};
+      if (q.first < q.end) {  // (the first part's weights travel while the barrier is waited for)
+        w = rows_out(p, sh, q.first / tiles, q.first % tiles, g);
+        load_round(frag, w.w0, w.w1, (warp & (q.ws - 1)) * ROUND, t, p.f);
+        if (part == start) prefetch_rows(w, t, p.f, q.ws);
+      }
+      if (part == start && !grid_wait(p, sh, ticket)) return;
+      for (int it = q.first; it < q.end; it += q.step) {
+        const int a = it / tiles, next = it + q.step;
+        const Rows wn = next < q.end ? rows_out(p, sh, next / tiles, next % tiles, g) : Rows{};
+        const int n = __popcll(sh.mask[sh.active[a]]);
+        by_columns(n, [&](auto c) { item_out<decltype(c)::value>(p, sh, red, frag, w, wn, a, it % tiles, n, q.ws); });
+        w = wn;
+      }
+      __syncthreads();
     }
   }
   if (!grid_barrier(p, sh)) return;
@@ -450,26 +669,18 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
     const int tok = i / quads, d = (i - tok * quads) * 4;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int j = 0; j < p.top_k; ++j) {
-      const int row = -1 - sh.sel[tok * p.top_k + j];
       const float w = sh.prob[tok * p.top_k + j];
-      const float4 o = __ldcg(reinterpret_cast<const float4*>(p.out + (long long)row * p.d + d));
+      const float4 o = __ldcg(reinterpret_cast<const float4*>(p.out + (long long)sh.row[tok * p.top_k + j] * p.d + d));
       s.x += w * o.x;
       s.y += w * o.y;
       s.z += w * o.z;
       s.w += w * o.w;
     }
     const long long at = tok * p.ldy + d;
-    const float v[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      if (p.y_f32) {
-        static_cast<float*>(p.y)[at + c] = v[c];
-      } else {
-        uint16_t r;
-        asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v[c]));
-        static_cast<uint16_t*>(p.y)[at + c] = r;
-      }
-    }
+    put_y(p, at, s.x);
+    put_y(p, at + 1, s.y);
+    put_y(p, at + 2, s.z);
+    put_y(p, at + 3, s.w);
   }
 }
 
@@ -562,8 +773,8 @@ apk_status forward(apk_moe* h, const apk_moe_io* io) {
   p.rsplit = std::max(1, std::min({h->sms / etiles, (c.d_model + moe::WARPS * moe::ROUND - 1) / (moe::WARPS * moe::ROUND), 8}));
   const size_t pairs = (size_t)io->tokens * c.top_k;
   const size_t b_log = up256((size_t)p.rsplit * io->tokens * c.experts * 4), b_hid = up256(pairs * c.d_ff * 2);
-  const size_t b_out = up256(pairs * c.d_model * 4);
-  APK_TRY(h->scratch.begin(256 + b_log + b_hid + b_out, 256, s, &h->err));
+  const size_t b_out = up256(pairs * c.d_model * 4), b_choice = up256(pairs * 8);
+  APK_TRY(h->scratch.begin(256 + b_log + b_hid + b_out + b_choice, 256, s, &h->err));
   uint8_t* b = h->scratch.data();
   p.x = static_cast<const uint16_t*>(io->x);
   p.router = static_cast<const uint16_t*>(c.router);
@@ -589,15 +800,20 @@ apk_status forward(apk_moe* h, const apk_moe_io* io) {
   p.logits = reinterpret_cast<float*>(b + 256);
   p.hid = reinterpret_cast<uint16_t*>(b + 256 + b_log);
   p.out = reinterpret_cast<float*>(b + 256 + b_log + b_hid);
+  p.choice = reinterpret_cast<float2*>(b + 256 + b_log + b_hid + b_out);
+  // a small router (16 tokens, 96 KB of weights at most) is read by every CTA
+  // from L2 in less time than a grid barrier takes
+  p.local = io->tokens <= 16 && io->tokens * c.experts <= moe::LOCAL_LOGITS &&
+            (long long)c.experts * c.d_model * 2 <= moe::LOCAL_BYTES;
   const int nt8 = io->tokens <= 8 ? 1 : io->tokens <= 16 ? 2 : io->tokens <= 32 ? 4 : 8;
-  p.red_stride = nt8 * 128;
+  p.red_stride = std::max(nt8, 2) * 128;  // (the router's items have two tiles of tokens)
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeCooperative;
   at[0].val.cooperative = 1;
   cfg.gridDim = dim3(h->sms);
   cfg.blockDim = dim3(moe::THREADS);
-  cfg.dynamicSmemBytes = moe::red_bytes(nt8);
+  cfg.dynamicSmemBytes = moe::red_bytes(std::max(nt8, 2));
   cfg.stream = s;
   cfg.attrs = at;
   cfg.numAttrs = 1;
