@@ -73,25 +73,38 @@ __device__ __forceinline__ uint16_t f2bf(float v) {
   return r;
 }
 
-// Copies an operand whose base or row stride is not a multiple of 16 bytes
-// (TMA cannot address it) to rows of ld elements, ld a multiple of 8.  One
-// thread per 8 elements, 2-byte loads along a warp.
-__global__ void __launch_bounds__(256) repack(const uint16_t* src, long long lds, int rows, int cols, uint16_t* dst,
-                                              int ld) {
-  const int chunks = ld / 8;
-  const long long n = (long long)rows * chunks;
+// Copies operands whose base or row stride is not a multiple of 16 bytes (TMA
+// cannot address them) to rows of ld elements, ld a multiple of 8.  One
+// thread per 8 elements.
+struct Repack {
+  const uint16_t* src;
+  uint16_t* dst;
+  long long lds;
+  int rows, cols, ld;
+  long long first;  // chunk index of this operand's first chunk
+};
+struct RepackParams {
+  Repack op[2];
+  int n;
+  long long chunks;
+};
+__global__ void __launch_bounds__(256) repack(const __grid_constant__ RepackParams p) {
   pdl_launch();
   pdl_wait();
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const long long r = i / chunks;
-    const int c = (int)(i % chunks) * 8;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < p.chunks; i += (long long)gridDim.x * 256) {
+    const Repack& o = p.op[p.n > 1 && i >= p.op[1].first ? 1 : 0];
+    const long long at = i - o.first;
+    const int per = o.ld / 8;
+    const long long r = at / per;
+    const int c = (int)(at - r * per) * 8;
     union {
       uint16_t h[8];
       uint4 v;
     } u;
+    const uint16_t* s = o.src + r * o.lds + c;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) u.h[j] = c + j < cols ? src[r * lds + c + j] : (uint16_t)0;
-    *reinterpret_cast<uint4*>(dst + r * ld + c) = u.v;
+    for (int j = 0; j < 8; ++j) u.h[j] = c + j < o.cols ? s[j] : (uint16_t)0;
+    *reinterpret_cast<uint4*>(o.dst + r * o.ld + c) = u.v;
   }
 }
 
@@ -126,7 +139,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzParams p) {
   auto colof = [&](int i) { return VEC ? lane * 8 + i : lane + 32 * i; };
   with_act(p.z ? p.act : APK_ACT_NONE, [&](auto tag) {
     constexpr int ACT = decltype(tag)::value;
-#pragma unroll 2
+#pragma unroll 4
     for (long long r = (long long)blockIdx.y * p.rows_per_block + warp; r < r1; r += 8) {
       union {
         uint16_t h[8];
@@ -183,6 +196,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzParams p) {
     __threadfence();
     s = 0.f;
     if (c < p.cols)
+#pragma unroll 8
       for (unsigned b = 0; b < gridDim.y; ++b) s += __ldcg(p.part + (long long)b * p.cols + c);
   }
   if (c < p.cols) {
@@ -217,15 +231,23 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 lin::Operand operand(const void* p, long long ld, int outer, int inner, bool mn) {
   return {p, outer == 1 ? (long long)up8(inner) : ld, outer, inner, mn};
 }
-apk_status launch_repack(const void* src, long long lds, int rows, int cols, void* dst, cudaStream_t s, Err* err) {
-  const int ld = up8(cols);
-  const long long n = (long long)rows * (ld / 8);
-  const int grid = (int)std::min<long long>((n + 255) / 256, 148 * 16);
-  Launch l(dim3(grid), 256, 0, s);
-  return cu_status(cudaLaunchKernelEx(&l.cfg, lin::repack, static_cast<const uint16_t*>(src), lds, rows, cols,
-                                      static_cast<uint16_t*>(dst), ld),
-                   "launching the repack kernel", err);
-}
+// The operands of one launch of the repack kernel.
+struct RepackList {
+  lin::RepackParams p{};
+  // `*src` becomes the copy at dst
+  void add(const void** src, long long* ld, int rows, int cols, void* dst) {
+    lin::Repack& o = p.op[p.n++];
+    o = {static_cast<const uint16_t*>(*src), static_cast<uint16_t*>(dst), *ld, rows, cols, up8(cols), p.chunks};
+    p.chunks += (long long)rows * (o.ld / 8);
+    *src = dst;
+    *ld = o.ld;
+  }
+  apk_status run(int sms, cudaStream_t s, Err* err) const {
+    if (p.n == 0) return APK_OK;
+    Launch l(dim3((unsigned)std::min<long long>((p.chunks + 255) / 256, sms * 16)), 256, 0, s);
+    return cu_status(cudaLaunchKernelEx(&l.cfg, lin::repack, p), "launching the repack kernel", err);
+  }
+};
 
 #define APK_TRY(x)                    \
   do {                                \
@@ -268,16 +290,10 @@ apk_status forward(apk_linear* h, const apk_linear_io* io) {
     const size_t bx = px ? up256((size_t)M * up8(K) * 2) : 0, bw = pw ? up256((size_t)w_outer * up8(w_inner) * 2) : 0;
     const size_t zeroed = up256((size_t)(N + lin::DZ_COLS - 1) / lin::DZ_COLS * 4);
     APK_TRY(h->scratch.begin(zeroed + bx + bw, zeroed, s, &h->err));
-    if (px) {
-      APK_TRY(launch_repack(x, ldx, M, K, h->scratch.data() + zeroed, s, &h->err));
-      x = h->scratch.data() + zeroed;
-      ldx = up8(K);
-    }
-    if (pw) {
-      APK_TRY(launch_repack(w, ldw, w_outer, w_inner, h->scratch.data() + zeroed + bx, s, &h->err));
-      w = h->scratch.data() + zeroed + bx;
-      ldw = up8(w_inner);
-    }
+    RepackList list;
+    if (px) list.add(&x, &ldx, M, K, h->scratch.data() + zeroed);
+    if (pw) list.add(&w, &ldw, w_outer, w_inner, h->scratch.data() + zeroed + bx);
+    APK_TRY(list.run(h->sms, s, &h->err));
   }
   lin::Product p{};
   p.P = operand(w, ldw, w_outer, w_inner, c.w_layout == APK_W_KN);
@@ -286,7 +302,7 @@ apk_status forward(apk_linear* h, const apk_linear_io* io) {
   p.cols = N;
   p.k = K;
   p.epi = epi;
-  APK_TRY(lin::run_products(&p, 1, h->sms, h->status, c.wait_limit_ns, s, &h->err.text));
+  APK_TRY(lin::run_products(&p, 1, h->sms, c.device, h->status, c.wait_limit_ns, s, &h->err.text));
   if (px || pw) APK_TRY(h->scratch.end(s, &h->err));
   return APK_OK;
 }
@@ -367,18 +383,10 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
   const void* x = g->x;
   const void* w = c.W;
   long long ldx = g->ldx, ldw = c.ldw;
-  if (px) {
-    void* q = base + zeroed + bpart + bdz;
-    APK_TRY(launch_repack(x, ldx, M, K, q, s, &h->err));
-    x = q;
-    ldx = up8(K);
-  }
-  if (pw) {
-    void* q = base + zeroed + bpart + bdz + bx;
-    APK_TRY(launch_repack(w, ldw, w_outer, w_inner, q, s, &h->err));
-    w = q;
-    ldw = up8(w_inner);
-  }
+  RepackList list;
+  if (px) list.add(&x, &ldx, M, K, base + zeroed + bpart + bdz);
+  if (pw) list.add(&w, &ldw, w_outer, w_inner, base + zeroed + bpart + bdz + bx);
+  APK_TRY(list.run(h->sms, s, &h->err));
   lin::Product p[2] = {};
   int n = 0;
   if (g->dx) {  // dx[m][k] = sum_n dz[m][n] W[k][n]
@@ -400,7 +408,7 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
     a.k = M;
     a.epi = {nullptr, nullptr, g->dw, nullptr, 0, g->ld_dw, 0, 0, 0, g->dw_dtype == APK_F32, APK_ACT_NONE};
   }
-  if (n) APK_TRY(lin::run_products(p, n, h->sms, h->status, c.wait_limit_ns, s, &h->err.text));
+  if (n) APK_TRY(lin::run_products(p, n, h->sms, c.device, h->status, c.wait_limit_ns, s, &h->err.text));
   if (scratch) APK_TRY(h->scratch.end(s, &h->err));
   return APK_OK;
 }
@@ -436,11 +444,11 @@ apk_status apk_linear_create(const apk_linear_config* cfg, apk_linear** out) {
     return h->err.fail(APK_ECUDA, "no CUDA device %d", c.device);
   }
   DeviceGuard guard(c.device);
-  int major = 0, sms = 0, pairs = 0;
+  int major = 0, sms = 0;
   APK_TRY(cu_status(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, c.device), "device query", &h->err));
   APK_TRY(cu_status(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c.device), "device query", &h->err));
   if (major != 10) return h->err.fail(APK_EUNSUPPORTED, "the kernels are built for sm_100a");
-  APK_TRY(cu_status(lin::prepare(&pairs), "preparing the linear kernels", &h->err));
+  APK_TRY(cu_status(lin::prepare(), "preparing the linear kernels", &h->err));
   h->sms = sms;
   if (c.sms < 0 || c.sms > sms) return h->err.fail(APK_EINVAL, "sms %d of %d", c.sms, sms);
   if (c.sms > 0) h->sms = c.sms;

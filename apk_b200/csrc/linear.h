@@ -55,17 +55,18 @@ struct Product {
   Epilogue epi;
 };
 
-// Launches one or two products (one launch). sms: the SMs it may fill.
+// Launches one or two products, in one launch where that is faster. sms: the SMs it may
+// fill; dev: the current device.
 // `why` receives a message on failure.
-apk_status run_products(const Product* pr, int n, int sms, int* status, long long limit, cudaStream_t stream,
+apk_status run_products(const Product* pr, int n, int sms, int dev, int* status, long long limit, cudaStream_t stream,
                         std::string* why);
 // A product of at most STREAM_ROWS rows with weights [n][k] (nk) or [k][n] of
 // any stride and alignment.
 constexpr int STREAM_ROWS = 16;
 cudaError_t run_stream(const void* x, long long ldx, const void* w, long long ldw, bool nk, int rows, int n, int k,
                        const Epilogue& epi, int sms, cudaStream_t stream);
-// The first use on a device sets the kernels' shared-memory attributes.
-cudaError_t prepare(int* pairs);
+// Sets the kernels' attributes on the current device, once; before its first run_products.
+cudaError_t prepare();
 
 }  // namespace lin
 

@@ -16,10 +16,11 @@
 // tail.  Edges are TMA's zero fill on load and a predicate on store.
 //
 // SPLIT: a tile's K range is shared by a cluster of 2-8 CTAs, for calls with
-// fewer tiles than SMs.  Each leaves its fp32 accumulator in its own shared
-// memory (the drained ring) and, past a cluster barrier, sums every
-// p.split-th row over the cluster in rank order: nothing goes through global
-// memory, and the order of the sum is fixed.
+// fewer tiles than SMs.  Rank r owns the rows r, r + split, ...: each CTA
+// stores its fp32 accumulator's rows into their owners' shared memory (stores
+// need not be waited for one by one, as loads from there would), and past one
+// cluster barrier the owners sum them in rank order and finish.  Nothing goes
+// through global memory, and the order of the sum is fixed.
 //
 // Every wait is bounded; one that runs out raises the status word and lets
 // every role unwind.
@@ -27,6 +28,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "act.cuh"
 #include "common.cuh"
@@ -52,10 +54,8 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, uint32_t bits) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(bits) : "memory");
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -156,14 +156,14 @@ __device__ __forceinline__ void store_elem(void* p, long long i, float v, int f3
 }
 
 // W rows of one output column: bias, pre-activation, activation, residual,
-// stores.  out and pre point at the first row's element.  The types and the
-// presence of the pre-activation are fixed per call of this function: with
-// run-time flags in the element loop and an address product per element the
-// epilogue took 51 instructions a row and twice the time of the MMAs of 2048 k.
-template <int ACT, bool PRE, bool F32, int W>
-__device__ __forceinline__ void finish_full(const Epilogue& e, const uint32_t (&v)[W], const float (&res)[W],
-                                            float bias, uint8_t* out, uint8_t* pre) {
-  const long long so = e.ld_out * (F32 ? 4 : 2), sp = e.ld_pre * 2;
+// stores.  out and pre point at the first row's element; so and sp are the
+// bytes to the next one.  The types and the presence of the pre-activation
+// are fixed per call of this function: with run-time flags in the element
+// loop and an address product per element the epilogue took 51 instructions a
+// row and twice the time of the MMAs of 2048 k.
+template <int ACT, bool PRE, bool F32, bool RES, int W>
+__device__ __forceinline__ void finish_full(const uint32_t (&v)[W], const uint32_t (&raw)[W], int shift, float bias,
+                                            uint8_t* out, uint8_t* pre, long long so, long long sp) {
 #pragma unroll
   for (int i = 0; i < W; ++i) {
     const float z = __uint_as_float(v[i]) + bias;
@@ -171,38 +171,101 @@ __device__ __forceinline__ void finish_full(const Epilogue& e, const uint32_t (&
       *reinterpret_cast<uint16_t*>(pre) = to_bf16(z);
       pre += sp;
     }
-    const float y = act_f<ACT>(z) + res[i];
+    float y = act_f<ACT>(z);
+    if (RES) y += __uint_as_float(raw[i] << shift);
     if (F32) *reinterpret_cast<float*>(out) = y;
     else *reinterpret_cast<uint16_t*>(out) = to_bf16(y);
     out += so;
   }
 }
-// The same for a block that reaches past the last row.
+// The same for n < W rows.
 template <int ACT, int W>
-__device__ __forceinline__ void finish_part(const Epilogue& e, const uint32_t (&v)[W], const float (&res)[W],
-                                            float bias, uint8_t* out, uint8_t* pre, int n) {
+__device__ __forceinline__ void finish_part(const Epilogue& e, const uint32_t (&v)[W], const uint32_t (&raw)[W],
+                                            int shift, float bias, uint8_t* out, uint8_t* pre, long long so,
+                                            long long sp, int n) {
 #pragma unroll
   for (int i = 0; i < W; ++i) {
     if (i < n) {
       const float z = __uint_as_float(v[i]) + bias;
-      if (e.pre) store_elem(pre, i * e.ld_pre, z, 0);
-      store_elem(out, i * e.ld_out, act_f<ACT>(z) + res[i], e.out_f32);
+      if (e.pre) store_elem(pre + i * sp, 0, z, 0);
+      const float res = e.res ? __uint_as_float(raw[i] << shift) : 0.f;
+      store_elem(out + i * so, 0, act_f<ACT>(z) + res, e.out_f32);
     }
   }
 }
+// min(n, W) rows r, r + step, ... of column c; raw: their residual's bits, if any.
 template <int W>
-__device__ __forceinline__ void load_residual(const Epilogue& e, float (&res)[W], int r, int n, long long c) {
+__device__ __forceinline__ void finish(const Epilogue& e, const uint32_t (&v)[W], const uint32_t (&raw)[W], float bias,
+                                       int r, int step, int n, long long c) {
+  const int es = e.out_f32 ? 4 : 2, shift = e.res_f32 ? 0 : 16;
+  uint8_t* out = static_cast<uint8_t*>(e.out) + (r * e.ld_out + c) * es;
+  uint8_t* pre = static_cast<uint8_t*>(e.pre) + (r * e.ld_pre + c) * 2;
+  const long long so = e.ld_out * step * es, sp = e.ld_pre * step * 2;
+  with_act(e.act, [&](auto a) {
+    constexpr int ACT = decltype(a)::value;
+    auto full = [&](auto pre_, auto f32_, auto res_) {
+      finish_full<ACT, decltype(pre_)::value, decltype(f32_)::value, decltype(res_)::value, W>(v, raw, shift, bias, out,
+                                                                                               pre, so, sp);
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    if (n < W) finish_part<ACT, W>(e, v, raw, shift, bias, out, pre, so, sp, n);
+    else if (e.res) e.out_f32 ? (e.pre ? full(yes, yes, yes) : full(no, yes, yes))
+                              : (e.pre ? full(yes, no, yes) : full(no, no, yes));
+    else e.out_f32 ? (e.pre ? full(yes, yes, no) : full(no, yes, no)) : (e.pre ? full(yes, no, no) : full(no, no, no));
+  });
+}
+// The residual of the rows r, r + step, ... (W, of which n exist), as loaded
+// bits.  With a condition on every load the loads went out one by one: a full
+// block has none.
+template <int W>
+__device__ __forceinline__ void load_residual(const Epilogue& e, uint32_t (&res)[W], int r, int step, int n,
+                                              long long c) {
+  const long long ld = e.ld_res * step;
   if (e.res_f32) {
-    const float* p = static_cast<const float*>(e.res) + r * e.ld_res + c;
+    const uint32_t* p = static_cast<const uint32_t*>(e.res) + r * e.ld_res + c;
+    if (n >= W) {
 #pragma unroll
-    for (int i = 0; i < W; ++i, p += e.ld_res) res[i] = i < n ? *p : 0.f;
+      for (int i = 0; i < W; ++i) res[i] = p[i * ld];
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) res[i] = i < n ? p[i * ld] : 0u;
+    }
   } else {
     const uint16_t* p = static_cast<const uint16_t*>(e.res) + r * e.ld_res + c;
-    uint16_t h[W];
+    if (n >= W) {
 #pragma unroll
-    for (int i = 0; i < W; ++i, p += e.ld_res) h[i] = i < n ? *p : (uint16_t)0;
+      for (int i = 0; i < W; ++i) res[i] = p[i * ld];
+    } else {
 #pragma unroll
-    for (int i = 0; i < W; ++i) res[i] = __uint_as_float((uint32_t)h[i] << 16);
+      for (int i = 0; i < W; ++i) res[i] = i < n ? p[i * ld] : 0u;
+    }
+  }
+}
+
+// The split K's sum for this thread's column c of the rows this rank owns
+// (`own` of them, the i-th is row rank + SPLIT i of n), i = i0, i0 + 2, ...
+// part: shared address of [rank][own][128] floats, at the column.
+template <int SPLIT>
+__device__ __forceinline__ void sum_ranks(const Epilogue& e, uint32_t part, int own, int rank, int i0, int n, int r0,
+                                          long long c, float bias) {
+  constexpr int U = 8, STEP = 2 * SPLIT;
+  for (int i = i0; rank + SPLIT * i < n; i += 2 * U) {
+    const int row = rank + SPLIT * i, left = (n - row + STEP - 1) / STEP;
+    uint32_t raw[U], v[U];
+    if (e.res) load_residual<U>(e, raw, r0 + row, STEP, left, c);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float z = 0.f;
+#pragma unroll
+      for (int s = 0; s < SPLIT; ++s) {
+        float w;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(w) : "r"(part + (s * own + min(i + 2 * u, own - 1)) * 512));
+        z += w;
+      }
+      v[u] = __float_as_uint(z);
+    }
+    finish<U>(e, v, raw, bias, r0 + row, STEP, left, c);
   }
 }
 
@@ -213,8 +276,7 @@ struct Cfg {
   static constexpr int STAGE = P_BYTES + Q_BYTES;
   static constexpr int NBUF = SPLIT ? 1 : 2;
   static constexpr int TMEM_COLS = NBUF * NT < 32 ? 32 : NBUF * NT;
-  static constexpr int SMEM = S * STAGE + 1024;
-  static_assert(!SPLIT || S * STAGE >= NT * 512, "the split sum reuses the ring");
+  static constexpr int SMEM = S * STAGE + (SPLIT ? NT * 512 : 0) + 1024;
   static_assert((TMEM_COLS & (TMEM_COLS - 1)) == 0 && TMEM_COLS <= 512, "");
 };
 
@@ -376,29 +438,34 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
     for (int t = t0; t < p.tiles; t += step, ++T) {
       int r0, c0;
       const Problem& pr = locate(t, r0, c0);
-      const Epilogue& e = pr.epi;
+      const Epilogue e = pr.epi;
       const int buf = T % C::NBUF;
       const int col = 32 * q + lane;
       const bool in = c0 + col < pr.cols;
       const long long c = c0 + col;
       float bias = 0.f;
       if (!SPLIT && in && e.bias) bias = load_elem(e.bias, c, e.bias_f32);
+      const bool has_res = !SPLIT && e.res && in;
+      uint32_t raw[W];
+      if (has_res && r0 + g * W < pr.rows) load_residual<W>(e, raw, r0 + g * W, 1, pr.rows - r0 - g * W, c);
       if (!bwait(&sh.tfull[buf], (T / C::NBUF) & 1, p, sh, DEV_WAIT_TIMEOUT_TMEM)) break;
       tc::fence_after_sync();
       const uint32_t ta = tbase + ((uint32_t)(32 * q) << 16) + (uint32_t)buf * NT;
       if constexpr (SPLIT) {
-        // the accumulator, [row][128 columns] in the drained ring; a CTA
-        // whose share of K is empty holds zero
+        // rows to their owners; a CTA whose share of K is empty sends zeros
         int kb, ke;
         k_range(pr, kb, ke);
-        float* part = reinterpret_cast<float*>(ring);
+        const uint32_t at = smem_u32(ring + S * C::STAGE) + (uint32_t)(krank * (NT / p.split) * 512 + col * 4);
 #pragma unroll 1
         for (int b = g; b < NT / W; b += 2) {
           uint32_t v[W];
           tc::ld_32x32b<W>(ta + b * W, v);
           tc::wait_ld();
 #pragma unroll
-          for (int i = 0; i < W; ++i) part[(b * W + i) * 128 + col] = kb < ke ? __uint_as_float(v[i]) : 0.f;
+          for (int i = 0; i < W; ++i) {
+            const int row = b * W + i;
+            st_cluster_f32(map_rank(at, row & (p.split - 1)) + (row / p.split) * 512, kb < ke ? v[i] : 0u);
+          }
         }
       } else {
 #pragma unroll 1
@@ -406,28 +473,16 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
           const int r = r0 + b * W;
           if (r >= pr.rows) break;  // (uniform; later blocks lie further out)
           uint32_t v[W];
-          float res[W];
           tc::ld_32x32b<W>(ta + b * W, v);
           const int n = pr.rows - r;
-          if (e.res && in) {
-            load_residual<W>(e, res, r, n, c);
-          } else {
+          uint32_t res[W];
+          if (e.res) {
 #pragma unroll
-            for (int i = 0; i < W; ++i) res[i] = 0.f;
+            for (int i = 0; i < W; ++i) res[i] = raw[i];
           }
+          if (has_res && b + 2 < NT / W && n > 2 * W) load_residual<W>(e, raw, r + 2 * W, 1, n - 2 * W, c);
           tc::wait_ld();
-          if (in) {
-            uint8_t* out = static_cast<uint8_t*>(e.out) + (r * e.ld_out + c) * (e.out_f32 ? 4 : 2);
-            uint8_t* pre = static_cast<uint8_t*>(e.pre) + (r * e.ld_pre + c) * 2;
-            with_act(e.act, [&](auto a) {
-              constexpr int ACT = decltype(a)::value;
-              if (n < W) finish_part<ACT, W>(e, v, res, bias, out, pre, n);
-              else if (e.out_f32 && e.pre) finish_full<ACT, true, true, W>(e, v, res, bias, out, pre);
-              else if (e.out_f32) finish_full<ACT, false, true, W>(e, v, res, bias, out, pre);
-              else if (e.pre) finish_full<ACT, true, false, W>(e, v, res, bias, out, pre);
-              else finish_full<ACT, false, false, W>(e, v, res, bias, out, pre);
-            });
-          }
+          if (in) finish<W>(e, v, res, bias, r, 1, n, c);
           __syncwarp();
         }
         tc::fence_before_sync();
@@ -443,37 +498,24 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
   tc::fence_before_sync();
   __syncthreads();
   if constexpr (SPLIT) {
-    cluster_sync();  // every rank's partial tile is in its shared memory
+    cluster_sync();  // every rank's rows have arrived
     int r0, c0;
     const Problem& pr = locate(t0, r0, c0);
-    const Epilogue& e = pr.epi;
+    const Epilogue e = pr.epi;  // in registers: a field of an indexed kernel parameter costs 80 cycles a use
     if (tid < 256 && !sh.abort) {
       const int col = tid & 127;
       const long long c = c0 + col;
       if (c < pr.cols) {
         const float bias = e.bias ? load_elem(e.bias, c, e.bias_f32) : 0.f;
-        const uint32_t base = smem_u32(ring) + col * 4;
-        for (int j = krank + p.split * (tid >> 7); j < NT && r0 + j < pr.rows; j += 2 * p.split) {
-          float part[8];
-#pragma unroll
-          for (int s = 0; s < 8; ++s)
-            part[s] = s < p.split ? ld_cluster_f32(map_rank(base, s) + j * 512) : 0.f;
-          float z = part[0];
-#pragma unroll
-          for (int s = 1; s < 8; ++s) z += part[s];
-          z += bias;
-          const long long r = r0 + j;
-          const float res = e.res ? load_elem(e.res, r * e.ld_res + c, e.res_f32) : 0.f;
-          if (e.pre) store_elem(e.pre, r * e.ld_pre + c, z, 0);
-          with_act(e.act, [&](auto a) {
-            store_elem(e.out, r * e.ld_out + c, act_f<decltype(a)::value>(z) + res, e.out_f32);
-          });
-        }
+        const uint32_t part = smem_u32(ring + S * C::STAGE) + col * 4;
+        const int n = min(NT, pr.rows - r0), i0 = tid >> 7, own = NT / p.split;
+        if (p.split == 2) sum_ranks<2>(e, part, own, krank, i0, n, r0, c, bias);
+        else if (p.split == 4) sum_ranks<4>(e, part, own, krank, i0, n, r0, c, bias);
+        else sum_ranks<8>(e, part, own, krank, i0, n, r0, c, bias);
       }
     }
-    __syncthreads();
   }
-  if constexpr (CG == 2 || SPLIT) cluster_sync();  // no access reaches a CTA that has left
+  if constexpr (CG == 2) cluster_sync();  // no access reaches a CTA that has left
   if (warp == 1) {
     __syncwarp();
     tc::fence_after_sync();
@@ -501,8 +543,8 @@ Variant variant() {
 }
 const Variant* variants(int* n) {
   static const Variant v[] = {variant<2, 256, 6, false>(), variant<1, 128, 6, false>(), variant<1, 64, 8, false>(),
-                              variant<1, 32, 8, false>(),  variant<1, 16, 8, false>(),  variant<1, 128, 6, true>(),
-                              variant<1, 64, 8, true>(),   variant<1, 32, 8, true>(),   variant<1, 16, 8, true>()};
+                              variant<1, 32, 8, false>(),  variant<1, 16, 8, false>(),  variant<1, 128, 4, true>(),
+                              variant<1, 64, 7, true>(),   variant<1, 32, 8, true>(),   variant<1, 16, 8, true>()};
   *n = (int)(sizeof v / sizeof v[0]);
   return v;
 }
@@ -535,22 +577,34 @@ struct Choice {
   double cost;
 };
 
-// The variant with the least estimated time for these products on `sms` SMs.
-// In SM clocks per 64-deep k-block of one tile: the MMA's own time (128 x NT
-// x 64 at 4096 MAC per clock and SM) or, for narrow tiles, the time its
-// stage takes to arrive; and per tile the ring's fill and the epilogue's
-// drain, which two accumulators hide behind the next tile.
-Choice choose(const Product* pr, int n, int sms) {
+// Clusters of 2, 4 and 8 CTAs (index log2) that can be resident at once: an
+// SM cluster lies within one GPC, so eight CTAs find fewer places than 148 / 8.
+int g_clusters[64][4];
+
+// The variant with the least estimated time for these products on `sms` SMs,
+// in SM clocks.  Per 64-deep k-block and tile: the MMA's own time (128 x NT x
+// 64 at 4096 MAC per clock and SM) or the time a stage takes to arrive at an
+// SM (37 bytes a clock measured with every SM loading, from L2 or memory: the
+// widest tile is bound by this); for the whole: its bytes at the memory's
+// rate (3300 a clock).  Per tile an epilogue that two accumulators hide but for the last;
+// for a split, two cluster barriers and the sum.
+Choice choose(const Product* pr, int n, int sms, int dev) {
   int nv;
   const Variant* vs = variants(&nv);
+  double bytes = 0;
+  for (int j = 0; j < n; ++j)
+    bytes += 2.0 * ((double)pr[j].rows * pr[j].k + (double)pr[j].cols * pr[j].k + (double)pr[j].rows * pr[j].cols);
   Choice best{nullptr, 1, 0};
   for (int i = 0; i < nv; ++i) {
     const Variant& v = vs[i];
     bool fits = true;
     for (int j = 0; j < n; ++j) fits = fits && !(pr[j].Q.mn && v.nt < 64);
     if (!fits) continue;
-    const double per_kb = std::max(v.nt / v.cg * 2.0 * v.cg, (P_BYTES + v.nt / v.cg * 128) / 60.0);
-    for (int sp = v.split ? 2 : 1; sp <= (v.split ? 8 : 1); sp *= 2) {
+    const double per_kb = std::max(v.nt * 2.0, (P_BYTES + v.nt / v.cg * 128) / 37.0);
+    for (int lg = v.split ? 1 : 0; lg <= (v.split ? 3 : 0); ++lg) {
+      const int sp = 1 << lg, per = v.cg * sp;
+      int slots = std::max(1, sms / per);
+      if (per > 1) slots = std::max(1, std::min(slots, g_clusters[dev][per == 2 ? 1 : lg]));
       long long tiles = 0;
       double work = 0, longest = 0;
       for (int j = 0; j < n; ++j) {
@@ -560,11 +614,11 @@ Choice choose(const Product* pr, int n, int sms) {
         work += t * one;
         longest = std::max(longest, one);
       }
-      const int slots = std::max(1, sms / (v.cg * sp));
-      if (v.split && (tiles > slots || tiles * sp > 65535 * 32ll)) continue;
-      double cost = 2500 + (tiles <= slots ? longest : std::max(longest, work / slots * (double)(ceil_div((int)std::min<long long>(tiles, 1 << 30), slots) * (double)slots / tiles)));
-      cost += v.nt * 6.0;                         // the last tile's epilogue
-      if (v.split) cost += 1200 + v.nt * 4.0;     // cluster barriers and the sum
+      if (v.split && tiles > slots) continue;  // one tile per cluster, all resident
+      const double waves = (double)((tiles + slots - 1) / slots) * slots / tiles;  // rounding up to whole sweeps
+      double cost = 2500 + std::max(bytes / 3300, tiles <= slots ? longest : std::max(longest, work / slots * waves));
+      cost += v.nt * 6.0;
+      if (v.split) cost += 1500 + v.nt / sp * 6.0;
       if (!best.v || cost < best.cost) best = {&v, sp, cost};
     }
   }
@@ -573,14 +627,15 @@ Choice choose(const Product* pr, int n, int sms) {
 
 }  // namespace
 
-cudaError_t prepare(int* pairs) {
+cudaError_t prepare() {
   std::lock_guard<std::mutex> lock(g_mu);
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   int nv;
   const Variant* vs = variants(&nv);
-  if (dev >= 64 || !g_ready[dev]) {
+  if (dev >= 64) return cudaErrorInvalidDevice;
+  if (!g_ready[dev]) {
     if (!g_enc) {
       cudaDriverEntryPointQueryResult q;
       void* fn = nullptr;
@@ -593,25 +648,34 @@ cudaError_t prepare(int* pairs) {
       e = cudaFuncSetAttribute(vs[i].fn, cudaFuncAttributeMaxDynamicSharedMemorySize, vs[i].smem);
       if (e != cudaSuccess) return e;
     }
-    if (dev < 64) g_ready[dev] = true;
+    // the largest shared memory of each cluster size decides
+    for (int lg = 1; lg <= 3; ++lg) {
+      g_clusters[dev][lg] = 1 << 20;
+      for (int i = 0; i < nv; ++i) {
+        if (!(vs[i].split || (vs[i].cg == 2 && lg == 1))) continue;
+        Launch l(dim3(1 << lg), THREADS, vs[i].smem, nullptr, 1 << lg);
+        int c = 0;
+        e = cudaOccupancyMaxActiveClusters(&c, vs[i].fn, &l.cfg);
+        if (e != cudaSuccess) return e;
+        g_clusters[dev][lg] = std::min(g_clusters[dev][lg], c);
+      }
+    }
+    g_ready[dev] = true;
   }
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = 2;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(2);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = vs[0].smem;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaOccupancyMaxActiveClusters(pairs, vs[0].fn, &cfg);
+  return cudaSuccess;
 }
 
-apk_status run_products(const Product* pr, int n, int sms, int* status, long long limit, cudaStream_t stream,
+apk_status run_products(const Product* pr, int n, int sms, int dev, int* status, long long limit, cudaStream_t stream,
                         std::string* why) {
-  const Choice ch = choose(pr, n, sms);
+  const Choice ch = choose(pr, n, sms, dev);
+  if (n == 2) {
+    // products that want different tiles run one after the other
+    const double apart = choose(pr, 1, sms, dev).cost + choose(pr + 1, 1, sms, dev).cost;
+    if (apart < ch.cost) {
+      const apk_status st = run_products(pr, 1, sms, dev, status, limit, stream, why);
+      return st != APK_OK ? st : run_products(pr + 1, 1, sms, dev, status, limit, stream, why);
+    }
+  }
   const Variant& v = *ch.v;
   GemmParams p;
   p.nprob = n;
