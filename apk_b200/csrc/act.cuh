@@ -2,43 +2,59 @@
 //   gelu       x Phi(x),  Phi the normal distribution function
 //   gelu_tanh  x (1 + tanh u) / 2 = x / (1 + exp(-2u)),  u = sqrt(2/pi) (x + 0.044715 x^3)
 //   silu       x / (1 + exp(-x))
-// exp through the hardware exponential and the division by its reciprocal
-// approximation: a few 2^-23 relative for the arguments where the result is
-// not negligible, far below the rounding of a bf16 result and within the
-// fp32 sums' own error for an fp32 one.
+// The sigmoid 1 / (1 + 2^(-x log2 e)) goes through the hardware's 2^x and
+// reciprocal approximations: a few 2^-23 relative where it is not negligible,
+// far below the rounding of a bf16 result and within an fp32 sum's own error.
 #pragma once
 #include "../../include/apk.h"
 
 namespace apk {
 
-__device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+// 1 / (1 + 2^t): 0 for t = inf, 1 for t = -inf
+__device__ __forceinline__ float rcp_1p_ex2(float t) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return r;
+}
+// min(max(x, -100), 100), a NaN staying one: beyond, every activation's
+// derivative is at its limit, and products like inf * 0 do not arise.
+__device__ __forceinline__ float clamp100(float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(-100.f));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(r), "f"(100.f));
+  return r;
+}
+
+constexpr float LOG2E = 1.44269504f;
+// 2u = x (GT1 + GT3 x^2)
+constexpr float GT1 = 1.59576912f, GT3 = 0.0713548162f;
 
 template <int ACT>
 __device__ __forceinline__ float act_f(float x) {
   if constexpr (ACT == APK_ACT_RELU) return x <= 0.f ? 0.f : x;  // a NaN stays one
   else if constexpr (ACT == APK_ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678f));
-  else if constexpr (ACT == APK_ACT_GELU_TANH) {
-    const float u2 = 1.59576912f * (x + 0.044715f * x * x * x);
-    return __fdividef(x, 1.f + __expf(-u2));
-  } else if constexpr (ACT == APK_ACT_SILU) return __fdividef(x, 1.f + __expf(-x));
+  else if constexpr (ACT == APK_ACT_GELU_TANH)
+    return x * rcp_1p_ex2(x * fmaf(-LOG2E * GT3, x * x, -LOG2E * GT1));
+  else if constexpr (ACT == APK_ACT_SILU) return x * rcp_1p_ex2(-LOG2E * x);
   else return x;
 }
 
 template <int ACT>
-__device__ __forceinline__ float act_grad_f(float x) {
-  if constexpr (ACT == APK_ACT_RELU) return x > 0.f ? 1.f : 0.f;
-  else if constexpr (ACT == APK_ACT_GELU)
-    return 0.5f * (1.f + erff(x * 0.70710678f)) + x * 0.39894228f * __expf(-0.5f * x * x);
-  else if constexpr (ACT == APK_ACT_GELU_TANH) {
-    // d/dx x s(v) = s + x s (1 - s) v',  v = 2u
-    // (where |x| > 100 the second term is 0; unclamped it would be 0 * inf)
-    const float s = sigmoid_f(1.59576912f * (x + 0.044715f * x * x * x));
-    const float c = fminf(fmaxf(x, -100.f), 100.f);
-    return s + c * s * (1.f - s) * 1.59576912f * (1.f + 0.134145f * c * c);
+__device__ __forceinline__ float act_grad_f(float z) {
+  if constexpr (ACT == APK_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  else if constexpr (ACT == APK_ACT_GELU) {
+    const float x = clamp100(z);
+    return fmaf(x * 0.39894228f, __expf(-0.5f * x * x), 0.5f * (1.f + erff(x * 0.70710678f)));
+  } else if constexpr (ACT == APK_ACT_GELU_TANH) {
+    // d/dx x s(v) = s (1 + x v' (1 - s)),  v = 2u
+    const float x = clamp100(z), x2 = x * x;
+    const float s = rcp_1p_ex2(x * fmaf(-LOG2E * GT3, x2, -LOG2E * GT1));
+    const float t = x * fmaf(3.f * GT3, x2, GT1);
+    return fmaf(s, fmaf(-s, t, t), s);
   } else if constexpr (ACT == APK_ACT_SILU) {
-    const float s = sigmoid_f(x);
-    const float c = fminf(fmaxf(x, -100.f), 100.f);
-    return s * (1.f + c * (1.f - s));
+    const float x = clamp100(z), s = rcp_1p_ex2(-LOG2E * x);
+    return fmaf(s, fmaf(-s, x, x), s);
   } else return 1.f;
 }
 

@@ -66,7 +66,6 @@ void Scratch::release() {
 
 namespace lin {
 
-__device__ __forceinline__ float bf2f(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 __device__ __forceinline__ uint16_t f2bf(float v) {
   uint16_t r;
   asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
@@ -113,7 +112,7 @@ struct DzParams {
   const uint16_t* z;  // null: no activation
   uint16_t* dz;       // null: not wanted (it is dy)
   void* db;           // null: no bias
-  float* part;        // [row blocks][cols] partial column sums
+  float* part;        // [row blocks][cols rounded up to 8] partial column sums
   unsigned* count;    // one per column block, zero between launches
   long long ld_dy, ld_z, ld_dz;
   int rows, cols, rows_per_block, act, db_f32;
@@ -137,42 +136,62 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzParams p) {
   pdl_launch();
   pdl_wait();
   auto colof = [&](int i) { return VEC ? lane * 8 + i : lane + 32 * i; };
+  struct Row {
+    uint4 y, z;
+  };
+  const uint4 zero = make_uint4(0, 0, 0, 0);
   with_act(p.z ? p.act : APK_ACT_NONE, [&](auto tag) {
     constexpr int ACT = decltype(tag)::value;
-#pragma unroll 4
-    for (long long r = (long long)blockIdx.y * p.rows_per_block + warp; r < r1; r += 8) {
-      union {
-        uint16_t h[8];
-        uint4 v;
-      } y, z;
-      z.v = make_uint4(0, 0, 0, 0);
+    auto load = [&](long long r) {
+      Row v = {zero, zero};
+      if (r >= r1) return v;
       if constexpr (VEC) {
-        if (c0 + lane * 8 >= p.cols) continue;
-        y.v = *reinterpret_cast<const uint4*>(p.dy + r * p.ld_dy + c0 + lane * 8);
-        if (ACT != APK_ACT_NONE) z.v = *reinterpret_cast<const uint4*>(p.z + r * p.ld_z + c0 + lane * 8);
+        if (c0 + lane * 8 < p.cols) {
+          v.y = __ldcs(reinterpret_cast<const uint4*>(p.dy + r * p.ld_dy + c0 + lane * 8));
+          if (ACT != APK_ACT_NONE) v.z = __ldcs(reinterpret_cast<const uint4*>(p.z + r * p.ld_z + c0 + lane * 8));
+        }
       } else {
+        union {
+          uint16_t h[8];
+          uint4 v;
+        } y, z;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const bool in = c0 + colof(i) < p.cols;
           y.h[i] = in ? p.dy[r * p.ld_dy + c0 + colof(i)] : (uint16_t)0;
-          if (ACT != APK_ACT_NONE) z.h[i] = in ? p.z[r * p.ld_z + c0 + colof(i)] : (uint16_t)0;
+          z.h[i] = ACT != APK_ACT_NONE && in ? p.z[r * p.ld_z + c0 + colof(i)] : (uint16_t)0;
         }
+        v = {y.v, z.v};
       }
+      return v;
+    };
+    long long r = (long long)blockIdx.y * p.rows_per_block + warp;
+    Row now = load(r);
+    for (; r < r1; r += 8) {
+      const Row next = load(r + 8);  // in flight while this row is worked on
+      uint4 out;
+      const uint32_t* y = &now.y.x;
+      const uint32_t* z = &now.z.x;
+      uint32_t* o = &out.x;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = bf2f(y.h[i]) * act_grad_f<ACT>(bf2f(z.h[i]));
-        acc[i] += d;
-        y.h[i] = f2bf(d);
+      for (int i = 0; i < 4; ++i) {
+        const float d0 = __uint_as_float(y[i] << 16) * act_grad_f<ACT>(__uint_as_float(z[i] << 16));
+        const float d1 = __uint_as_float(y[i] & 0xFFFF0000u) * act_grad_f<ACT>(__uint_as_float(z[i] & 0xFFFF0000u));
+        acc[2 * i] += d0;
+        acc[2 * i + 1] += d1;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[i]) : "f"(d1), "f"(d0));
       }
       if (p.dz) {
         if constexpr (VEC) {
-          *reinterpret_cast<uint4*>(p.dz + r * p.ld_dz + c0 + lane * 8) = y.v;
+          if (c0 + lane * 8 < p.cols) *reinterpret_cast<uint4*>(p.dz + r * p.ld_dz + c0 + lane * 8) = out;
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (c0 + colof(i) < p.cols) p.dz[r * p.ld_dz + c0 + colof(i)] = y.h[i];
+            if (c0 + colof(i) < p.cols)
+              p.dz[r * p.ld_dz + c0 + colof(i)] = (uint16_t)(o[i / 2] >> (16 * (i & 1)));
         }
       }
+      now = next;
     }
   });
   if (!p.db) return;
@@ -184,7 +203,8 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzParams p) {
 #pragma unroll
   for (int w = 0; w < 8; ++w) s += sum[w][threadIdx.x];
   if (gridDim.y > 1) {
-    if (c < p.cols) p.part[(long long)blockIdx.y * p.cols + c] = s;
+    const int ldp = (p.cols + 7) / 8 * 8;
+    if (c < p.cols) p.part[(long long)blockIdx.y * ldp + c] = s;
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -194,10 +214,29 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzParams p) {
     __syncthreads();
     if (!last) return;
     __threadfence();
+    // warp w adds the row blocks w, w + 8, ..., then the warps are added in order
+    float t[8] = {};
+    if (c0 + lane * 8 < ldp) {
+#pragma unroll 4
+      for (unsigned b = warp; b < gridDim.y; b += 8) {
+        const float4* q = reinterpret_cast<const float4*>(p.part + (long long)b * ldp + c0 + lane * 8);
+        const float4 lo = __ldcg(q), hi = __ldcg(q + 1);
+        t[0] += lo.x;
+        t[1] += lo.y;
+        t[2] += lo.z;
+        t[3] += lo.w;
+        t[4] += hi.x;
+        t[5] += hi.y;
+        t[6] += hi.z;
+        t[7] += hi.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[warp][lane * 8 + i] = t[i];
+    __syncthreads();
     s = 0.f;
-    if (c < p.cols)
-#pragma unroll 8
-      for (unsigned b = 0; b < gridDim.y; ++b) s += __ldcg(p.part + (long long)b * p.cols + c);
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += sum[w][threadIdx.x];
   }
   if (c < p.cols) {
     if (p.db_f32) static_cast<float*>(p.db)[c] = s;
@@ -346,7 +385,7 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
   const int per = ((M + rblocks - 1) / rblocks + 7) / 8 * 8;
   rblocks = (M + per - 1) / per;
   const size_t zeroed = up256((size_t)cblocks * 4);
-  const size_t bpart = g->db ? up256((size_t)rblocks * N * 4) : 0;
+  const size_t bpart = g->db ? up256((size_t)rblocks * up8(N) * 4) : 0;
   const size_t bdz = own_dz ? up256((size_t)M * up8(N) * 2) : 0;
   const size_t bx = px ? up256((size_t)M * up8(K) * 2) : 0, bw = pw ? up256((size_t)w_outer * up8(w_inner) * 2) : 0;
   const bool scratch = g->db || own_dz || px || pw;

@@ -37,6 +37,7 @@ struct GemmParams {
   Problem pr[2];
   int nprob;
   int tiles0, tiles;  // tiles of problem 0 / of all
+  int extra;          // tiles of problem 1 that take the time of one of problem 0
   int split;          // CTAs of a cluster that share one tile's K range (1: none)
   int* status;
   long long limit;

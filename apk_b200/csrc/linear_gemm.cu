@@ -9,11 +9,19 @@
 // the bias is one register per lane, and a call with few rows takes an MMA
 // with a small N (16, 32, 64) instead of padding them to 128.
 //
-// Kernel<CG, NT, S, SPLIT>: CG CTAs (a pair for CG = 2) compute 128 CG columns
-// by NT rows.  Warp 0 feeds a ring of S TMA stages of 64 k, warp 1 issues
-// the MMAs into one of two TMEM accumulators, warps 2-9 drain the other:
-// persistent CTAs walk the tiles of up to two products, so a launch has one
-// tail.  Edges are TMA's zero fill on load and a predicate on store.
+// Kernel<CG, FM, NT, S, SPLIT>: CG CTAs (a pair for CG = 2) compute 128 CG FM
+// columns by NT rows.  Warp 0 feeds a ring of S TMA stages of 64 k, warp 1
+// issues the MMAs into one of two TMEM accumulators, warps 2-9 drain the
+// other: persistent CTAs walk the tiles of up to two products, so a launch
+// has one tail.  Edges are TMA's zero fill on load and a predicate on store.
+//
+// FM = 2 (512 columns by 256 rows a pair): both accumulators belong to one
+// tile, whose rows are loaded once for both.  What bounds the largest
+// products is the operands' way into the SMs (37 bytes a clock and SM, 885
+// clocks for a stage whose MMAs take 512); this tile loads 48 KB for two such
+// steps instead of 64.  Its epilogue hides less, so the MMAs are reordered at
+// both ends of a tile: the first stages feed accumulator 0 while 1 is still
+// being drained, and the last ones finish 0 before 1.
 //
 // SPLIT: a tile's K range is shared by a cluster of 2-8 CTAs, for calls with
 // fewer tiles than SMs.  Rank r owns the rows r, r + split, ...: each CTA
@@ -269,20 +277,45 @@ __device__ __forceinline__ void sum_ranks(const Epilogue& e, uint32_t part, int 
   }
 }
 
-template <int CG, int NT, int S, bool SPLIT>
+template <int CG, int FM, int NT, int S, bool SPLIT>
 struct Cfg {
   static constexpr int QROWS = NT / CG;
   static constexpr int Q_BYTES = QROWS * BK * 2;
-  static constexpr int STAGE = P_BYTES + Q_BYTES;
+  static constexpr int Q_AT = FM * P_BYTES;
+  static constexpr int STAGE = Q_AT + Q_BYTES;
+  static constexpr int COLS = 128 * CG * FM;  // of a tile
   static constexpr int NBUF = SPLIT ? 1 : 2;
   static constexpr int TMEM_COLS = NBUF * NT < 32 ? 32 : NBUF * NT;
   static constexpr int SMEM = S * STAGE + (SPLIT ? NT * 512 : 0) + 1024;
+  static_assert(FM == 1 || (CG == 2 && !SPLIT), "");
   static_assert((TMEM_COLS & (TMEM_COLS - 1)) == 0 && TMEM_COLS <= 512, "");
 };
 
-template <int CG, int NT, int S, bool SPLIT>
+// The q-th tile of group `g` of G, or -1.  Of two products the one with the
+// longer tiles comes first; groups that get one of those fewer take `extra`
+// of the shorter ones each before the rest is dealt out (to them first), so
+// that all end together.
+__device__ __forceinline__ int tile_of(const GemmParams& p, int g, int G, int q) {
+  const int n0 = p.tiles0, n1 = p.tiles - n0;
+  const int mine = g < n0 ? (n0 - g + G - 1) / G : 0;
+  if (q < mine) return g + q * G;
+  q -= mine;
+  const int rem = n0 % G, extra = rem ? p.extra : 0, others = rem ? G - rem : 0;
+  const int head = min(n1, others * extra);
+  if (extra && g >= rem) {
+    if (q < extra) {
+      const int j = (g - rem) * extra + q;
+      return j < head ? n0 + j : -1;
+    }
+    q -= extra;
+  }
+  const int j = head + (g >= rem ? g - rem : g - rem + G) + q * G;
+  return j < n1 ? n0 + j : -1;
+}
+
+template <int CG, int FM, int NT, int S, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ GemmParams p) {
-  using C = Cfg<CG, NT, S, SPLIT>;
+  using C = Cfg<CG, FM, NT, S, SPLIT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ Shared<S> sh;
@@ -328,16 +361,17 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
   pdl_wait();
   const uint32_t tbase = sh.tmem_base;
 
-  // The tiles of this CTA (pair, cluster): t0, t0 + step, ...
+  // The tiles of this CTA (pair, cluster): tile_of(q), q = 0, 1, ...
   const int group = CG == 2 ? 2 : SPLIT ? p.split : 1;
-  const int t0 = (int)blockIdx.x / group, step = (int)gridDim.x / group;
+  const int gi = (int)blockIdx.x / group, groups = (int)gridDim.x / group;
+  auto tile = [&](int q) { return tile_of(p, gi, groups, q); };
   // tile t: its product, and its first row and column (this CTA's column in a pair)
   auto locate = [&](int t, int& r0, int& c0) -> const Problem& {
     const Problem& pr = p.pr[t < p.tiles0 ? 0 : 1];
     int tr, tc_;
     tile_coords(t < p.tiles0 ? t : t - p.tiles0, pr.tiles_r, pr.tiles_c, RASTER_GROUP, tr, tc_);
     r0 = tr * NT;
-    c0 = tc_ * 128 * CG + 128 * (int)prank;
+    c0 = tc_ * C::COLS + 128 * (int)prank;
     return pr;
   };
   auto k_range = [&](const Problem& pr, int& kb, int& ke) {
@@ -349,7 +383,7 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
     // ================================ producer ================================
     uint32_t P = 0;
     bool ok = true;
-    for (int t = t0; t < p.tiles && ok; t += step) {
+    for (int q = 0, t; ok && (t = tile(q)) >= 0; ++q) {
       int r0, c0, kb, ke;
       const Problem& pr = locate(t, r0, c0);
       k_range(pr, kb, ke);
@@ -364,18 +398,23 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
         if (leader) mbar_arrive_expect_tx(&sh.full[s], CG * C::STAGE);
         const uint32_t d = smem_u32(ring + s * C::STAGE);
         const int k = kb * BK;
-        if (pr.p_mn) {
-          load_box<CG>(d, &pr.tmP, c0, k, bar);
-          load_box<CG>(d + 8192, &pr.tmP, c0 + 64, k, bar);
-        } else {
-          load_box<CG>(d, &pr.tmP, k, c0, bar);
+#pragma unroll
+        for (int h = 0; h < FM; ++h) {
+          const uint32_t at = d + h * P_BYTES;
+          const int c = c0 + 128 * CG * h;
+          if (pr.p_mn) {
+            load_box<CG>(at, &pr.tmP, c, k, bar);
+            load_box<CG>(at + 8192, &pr.tmP, c + 64, k, bar);
+          } else {
+            load_box<CG>(at, &pr.tmP, k, c, bar);
+          }
         }
         if (NT >= 64 && pr.q_mn) {
 #pragma unroll
           for (int b = 0; b < C::QROWS / 64; ++b)
-            load_box<CG>(d + P_BYTES + b * 8192, &pr.tmQ, r0 + 64 * b, k, bar);
+            load_box<CG>(d + C::Q_AT + b * 8192, &pr.tmQ, r0 + 64 * b, k, bar);
         } else {
-          load_box<CG>(d + P_BYTES, &pr.tmQ, k, r0, bar);
+          load_box<CG>(d + C::Q_AT, &pr.tmQ, k, r0, bar);
         }
       }
     }
@@ -386,44 +425,85 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
     }
   } else if (warp == 1 && lane == 0 && leader) {
     // =================================== MMA ===================================
-    uint32_t Q = 0, T = 0;
+    uint32_t Q = 0;
     bool ok = true;
-    for (int t = t0; t < p.tiles && ok; t += step, ++T) {
+    // an arrival in every CTA of the pair once the MMAs issued so far are done
+    auto commit_all = [&](uint64_t* bar) {
+      const uint32_t a = smem_u32(bar);
+      if constexpr (CG == 2) {
+        commit_to<CG>(map_rank(a, 0));
+        commit_to<CG>(map_rank(a, 1));
+      } else {
+        commit_to<CG>(a);
+      }
+    };
+    for (int T = 0, t; ok && (t = tile(T)) >= 0; ++T) {
       int r0, c0, kb, ke;
       const Problem& pr = locate(t, r0, c0);
       k_range(pr, kb, ke);
-      const int buf = T % C::NBUF;
-      ok = bwait(&sh.tempty[buf], ((T / C::NBUF) & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
-      if (!ok) break;
-      tc::fence_after_sync();
-      const uint32_t d = tbase + (uint32_t)buf * NT;
       const uint32_t idesc = pr.idesc;
       const uint32_t p_step = pr.p_mn ? 2048 : 32, q_step = pr.q_mn ? 2048 : 32;
       const uint32_t p_lbo = pr.p_mn ? 8192 : 16, q_lbo = pr.q_mn ? 8192 : 16;
-      for (int k = kb; k < ke; ++k, ++Q) {
-        const int s = Q % S;
-        ok = bwait(&sh.full[s], (Q / S) & 1, p, sh, DEV_WAIT_TIMEOUT_FULL);
-        if (!ok) break;
-        const uint32_t sp = smem_u32(ring + s * C::STAGE), sq = sp + P_BYTES;
+      auto full = [&](uint32_t i) { return bwait(&sh.full[i % S], (i / S) & 1, p, sh, DEV_WAIT_TIMEOUT_FULL); };
+      // stage i's MMAs with the h-th 128 columns of each CTA into accumulator buf
+      auto mmas = [&](uint32_t i, int h, int buf, bool first) {
+        const uint32_t sp = smem_u32(ring + (i % S) * C::STAGE) + h * P_BYTES, sq = smem_u32(ring + (i % S) * C::STAGE) + C::Q_AT;
 #pragma unroll
         for (int kk = 0; kk < BK / 16; ++kk)
-          mma<CG>(d, tc::smem_desc(sp + kk * p_step, p_lbo, 1024, tc::LAYOUT_SW128),
-                  tc::smem_desc(sq + kk * q_step, q_lbo, 1024, tc::LAYOUT_SW128), idesc, (k > kb || kk > 0) ? 1u : 0u);
-        const uint32_t e = smem_u32(&sh.empty[s]);
-        if constexpr (CG == 2) {
-          commit_to<CG>(map_rank(e, 0));
-          commit_to<CG>(map_rank(e, 1));
-        } else {
-          commit_to<CG>(e);
+          mma<CG>(tbase + (uint32_t)buf * NT, tc::smem_desc(sp + kk * p_step, p_lbo, 1024, tc::LAYOUT_SW128),
+                  tc::smem_desc(sq + kk * q_step, q_lbo, 1024, tc::LAYOUT_SW128), idesc, (!first || kk > 0) ? 1u : 0u);
+      };
+      const int n = ke - kb;
+      if constexpr (FM == 1) {
+        const int buf = T % C::NBUF;
+        ok = bwait(&sh.tempty[buf], ((T / C::NBUF) & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
+        if (!ok) break;
+        tc::fence_after_sync();
+        for (int i = 0; i < n; ++i, ++Q) {
+          ok = full(Q);
+          if (!ok) break;
+          mmas(Q, 0, buf, i == 0);
+          commit_all(&sh.empty[Q % S]);
         }
-      }
-      if (!ok) break;
-      const uint32_t f = smem_u32(&sh.tfull[buf]);
-      if constexpr (CG == 2) {
-        commit_to<CG>(map_rank(f, 0));
-        commit_to<CG>(map_rank(f, 1));
+        if (!ok) break;
+        commit_all(&sh.tfull[buf]);
       } else {
-        commit_to<CG>(f);
+        // stages i = 0 .. w: accumulator 0 first; n - l .. n: 0 before 1
+        const int w = n < S - 1 ? n : S - 1, l = n - w < S - 1 ? n - w : S - 1;
+        ok = bwait(&sh.tempty[0], (T & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
+        if (!ok) break;
+        tc::fence_after_sync();
+        for (int i = 0; i < w && ok; ++i) {
+          ok = full(Q + i);
+          if (ok) mmas(Q + i, 0, 0, i == 0);
+        }
+        ok = ok && bwait(&sh.tempty[1], (T & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
+        if (!ok) break;
+        tc::fence_after_sync();
+        if (l == 0) commit_all(&sh.tfull[0]);
+        for (int i = 0; i < w; ++i) {
+          mmas(Q + i, 1, 1, i == 0);
+          commit_all(&sh.empty[(Q + i) % S]);
+        }
+        for (int i = w; i < n - l && ok; ++i) {
+          ok = full(Q + i);
+          if (!ok) break;
+          mmas(Q + i, 0, 0, false);
+          mmas(Q + i, 1, 1, false);
+          commit_all(&sh.empty[(Q + i) % S]);
+        }
+        for (int i = n - l; i < n && ok; ++i) {
+          ok = full(Q + i);
+          if (ok) mmas(Q + i, 0, 0, false);
+        }
+        if (!ok) break;
+        if (l > 0) commit_all(&sh.tfull[0]);
+        for (int i = n - l; i < n; ++i) {
+          mmas(Q + i, 1, 1, false);
+          commit_all(&sh.empty[(Q + i) % S]);
+        }
+        commit_all(&sh.tfull[1]);
+        Q += n;
       }
     }
     if (!ok) {
@@ -434,12 +514,13 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
     // ================================ epilogue ================================
     constexpr int W = NT >= 64 ? 32 : 8;  // rows of one TMEM load
     const int q = warp & 3, g = (warp - 2) >> 2;
-    uint32_t T = 0;
-    for (int t = t0; t < p.tiles; t += step, ++T) {
+    // U: half tiles of FM = 2, tiles otherwise
+    for (int U = 0, t; (t = tile(U / FM)) >= 0; ++U) {
       int r0, c0;
       const Problem& pr = locate(t, r0, c0);
+      c0 += 128 * CG * (U % FM);
       const Epilogue e = pr.epi;
-      const int buf = T % C::NBUF;
+      const int buf = U % C::NBUF;
       const int col = 32 * q + lane;
       const bool in = c0 + col < pr.cols;
       const long long c = c0 + col;
@@ -448,7 +529,7 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
       const bool has_res = !SPLIT && e.res && in;
       uint32_t raw[W];
       if (has_res && r0 + g * W < pr.rows) load_residual<W>(e, raw, r0 + g * W, 1, pr.rows - r0 - g * W, c);
-      if (!bwait(&sh.tfull[buf], (T / C::NBUF) & 1, p, sh, DEV_WAIT_TIMEOUT_TMEM)) break;
+      if (!bwait(&sh.tfull[buf], (U / C::NBUF) & 1, p, sh, DEV_WAIT_TIMEOUT_TMEM)) break;
       tc::fence_after_sync();
       const uint32_t ta = tbase + ((uint32_t)(32 * q) << 16) + (uint32_t)buf * NT;
       if constexpr (SPLIT) {
@@ -500,7 +581,7 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
   if constexpr (SPLIT) {
     cluster_sync();  // every rank's rows have arrived
     int r0, c0;
-    const Problem& pr = locate(t0, r0, c0);
+    const Problem& pr = locate(gi, r0, c0);
     const Epilogue e = pr.epi;  // in registers: a field of an indexed kernel parameter costs 80 cycles a use
     if (tid < 256 && !sh.abort) {
       const int col = tid & 127;
@@ -532,19 +613,22 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
 namespace {
 
 struct Variant {
-  int cg, nt, stages;
+  int cg, fm, nt, stages;
   bool split;
   const void* fn;
   int smem;
 };
-template <int CG, int NT, int S, bool SPLIT>
+template <int CG, int FM, int NT, int S, bool SPLIT>
 Variant variant() {
-  return {CG, NT, S, SPLIT, reinterpret_cast<const void*>(&lin_gemm<CG, NT, S, SPLIT>), Cfg<CG, NT, S, SPLIT>::SMEM};
+  return {CG, FM, NT, S, SPLIT, reinterpret_cast<const void*>(&lin_gemm<CG, FM, NT, S, SPLIT>),
+          Cfg<CG, FM, NT, S, SPLIT>::SMEM};
 }
 const Variant* variants(int* n) {
-  static const Variant v[] = {variant<2, 256, 6, false>(), variant<1, 128, 6, false>(), variant<1, 64, 8, false>(),
-                              variant<1, 32, 8, false>(),  variant<1, 16, 8, false>(),  variant<1, 128, 4, true>(),
-                              variant<1, 64, 7, true>(),   variant<1, 32, 8, true>(),   variant<1, 16, 8, true>()};
+  static const Variant v[] = {
+      variant<2, 2, 256, 4, false>(), variant<2, 1, 256, 6, false>(), variant<1, 1, 128, 6, false>(),
+      variant<1, 1, 64, 8, false>(),  variant<1, 1, 32, 8, false>(),  variant<1, 1, 16, 8, false>(),
+      variant<1, 1, 128, 4, true>(),  variant<1, 1, 64, 7, true>(),   variant<1, 1, 32, 8, true>(),
+      variant<1, 1, 16, 8, true>()};
   *n = (int)(sizeof v / sizeof v[0]);
   return v;
 }
@@ -586,12 +670,16 @@ int g_clusters[64][4];
 // 64 at 4096 MAC per clock and SM) or the time a stage takes to arrive at an
 // SM (37 bytes a clock measured with every SM loading, from L2 or memory: the
 // widest tile is bound by this); for the whole: its bytes at the memory's
-// rate (3300 a clock).  Per tile an epilogue that two accumulators hide but for the last;
-// for a split, two cluster barriers and the sum.
+// rate (3300 a clock).  A tile's epilogue takes 8500 clocks per 256 rows of a
+// CTA's 128 columns (measured without residual or activation; they add about
+// 4000 and 3000); a second accumulator hides it behind the next tile, or half
+// of it where both belong to one tile.  A split adds its barrier and sum.
 Choice choose(const Product* pr, int n, int sms, int dev) {
   int nv;
   const Variant* vs = variants(&nv);
-  double bytes = 0;
+  double bytes = 0, epi = 0;
+  for (int j = 0; j < n; ++j)
+    epi = std::max(epi, 8500.0 + (pr[j].epi.act != APK_ACT_NONE ? 3000 : 0) + (pr[j].epi.res ? 4000 : 0));
   for (int j = 0; j < n; ++j)
     bytes += 2.0 * ((double)pr[j].rows * pr[j].k + (double)pr[j].cols * pr[j].k + (double)pr[j].rows * pr[j].cols);
   Choice best{nullptr, 1, 0};
@@ -600,7 +688,7 @@ Choice choose(const Product* pr, int n, int sms, int dev) {
     bool fits = true;
     for (int j = 0; j < n; ++j) fits = fits && !(pr[j].Q.mn && v.nt < 64);
     if (!fits) continue;
-    const double per_kb = std::max(v.nt * 2.0, (P_BYTES + v.nt / v.cg * 128) / 37.0);
+    const double per_kb = std::max(v.nt * 2.0 * v.fm, (v.fm * P_BYTES + v.nt / v.cg * 128) / 37.0);
     for (int lg = v.split ? 1 : 0; lg <= (v.split ? 3 : 0); ++lg) {
       const int sp = 1 << lg, per = v.cg * sp;
       int slots = std::max(1, sms / per);
@@ -608,16 +696,18 @@ Choice choose(const Product* pr, int n, int sms, int dev) {
       long long tiles = 0;
       double work = 0, longest = 0;
       for (int j = 0; j < n; ++j) {
-        const long long t = (long long)ceil_div(pr[j].rows, v.nt) * ceil_div(pr[j].cols, 128 * v.cg);
-        const double one = ceil_div(ceil_div(pr[j].k, BK), sp) * per_kb + (v.nt >= 128 ? 300 : 150);
+        const long long t = (long long)ceil_div(pr[j].rows, v.nt) * ceil_div(pr[j].cols, 128 * v.cg * v.fm);
+        const double mma = ceil_div(ceil_div(pr[j].k, BK), sp) * per_kb, drain = epi * v.nt / 256;
+        const double one = v.fm == 2 ? mma + 1.5 * drain : v.split ? mma : std::max(mma, drain) + 150;
         tiles += t;
         work += t * one;
         longest = std::max(longest, one);
       }
       if (v.split && tiles > slots) continue;  // one tile per cluster, all resident
-      const double waves = (double)((tiles + slots - 1) / slots) * slots / tiles;  // rounding up to whole sweeps
-      double cost = 2500 + std::max(bytes / 3300, tiles <= slots ? longest : std::max(longest, work / slots * waves));
-      cost += v.nt * 6.0;
+      // one product runs in whole sweeps; two are dealt out evenly but for half a tile
+      const double sweeps = n == 1 ? (double)((tiles + slots - 1) / slots) * longest : work / slots + longest / 2;
+      double cost = 6000 + std::max(bytes / 3300, std::max(longest, sweeps));
+      if (v.fm == 1) cost += v.nt * 20.0;  // the last tile's epilogue
       if (v.split) cost += 1500 + v.nt / sp * 6.0;
       if (!best.v || cost < best.cost) best = {&v, sp, cost};
     }
@@ -667,6 +757,12 @@ cudaError_t prepare() {
 
 apk_status run_products(const Product* pr, int n, int sms, int dev, int* status, long long limit, cudaStream_t stream,
                         std::string* why) {
+  Product longer_first[2];
+  if (n == 2 && pr[0].k < pr[1].k) {
+    longer_first[0] = pr[1];
+    longer_first[1] = pr[0];
+    pr = longer_first;
+  }
   const Choice ch = choose(pr, n, sms, dev);
   if (n == 2) {
     // products that want different tiles run one after the other
@@ -682,6 +778,7 @@ apk_status run_products(const Product* pr, int n, int sms, int dev, int* status,
   p.tiles = 0;
   p.tiles0 = 0;
   p.split = ch.split;
+  p.extra = n == 2 && !v.split ? ceil_div(pr[0].k, BK) / ceil_div(pr[1].k, BK) : 0;
   p.status = status;
   p.limit = limit;
   for (int j = 0; j < n; ++j) {
@@ -691,7 +788,7 @@ apk_status run_products(const Product* pr, int n, int sms, int dev, int* status,
     q.cols = pr[j].cols;
     q.nkb = ceil_div(pr[j].k, BK);
     q.tiles_r = ceil_div(q.rows, v.nt);
-    q.tiles_c = ceil_div(q.cols, 128 * v.cg);
+    q.tiles_c = ceil_div(q.cols, 128 * v.cg * v.fm);
     q.p_mn = pr[j].P.mn;
     q.q_mn = pr[j].Q.mn;
     q.idesc = tc::idesc_bf16_f32(128 * v.cg, v.nt, q.p_mn, q.q_mn);
