@@ -30,6 +30,12 @@
 // cluster barrier the owners sum them in rank order and finish.  Nothing goes
 // through global memory, and the order of the sum is fixed.
 //
+// EXACT: for fp32 results of long sums.  The tensor core adds each product of
+// 16 k to the accumulator with truncation, a bias of about 1e-9 k of the
+// result (1e-6 at 1024 k, 9e-6 at 8192); an fp32 result would show it, a bf16
+// one does not.  So K is taken 512 at a time in alternating accumulators, and
+// the epilogue warps add the pieces in registers with rounding.
+//
 // Every wait is bounded; one that runs out raises the status word and lets
 // every role unwind.
 #include <cudaTypedefs.h>
@@ -51,6 +57,7 @@ constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 32 * (2 + EPI_WARPS);
 constexpr int P_BYTES = 128 * BK * 2;
 constexpr int RASTER_GROUP = 8;
+constexpr int EXACT_KB = 8;  // k-blocks of one accumulator under EXACT
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -201,8 +208,9 @@ __device__ __forceinline__ void finish_part(const Epilogue& e, const uint32_t (&
     }
   }
 }
-// min(n, W) rows r, r + step, ... of column c; raw: their residual's bits, if any.
-template <int W>
+// min(n, W) rows r, r + step, ... of column c; raw: their residual's bits, if
+// any.  SMALL: only the code with run-time flags (where it is inlined often).
+template <int W, bool SMALL = false>
 __device__ __forceinline__ void finish(const Epilogue& e, const uint32_t (&v)[W], const uint32_t (&raw)[W], float bias,
                                        int r, int step, int n, long long c) {
   const int es = e.out_f32 ? 4 : 2, shift = e.res_f32 ? 0 : 16;
@@ -217,7 +225,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, const uint32_t (&v)[W]
     };
     const std::true_type yes;
     const std::false_type no;
-    if (n < W) finish_part<ACT, W>(e, v, raw, shift, bias, out, pre, so, sp, n);
+    if (SMALL || n < W) finish_part<ACT, W>(e, v, raw, shift, bias, out, pre, so, sp, n);
     else if (e.res) e.out_f32 ? (e.pre ? full(yes, yes, yes) : full(no, yes, yes))
                               : (e.pre ? full(yes, no, yes) : full(no, no, yes));
     else e.out_f32 ? (e.pre ? full(yes, yes, no) : full(no, yes, no)) : (e.pre ? full(yes, no, no) : full(no, no, no));
@@ -277,17 +285,17 @@ __device__ __forceinline__ void sum_ranks(const Epilogue& e, uint32_t part, int 
   }
 }
 
-template <int CG, int FM, int NT, int S, bool SPLIT>
+template <int CG, int FM, int NT, int S, bool SPLIT, bool EXACT>
 struct Cfg {
   static constexpr int QROWS = NT / CG;
   static constexpr int Q_BYTES = QROWS * BK * 2;
   static constexpr int Q_AT = FM * P_BYTES;
   static constexpr int STAGE = Q_AT + Q_BYTES;
   static constexpr int COLS = 128 * CG * FM;  // of a tile
-  static constexpr int NBUF = SPLIT ? 1 : 2;
+  static constexpr int NBUF = SPLIT && !EXACT ? 1 : 2;
   static constexpr int TMEM_COLS = NBUF * NT < 32 ? 32 : NBUF * NT;
   static constexpr int SMEM = S * STAGE + (SPLIT ? NT * 512 : 0) + 1024;
-  static_assert(FM == 1 || (CG == 2 && !SPLIT), "");
+  static_assert(FM == 1 || (CG == 2 && !SPLIT && !EXACT), "");
   static_assert((TMEM_COLS & (TMEM_COLS - 1)) == 0 && TMEM_COLS <= 512, "");
 };
 
@@ -313,9 +321,9 @@ __device__ __forceinline__ int tile_of(const GemmParams& p, int g, int G, int q)
   return j < n1 ? n0 + j : -1;
 }
 
-template <int CG, int FM, int NT, int S, bool SPLIT>
+template <int CG, int FM, int NT, int S, bool SPLIT, bool EXACT>
 __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ GemmParams p) {
-  using C = Cfg<CG, FM, NT, S, SPLIT>;
+  using C = Cfg<CG, FM, NT, S, SPLIT, EXACT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ Shared<S> sh;
@@ -379,6 +387,9 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
     ke = SPLIT ? pr.nkb * (krank + 1) / p.split : pr.nkb;
   };
 
+  // accumulators that a tile's n k-blocks are spread over
+  auto pieces = [](int n) { return EXACT ? max(1, (n + EXACT_KB - 1) / EXACT_KB) : 1; };
+
   if (warp == 0 && lane == 0) {
     // ================================ producer ================================
     uint32_t P = 0;
@@ -425,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
     }
   } else if (warp == 1 && lane == 0 && leader) {
     // =================================== MMA ===================================
-    uint32_t Q = 0;
+    uint32_t Q = 0, U = 0;  // stages and accumulators used
     bool ok = true;
     // an arrival in every CTA of the pair once the MMAs issued so far are done
     auto commit_all = [&](uint64_t* bar) {
@@ -455,18 +466,19 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
       };
       const int n = ke - kb;
       if constexpr (FM == 1) {
-        const int buf = T % C::NBUF;
-        ok = bwait(&sh.tempty[buf], ((T / C::NBUF) & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
-        if (!ok) break;
-        tc::fence_after_sync();
-        for (int i = 0; i < n; ++i, ++Q) {
-          ok = full(Q);
+        for (int c = 0; c < pieces(n) && ok; ++c, ++U) {
+          const int buf = U % C::NBUF, i0 = EXACT ? c * EXACT_KB : 0, i1 = EXACT ? min(n, i0 + EXACT_KB) : n;
+          ok = bwait(&sh.tempty[buf], ((U / C::NBUF) & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
           if (!ok) break;
-          mmas(Q, 0, buf, i == 0);
-          commit_all(&sh.empty[Q % S]);
+          tc::fence_after_sync();
+          for (int i = i0; i < i1; ++i, ++Q) {
+            ok = full(Q);
+            if (!ok) break;
+            mmas(Q, 0, buf, i == i0);
+            commit_all(&sh.empty[Q % S]);
+          }
+          if (ok) commit_all(&sh.tfull[buf]);
         }
-        if (!ok) break;
-        commit_all(&sh.tfull[buf]);
       } else {
         // stages i = 0 .. w: accumulator 0 first; n - l .. n: 0 before 1
         const int w = n < S - 1 ? n : S - 1, l = n - w < S - 1 ? n - w : S - 1;
@@ -514,13 +526,14 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
     // ================================ epilogue ================================
     constexpr int W = NT >= 64 ? 32 : 8;  // rows of one TMEM load
     const int q = warp & 3, g = (warp - 2) >> 2;
-    // U: half tiles of FM = 2, tiles otherwise
-    for (int U = 0, t; (t = tile(U / FM)) >= 0; ++U) {
-      int r0, c0;
+    // i: tiles, or half tiles of FM = 2; U: accumulators drained
+    uint32_t U = 0;
+    for (int i = 0, t; (t = tile(i / FM)) >= 0; ++i) {
+      int r0, c0, kb, ke;
       const Problem& pr = locate(t, r0, c0);
-      c0 += 128 * CG * (U % FM);
+      k_range(pr, kb, ke);
+      c0 += 128 * CG * (i % FM);
       const Epilogue e = pr.epi;
-      const int buf = U % C::NBUF;
       const int col = 32 * q + lane;
       const bool in = c0 + col < pr.cols;
       const long long c = c0 + col;
@@ -529,50 +542,87 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
       const bool has_res = !SPLIT && e.res && in;
       uint32_t raw[W];
       if (has_res && r0 + g * W < pr.rows) load_residual<W>(e, raw, r0 + g * W, 1, pr.rows - r0 - g * W, c);
-      if (!bwait(&sh.tfull[buf], (U / C::NBUF) & 1, p, sh, DEV_WAIT_TIMEOUT_TMEM)) break;
-      tc::fence_after_sync();
-      const uint32_t ta = tbase + ((uint32_t)(32 * q) << 16) + (uint32_t)buf * NT;
-      if constexpr (SPLIT) {
-        // rows to their owners; a CTA whose share of K is empty sends zeros
-        int kb, ke;
-        k_range(pr, kb, ke);
+      const uint32_t tcol = tbase + ((uint32_t)(32 * q) << 16);
+      auto wait_acc = [&]() {
+        const bool ok = bwait(&sh.tfull[U % C::NBUF], (U / C::NBUF) & 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
+        tc::fence_after_sync();
+        return ok;
+      };
+      auto free_acc = [&]() {
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 2) arrive_cluster(map_rank(smem_u32(&sh.tempty[U % C::NBUF]), 0));
+          else mbar_arrive(&sh.tempty[U % C::NBUF]);
+        }
+        ++U;
+      };
+      // a split tile's rows to their owners; a CTA whose share of K is empty sends zeros
+      auto push = [&](int b, const uint32_t(&v)[W]) {
         const uint32_t at = smem_u32(ring + S * C::STAGE) + (uint32_t)(krank * (NT / p.split) * 512 + col * 4);
-#pragma unroll 1
-        for (int b = g; b < NT / W; b += 2) {
-          uint32_t v[W];
-          tc::ld_32x32b<W>(ta + b * W, v);
-          tc::wait_ld();
 #pragma unroll
-          for (int i = 0; i < W; ++i) {
-            const int row = b * W + i;
-            st_cluster_f32(map_rank(at, row & (p.split - 1)) + (row / p.split) * 512, kb < ke ? v[i] : 0u);
+        for (int k = 0; k < W; ++k) {
+          const int row = b * W + k;
+          st_cluster_f32(map_rank(at, row & (p.split - 1)) + (row / p.split) * 512, kb < ke ? v[k] : 0u);
+        }
+      };
+      if constexpr (EXACT) {
+        constexpr int NB = NT / W / 2;  // this warp's blocks
+        uint32_t acc[NB][W] = {};
+        bool ok = true;
+        for (int k = pieces(ke - kb); k > 0; --k) {
+          ok = wait_acc();
+          if (!ok) break;
+          const uint32_t ta = tcol + (U % C::NBUF) * NT;
+#pragma unroll
+          for (int j = 0; j < NB; ++j) {
+            uint32_t v[W];
+            tc::ld_32x32b<W>(ta + (g + 2 * j) * W, v);
+            tc::wait_ld();
+#pragma unroll
+            for (int x = 0; x < W; ++x) acc[j][x] = __float_as_uint(__uint_as_float(acc[j][x]) + __uint_as_float(v[x]));
+          }
+          free_acc();
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const int b = g + 2 * j, r = r0 + b * W, n = pr.rows - r;
+          if constexpr (SPLIT) {
+            push(b, acc[j]);
+          } else if (in && n > 0) {
+            if (has_res && j > 0) load_residual<W>(e, raw, r, 1, n, c);
+            finish<W, true>(e, acc[j], raw, bias, r, 1, n, c);
           }
         }
-      } else {
+        continue;
+      }
+      if (!wait_acc()) break;
+      const uint32_t ta = tcol + (U % C::NBUF) * NT;
 #pragma unroll 1
-        for (int b = g; b < NT / W; b += 2) {
-          const int r = r0 + b * W;
-          if (r >= pr.rows) break;  // (uniform; later blocks lie further out)
-          uint32_t v[W];
+      for (int b = g; b < NT / W; b += 2) {
+        const int r = r0 + b * W, n = pr.rows - r;
+        uint32_t v[W];
+        if constexpr (SPLIT) {
           tc::ld_32x32b<W>(ta + b * W, v);
-          const int n = pr.rows - r;
+          tc::wait_ld();
+          push(b, v);
+        } else {
+          if (n <= 0) break;  // (uniform; later blocks lie further out)
+          tc::ld_32x32b<W>(ta + b * W, v);
           uint32_t res[W];
           if (e.res) {
 #pragma unroll
-            for (int i = 0; i < W; ++i) res[i] = raw[i];
+            for (int k = 0; k < W; ++k) res[k] = raw[k];
           }
           if (has_res && b + 2 < NT / W && n > 2 * W) load_residual<W>(e, raw, r + 2 * W, 1, n - 2 * W, c);
           tc::wait_ld();
           if (in) finish<W>(e, v, res, bias, r, 1, n, c);
           __syncwarp();
         }
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (CG == 2) arrive_cluster(map_rank(smem_u32(&sh.tempty[buf]), 0));
-          else mbar_arrive(&sh.tempty[buf]);
-        }
       }
+      if constexpr (SPLIT) break;  // one tile a cluster
+      free_acc();
     }
   }
 
@@ -614,21 +664,22 @@ namespace {
 
 struct Variant {
   int cg, fm, nt, stages;
-  bool split;
+  bool split, exact;
   const void* fn;
   int smem;
 };
-template <int CG, int FM, int NT, int S, bool SPLIT>
+template <int CG, int FM, int NT, int S, bool SPLIT, bool EXACT = false>
 Variant variant() {
-  return {CG, FM, NT, S, SPLIT, reinterpret_cast<const void*>(&lin_gemm<CG, FM, NT, S, SPLIT>),
-          Cfg<CG, FM, NT, S, SPLIT>::SMEM};
+  return {CG,    FM, NT, S, SPLIT, EXACT, reinterpret_cast<const void*>(&lin_gemm<CG, FM, NT, S, SPLIT, EXACT>),
+          Cfg<CG, FM, NT, S, SPLIT, EXACT>::SMEM};
 }
 const Variant* variants(int* n) {
   static const Variant v[] = {
       variant<2, 2, 256, 4, false>(), variant<2, 1, 256, 6, false>(), variant<1, 1, 128, 6, false>(),
       variant<1, 1, 64, 8, false>(),  variant<1, 1, 32, 8, false>(),  variant<1, 1, 16, 8, false>(),
       variant<1, 1, 128, 4, true>(),  variant<1, 1, 64, 7, true>(),   variant<1, 1, 32, 8, true>(),
-      variant<1, 1, 16, 8, true>()};
+      variant<1, 1, 16, 8, true>(),   variant<2, 1, 128, 8, false, true>(), variant<1, 1, 64, 8, false, true>(),
+      variant<1, 1, 64, 7, true, true>()};
   *n = (int)(sizeof v / sizeof v[0]);
   return v;
 }
@@ -682,10 +733,12 @@ Choice choose(const Product* pr, int n, int sms, int dev) {
     epi = std::max(epi, 8500.0 + (pr[j].epi.act != APK_ACT_NONE ? 3000 : 0) + (pr[j].epi.res ? 4000 : 0));
   for (int j = 0; j < n; ++j)
     bytes += 2.0 * ((double)pr[j].rows * pr[j].k + (double)pr[j].cols * pr[j].k + (double)pr[j].rows * pr[j].cols);
+  bool exact = false;  // a long sum that is not rounded to bf16
+  for (int j = 0; j < n; ++j) exact = exact || (pr[j].epi.out_f32 && pr[j].k > EXACT_KB * BK);
   Choice best{nullptr, 1, 0};
   for (int i = 0; i < nv; ++i) {
     const Variant& v = vs[i];
-    bool fits = true;
+    bool fits = v.exact == exact;
     for (int j = 0; j < n; ++j) fits = fits && !(pr[j].Q.mn && v.nt < 64);
     if (!fits) continue;
     const double per_kb = std::max(v.nt * 2.0 * v.fm, (v.fm * P_BYTES + v.nt / v.cg * 128) / 37.0);

@@ -48,6 +48,21 @@ __device__ __forceinline__ void st_epi(void* p, long long i, float v, int f32) {
   }
 }
 
+// The tensor core truncates as it adds, a bias that grows with the length of
+// the chain (1e-6 of the result at 1024 k): every FLUSH k a warp adds its sum
+// to a total with rounding.
+constexpr int FLUSH = 512;
+template <int N>
+__device__ __forceinline__ void flush(float (&acc)[N][4], float (&total)[N][4]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      total[i][j] += acc[i][j];
+      acc[i][j] = 0.f;
+    }
+}
+
 template <bool NK, int NT8, bool VEC>
 __global__ void __launch_bounds__(32 * WARPS, NK ? (NT8 == 1 && VEC ? 4 : 3) : 2) lin_stream(const __grid_constant__ StreamParams p) {
   constexpr int FT = FEATURES<NK>, KC = CHUNK<NK>, TOK = 8 * NT8;
@@ -62,7 +77,8 @@ __global__ void __launch_bounds__(32 * WARPS, NK ? (NT8 == 1 && VEC ? 4 : 3) : 2
   for (int i = 0; i < NT8; ++i) xr[i] = p.x + min(8 * i + g, p.rows - 1) * p.ldx;
 
   if constexpr (NK) {
-    float acc[NT8][4] = {};
+    float acc[NT8][4] = {}, total[NT8][4] = {};
+    int round = 0;
     const uint16_t* w0 = p.w + min(f0 + g, p.n - 1) * p.ldw;
     const uint16_t* w1 = p.w + min(f0 + g + 8, p.n - 1) * p.ldw;
 #pragma unroll 1
@@ -92,13 +108,16 @@ __global__ void __launch_bounds__(32 * WARPS, NK ? (NT8 == 1 && VEC ? 4 : 3) : 2
           stream::mma_bf16(acc[i], a[u].x, b[u].x, a[u].y, b[u].y, c[i][u].x, c[i][u].y);
           stream::mma_bf16(acc[i], a[u].z, b[u].z, a[u].w, b[u].w, c[i][u].z, c[i][u].w);
         }
+      if ((++round & (FLUSH / KC - 1)) == 0) flush(acc, total);
     }
+    flush(acc, total);
 #pragma unroll
     for (int i = 0; i < NT8; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) part[warp][8 * i + 2 * t + (j & 1)][g + 8 * (j >> 1)] = acc[i][j];
+      for (int j = 0; j < 4; ++j) part[warp][8 * i + 2 * t + (j & 1)][g + 8 * (j >> 1)] = total[i][j];
   } else {
-    float acc[4][NT8][4] = {};
+    float acc[4][NT8][4] = {}, total[4][NT8][4] = {};
+    int round = 0;
     const int f = f0 + 8 * g;
     const uint16_t* w = p.w + (VEC ? min(f, p.n - 8) : f);
 #pragma unroll 1
@@ -138,7 +157,12 @@ __global__ void __launch_bounds__(32 * WARPS, NK ? (NT8 == 1 && VEC ? 4 : 3) : 2
           }
         }
       }
+      if ((++round & (FLUSH / KC - 1)) == 0)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) flush(acc[m], total[m]);
     }
+#pragma unroll
+    for (int m = 0; m < 4; ++m) flush(acc[m], total[m]);
     // MMA m's rows g and g + 8 are the features 8g + 2m and 8g + 2m + 1
 #pragma unroll
     for (int m = 0; m < 4; ++m)
@@ -146,7 +170,7 @@ __global__ void __launch_bounds__(32 * WARPS, NK ? (NT8 == 1 && VEC ? 4 : 3) : 2
       for (int i = 0; i < NT8; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          part[warp][8 * i + 2 * t + (j & 1)][8 * g + 2 * m + (j >> 1)] = acc[m][i][j];
+          part[warp][8 * i + 2 * t + (j & 1)][8 * g + 2 * m + (j >> 1)] = total[m][i][j];
   }
   __syncthreads();
   if (p.split > 1)

@@ -20,6 +20,7 @@ _ACT = {"none": L.APK_ACT_NONE, "relu": L.APK_ACT_RELU, "gelu": L.APK_ACT_GELU,
 _LAYOUT = {"kn": L.APK_W_KN, "nk": L.APK_W_NK}
 _TORCH = {"f32": torch.float32, "bf16": torch.bfloat16}
 _CODE = {torch.float32: L.APK_F32, torch.bfloat16: L.APK_BF16}
+_ANY = tuple(_CODE)
 # the current stream's handle; building a torch.cuda.Stream for it costs 2 us a call
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
@@ -47,16 +48,32 @@ def _tensor(t, what, device=None, dtypes=(torch.bfloat16,), dim=None):
 
 
 def _rows(t, what, device, width, dtypes=(torch.bfloat16,)):
-    """(2-D view, row stride) of a [..., width] tensor; the last axis has to be contiguous."""
+    """(address, rows, row stride) of a [..., width] tensor whose last axis is
+    contiguous.  Called for every operand of every call: the usual case first."""
+    try:
+        shape = t.shape
+        if len(shape) == 2 and shape[1] == width and t.dtype in dtypes and t.device == device:
+            s0, s1 = t.stride()
+            if s1 == 1 or width == 1:
+                m = shape[0]
+                return t.data_ptr(), m, (s0 if m > 1 else width)
+    except (AttributeError, TypeError):
+        pass
     _tensor(t, what, device, dtypes)
     if t.dim() < 1 or t.shape[-1] != width:
         raise ValueError(f"{what} is {tuple(t.shape)}: its last axis has to be {width}")
-    if t.dim() != 2:
-        t = t.reshape(-1, width)
-    s0, s1 = t.stride()
-    if s1 != 1 and width > 1:
-        raise ValueError(f"{what}: its last axis has stride {s1}, not 1")
-    return t, (s0 if t.shape[0] > 1 else width)
+    if width > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: its last axis has stride {t.stride(-1)}, not 1")
+    try:
+        v = t.view(-1, width) if t.numel() else t.new_empty((t.numel() // width, width))
+    except RuntimeError:
+        raise ValueError(f"{what}: its leading axes, of strides {t.stride()}, are not rows of one stride") from None
+    return v.data_ptr(), v.shape[0], (v.stride(0) if v.shape[0] > 1 else width)
+
+
+def _like(t, shape):
+    """A new tensor of t's type and device; of t's own shape the cheaper way."""
+    return torch.empty_like(t) if t.shape == shape and t.is_contiguous() else t.new_empty(shape)
 
 
 class _Handle:
@@ -86,7 +103,7 @@ class _Handle:
         return st.value
 
     def _stream(self):
-        return _raw_stream(self.device.index)
+        return _raw_stream(self._index)
 
     def close(self):
         if getattr(self, "_h", None) is not None and self._h.value:
@@ -120,9 +137,9 @@ class Linear(_Handle):
                  sms: int = 0, wait_limit_ns: int = _DEFAULT_WAIT_NS):
         _tensor(weight, "weight", dim=2)
         kn = _pick(_LAYOUT, layout, "layout") == L.APK_W_KN
-        self.device = weight.device
+        self.device, self._index = weight.device, weight.device.index
         self.in_features, self.out_features = weight.shape if kn else weight.shape[::-1]
-        w, ldw = _rows(weight, "weight", self.device, weight.shape[1])
+        w, _, ldw = _rows(weight, "weight", self.device, weight.shape[1])
         if bias is not None:
             _tensor(bias, "bias", self.device, tuple(_CODE), 1)
             if bias.shape[0] != self.out_features or (bias.shape[0] > 1 and bias.stride(0) != 1):
@@ -130,9 +147,10 @@ class Linear(_Handle):
                                  f"{self.out_features} contiguous values are wanted")
         self.weight, self.bias, self.act, self.layout = weight, bias, act, layout
         self.out_dtype = _pick(_TORCH, out_dtype, "out_dtype")
+        self._y_code = _CODE[self.out_dtype]
         self._act = _pick(_ACT, act, "act")
         self._open(L.LinearConfig(self.device.index, self.in_features, self.out_features, _LAYOUT[layout], self._act,
-                                  _CODE[bias.dtype] if bias is not None else L.APK_F32, w.data_ptr(), ldw,
+                                  _CODE[bias.dtype] if bias is not None else L.APK_F32, w, ldw,
                                   bias.data_ptr() if bias is not None else None, sms, wait_limit_ns))
         self._io, self._grads = L.LinearIO(), L.LinearGrads()
         self._io_ref, self._grads_ref = ctypes.byref(self._io), ctypes.byref(self._grads)
@@ -142,34 +160,30 @@ class Linear(_Handle):
         x W + b in bf16, as backward() takes it.  out: the output's tensor;
         it may be the residual."""
         io, n = self._io, self.out_features
-        x2, io.ldx = _rows(x, "x", self.device, self.in_features)
-        m = x2.shape[0]
-        shape = (*x.shape[:-1], n)
+        io.x, io.rows, io.ldx = _rows(x, "x", self.device, self.in_features)
+        shape = (io.rows, n) if len(x.shape) == 2 else (*x.shape[:-1], n)
         if out is None:
-            y = torch.empty(shape, dtype=self.out_dtype, device=self.device)
-            y_ptr, io.ldy = y.data_ptr(), n
+            y = x.new_empty(shape) if self._y_code == L.APK_BF16 else x.new_empty(shape, dtype=self.out_dtype)
+            io.y, io.ldy = y.data_ptr(), n
         else:
             y = out
             if y.shape != shape:
                 raise ValueError(f"out is {tuple(y.shape)}, not {shape}")
-            y2, io.ldy = _rows(y, "out", self.device, n, (self.out_dtype,))
-            y_ptr = y2.data_ptr()
-            if y_ptr != y.data_ptr():
-                raise ValueError("out cannot be written as rows of one stride")
+            io.y, _, io.ldy = _rows(y, "out", self.device, n, (self.out_dtype,))
         if residual is None:
             io.residual = None
         else:
             if residual.shape != shape:
                 raise ValueError(f"residual is {tuple(residual.shape)}, not {shape}")
-            r2, io.ld_residual = _rows(residual, "residual", self.device, n, tuple(_CODE))
-            io.residual, io.residual_dtype = r2.data_ptr(), _CODE[residual.dtype]
+            io.residual, _, io.ld_residual = _rows(residual, "residual", self.device, n, _ANY)
+            io.residual_dtype = _CODE[residual.dtype]
         z = None
         if save_preact:
-            z = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            z = x.new_empty(shape)
             io.preact, io.ld_preact = z.data_ptr(), n
         else:
             io.preact = None
-        io.x, io.y, io.rows, io.y_dtype, io.stream = x2.data_ptr(), y_ptr, m, _CODE[self.out_dtype], self._stream()
+        io.y_dtype, io.stream = self._y_code, self._stream()
         st = self._lib.apk_linear_forward(self._h, self._io_ref)
         if st:
             self._check(st)
@@ -184,36 +198,30 @@ class Linear(_Handle):
         preact: what forward(save_preact=True) returned, for a layer with an
         activation."""
         g, n, k = self._grads, self.out_features, self.in_features
-        dy2, g.ld_dy = _rows(dy, "dy", self.device, n)
-        m = dy2.shape[0]
+        g.dy, g.rows, g.ld_dy = _rows(dy, "dy", self.device, n)
         if dy.shape[:-1] != x.shape[:-1]:
             raise ValueError(f"dy is {tuple(dy.shape)} and x {tuple(x.shape)}")
-        x2, g.ldx = _rows(x, "x", self.device, k)
+        g.x, _, g.ldx = _rows(x, "x", self.device, k)
         if self._act != L.APK_ACT_NONE:
             if preact is None or preact.shape != dy.shape:
                 raise ValueError("preact: the pre-activation that forward(save_preact=True) returned is wanted")
-            z2, g.ld_preact = _rows(preact, "preact", self.device, n)
-            g.preact = z2.data_ptr()
+            g.preact, _, g.ld_preact = _rows(preact, "preact", self.device, n)
         else:
             g.preact = None
+        g.dx = g.dw = g.db = None
         dx = dw = db = None
         if need_dx:
-            dx = torch.empty(x.shape, dtype=torch.bfloat16, device=self.device)
+            dx = _like(x, x.shape)
             g.dx, g.ld_dx = dx.data_ptr(), k
-        else:
-            g.dx = None
         if need_dw:
             dt = _pick(_TORCH, dw_dtype, "dw_dtype")
-            dw = torch.empty(self.weight.shape, dtype=dt, device=self.device)
-            g.dw, g.ld_dw, g.dw_dtype = dw.data_ptr(), self.weight.shape[1], _CODE[dt]
-        else:
-            g.dw = None
+            shape = self.weight.shape
+            dw = _like(self.weight, shape) if dt is torch.bfloat16 else self.weight.new_empty(shape, dtype=dt)
+            g.dw, g.ld_dw, g.dw_dtype = dw.data_ptr(), shape[1], _CODE[dt]
         if need_db and self.bias is not None:
             db = torch.empty_like(self.bias)
             g.db = db.data_ptr()
-        else:
-            g.db = None
-        g.dy, g.x, g.rows, g.stream = dy2.data_ptr(), x2.data_ptr(), m, self._stream()
+        g.stream = self._stream()
         if dx is not None or dw is not None or db is not None:
             st = self._lib.apk_linear_backward(self._h, self._grads_ref)
             if st:
@@ -235,7 +243,7 @@ class MoE(_Handle):
                  renormalize: bool = True, out_dtype: str = "bf16", sms: int = 0,
                  wait_limit_ns: int = _DEFAULT_WAIT_NS):
         _tensor(router, "router", dim=2)
-        self.device = router.device
+        self.device, self._index = router.device, router.device.index
         self.experts, self.d_model = router.shape
         _tensor(w_in, "w_in", self.device, dim=3)
         _tensor(w_out, "w_out", self.device, dim=3)
@@ -249,6 +257,7 @@ class MoE(_Handle):
                 raise ValueError(f"{what} is not contiguous")
         self.router, self.w_in, self.w_out, self.top_k = router, w_in, w_out, top_k
         self.out_dtype = _pick(_TORCH, out_dtype, "out_dtype")
+        self._y_code = _CODE[self.out_dtype]
         self._open(L.MoeConfig(self.device.index, self.experts, top_k, self.d_model, self.d_ff, _pick(_ACT, act, "act"),
                                int(gated), int(renormalize), router.data_ptr(), w_in.data_ptr(), w_out.data_ptr(),
                                sms, wait_limit_ns))
@@ -259,18 +268,17 @@ class MoE(_Handle):
         """The layer's output for x [..., D]; with return_routing also the
         chosen experts (int32 [..., top_k]) and their weights (fp32)."""
         io = self._io
-        x2, io.ldx = _rows(x, "x", self.device, self.d_model)
-        y = torch.empty(x.shape, dtype=self.out_dtype, device=self.device)
+        io.x, io.tokens, io.ldx = _rows(x, "x", self.device, self.d_model)
+        y = _like(x, x.shape) if self._y_code == L.APK_BF16 else x.new_empty(x.shape, dtype=self.out_dtype)
+        io.y, io.ldy, io.y_dtype = y.data_ptr(), self.d_model, self._y_code
         ids = probs = None
         if return_routing:
             shape = (*x.shape[:-1], self.top_k)
-            ids = torch.empty(shape, dtype=torch.int32, device=self.device)
-            probs = torch.empty(shape, dtype=torch.float32, device=self.device)
+            ids, probs = x.new_empty(shape, dtype=torch.int32), x.new_empty(shape, dtype=torch.float32)
             io.ids, io.probs = ids.data_ptr(), probs.data_ptr()
         else:
             io.ids = io.probs = None
-        io.x, io.tokens, io.y, io.ldy = x2.data_ptr(), x2.shape[0], y.data_ptr(), self.d_model
-        io.y_dtype, io.stream = _CODE[self.out_dtype], self._stream()
+        io.stream = self._stream()
         st = self._lib.apk_moe_forward(self._h, self._io_ref)
         if st:
             self._check(st)
