@@ -318,7 +318,7 @@ apk_status forward(apk_linear* h, const apk_linear_io* io) {
   const int w_outer = c.w_layout == APK_W_KN ? K : N, w_inner = c.w_layout == APK_W_KN ? N : K;
   const lin::Epilogue epi = {c.bias, io->residual, io->y, io->preact, io->ld_residual, io->ldy, io->ld_preact,
                              c.bias_dtype == APK_F32, io->residual_dtype == APK_F32, io->y_dtype == APK_F32, c.act};
-  if (M <= lin::STREAM_ROWS)
+  if (lin::streams(M, (long long)K * N * 2, c.w_layout == APK_W_NK, tma_ok(c.W, c.ldw, w_outer)))
     return cu_status(lin::run_stream(io->x, io->ldx, c.W, c.ldw, c.w_layout == APK_W_NK, M, N, K, epi, h->sms, s),
                      "launching the streaming kernel", &h->err);
   const void* x = io->x;
@@ -452,16 +452,7 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
   return APK_OK;
 }
 
-}  // namespace
-
-extern "C" {
-
-apk_status apk_linear_create(const apk_linear_config* cfg, apk_linear** out) {
-  if (!out) return APK_EINVAL;
-  *out = nullptr;
-  apk_linear* h = new (std::nothrow) apk_linear;
-  if (!h) return APK_ENOMEM;
-  *out = h;  // also on failure: apk_linear_last_error says why, apk_linear_destroy frees it
+apk_status create(const apk_linear_config* cfg, apk_linear* h) {
   if (!cfg) return h->err.fail(APK_EINVAL, "cfg is NULL");
   h->cfg = *cfg;
   const apk_linear_config& c = h->cfg;
@@ -496,6 +487,21 @@ apk_status apk_linear_create(const apk_linear_config* cfg, apk_linear** out) {
   h->status = static_cast<int*>(st);
   APK_TRY(cu_status(cudaMemset(st, 0, 256), "cudaMemset", &h->err));
   return cu_status(cudaStreamSynchronize(nullptr), "cudaStreamSynchronize", &h->err);
+}
+
+}  // namespace
+
+extern "C" {
+
+apk_status apk_linear_create(const apk_linear_config* cfg, apk_linear** out) {
+  if (!out) return APK_EINVAL;
+  *out = new (std::nothrow) apk_linear;
+  if (!*out) return APK_ENOMEM;
+  try {
+    return create(cfg, *out);  // *out is set on failure too: its last_error says why
+  } catch (...) {
+    return APK_ENOMEM;
+  }
 }
 
 apk_status apk_linear_destroy(apk_linear* h) {

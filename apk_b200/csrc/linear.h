@@ -59,11 +59,23 @@ struct Product {
 // Launches one or two products, in one launch where that is faster. sms: the SMs it may
 // fill; dev: the current device.
 // `why` receives a message on failure.
+// Whether a product is faster through run_stream than through run_products.  Up to 8 rows
+// [n][k] weights always are (8 x 4096 x 8192: 13.7 against 15.6 us); two MMA
+// tiles of rows, or the narrower row pieces of [k][n], cost it bandwidth, so
+// that only its smaller latency counts (16 x 2048 x 2048: 5.3 against 7.0 us;
+// 16 x 4096 x 8192: 19.8 against 15.7; [k][n] 8 x 4096 x 8192: 21 against 15.2,
+// 1 x 2048 x 2048: 5.3 against 6.8).  Weights that TMA cannot address save it
+// their copy.
+inline bool streams(int rows, long long weight_bytes, bool nk, bool tma) {
+  if (rows > 16) return false;
+  const long long mb = weight_bytes >> 20;
+  if (!tma) return mb < 16;
+  return nk ? rows <= 8 || mb < 16 : mb < (rows <= 8 ? 16 : 4);
+}
 apk_status run_products(const Product* pr, int n, int sms, int dev, int* status, long long limit, cudaStream_t stream,
                         std::string* why);
-// A product of at most STREAM_ROWS rows with weights [n][k] (nk) or [k][n] of
-// any stride and alignment.
-constexpr int STREAM_ROWS = 16;
+// A product of at most 16 rows with weights [n][k] (nk) or [k][n] of any
+// stride and alignment.
 cudaError_t run_stream(const void* x, long long ldx, const void* w, long long ldw, bool nk, int rows, int n, int k,
                        const Epilogue& epi, int sms, cudaStream_t stream);
 // Sets the kernels' attributes on the current device, once; before its first run_products.

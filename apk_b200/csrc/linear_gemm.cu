@@ -150,10 +150,11 @@ __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t parity, const Gemm
     }
   }
 }
-__device__ __forceinline__ void bwait_unwind(uint64_t* bar, uint32_t parity, long long limit) {
+// While unwinding: up to a second, however short the caller's limit is.
+__device__ __forceinline__ void bwait_unwind(uint64_t* bar, uint32_t parity) {
   const long long t0 = globaltimer_ns();
   while (!try_wait_cluster(bar, parity))
-    if (globaltimer_ns() - t0 > limit) return;
+    if (globaltimer_ns() - t0 > 1000000000ll) return;
 }
 
 __device__ __forceinline__ float load_elem(const void* p, long long i, int f32) {
@@ -429,10 +430,14 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
         }
       }
     }
-    if (!ok && leader) {
+    if (!ok) {
       // unwinding: the loads in flight land before the shared memory goes away
-      for (uint32_t q = P > (uint32_t)S ? P - S : 0; q < P; ++q)
-        bwait_unwind(&sh.full[q % S], (q / S) & 1, p.limit);
+      if (leader)
+        for (uint32_t q = P > (uint32_t)S ? P - S : 0; q < P; ++q) bwait_unwind(&sh.full[q % S], (q / S) & 1);
+      // (a pair's second CTA has no barrier of its own to ask: a millisecond is
+      // a thousand times what a load takes)
+      const long long t0 = globaltimer_ns();
+      while (CG == 2 && globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
     }
   } else if (warp == 1 && lane == 0 && leader) {
     // =================================== MMA ===================================
@@ -520,7 +525,7 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
     }
     if (!ok) {
       commit_to<CG>(smem_u32(&sh.drain));
-      bwait_unwind(&sh.drain, 0, p.limit);
+      bwait_unwind(&sh.drain, 0);
     }
   } else if (warp >= 2) {
     // ================================ epilogue ================================
@@ -744,6 +749,7 @@ Choice choose(const Product* pr, int n, int sms, int dev) {
     const double per_kb = std::max(v.nt * 2.0 * v.fm, (v.fm * P_BYTES + v.nt / v.cg * 128) / 37.0);
     for (int lg = v.split ? 1 : 0; lg <= (v.split ? 3 : 0); ++lg) {
       const int sp = 1 << lg, per = v.cg * sp;
+      if (per > sms) continue;
       int slots = std::max(1, sms / per);
       if (per > 1) slots = std::max(1, std::min(slots, g_clusters[dev][per == 2 ? 1 : lg]));
       long long tiles = 0;

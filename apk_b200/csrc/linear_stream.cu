@@ -1,8 +1,8 @@
 // The linear layer for up to 16 rows (decoding): weights streamed once from
 // global memory into MMA fragments (stream.cuh).
 //
-// A CTA of 8 warps owns 16 output columns ([N][K] weights) or 64 ([K][N]:
-// 128-byte row pieces) and splits K over its warps in chunks of 128 (64); a
+// A CTA owns 16 output columns ([N][K] weights, 16 warps) or 32 ([K][N]:
+// 64-byte row pieces, 8 warps) and splits K over its warps in chunks of 128 (64); a
 // cluster of 2, 4 or 8 CTAs splits it further where the columns alone give
 // too few CTAs.  The warps' partial sums meet in shared memory and are added
 // in the order of (CTA rank, warp): the result does not depend on timing.
@@ -28,11 +28,12 @@ struct StreamParams {
 
 namespace {
 
-constexpr int WARPS = 8;
 template <bool NK>
-constexpr int FEATURES = NK ? 16 : 64;
+constexpr int WARPS_OF = NK ? 16 : 8;
 template <bool NK>
-constexpr int CHUNK = NK ? 128 : 64;  // k of one warp's round: 8 16-byte loads a lane
+constexpr int FEATURES = NK ? 16 : 32;
+template <bool NK>
+constexpr int CHUNK = NK ? 128 : 64;  // k of one warp's round: 128 bytes a lane
 
 __device__ __forceinline__ float ld_epi(const void* p, long long i, int f32) {
   return f32 ? static_cast<const float*>(p)[i]
@@ -63,8 +64,11 @@ __device__ __forceinline__ void flush(float (&acc)[N][4], float (&total)[N][4]) 
     }
 }
 
-template <bool NK, int NT8, bool VEC>
-__global__ void __launch_bounds__(32 * WARPS, NK ? (NT8 == 1 && VEC ? 4 : 3) : 2) lin_stream(const __grid_constant__ StreamParams p) {
+// LONG: a warp's share of K exceeds FLUSH.
+template <bool NK, int NT8, bool VEC, bool LONG>
+__global__ void __launch_bounds__(32 * WARPS_OF<NK>, NT8 == 1 && VEC ? (NK ? 2 : 3) : NK ? 1 : VEC ? 3 : 2)
+lin_stream(const __grid_constant__ StreamParams p) {
+  constexpr int WARPS = WARPS_OF<NK>;
   constexpr int FT = FEATURES<NK>, KC = CHUNK<NK>, TOK = 8 * NT8;
   __shared__ float part[WARPS][TOK][FT];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -108,7 +112,7 @@ __global__ void __launch_bounds__(32 * WARPS, NK ? (NT8 == 1 && VEC ? 4 : 3) : 2
           stream::mma_bf16(acc[i], a[u].x, b[u].x, a[u].y, b[u].y, c[i][u].x, c[i][u].y);
           stream::mma_bf16(acc[i], a[u].z, b[u].z, a[u].w, b[u].w, c[i][u].z, c[i][u].w);
         }
-      if ((++round & (FLUSH / KC - 1)) == 0) flush(acc, total);
+      if (LONG && (++round & (FLUSH / KC - 1)) == 0) flush(acc, total);
     }
     flush(acc, total);
 #pragma unroll
@@ -116,61 +120,54 @@ __global__ void __launch_bounds__(32 * WARPS, NK ? (NT8 == 1 && VEC ? 4 : 3) : 2
 #pragma unroll
       for (int j = 0; j < 4; ++j) part[warp][8 * i + 2 * t + (j & 1)][g + 8 * (j >> 1)] = total[i][j];
   } else {
-    float acc[4][NT8][4] = {}, total[4][NT8][4] = {};
+    float acc[2][NT8][4] = {}, total[2][NT8][4] = {};
     int round = 0;
-    const int f = f0 + 8 * g;
-    const uint16_t* w = p.w + (VEC ? min(f, p.n - 8) : f);
+    const int f = f0 + 4 * g;
+    const uint16_t* w = p.w + (VEC ? min(f, p.n - 4) : f);
 #pragma unroll 1
     for (int k0 = (rank * WARPS + warp) * KC; k0 < p.k; k0 += p.split * WARPS * KC) {
       constexpr int U = KC / 16;
-      uint4 a[U / 2][4];
+      uint2 a[U][4], c[U][NT8];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint2 c[U / 2][NT8];
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + 16 * u + 4 * t;
 #pragma unroll
-        for (int u = 0; u < U / 2; ++u) {
-          const int k = k0 + 16 * (h * U / 2 + u) + 4 * t;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool in = k + r < p.k;
-            if (VEC) a[u][r] = in ? stream::ld_weights(w + (long long)(k + r) * p.ldw) : make_uint4(0, 0, 0, 0);
-            else a[u][r] = stream::ld8_any(w + (long long)(k + r) * p.ldw, in ? p.n - f : 0);
-          }
-#pragma unroll
-          for (int i = 0; i < NT8; ++i) {
-            if (VEC) c[u][i] = k < p.k ? __ldg(reinterpret_cast<const uint2*>(xr[i] + k)) : make_uint2(0, 0);
-            else c[u][i] = stream::ld4_any(xr[i] + k, p.k - k);
-          }
+        for (int r = 0; r < 4; ++r) {
+          const bool in = k + r < p.k;
+          if (VEC) a[u][r] = in ? stream::ld_weights8(w + (long long)(k + r) * p.ldw) : make_uint2(0, 0);
+          else a[u][r] = stream::ld4_any(w + (long long)(k + r) * p.ldw, in ? p.n - f : 0);
         }
 #pragma unroll
-        for (int u = 0; u < U / 2; ++u) {
-          const uint32_t* r0 = &a[u][0].x;
-          const uint32_t* r1 = &a[u][1].x;
-          const uint32_t* r2 = &a[u][2].x;
-          const uint32_t* r3 = &a[u][3].x;
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            const uint32_t a0 = __byte_perm(r0[m], r1[m], 0x5410), a1 = __byte_perm(r0[m], r1[m], 0x7632);
-            const uint32_t a2 = __byte_perm(r2[m], r3[m], 0x5410), a3 = __byte_perm(r2[m], r3[m], 0x7632);
-#pragma unroll
-            for (int i = 0; i < NT8; ++i) stream::mma_bf16(acc[m][i], a0, a1, a2, a3, c[u][i].x, c[u][i].y);
-          }
+        for (int i = 0; i < NT8; ++i) {
+          if (VEC) c[u][i] = k < p.k ? __ldg(reinterpret_cast<const uint2*>(xr[i] + k)) : make_uint2(0, 0);
+          else c[u][i] = stream::ld4_any(xr[i] + k, p.k - k);
         }
       }
-      if ((++round & (FLUSH / KC - 1)) == 0)
 #pragma unroll
-        for (int m = 0; m < 4; ++m) flush(acc[m], total[m]);
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const uint32_t r0 = m ? a[u][0].y : a[u][0].x, r1 = m ? a[u][1].y : a[u][1].x;
+          const uint32_t r2 = m ? a[u][2].y : a[u][2].x, r3 = m ? a[u][3].y : a[u][3].x;
+          const uint32_t a0 = __byte_perm(r0, r1, 0x5410), a1 = __byte_perm(r0, r1, 0x7632);
+          const uint32_t a2 = __byte_perm(r2, r3, 0x5410), a3 = __byte_perm(r2, r3, 0x7632);
+#pragma unroll
+          for (int i = 0; i < NT8; ++i) stream::mma_bf16(acc[m][i], a0, a1, a2, a3, c[u][i].x, c[u][i].y);
+        }
+      if (LONG && (++round & (FLUSH / KC - 1)) == 0)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) flush(acc[m], total[m]);
     }
 #pragma unroll
-    for (int m = 0; m < 4; ++m) flush(acc[m], total[m]);
-    // MMA m's rows g and g + 8 are the features 8g + 2m and 8g + 2m + 1
+    for (int m = 0; m < 2; ++m) flush(acc[m], total[m]);
+    // MMA m's rows g and g + 8 are the features 4g + 2m and 4g + 2m + 1
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int i = 0; i < NT8; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          part[warp][8 * i + 2 * t + (j & 1)][8 * g + 2 * m + (j >> 1)] = total[m][i][j];
+          part[warp][8 * i + 2 * t + (j & 1)][4 * g + 2 * m + (j >> 1)] = total[m][i][j];
   }
   __syncthreads();
   if (p.split > 1)
@@ -208,8 +205,9 @@ __global__ void __launch_bounds__(32 * WARPS, NK ? (NT8 == 1 && VEC ? 4 : 3) : 2
 }
 
 template <bool NK, int NT8, bool VEC>
-const void* fn() {
-  return reinterpret_cast<const void*>(&lin_stream<NK, NT8, VEC>);
+const void* fn(bool longer) {
+  return longer ? reinterpret_cast<const void*>(&lin_stream<NK, NT8, VEC, true>)
+                : reinterpret_cast<const void*>(&lin_stream<NK, NT8, VEC, false>);
 }
 
 }  // namespace
@@ -220,15 +218,18 @@ cudaError_t run_stream(const void* x, long long ldx, const void* w, long long ld
   auto a16 = [](const void* q, long long ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ld % 8 == 0; };
   const bool vec = k % 8 == 0 && (nk || n % 8 == 0) && a16(w, ldw) && (a16(x, ldx) || (rows == 1 && a16(x, 8)));
   const int nt = rows <= 8 ? 1 : 2;
-  const void* f = nk ? (nt == 1 ? (vec ? fn<true, 1, true>() : fn<true, 1, false>())
-                                : (vec ? fn<true, 2, true>() : fn<true, 2, false>()))
-                     : (nt == 1 ? (vec ? fn<false, 1, true>() : fn<false, 1, false>())
-                                : (vec ? fn<false, 2, true>() : fn<false, 2, false>()));
   const int ft = nk ? FEATURES<true> : FEATURES<false>, kc = nk ? CHUNK<true> : CHUNK<false>;
+  const int warps = nk ? WARPS_OF<true> : WARPS_OF<false>;
   const int tiles = (n + ft - 1) / ft;
   // split K while a round of every warp remains and the CTAs do not exceed two per SM
-  while (p.split < 8 && 2 * p.split * tiles <= 2 * sms && 2 * p.split * WARPS * kc <= k) p.split *= 2;
-  Launch l(dim3(tiles * p.split), 32 * WARPS, 0, stream, p.split);
+  while (p.split < 8 && 2 * p.split * tiles <= 2 * sms && 2 * p.split * warps * kc <= k) p.split *= 2;
+  const int round = p.split * warps * kc;
+  const bool longer = (k + round - 1) / round * kc > FLUSH;
+  const void* f = nk ? (nt == 1 ? (vec ? fn<true, 1, true>(longer) : fn<true, 1, false>(longer))
+                                : (vec ? fn<true, 2, true>(longer) : fn<true, 2, false>(longer)))
+                     : (nt == 1 ? (vec ? fn<false, 1, true>(longer) : fn<false, 1, false>(longer))
+                                : (vec ? fn<false, 2, true>(longer) : fn<false, 2, false>(longer)));
+  Launch l(dim3(tiles * p.split), 32 * warps, 0, stream, p.split);
   void* args[] = {&p};
   return cudaLaunchKernelExC(&l.cfg, f, args);
 }

@@ -6,12 +6,12 @@
 // tensor pipe's rate does not matter.
 //
 // A fragment's k order is free as long as A and B agree, so a thread loads 16
-// contiguous bytes and deals them over the fragments:
+// (8) contiguous bytes and deals them over the fragments:
 //   [feature][k] weights: lane (g, t) holds features g and g + 8 at k = 8t..8t+7
 //     of 32, two MMAs; its B values are token g at the same k.
-//   [k][feature] weights: lane (g, t) holds features 8g..8g+7 of 64 at the
-//     rows k = 4t..4t+3 of 16; byte permutes pair two rows into the four
-//     MMAs' A registers.
+//   [k][feature] weights: lane (g, t) holds features 4g..4g+3 of 32 at the
+//     rows k = 4t..4t+3 of 16; byte permutes pair two rows into the two MMAs'
+//     A registers.
 #pragma once
 #include <stdint.h>
 
@@ -33,6 +33,12 @@ __device__ __forceinline__ uint4 ld_weights(const void* p) {
   asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ uint2 ld_weights8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 

@@ -523,7 +523,7 @@ typedef struct apk_linear_config {
   const void* W;            /* bf16                                           */
   long long ldw;
   const void* bias;         /* out_features values, or NULL                   */
-  int sms;                  /* SMs the products may fill; 0 = all             */
+  int sms;                  /* SMs the persistent products fill; 0 = all      */
   long long wait_limit_ns;
 } apk_linear_config;
 typedef struct apk_linear apk_linear;
