@@ -171,6 +171,16 @@ __device__ __forceinline__ void store_elem(void* p, long long i, float v, int f3
   else static_cast<uint16_t*>(p)[i] = to_bf16(v);
 }
 
+// The fields in registers.  The compiler would rather load them again from
+// the indexed kernel parameter at every use.
+__device__ __forceinline__ Epilogue pinned(const Epilogue& c) {
+  Epilogue e = c;
+  asm volatile("" : "+l"(e.bias), "+l"(e.res), "+l"(e.out), "+l"(e.pre));
+  asm volatile("" : "+l"(e.ld_res), "+l"(e.ld_out), "+l"(e.ld_pre));
+  asm volatile("" : "+r"(e.bias_f32), "+r"(e.res_f32), "+r"(e.out_f32), "+r"(e.act));
+  return e;
+}
+
 // W rows of one output column: bias, pre-activation, activation, residual,
 // stores.  out and pre point at the first row's element; so and sp are the
 // bytes to the next one.  The types and the presence of the pre-activation
@@ -313,7 +323,7 @@ __device__ __forceinline__ int tile_of(const GemmParams& p, int g, int G, int q)
   const int head = min(n1, others * extra);
   if (extra && g >= rem) {
     if (q < extra) {
-      const int j = (g - rem) * extra + q;
+      const int j = g - rem + q * others;
       return j < head ? n0 + j : -1;
     }
     q -= extra;
@@ -538,7 +548,7 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
       const Problem& pr = locate(t, r0, c0);
       k_range(pr, kb, ke);
       c0 += 128 * CG * (i % FM);
-      const Epilogue e = pr.epi;
+      const Epilogue e = pinned(pr.epi);
       const int col = 32 * q + lane;
       const bool in = c0 + col < pr.cols;
       const long long c = c0 + col;
@@ -724,8 +734,8 @@ int g_clusters[64][4];
 // The variant with the least estimated time for these products on `sms` SMs,
 // in SM clocks.  Per 64-deep k-block and tile: the MMA's own time (128 x NT x
 // 64 at 4096 MAC per clock and SM) or the time a stage takes to arrive at an
-// SM (37 bytes a clock measured with every SM loading, from L2 or memory: the
-// widest tile is bound by this); for the whole: its bytes at the memory's
+// SM (37 bytes a clock measured for the pairs, 45 for single CTAs: the widest
+// tile is bound by this); for the whole: its bytes at the memory's
 // rate (3300 a clock).  A tile's epilogue takes 8500 clocks per 256 rows of a
 // CTA's 128 columns (measured without residual or activation; they add about
 // 4000 and 3000); a second accumulator hides it behind the next tile, or half
@@ -746,7 +756,7 @@ Choice choose(const Product* pr, int n, int sms, int dev) {
     bool fits = v.exact == exact;
     for (int j = 0; j < n; ++j) fits = fits && !(pr[j].Q.mn && v.nt < 64);
     if (!fits) continue;
-    const double per_kb = std::max(v.nt * 2.0 * v.fm, (v.fm * P_BYTES + v.nt / v.cg * 128) / 37.0);
+    const double per_kb = std::max(v.nt * 2.0 * v.fm, (v.fm * P_BYTES + v.nt / v.cg * 128) / (v.cg == 2 ? 37.0 : 45.0));
     for (int lg = v.split ? 1 : 0; lg <= (v.split ? 3 : 0); ++lg) {
       const int sp = 1 << lg, per = v.cg * sp;
       if (per > sms) continue;
@@ -826,7 +836,7 @@ apk_status run_products(const Product* pr, int n, int sms, int dev, int* status,
   if (n == 2) {
     // products that want different tiles run one after the other
     const double apart = choose(pr, 1, sms, dev).cost + choose(pr + 1, 1, sms, dev).cost;
-    if (apart < ch.cost) {
+    if (apart + 8000 < ch.cost) {  // (a second launch, and a second tail)
       const apk_status st = run_products(pr, 1, sms, dev, status, limit, stream, why);
       return st != APK_OK ? st : run_products(pr + 1, 1, sms, dev, status, limit, stream, why);
     }
