@@ -87,10 +87,8 @@ struct RepackParams {
   int n;
   long long chunks;
 };
-__global__ void __launch_bounds__(256) repack(const __grid_constant__ RepackParams p) {
-  pdl_launch();
-  pdl_wait();
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < p.chunks; i += (long long)gridDim.x * 256) {
+__device__ __forceinline__ void repack_block(const RepackParams& p, int block, int blocks) {
+  for (long long i = (long long)block * 256 + threadIdx.x; i < p.chunks; i += (long long)blocks * 256) {
     const Repack& o = p.op[p.n > 1 && i >= p.op[1].first ? 1 : 0];
     const long long at = i - o.first;
     const int per = o.ld / 8;
@@ -106,6 +104,11 @@ __global__ void __launch_bounds__(256) repack(const __grid_constant__ RepackPara
     *reinterpret_cast<uint4*>(o.dst + r * o.ld + c) = u.v;
   }
 }
+__global__ void __launch_bounds__(256) repack(const __grid_constant__ RepackParams p) {
+  pdl_launch();
+  pdl_wait();
+  repack_block(p, blockIdx.x, gridDim.x);
+}
 
 struct DzParams {
   const uint16_t* dy;
@@ -116,6 +119,7 @@ struct DzParams {
   unsigned* count;    // one per column block, zero between launches
   long long ld_dy, ld_z, ld_dz;
   int rows, cols, rows_per_block, act, db_f32;
+  int cblocks, rblocks;  // column ranges, row ranges; further blocks repack
 };
 
 constexpr int DZ_COLS = 256;  // columns of a block: 8 per lane
@@ -125,13 +129,24 @@ constexpr int DZ_COLS = 256;  // columns of a block: 8 per lane
 // rows in registers and shared memory; the last block of a column range adds
 // the row blocks' sums in their order, so db does not depend on the order of
 // arrival.  VEC: rows of 16-byte aligned 8-element chunks.
+// Blocks past the first cblocks * rblocks copy operands for the products that
+// follow (one launch for both).
 template <bool VEC>
-__global__ void __launch_bounds__(256) dz_kernel(const DzParams p) {
+__global__ void __launch_bounds__(256) dz_kernel(const __grid_constant__ DzParams p,
+                                                 const __grid_constant__ RepackParams copies) {
   __shared__ float sum[8][DZ_COLS];
   __shared__ bool last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c0 = (int)blockIdx.x * DZ_COLS;
-  const long long r1 = min((long long)p.rows, (long long)(blockIdx.y + 1) * p.rows_per_block);
+  const int own = p.cblocks * p.rblocks;
+  if ((int)blockIdx.x >= own) {
+    pdl_launch();
+    pdl_wait();
+    repack_block(copies, (int)blockIdx.x - own, (int)gridDim.x - own);
+    return;
+  }
+  const int cb = (int)blockIdx.x % p.cblocks, rb = (int)blockIdx.x / p.cblocks;
+  const int c0 = cb * DZ_COLS;
+  const long long r1 = min((long long)p.rows, (long long)(rb + 1) * p.rows_per_block);
   float acc[8] = {};
   pdl_launch();
   pdl_wait();
@@ -165,7 +180,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzParams p) {
       }
       return v;
     };
-    long long r = (long long)blockIdx.y * p.rows_per_block + warp;
+    long long r = (long long)rb * p.rows_per_block + warp;
     Row now = load(r);
     for (; r < r1; r += 8) {
       const Row next = load(r + 8);  // in flight while this row is worked on
@@ -202,14 +217,14 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzParams p) {
   float s = 0.f;
 #pragma unroll
   for (int w = 0; w < 8; ++w) s += sum[w][threadIdx.x];
-  if (gridDim.y > 1) {
+  if (p.rblocks > 1) {
     const int ldp = (p.cols + 7) / 8 * 8;
-    if (c < p.cols) p.part[(long long)blockIdx.y * ldp + c] = s;
+    if (c < p.cols) p.part[(long long)rb * ldp + c] = s;
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
-      last = atomicAdd(&p.count[blockIdx.x], 1u) == gridDim.y - 1;
-      if (last) p.count[blockIdx.x] = 0;
+      last = atomicAdd(&p.count[cb], 1u) == (unsigned)p.rblocks - 1;
+      if (last) p.count[cb] = 0;
     }
     __syncthreads();
     if (!last) return;
@@ -218,7 +233,7 @@ __global__ void __launch_bounds__(256) dz_kernel(const DzParams p) {
     float t[8] = {};
     if (c0 + lane * 8 < ldp) {
 #pragma unroll 4
-      for (unsigned b = warp; b < gridDim.y; b += 8) {
+      for (int b = warp; b < p.rblocks; b += 8) {
         const float4* q = reinterpret_cast<const float4*>(p.part + (long long)b * ldp + c0 + lane * 8);
         const float4 lo = __ldcg(q), hi = __ldcg(q + 1);
         t[0] += lo.x;
@@ -281,9 +296,10 @@ struct RepackList {
     *src = dst;
     *ld = o.ld;
   }
+  unsigned blocks(int sms) const { return (unsigned)std::min<long long>((p.chunks + 255) / 256, sms * 16); }
   apk_status run(int sms, cudaStream_t s, Err* err) const {
     if (p.n == 0) return APK_OK;
-    Launch l(dim3((unsigned)std::min<long long>((p.chunks + 255) / 256, sms * 16)), 256, 0, s);
+    Launch l(dim3(blocks(sms)), 256, 0, s);
     return cu_status(cudaLaunchKernelEx(&l.cfg, lin::repack, p), "launching the repack kernel", err);
   }
 };
@@ -391,9 +407,17 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
   const bool scratch = g->db || own_dz || px || pw;
   if (scratch) APK_TRY(h->scratch.begin(zeroed + bpart + bdz + bx + bw, zeroed, s, &h->err));
   uint8_t* base = h->scratch.data();
+  const void* x = g->x;
+  const void* w = c.W;
+  long long ldx = g->ldx, ldw = c.ldw;
+  RepackList list;
+  if (px) list.add(&x, &ldx, M, K, base + zeroed + bpart + bdz);
+  if (pw) list.add(&w, &ldw, w_outer, w_inner, base + zeroed + bpart + bdz + bx);
   const void* dz = g->dy;
   long long ld_dz = g->ld_dy;
-  if (g->db || own_dz) {
+  if (!g->db && !own_dz) {
+    APK_TRY(list.run(h->sms, s, &h->err));
+  } else {
     lin::DzParams d{};
     d.dy = static_cast<const uint16_t*>(g->dy);
     d.z = act ? static_cast<const uint16_t*>(g->preact) : nullptr;
@@ -414,18 +438,12 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
     d.act = c.act;
     // (the last chunk of a row may reach past N: only within an 8-multiple row)
     const bool vec = N % 8 == 0 && tma_ok(g->dy, g->ld_dy, M) && (!act || tma_ok(g->preact, g->ld_preact, M));
-    if (rblocks > 65535) return h->err.fail(APK_EINVAL, "%d rows", M);
-    Launch l(dim3(cblocks, rblocks), 256, 0, s);
-    APK_TRY(cu_status(cudaLaunchKernelEx(&l.cfg, vec ? lin::dz_kernel<true> : lin::dz_kernel<false>, d),
+    d.cblocks = cblocks;
+    d.rblocks = rblocks;
+    Launch l(dim3(cblocks * rblocks + list.blocks(h->sms)), 256, 0, s);
+    APK_TRY(cu_status(cudaLaunchKernelEx(&l.cfg, vec ? lin::dz_kernel<true> : lin::dz_kernel<false>, d, list.p),
                       "launching the dz kernel", &h->err));
   }
-  const void* x = g->x;
-  const void* w = c.W;
-  long long ldx = g->ldx, ldw = c.ldw;
-  RepackList list;
-  if (px) list.add(&x, &ldx, M, K, base + zeroed + bpart + bdz);
-  if (pw) list.add(&w, &ldw, w_outer, w_inner, base + zeroed + bpart + bdz + bx);
-  APK_TRY(list.run(h->sms, s, &h->err));
   lin::Product p[2] = {};
   int n = 0;
   if (g->dx) {  // dx[m][k] = sum_n dz[m][n] W[k][n]
