@@ -28,9 +28,11 @@ apk_status Scratch::begin(size_t bytes, size_t zeroed, cudaStream_t stream, Err*
                        bytes);
     if (ev_ && used_ && (st = cu_status(cudaEventSynchronize(ev_), "waiting for the scratch", err)) != APK_OK) return st;
     used_ = false;
-    if (p_) cudaFree(p_);
+    if (p_ && captured_) kept_.push_back(p_);
+    else if (p_) cudaFree(p_);
     p_ = nullptr;
     bytes_ = 0;
+    captured_ = false;
     void* q = nullptr;
     if ((st = cu_status(cudaMalloc(&q, bytes), "cudaMalloc(scratch)", err)) != APK_OK) return st;
     p_ = static_cast<uint8_t*>(q);
@@ -39,8 +41,9 @@ apk_status Scratch::begin(size_t bytes, size_t zeroed, cudaStream_t stream, Err*
     if ((st = cu_status(cudaStreamSynchronize(nullptr), "cudaStreamSynchronize", err)) != APK_OK) return st;
     bytes_ = bytes;
   }
-  if (!capturing_ && used_ && last_ != stream)
-    return cu_status(cudaStreamWaitEvent(stream, ev_, 0), "cudaStreamWaitEvent", err);
+  captured_ = captured_ || capturing_;
+  // (on the same stream too: a handle's value may name another stream by now)
+  if (!capturing_ && used_) return cu_status(cudaStreamWaitEvent(stream, ev_, 0), "cudaStreamWaitEvent", err);
   return APK_OK;
 }
 
@@ -50,13 +53,14 @@ apk_status Scratch::end(cudaStream_t stream, Err* err) {
   if (!ev_ && (st = cu_status(cudaEventCreateWithFlags(&ev_, cudaEventDisableTiming), "cudaEventCreate", err)) != APK_OK)
     return st;
   if ((st = cu_status(cudaEventRecord(ev_, stream), "cudaEventRecord", err)) != APK_OK) return st;
-  last_ = stream;
   used_ = true;
   return APK_OK;
 }
 
 void Scratch::release() {
   if (p_) cudaFree(p_);  // waits for the device
+  for (uint8_t* q : kept_) cudaFree(q);
+  kept_.clear();
   if (ev_) cudaEventDestroy(ev_);
   p_ = nullptr;
   ev_ = nullptr;
@@ -341,10 +345,11 @@ apk_status forward(apk_linear* h, const apk_linear_io* io) {
   const void* w = c.W;
   long long ldx = io->ldx, ldw = c.ldw;
   const bool px = !tma_ok(x, ldx, M), pw = !tma_ok(w, ldw, w_outer);
+  ScratchUse use(&h->scratch, s, &h->err);
   if (px || pw) {
     const size_t bx = px ? up256((size_t)M * up8(K) * 2) : 0, bw = pw ? up256((size_t)w_outer * up8(w_inner) * 2) : 0;
     const size_t zeroed = up256((size_t)(N + lin::DZ_COLS - 1) / lin::DZ_COLS * 4);
-    APK_TRY(h->scratch.begin(zeroed + bx + bw, zeroed, s, &h->err));
+    APK_TRY(use.begin(zeroed + bx + bw, zeroed));
     RepackList list;
     if (px) list.add(&x, &ldx, M, K, h->scratch.data() + zeroed);
     if (pw) list.add(&w, &ldw, w_outer, w_inner, h->scratch.data() + zeroed + bx);
@@ -358,8 +363,7 @@ apk_status forward(apk_linear* h, const apk_linear_io* io) {
   p.k = K;
   p.epi = epi;
   APK_TRY(lin::run_products(&p, 1, h->sms, c.device, h->status, c.wait_limit_ns, s, &h->err.text));
-  if (px || pw) APK_TRY(h->scratch.end(s, &h->err));
-  return APK_OK;
+  return use.end();
 }
 
 apk_status backward(apk_linear* h, const apk_linear_grads* g) {
@@ -404,8 +408,8 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
   const size_t bpart = g->db ? up256((size_t)rblocks * up8(N) * 4) : 0;
   const size_t bdz = own_dz ? up256((size_t)M * up8(N) * 2) : 0;
   const size_t bx = px ? up256((size_t)M * up8(K) * 2) : 0, bw = pw ? up256((size_t)w_outer * up8(w_inner) * 2) : 0;
-  const bool scratch = g->db || own_dz || px || pw;
-  if (scratch) APK_TRY(h->scratch.begin(zeroed + bpart + bdz + bx + bw, zeroed, s, &h->err));
+  ScratchUse use(&h->scratch, s, &h->err);
+  if (g->db || own_dz || px || pw) APK_TRY(use.begin(zeroed + bpart + bdz + bx + bw, zeroed));
   uint8_t* base = h->scratch.data();
   const void* x = g->x;
   const void* w = c.W;
@@ -466,8 +470,7 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
     a.epi = {nullptr, nullptr, g->dw, nullptr, 0, g->ld_dw, 0, 0, 0, g->dw_dtype == APK_F32, APK_ACT_NONE};
   }
   if (n) APK_TRY(lin::run_products(p, n, h->sms, c.device, h->status, c.wait_limit_ns, s, &h->err.text));
-  if (scratch) APK_TRY(h->scratch.end(s, &h->err));
-  return APK_OK;
+  return use.end();
 }
 
 apk_status create(const apk_linear_config* cfg, apk_linear* h) {

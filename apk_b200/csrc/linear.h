@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <string>
+#include <vector>
 
 #include "../../include/apk.h"
 
@@ -116,7 +117,8 @@ class DeviceGuard {
 // Device scratch of one handle.  Calls on one handle may come from different
 // streams: a call that uses the scratch waits for the last one that did.  In
 // a stream capture the events are left out (the order of a graph's launches
-// and of other calls is the caller's), and the scratch may not grow.
+// and of other calls is the caller's), and the scratch may not grow; a
+// buffer that a graph refers to is kept until the handle is destroyed.
 class Scratch {
  public:
   // At least `bytes` of scratch, the first `zeroed` of them zero when it was
@@ -130,8 +132,36 @@ class Scratch {
   uint8_t* p_ = nullptr;
   size_t bytes_ = 0;
   cudaEvent_t ev_ = nullptr;
-  cudaStream_t last_ = nullptr;
-  bool used_ = false, capturing_ = false;
+  bool used_ = false, capturing_ = false, captured_ = false;
+  std::vector<uint8_t*> kept_;  // earlier buffers that graphs refer to
+};
+
+// Ends the use of the scratch on every way out of a call.
+class ScratchUse {
+ public:
+  ScratchUse(Scratch* s, cudaStream_t stream, Err* err) : s_(s), stream_(stream), err_(err) {}
+  ~ScratchUse() {
+    if (begun_) {
+      Err ignored;
+      s_->end(stream_, &ignored);
+    }
+  }
+  apk_status begin(size_t bytes, size_t zeroed) {
+    const apk_status st = s_->begin(bytes, zeroed, stream_, err_);
+    begun_ = st == APK_OK;
+    return st;
+  }
+  apk_status end() {
+    if (!begun_) return APK_OK;
+    begun_ = false;
+    return s_->end(stream_, err_);
+  }
+
+ private:
+  Scratch* s_;
+  cudaStream_t stream_;
+  Err* err_;
+  bool begun_ = false;
 };
 
 // Launch configuration with a cluster size and programmatic stream

@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
   // -------- 1: routing (by every CTA), then the hidden values --------
   // A logit is the sum of its slices.  Up to 16 tokens: warp w of every CTA
   // routes token w.  More: warp 0 of CTA b routes token b for all, and another
-  // barrier passes the choices on (64 tokens of 128 experts took every CTA 13 us).
+  // barrier passes the choices on (64 tokens of 128 experts: 8 us instead of 15).
   const bool shared_out = p.tokens > WARPS;
   auto each_token = [&](int tok) {
     int my_e;
@@ -774,7 +774,8 @@ apk_status forward(apk_moe* h, const apk_moe_io* io) {
   const size_t pairs = (size_t)io->tokens * c.top_k;
   const size_t b_log = up256((size_t)p.rsplit * io->tokens * c.experts * 4), b_hid = up256(pairs * c.d_ff * 2);
   const size_t b_out = up256(pairs * c.d_model * 4), b_choice = up256(pairs * 8);
-  APK_TRY(h->scratch.begin(256 + b_log + b_hid + b_out + b_choice, 256, s, &h->err));
+  ScratchUse use(&h->scratch, s, &h->err);
+  APK_TRY(use.begin(256 + b_log + b_hid + b_out + b_choice, 256));
   uint8_t* b = h->scratch.data();
   p.x = static_cast<const uint16_t*>(io->x);
   p.router = static_cast<const uint16_t*>(c.router);
@@ -818,7 +819,7 @@ apk_status forward(apk_moe* h, const apk_moe_io* io) {
   cfg.attrs = at;
   cfg.numAttrs = 1;
   APK_TRY(cu_status(cudaLaunchKernelEx(&cfg, moe::moe_layer, p), "launching the expert kernel", &h->err));
-  return h->scratch.end(s, &h->err);
+  return use.end();
 }
 
 }  // namespace

@@ -9,6 +9,7 @@ reference, which multiplies bare matrices (src/tcyield.cu:91-356).
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import torch
 
@@ -82,6 +83,9 @@ class _Handle:
 
     def _open(self, cfg):
         self._lib = L.load()
+        # a layer's argument structures are reused from call to call, and the
+        # interpreter lets other threads run during one
+        self._lock = threading.Lock()
         self._h = ctypes.c_void_p()
         st = getattr(self._lib, self._create)(ctypes.byref(cfg), ctypes.byref(self._h))
         if st != L.APK_OK:
@@ -159,35 +163,36 @@ class Linear(_Handle):
         """act(x W + b) + residual for x [..., in]; with save_preact also
         x W + b in bf16, as backward() takes it.  out: the output's tensor;
         it may be the residual."""
-        io, n = self._io, self.out_features
-        io.x, io.rows, io.ldx = _rows(x, "x", self.device, self.in_features)
-        shape = (io.rows, n) if len(x.shape) == 2 else (*x.shape[:-1], n)
-        if out is None:
-            y = x.new_empty(shape) if self._y_code == L.APK_BF16 else x.new_empty(shape, dtype=self.out_dtype)
-            io.y, io.ldy = y.data_ptr(), n
-        else:
-            y = out
-            if y.shape != shape:
-                raise ValueError(f"out is {tuple(y.shape)}, not {shape}")
-            io.y, _, io.ldy = _rows(y, "out", self.device, n, (self.out_dtype,))
-        if residual is None:
-            io.residual = None
-        else:
-            if residual.shape != shape:
-                raise ValueError(f"residual is {tuple(residual.shape)}, not {shape}")
-            io.residual, _, io.ld_residual = _rows(residual, "residual", self.device, n, _ANY)
-            io.residual_dtype = _CODE[residual.dtype]
-        z = None
-        if save_preact:
-            z = x.new_empty(shape)
-            io.preact, io.ld_preact = z.data_ptr(), n
-        else:
-            io.preact = None
-        io.y_dtype, io.stream = self._y_code, self._stream()
-        st = self._lib.apk_linear_forward(self._h, self._io_ref)
-        if st:
-            self._check(st)
-        return (y, z) if save_preact else y
+        with self._lock:
+            io, n = self._io, self.out_features
+            io.x, io.rows, io.ldx = _rows(x, "x", self.device, self.in_features)
+            shape = (io.rows, n) if len(x.shape) == 2 else (*x.shape[:-1], n)
+            if out is None:
+                y = x.new_empty(shape) if self._y_code == L.APK_BF16 else x.new_empty(shape, dtype=self.out_dtype)
+                io.y, io.ldy = y.data_ptr(), n
+            else:
+                y = out
+                if y.shape != shape:
+                    raise ValueError(f"out is {tuple(y.shape)}, not {shape}")
+                io.y, _, io.ldy = _rows(y, "out", self.device, n, (self.out_dtype,))
+            if residual is None:
+                io.residual = None
+            else:
+                if residual.shape != shape:
+                    raise ValueError(f"residual is {tuple(residual.shape)}, not {shape}")
+                io.residual, _, io.ld_residual = _rows(residual, "residual", self.device, n, _ANY)
+                io.residual_dtype = _CODE[residual.dtype]
+            z = None
+            if save_preact:
+                z = x.new_empty(shape)
+                io.preact, io.ld_preact = z.data_ptr(), n
+            else:
+                io.preact = None
+            io.y_dtype, io.stream = self._y_code, self._stream()
+            st = self._lib.apk_linear_forward(self._h, self._io_ref)
+            if st:
+                self._check(st)
+            return (y, z) if save_preact else y
 
     __call__ = forward
 
@@ -197,36 +202,37 @@ class Linear(_Handle):
         itself); None where one is not needed or the layer has no bias.
         preact: what forward(save_preact=True) returned, for a layer with an
         activation."""
-        g, n, k = self._grads, self.out_features, self.in_features
-        g.dy, g.rows, g.ld_dy = _rows(dy, "dy", self.device, n)
-        if dy.shape[:-1] != x.shape[:-1]:
-            raise ValueError(f"dy is {tuple(dy.shape)} and x {tuple(x.shape)}")
-        g.x, _, g.ldx = _rows(x, "x", self.device, k)
-        if self._act != L.APK_ACT_NONE:
-            if preact is None or preact.shape != dy.shape:
-                raise ValueError("preact: the pre-activation that forward(save_preact=True) returned is wanted")
-            g.preact, _, g.ld_preact = _rows(preact, "preact", self.device, n)
-        else:
-            g.preact = None
-        g.dx = g.dw = g.db = None
-        dx = dw = db = None
-        if need_dx:
-            dx = _like(x, x.shape)
-            g.dx, g.ld_dx = dx.data_ptr(), k
-        if need_dw:
-            dt = _pick(_TORCH, dw_dtype, "dw_dtype")
-            shape = self.weight.shape
-            dw = _like(self.weight, shape) if dt is torch.bfloat16 else self.weight.new_empty(shape, dtype=dt)
-            g.dw, g.ld_dw, g.dw_dtype = dw.data_ptr(), shape[1], _CODE[dt]
-        if need_db and self.bias is not None:
-            db = torch.empty_like(self.bias)
-            g.db = db.data_ptr()
-        g.stream = self._stream()
-        if dx is not None or dw is not None or db is not None:
-            st = self._lib.apk_linear_backward(self._h, self._grads_ref)
-            if st:
-                self._check(st)
-        return dx, dw, db
+        with self._lock:
+            g, n, k = self._grads, self.out_features, self.in_features
+            g.dy, g.rows, g.ld_dy = _rows(dy, "dy", self.device, n)
+            if dy.shape[:-1] != x.shape[:-1]:
+                raise ValueError(f"dy is {tuple(dy.shape)} and x {tuple(x.shape)}")
+            g.x, _, g.ldx = _rows(x, "x", self.device, k)
+            if self._act != L.APK_ACT_NONE:
+                if preact is None or preact.shape != dy.shape:
+                    raise ValueError("preact: the pre-activation that forward(save_preact=True) returned is wanted")
+                g.preact, _, g.ld_preact = _rows(preact, "preact", self.device, n)
+            else:
+                g.preact = None
+            g.dx = g.dw = g.db = None
+            dx = dw = db = None
+            if need_dx:
+                dx = _like(x, x.shape)
+                g.dx, g.ld_dx = dx.data_ptr(), k
+            if need_dw:
+                dt = _pick(_TORCH, dw_dtype, "dw_dtype")
+                shape = self.weight.shape
+                dw = _like(self.weight, shape) if dt is torch.bfloat16 else self.weight.new_empty(shape, dtype=dt)
+                g.dw, g.ld_dw, g.dw_dtype = dw.data_ptr(), shape[1], _CODE[dt]
+            if need_db and self.bias is not None:
+                db = torch.empty_like(self.bias)
+                g.db = db.data_ptr()
+            g.stream = self._stream()
+            if dw is not None or db is not None or (dx is not None and g.rows > 0):
+                st = self._lib.apk_linear_backward(self._h, self._grads_ref)
+                if st:
+                    self._check(st)
+            return dx, dw, db
 
 
 class MoE(_Handle):
@@ -267,21 +273,22 @@ class MoE(_Handle):
     def forward(self, x, return_routing: bool = False):
         """The layer's output for x [..., D]; with return_routing also the
         chosen experts (int32 [..., top_k]) and their weights (fp32)."""
-        io = self._io
-        io.x, io.tokens, io.ldx = _rows(x, "x", self.device, self.d_model)
-        y = _like(x, x.shape) if self._y_code == L.APK_BF16 else x.new_empty(x.shape, dtype=self.out_dtype)
-        io.y, io.ldy, io.y_dtype = y.data_ptr(), self.d_model, self._y_code
-        ids = probs = None
-        if return_routing:
-            shape = (*x.shape[:-1], self.top_k)
-            ids, probs = x.new_empty(shape, dtype=torch.int32), x.new_empty(shape, dtype=torch.float32)
-            io.ids, io.probs = ids.data_ptr(), probs.data_ptr()
-        else:
-            io.ids = io.probs = None
-        io.stream = self._stream()
-        st = self._lib.apk_moe_forward(self._h, self._io_ref)
-        if st:
-            self._check(st)
-        return (y, ids, probs) if return_routing else y
+        with self._lock:
+            io = self._io
+            io.x, io.tokens, io.ldx = _rows(x, "x", self.device, self.d_model)
+            y = _like(x, x.shape) if self._y_code == L.APK_BF16 else x.new_empty(x.shape, dtype=self.out_dtype)
+            io.y, io.ldy, io.y_dtype = y.data_ptr(), self.d_model, self._y_code
+            ids = probs = None
+            if return_routing:
+                shape = (*x.shape[:-1], self.top_k)
+                ids, probs = x.new_empty(shape, dtype=torch.int32), x.new_empty(shape, dtype=torch.float32)
+                io.ids, io.probs = ids.data_ptr(), probs.data_ptr()
+            else:
+                io.ids = io.probs = None
+            io.stream = self._stream()
+            st = self._lib.apk_moe_forward(self._h, self._io_ref)
+            if st:
+                self._check(st)
+            return (y, ids, probs) if return_routing else y
 
     __call__ = forward

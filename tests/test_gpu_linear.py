@@ -326,3 +326,59 @@ def test_c_entry_refuses_what_python_cannot_send():
     assert f(None, None) == L.APK_EINVAL and b(lin._h, None) == L.APK_EINVAL
     torch.cuda.synchronize()
     assert lin.status() == 0
+
+
+def test_a_graph_keeps_its_scratch_when_it_grows():
+    import torch
+    lin, _ = _layer(1001, 333, act="silu", bias="f32")
+    x, dy = _rand(40, 1001, seed=3), _rand(40, 333, seed=4)
+    y, z = lin.forward(x, save_preact=True)
+    want = lin.backward(dy, x, preact=z)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        yg = lin.forward(x)
+        gg = lin.backward(dy, x, preact=z)
+    big, dbig = _rand(900, 1001, seed=5), _rand(900, 333, seed=6)
+    for _ in range(3):
+        lin.backward(dbig, big, preact=lin.forward(big, save_preact=True)[1])
+        filler = torch.full((1 << 22,), -1, dtype=torch.int32, device="cuda")  # would reuse freed memory
+        yg.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(yg, y) and all(torch.equal(a, b) for a, b in zip(gg, want))
+        assert bool((filler == -1).all())
+
+
+def test_threads_share_a_layer():
+    import threading
+
+    import torch
+    lin, _ = _layer(264, 136, act="gelu", bias="bf16")
+    xs = [_rand(10 + 30 * i, 264, seed=i) for i in range(4)]
+    want = [lin.forward(x) for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(200):
+                y = lin.forward(xs[i])
+            torch.cuda.current_stream().synchronize()
+            if not torch.equal(y, want[i]):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and lin.status() == 0
+
+
+def test_no_rows_one_gradient_at_a_time():
+    lin, _ = _layer(16, 8, bias="f32")
+    x, dy = _rand(0, 16, seed=1), _rand(0, 8, seed=2)
+    for need in ("need_dx", "need_dw", "need_db"):
+        got = lin.backward(dy, x, **{n: n == need for n in ("need_dx", "need_dw", "need_db")})
+        assert [g is not None for g in got] == [n == need for n in ("need_dx", "need_dw", "need_db")]
+        assert not any(bool(g.any()) for g in got if g is not None)
