@@ -54,7 +54,7 @@ struct Params {
   int red_stride;  // floats of a warp's place in the shared sums
   int rsplit;    // slices of d_model in phase 0
   int local;     // every CTA computes all logits itself
-  unsigned* barrier;  // {arrived, generation}
+  unsigned* barrier;  // [0] arrivals, [32] their number when this launch began
   int* status;
   long long limit;
   float* logits;  // [rsplit][tokens][experts]
@@ -75,43 +75,31 @@ struct Shared {
   int warp_n[WARPS], warp_rows[WARPS];
   int n_active;
   int abort;
+  unsigned target;  // thread 0: the arrivals that the current barrier waits for
 };
 
 // A grid barrier in two halves, so that loads which do not depend on it can
 // be issued between them (issued before the first, they would delay its
-// fence).  After the second every CTA has arrived, and what it wrote before
-// is visible.  The last to arrive clears the count and advances the
-// generation (on another line, which the others poll), so the words need no
-// reset between launches.
-struct Ticket {
-  unsigned gen;
-  bool last;
-};
-__device__ __forceinline__ Ticket grid_arrive(const Params& p) {
-  Ticket k = {0, false};
+// fence).  After the second every CTA has arrived, and what it wrote before is
+// visible.  One word counts arrivals and is never reset: a barrier is passed
+// when it has grown by the grid's size, so the last arrival itself releases
+// the others.  Another word holds the count at which a launch begins; it is
+// moved on when the launch's last barrier lies behind every CTA.
+__device__ __forceinline__ void grid_arrive(const Params& p, Shared& sh) {
   __syncthreads();
   if (threadIdx.x == 0) {
-    unsigned old;
-    unsigned* const word = p.barrier + 32;
-    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(k.gen) : "l"(word) : "memory");
+    sh.target += gridDim.x;
     __threadfence();
-    asm volatile("atom.relaxed.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(p.barrier) : "memory");
-    k.last = old == gridDim.x - 1;
-    if (k.last) {
-      asm volatile("st.relaxed.gpu.global.u32 [%0], 0;" ::"l"(p.barrier) : "memory");
-      __threadfence();
-      asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(word), "r"(k.gen + 1) : "memory");
-    }
+    asm volatile("red.relaxed.gpu.global.add.u32 [%0], 1;" ::"l"(p.barrier) : "memory");
   }
-  return k;
 }
-__device__ __forceinline__ bool grid_wait(const Params& p, Shared& sh, const Ticket k) {
+__device__ __forceinline__ bool grid_wait(const Params& p, Shared& sh) {
   if (threadIdx.x == 0) {
     long long t0 = 0;
-    for (int n = 1; !k.last; ++n) {
+    for (int n = 1;; ++n) {
       unsigned now;
-      asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(p.barrier + 32) : "memory");
-      if (now != k.gen) break;
+      asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(p.barrier) : "memory");
+      if ((int)(now - sh.target) >= 0) break;
       if ((n & 63) == 0) {
         const long long t = globaltimer_ns();
         if (t0 == 0) t0 = t;
@@ -127,7 +115,14 @@ __device__ __forceinline__ bool grid_wait(const Params& p, Shared& sh, const Tic
   __syncthreads();
   return sh.abort == 0;
 }
-__device__ __forceinline__ bool grid_barrier(const Params& p, Shared& sh) { return grid_wait(p, sh, grid_arrive(p)); }
+__device__ __forceinline__ bool grid_barrier(const Params& p, Shared& sh) {
+  grid_arrive(p, sh);
+  return grid_wait(p, sh);
+}
+// The next launch begins where this one's last barrier ended.
+__device__ __forceinline__ void grid_done(const Params& p, const Shared& sh) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.barrier[32] = sh.target;
+}
 
 struct Frag {
   uint4 a[4], b[4];
@@ -213,16 +208,17 @@ __device__ __forceinline__ void join_warps(float (&acc)[NT8][4], float* red, int
 // Warps that share an item: 1, 2, ... 16, by the least time of a warp in
 // rounds: its items times the rounds of one and about three more for the join
 // and what the loads lose at an item's end.
-__device__ __forceinline__ int warps_per_item(long long items, int k) {
+__device__ __forceinline__ int warps_per_item(unsigned items, int k) {
   int best = 1;
-  long long least = 1ll << 60;
-  const int rounds = (k + ROUND - 1) / ROUND;
-  for (int ws = 1; ws <= WARPS; ws *= 2) {
-    const int slots = gridDim.x * (WARPS / ws);
-    const long long cost = (items + slots - 1) / slots * ((rounds + ws - 1) / ws + 3);
+  unsigned least = ~0u;
+  const unsigned rounds = (k + ROUND - 1) / ROUND;
+#pragma unroll
+  for (int lg = 0; lg <= 4; ++lg) {
+    const unsigned slots = gridDim.x * (WARPS >> lg);
+    const unsigned cost = (items + slots - 1) / slots * (((rounds + (1u << lg) - 1) >> lg) + 3);
     if (cost < least) {
       least = cost;
-      best = ws;
+      best = 1 << lg;
     }
   }
   return best;
@@ -249,18 +245,6 @@ struct Walk {
     return {ws, bulk + warp / ws * (int)gridDim.x + (int)blockIdx.x, items, (int)gridDim.x * (WARPS / ws)};
   }
 };
-
-// Starts bringing a warp's first rows into L2, past the round that is loaded
-// already: while a barrier is waited for, memory would be idle.  A kilobyte a
-// row keeps it busy for about that time (38 MB over the chip).
-__device__ __forceinline__ void prefetch_rows(const Rows w, int t, int k, int ws) {
-  constexpr int LEAD = 512;
-  if (ws != 1 || t > 1) return;
-  const uint16_t* r = t ? w.w1 : w.w0;
-  const int n = min(k - ROUND, LEAD);
-  if (n > 0)
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(r + ROUND), "r"((n & ~7) * 2) : "memory");
-}
 
 // Rows of expert a's tile in the first product.  Gated: MMA row g is gate
 // f0 + g and row g + 8 its up; else features f0 + g and f0 + g + 8.
@@ -454,9 +438,9 @@ __device__ __forceinline__ bool one_token_out(const Params& p, Shared& sh, float
     load_round<ROWS == 16>(f, w + r0 * p.f, w + r1 * p.f, (u - j * rounds) * ROUND, t, p.f);
   };
   Frag f;
-  const Ticket ticket = grid_arrive(p);
+  grid_arrive(p, sh);
   if (warp < units && (int)blockIdx.x * ROWS < p.d) load(f, blockIdx.x, warp);
-  if (!grid_wait(p, sh, ticket)) return false;
+  if (!grid_wait(p, sh)) return false;
   for (int tile = blockIdx.x; tile * ROWS < p.d; tile += gridDim.x) {
     float s0 = 0.f, s1 = 0.f;
     for (int u = warp; u < units; u += WARPS) {
@@ -499,7 +483,10 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
   extern __shared__ float red[];
   __shared__ Shared sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  if (tid == 0) sh.abort = 0;
+  if (tid == 0) {
+    sh.abort = 0;
+    sh.target = *reinterpret_cast<volatile unsigned*>(p.barrier + 32);
+  }
   for (int e = tid; e < p.experts; e += THREADS) sh.mask[e] = 0;
 
   // -------- 0: logits --------
@@ -577,9 +564,12 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
     }
     __syncthreads();
     int a = __popc(some & ((1u << lane) - 1)), r = rows - n;
-    for (int w = 0; w < warp; ++w) {
-      a += sh.warp_n[w];
-      r += sh.warp_rows[w];
+    if (n > 0 || tid == THREADS - 1) {
+      const int before = min(warp, (p.experts + 31) / 32);  // warps with experts below this one
+      for (int w = 0; w < before; ++w) {
+        a += sh.warp_n[w];
+        r += sh.warp_rows[w];
+      }
     }
     if (n > 0) {
       sh.active[a] = (short)tid;
@@ -633,24 +623,23 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
 
   // -------- 2: output rows of the pairs --------
   if (p.tokens == 1) {
-    if ((p.d + 7) / 8 <= 2 * (int)gridDim.x) one_token_out<8>(p, sh, red);
-    else one_token_out<16>(p, sh, red);
+    const bool ok = (p.d + 7) / 8 <= 2 * (int)gridDim.x ? one_token_out<8>(p, sh, red) : one_token_out<16>(p, sh, red);
+    if (ok) grid_done(p, sh);
     return;
   }
   {
     const int tiles = (p.d + 15) / 16;
     const Walk walk(n_active * tiles, p.f);
     const int start = walk.bulk ? 0 : 1;
-    const Ticket ticket = grid_arrive(p);
+    grid_arrive(p, sh);
     for (int part = start; part < 2; ++part) {
       const Walk::Part q = walk.part(part, warp);
       Rows w = {};
       if (q.first < q.end) {  // (the first part's weights travel while the barrier is waited for)
         w = rows_out(p, sh, q.first / tiles, q.first % tiles, g);
         load_round(frag, w.w0, w.w1, (warp & (q.ws - 1)) * ROUND, t, p.f);
-        if (part == start) prefetch_rows(w, t, p.f, q.ws);
       }
-      if (part == start && !grid_wait(p, sh, ticket)) return;
+      if (part == start && !grid_wait(p, sh)) return;
       for (int it = q.first; it < q.end; it += q.step) {
         const int a = it / tiles, next = it + q.step;
         const Rows wn = next < q.end ? rows_out(p, sh, next / tiles, next % tiles, g) : Rows{};
@@ -662,6 +651,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
     }
   }
   if (!grid_barrier(p, sh)) return;
+  grid_done(p, sh);
 
   // -------- 3: weighted sum --------
   const int quads = p.d / 4;
