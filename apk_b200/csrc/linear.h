@@ -60,18 +60,19 @@ struct Product {
 // Launches one or two products, in one launch where that is faster. sms: the SMs it may
 // fill; dev: the current device.
 // `why` receives a message on failure.
-// Whether a product is faster through run_stream than through run_products.  Up to 8 rows
-// [n][k] weights always are (8 x 4096 x 8192: 13.7 against 15.6 us); two MMA
-// tiles of rows, or the narrower row pieces of [k][n], cost it bandwidth, so
-// that only its smaller latency counts (16 x 2048 x 2048: 5.3 against 7.0 us;
-// 16 x 4096 x 8192: 19.8 against 15.7; [k][n] 8 x 4096 x 8192: 21 against 15.2,
-// 1 x 2048 x 2048: 5.3 against 6.8).  Weights that TMA cannot address save it
-// their copy.
+// Whether a product is faster through run_stream than through run_products.
+// Up to 8 rows [n][k] weights always are (8 x 4096 x 8192: 14.0 against 15.6
+// us).  Two MMA tiles of rows, or the narrower row pieces of [k][n], cost it
+// bandwidth, so that only its smaller latency counts (16 rows, [n][k]: 2048 x
+// 2048 3.2 against 7.0, 2048 x 4096 6.1 against 7.4, 4096 x 8192 20.6 against
+// 16.1; [k][n]: 1 x 2048 x 2048 5.2 against 6.8, 8 x 2048 x 4096 8.4 against
+// 7.4, 8 x 4096 x 8192 21.2 against 15.1).  Weights that TMA cannot address
+// save it their copy.
 inline bool streams(int rows, long long weight_bytes, bool nk, bool tma) {
   if (rows > 16) return false;
   const long long mb = weight_bytes >> 20;
   if (!tma) return mb < 16;
-  return nk ? rows <= 8 || mb < 16 : mb < (rows <= 8 ? 16 : 4);
+  return nk ? rows <= 8 || mb < 24 : mb < (rows <= 8 ? 16 : 4);
 }
 apk_status run_products(const Product* pr, int n, int sms, int dev, int* status, long long limit, cudaStream_t stream,
                         std::string* why);
