@@ -37,7 +37,8 @@
 // the epilogue warps add the pieces in registers with rounding.
 //
 // Every wait is bounded; one that runs out raises the status word and lets
-// every role unwind.
+// every role unwind: nothing leaves (shared memory, TMEM) before the loads and
+// MMAs in flight have ended, whichever role gave up.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -132,7 +133,16 @@ struct __align__(16) Shared {
   int abort;
 };
 
-template <int S>
+// The CTA that gives up tells the other one of its pair, whose waits depend on it.
+template <int CG, int S>
+__device__ __forceinline__ void give_up(Shared<S>& sh) {
+  *reinterpret_cast<volatile int*>(&sh.abort) = 1;
+  if constexpr (CG == 2)
+    asm volatile("st.volatile.shared::cluster.u32 [%0], %1;" ::"r"(map_rank(smem_u32(&sh.abort), cluster_rank() ^ 1)),
+                 "r"(1)
+                 : "memory");
+}
+template <int CG, int S>
 __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t parity, const GemmParams& p, Shared<S>& sh, int code) {
   if (try_wait_cluster(bar, parity)) return true;
   const long long t0 = globaltimer_ns();
@@ -143,16 +153,16 @@ __device__ __forceinline__ bool bwait(uint64_t* bar, uint32_t parity, const Gemm
       n = 0;
       if (*reinterpret_cast<volatile int*>(&sh.abort)) return false;
       if (globaltimer_ns() - t0 > p.limit) {
-        *reinterpret_cast<volatile int*>(&sh.abort) = 1;
+        give_up<CG>(sh);
         report_status(p.status, code, nullptr);
         return false;
       }
     }
   }
 }
-// While unwinding: up to a second, however short the caller's limit is.
-__device__ __forceinline__ void bwait_unwind(uint64_t* bar, uint32_t parity) {
-  const long long t0 = globaltimer_ns();
+// At a role's end, for what it has in flight: until a second after t0, however
+// short the caller's limit is.
+__device__ __forceinline__ void bwait_end(uint64_t* bar, uint32_t parity, long long t0) {
   while (!try_wait_cluster(bar, parity))
     if (globaltimer_ns() - t0 > 1000000000ll) return;
 }
@@ -412,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
       r0 += C::QROWS * (int)prank;
       for (; kb < ke; ++kb, ++P) {
         const int s = P % S;
-        ok = bwait(&sh.empty[s], ((P / S) & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_FULL);
+        ok = bwait<CG>(&sh.empty[s], ((P / S) & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_FULL);
         if (!ok) break;
         // both CTAs' loads of a pair complete on the leader's barrier
         uint32_t bar = smem_u32(&sh.full[s]);
@@ -440,14 +450,12 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
         }
       }
     }
-    if (!ok) {
-      // unwinding: the loads in flight land before the shared memory goes away
-      if (leader)
-        for (uint32_t q = P > (uint32_t)S ? P - S : 0; q < P; ++q) bwait_unwind(&sh.full[q % S], (q / S) & 1);
-      // (a pair's second CTA has no barrier of its own to ask: a millisecond is
-      // a thousand times what a load takes)
+    // The loads in flight land before the shared memory goes away.  They have
+    // landed already unless another role gave up, which this one may not have
+    // noticed.  (A pair's loads complete on the leader's barriers.)
+    if (leader) {
       const long long t0 = globaltimer_ns();
-      while (CG == 2 && globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
+      for (uint32_t q = P > (uint32_t)S ? P - S : 0; q < P; ++q) bwait_end(&sh.full[q % S], (q / S) & 1, t0);
     }
   } else if (warp == 1 && lane == 0 && leader) {
     // =================================== MMA ===================================
@@ -470,7 +478,7 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
       const uint32_t idesc = pr.idesc;
       const uint32_t p_step = pr.p_mn ? 2048 : 32, q_step = pr.q_mn ? 2048 : 32;
       const uint32_t p_lbo = pr.p_mn ? 8192 : 16, q_lbo = pr.q_mn ? 8192 : 16;
-      auto full = [&](uint32_t i) { return bwait(&sh.full[i % S], (i / S) & 1, p, sh, DEV_WAIT_TIMEOUT_FULL); };
+      auto full = [&](uint32_t i) { return bwait<CG>(&sh.full[i % S], (i / S) & 1, p, sh, DEV_WAIT_TIMEOUT_FULL); };
       // stage i's MMAs with the h-th 128 columns of each CTA into accumulator buf
       auto mmas = [&](uint32_t i, int h, int buf, bool first) {
         const uint32_t sp = smem_u32(ring + (i % S) * C::STAGE) + h * P_BYTES, sq = smem_u32(ring + (i % S) * C::STAGE) + C::Q_AT;
@@ -483,7 +491,7 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
       if constexpr (FM == 1) {
         for (int c = 0; c < pieces(n) && ok; ++c, ++U) {
           const int buf = U % C::NBUF, i0 = EXACT ? c * EXACT_KB : 0, i1 = EXACT ? min(n, i0 + EXACT_KB) : n;
-          ok = bwait(&sh.tempty[buf], ((U / C::NBUF) & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
+          ok = bwait<CG>(&sh.tempty[buf], ((U / C::NBUF) & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
           if (!ok) break;
           tc::fence_after_sync();
           for (int i = i0; i < i1; ++i, ++Q) {
@@ -497,14 +505,14 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
       } else {
         // stages i = 0 .. w: accumulator 0 first; n - l .. n: 0 before 1
         const int w = n < S - 1 ? n : S - 1, l = n - w < S - 1 ? n - w : S - 1;
-        ok = bwait(&sh.tempty[0], (T & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
+        ok = bwait<CG>(&sh.tempty[0], (T & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
         if (!ok) break;
         tc::fence_after_sync();
         for (int i = 0; i < w && ok; ++i) {
           ok = full(Q + i);
           if (ok) mmas(Q + i, 0, 0, i == 0);
         }
-        ok = ok && bwait(&sh.tempty[1], (T & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
+        ok = ok && bwait<CG>(&sh.tempty[1], (T & 1) ^ 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
         if (!ok) break;
         tc::fence_after_sync();
         if (l == 0) commit_all(&sh.tfull[0]);
@@ -533,10 +541,10 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
         Q += n;
       }
     }
-    if (!ok) {
-      commit_to<CG>(smem_u32(&sh.drain));
-      bwait_unwind(&sh.drain, 0);
-    }
+    // The MMAs in flight end before the tensor memory and the operands go
+    // away.  The epilogue has waited for them, unless it gave up.
+    commit_to<CG>(smem_u32(&sh.drain));
+    bwait_end(&sh.drain, 0, globaltimer_ns());
   } else if (warp >= 2) {
     // ================================ epilogue ================================
     constexpr int W = NT >= 64 ? 32 : 8;  // rows of one TMEM load
@@ -559,7 +567,7 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
       if (has_res && r0 + g * W < pr.rows) load_residual<W>(e, raw, r0 + g * W, 1, pr.rows - r0 - g * W, c);
       const uint32_t tcol = tbase + ((uint32_t)(32 * q) << 16);
       auto wait_acc = [&]() {
-        const bool ok = bwait(&sh.tfull[U % C::NBUF], (U / C::NBUF) & 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
+        const bool ok = bwait<CG>(&sh.tfull[U % C::NBUF], (U / C::NBUF) & 1, p, sh, DEV_WAIT_TIMEOUT_TMEM);
         tc::fence_after_sync();
         return ok;
       };
@@ -661,7 +669,16 @@ __global__ void __launch_bounds__(THREADS, 1) lin_gemm(const __grid_constant__ G
       }
     }
   }
-  if constexpr (CG == 2) cluster_sync();  // no access reaches a CTA that has left
+  if constexpr (CG == 2) {
+    cluster_sync();  // no access reaches a CTA that has left
+    // After a wait ran out the leader may have stopped before it expected the
+    // other CTA's last loads, so that no barrier tells when they have landed: a
+    // millisecond is a thousand times what a load takes.
+    if (warp == 0 && *reinterpret_cast<volatile int*>(&sh.abort)) {
+      const long long t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
+    }
+  }
   if (warp == 1) {
     __syncwarp();
     tc::fence_after_sync();
