@@ -57,6 +57,16 @@ apk_status Scratch::end(cudaStream_t stream, Err* err) {
   return APK_OK;
 }
 
+apk_status Scratch::clear(size_t bytes, cudaStream_t stream, Err* err) {
+  std::vector<uint8_t*> all = kept_;
+  if (p_) all.push_back(p_);
+  for (uint8_t* q : all) {
+    const apk_status st = cu_status(cudaMemsetAsync(q, 0, bytes, stream), "clearing the scratch", err);
+    if (st != APK_OK) return st;
+  }
+  return cu_status(cudaStreamSynchronize(stream), "cudaStreamSynchronize", err);
+}
+
 void Scratch::release() {
   if (p_) cudaFree(p_);  // waits for the device
   for (uint8_t* q : kept_) cudaFree(q);

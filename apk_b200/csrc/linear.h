@@ -127,6 +127,8 @@ class Scratch {
   apk_status begin(size_t bytes, size_t zeroed, cudaStream_t stream, Err* err);
   apk_status end(cudaStream_t stream, Err* err);
   uint8_t* data() const { return p_; }
+  // Zeroes the first `bytes` of every buffer, those of graphs too, and waits for it.
+  apk_status clear(size_t bytes, cudaStream_t stream, Err* err);
   void release();
 
  private:

@@ -93,10 +93,13 @@ __device__ __forceinline__ void grid_arrive(const Params& p, Shared& sh) {
     asm volatile("red.relaxed.gpu.global.add.u32 [%0], 1;" ::"l"(p.barrier) : "memory");
   }
 }
+// False: a barrier of this launch, or one before it that apk_moe_status has
+// not been asked about, ran out.  The count is of no use then, and a CTA that
+// went on by it could read what others have yet to write.
 __device__ __forceinline__ bool grid_wait(const Params& p, Shared& sh) {
   if (threadIdx.x == 0) {
     long long t0 = 0;
-    for (int n = 1;; ++n) {
+    for (int n = 1; !sh.abort; ++n) {
       unsigned now;
       asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(p.barrier) : "memory");
       if ((int)(now - sh.target) >= 0) break;
@@ -484,7 +487,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
   __shared__ Shared sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   if (tid == 0) {
-    sh.abort = 0;
+    sh.abort = *reinterpret_cast<volatile int*>(p.status) != 0;
     sh.target = *reinterpret_cast<volatile unsigned*>(p.barrier + 32);
   }
   for (int e = tid; e < p.experts; e += THREADS) sh.mask[e] = 0;
@@ -539,7 +542,8 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
     if (!grid_barrier(p, sh)) return;
     for (int i = tid; i < p.tokens * p.top_k; i += THREADS) {
       const float2 c = __ldcg(p.choice + i);
-      const int e = __float_as_int(c.x);
+      // (an index even if, against the rules, another launch uses this buffer at the same time)
+      const int e = (int)min(__float_as_uint(c.x), (unsigned)p.experts - 1);
       sh.sel[i] = (short)e;
       sh.prob[i] = c.y;
       atomicOr(&sh.mask[e], 1ull << (i / p.top_k));
@@ -586,7 +590,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
   }
   __syncthreads();
   const int n_active = sh.n_active;
-  if (blockIdx.x == 0) {
+  if (blockIdx.x == 0 && !sh.abort) {
     for (int i = tid; i < p.tokens * p.top_k; i += THREADS) {
       if (p.ids) p.ids[i] = sh.sel[i];
       if (p.probs) p.probs[i] = sh.prob[i];
@@ -860,12 +864,9 @@ apk_status apk_moe_status(apk_moe* h, void* stream, int* device_status) {
                       &h->err));
     APK_TRY(cu_status(cudaMemsetAsync(h->status, 0, sizeof(int), s), "status clear", &h->err));
     APK_TRY(cu_status(cudaStreamSynchronize(s), "cudaStreamSynchronize", &h->err));
-    // a barrier that was given up has left its words half counted
-    if (*device_status != 0 && h->scratch.data()) {
-      APK_TRY(cu_status(cudaMemsetAsync(h->scratch.data(), 0, 256, s), "barrier clear", &h->err));
-      APK_TRY(cu_status(cudaStreamSynchronize(s), "cudaStreamSynchronize", &h->err));
-    }
-    return APK_OK;
+    // a barrier that was given up has left its words half counted, a graph's in
+    // the buffer that it was captured with
+    return *device_status != 0 ? h->scratch.clear(256, s, &h->err) : APK_OK;
   } catch (...) {
     return APK_ENOMEM;
   }

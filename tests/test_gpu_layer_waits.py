@@ -1,6 +1,7 @@
 """Layer operators whose device waits run out.  A limit of one nanosecond makes
 ordinary waits give up (nothing is faulted or held up): the kernel has to end
 by itself, report a status and leave the GPU as it found it."""
+import ctypes
 import time
 
 import pytest
@@ -74,3 +75,55 @@ def test_gradients_that_give_up_end(layout, sms):
     for g, (ref, bound), what in zip((got[0], got[1] if layout == "kn" else got[1].t(), got[2]), want, ("dx", "dw", "db")):
         lb.check(g, ref, bound, what)
     assert lin.status() == 0
+
+
+def _slow_moe(wait_limit_ns, tokens=1):
+    """One expert of 8 hidden values over 2^20 inputs: one CTA reads it for a
+    few hundred microseconds while the others wait at the grid barrier."""
+    import apk_b200
+    D = 1 << 20
+    moe = apk_b200.MoE(_rand(1, D, seed=1, scale=D ** -0.5), _rand(1, 16, D, seed=2, scale=D ** -0.5),
+                       _rand(1, D, 8, seed=3, scale=8 ** -0.5), top_k=1, wait_limit_ns=wait_limit_ns)
+    return moe, _rand(tokens, D, seed=4)
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 20])
+def test_a_grid_barrier_that_gives_up_every_time(tokens):
+    import torch
+
+    from apk_b200 import _lib as L
+    moe, x = _slow_moe(1, tokens)
+    for _ in range(3):
+        # a barrier whose words were left half counted would let a second call pass
+        moe.forward(x)
+        assert moe.status() == 3 and moe.status() == 0
+    # until status() has been asked, further calls touch no output
+    moe.forward(x)
+    y, ids, probs = moe.forward(x, return_routing=True)
+    y.fill_(7.0)
+    io = L.MoeIO(x=x.data_ptr(), ldx=x.shape[1], tokens=tokens, y=y.data_ptr(), ldy=x.shape[1], y_dtype=L.APK_BF16,
+                 stream=torch.cuda.current_stream().cuda_stream)
+    assert moe._lib.apk_moe_forward(moe._h, ctypes.byref(io)) == L.APK_OK
+    torch.cuda.synchronize()
+    assert bool((y == 7.0).all())
+    assert moe.status() == 3
+    ok, _ = _slow_moe(0, tokens)
+    first = ok.forward(x)
+    assert bool(torch.isfinite(first).all()) and torch.equal(first, ok.forward(x)) and ok.status() == 0
+
+
+def test_a_graph_whose_barrier_gave_up_starts_anew():
+    import torch
+    moe, x = _slow_moe(1)
+    moe.forward(x)
+    assert moe.status() == 3
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        moe.forward(x)
+    more = _rand(20, x.shape[1], seed=5)
+    moe.forward(more)                                # the scratch grows: the graph has a buffer of its own
+    assert moe.status() == 3
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert moe.status() == 3 and moe.status() == 0
