@@ -12,72 +12,6 @@
 
 namespace apk {
 
-apk_status cu_status(cudaError_t e, const char* what, Err* err) {
-  if (e == cudaSuccess) return APK_OK;
-  return err->fail(e == cudaErrorMemoryAllocation ? APK_ENOMEM : APK_ECUDA, "%s: %s", what, cudaGetErrorString(e));
-}
-
-apk_status Scratch::begin(size_t bytes, size_t zeroed, cudaStream_t stream, Err* err) {
-  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  apk_status st = cu_status(cudaStreamIsCapturing(stream, &cap), "cudaStreamIsCapturing", err);
-  if (st != APK_OK) return st;
-  capturing_ = cap != cudaStreamCaptureStatusNone;
-  if (bytes > bytes_) {
-    if (capturing_)
-      return err->fail(APK_ESTATE, "the scratch has to grow to %zu bytes: make one call of this size before the capture",
-                       bytes);
-    if (ev_ && used_ && (st = cu_status(cudaEventSynchronize(ev_), "waiting for the scratch", err)) != APK_OK) return st;
-    used_ = false;
-    if (p_ && captured_) kept_.push_back(p_);
-    else if (p_) cudaFree(p_);
-    p_ = nullptr;
-    bytes_ = 0;
-    captured_ = false;
-    void* q = nullptr;
-    if ((st = cu_status(cudaMalloc(&q, bytes), "cudaMalloc(scratch)", err)) != APK_OK) return st;
-    p_ = static_cast<uint8_t*>(q);
-    if ((st = cu_status(cudaMemset(p_, 0, zeroed), "cudaMemset", err)) != APK_OK) return st;
-    // the memset of the legacy stream is not ordered before a non-blocking stream's work
-    if ((st = cu_status(cudaStreamSynchronize(nullptr), "cudaStreamSynchronize", err)) != APK_OK) return st;
-    bytes_ = bytes;
-  }
-  captured_ = captured_ || capturing_;
-  // (on the same stream too: a handle's value may name another stream by now)
-  if (!capturing_ && used_) return cu_status(cudaStreamWaitEvent(stream, ev_, 0), "cudaStreamWaitEvent", err);
-  return APK_OK;
-}
-
-apk_status Scratch::end(cudaStream_t stream, Err* err) {
-  if (capturing_) return APK_OK;
-  apk_status st = APK_OK;
-  if (!ev_ && (st = cu_status(cudaEventCreateWithFlags(&ev_, cudaEventDisableTiming), "cudaEventCreate", err)) != APK_OK)
-    return st;
-  if ((st = cu_status(cudaEventRecord(ev_, stream), "cudaEventRecord", err)) != APK_OK) return st;
-  used_ = true;
-  return APK_OK;
-}
-
-apk_status Scratch::clear(size_t bytes, cudaStream_t stream, Err* err) {
-  std::vector<uint8_t*> all = kept_;
-  if (p_) all.push_back(p_);
-  for (uint8_t* q : all) {
-    const apk_status st = cu_status(cudaMemsetAsync(q, 0, bytes, stream), "clearing the scratch", err);
-    if (st != APK_OK) return st;
-  }
-  return cu_status(cudaStreamSynchronize(stream), "cudaStreamSynchronize", err);
-}
-
-void Scratch::release() {
-  if (p_) cudaFree(p_);  // waits for the device
-  for (uint8_t* q : kept_) cudaFree(q);
-  kept_.clear();
-  if (ev_) cudaEventDestroy(ev_);
-  p_ = nullptr;
-  ev_ = nullptr;
-  bytes_ = 0;
-  used_ = false;
-}
-
 namespace lin {
 
 __device__ __forceinline__ uint16_t f2bf(float v) {
@@ -285,7 +219,6 @@ struct apk_linear {
   apk_linear_config cfg{};
   Err err;
   int sms = 0;
-  int* status = nullptr;  // device word
   Scratch scratch;
   std::mutex mu;  // calls from several host threads are taken one at a time
 };
@@ -354,11 +287,12 @@ apk_status forward(apk_linear* h, const apk_linear_io* io) {
   if (lin::streams(M, (long long)K * N * 2, c.w_layout == APK_W_NK, tma_ok(c.W, c.ldw, w_outer)))
     return cu_status(lin::run_stream(io->x, io->ldx, c.W, c.ldw, c.w_layout == APK_W_NK, M, N, K, epi, h->sms, s),
                      "launching the streaming kernel", &h->err);
+  APK_TRY(h->scratch.enter(s, &h->err));
   const void* x = io->x;
   const void* w = c.W;
   long long ldx = io->ldx, ldw = c.ldw;
   const bool px = !tma_ok(x, ldx, M), pw = !tma_ok(w, ldw, w_outer);
-  ScratchUse use(&h->scratch, s, &h->err);
+  ScratchUse use(&h->scratch, &h->err);
   if (px || pw) {
     const size_t bx = px ? up256((size_t)M * up8(K) * 2) : 0, bw = pw ? up256((size_t)w_outer * up8(w_inner) * 2) : 0;
     const size_t zeroed = up256((size_t)(N + lin::DZ_COLS - 1) / lin::DZ_COLS * 4);
@@ -375,7 +309,7 @@ apk_status forward(apk_linear* h, const apk_linear_io* io) {
   p.cols = N;
   p.k = K;
   p.epi = epi;
-  APK_TRY(lin::run_products(&p, 1, h->sms, c.device, h->status, c.wait_limit_ns, s, &h->err.text));
+  APK_TRY(lin::run_products(&p, 1, h->sms, c.device, h->scratch.status(), c.wait_limit_ns, s, &h->err.text));
   return use.end();
 }
 
@@ -408,6 +342,7 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
     if (g->db) APK_TRY(cu_status(cudaMemsetAsync(g->db, 0, (size_t)N * esize[c.bias_dtype], s), "clearing db", &h->err));
     return APK_OK;
   }
+  APK_TRY(h->scratch.enter(s, &h->err));
   const bool act = c.act != APK_ACT_NONE;
   const bool products = g->dx || g->dw;
   const bool own_dz = products && (act || !tma_ok(g->dy, g->ld_dy, M));
@@ -421,7 +356,7 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
   const size_t bpart = g->db ? up256((size_t)rblocks * up8(N) * 4) : 0;
   const size_t bdz = own_dz ? up256((size_t)M * up8(N) * 2) : 0;
   const size_t bx = px ? up256((size_t)M * up8(K) * 2) : 0, bw = pw ? up256((size_t)w_outer * up8(w_inner) * 2) : 0;
-  ScratchUse use(&h->scratch, s, &h->err);
+  ScratchUse use(&h->scratch, &h->err);
   if (g->db || own_dz || px || pw) APK_TRY(use.begin(zeroed + bpart + bdz + bx + bw, zeroed));
   uint8_t* base = h->scratch.data();
   const void* x = g->x;
@@ -482,7 +417,7 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
     a.k = M;
     a.epi = {nullptr, nullptr, g->dw, nullptr, 0, g->ld_dw, 0, 0, 0, g->dw_dtype == APK_F32, APK_ACT_NONE};
   }
-  if (n) APK_TRY(lin::run_products(p, n, h->sms, c.device, h->status, c.wait_limit_ns, s, &h->err.text));
+  if (n) APK_TRY(lin::run_products(p, n, h->sms, c.device, h->scratch.status(), c.wait_limit_ns, s, &h->err.text));
   return use.end();
 }
 
@@ -516,11 +451,7 @@ apk_status create(const apk_linear_config* cfg, apk_linear* h) {
   h->sms = sms;
   if (c.sms < 0 || c.sms > sms) return h->err.fail(APK_EINVAL, "sms %d of %d", c.sms, sms);
   if (c.sms > 0) h->sms = c.sms;
-  void* st = nullptr;
-  APK_TRY(cu_status(cudaMalloc(&st, 256), "cudaMalloc", &h->err));
-  h->status = static_cast<int*>(st);
-  APK_TRY(cu_status(cudaMemset(st, 0, 256), "cudaMemset", &h->err));
-  return cu_status(cudaStreamSynchronize(nullptr), "cudaStreamSynchronize", &h->err);
+  return h->scratch.open(c.device, &h->err);
 }
 
 }  // namespace
@@ -540,11 +471,6 @@ apk_status apk_linear_create(const apk_linear_config* cfg, apk_linear** out) {
 
 apk_status apk_linear_destroy(apk_linear* h) {
   if (!h) return APK_OK;
-  if (h->status) {
-    DeviceGuard guard(h->cfg.device);
-    h->scratch.release();
-    cudaFree(h->status);
-  }
   delete h;
   return APK_OK;
 }
@@ -552,7 +478,7 @@ apk_status apk_linear_destroy(apk_linear* h) {
 const char* apk_linear_last_error(const apk_linear* h) { return h ? h->err.text.c_str() : "NULL handle"; }
 
 apk_status apk_linear_forward(apk_linear* h, const apk_linear_io* io) {
-  if (!h || !h->status || !io) return APK_EINVAL;
+  if (!h || !h->scratch.status() || !io) return APK_EINVAL;
   try {
     std::lock_guard<std::mutex> lock(h->mu);
     return forward(h, io);
@@ -562,7 +488,7 @@ apk_status apk_linear_forward(apk_linear* h, const apk_linear_io* io) {
 }
 
 apk_status apk_linear_backward(apk_linear* h, const apk_linear_grads* g) {
-  if (!h || !h->status || !g) return APK_EINVAL;
+  if (!h || !h->scratch.status() || !g) return APK_EINVAL;
   try {
     std::lock_guard<std::mutex> lock(h->mu);
     return backward(h, g);
@@ -572,14 +498,14 @@ apk_status apk_linear_backward(apk_linear* h, const apk_linear_grads* g) {
 }
 
 apk_status apk_linear_status(apk_linear* h, void* stream, int* device_status) {
-  if (!h || !h->status || !device_status) return APK_EINVAL;
+  if (!h || !h->scratch.status() || !device_status) return APK_EINVAL;
   try {
     std::lock_guard<std::mutex> lock(h->mu);
     DeviceGuard guard(h->cfg.device);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    APK_TRY(cu_status(cudaMemcpyAsync(device_status, h->status, sizeof(int), cudaMemcpyDeviceToHost, s), "status copy",
+    APK_TRY(cu_status(cudaMemcpyAsync(device_status, h->scratch.status(), sizeof(int), cudaMemcpyDeviceToHost, s), "status copy",
                       &h->err));
-    APK_TRY(cu_status(cudaMemsetAsync(h->status, 0, sizeof(int), s), "status clear", &h->err));
+    APK_TRY(cu_status(cudaMemsetAsync(h->scratch.status(), 0, sizeof(int), s), "status clear", &h->err));
     return cu_status(cudaStreamSynchronize(s), "cudaStreamSynchronize", &h->err);
   } catch (...) {
     return APK_ENOMEM;

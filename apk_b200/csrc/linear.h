@@ -7,6 +7,7 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <memory>
 #include <string>
 #include <vector>
 
@@ -115,54 +116,98 @@ class DeviceGuard {
   int old_ = -1;
 };
 
-// Device scratch of one handle.  Calls on one handle may come from different
-// streams: a call that uses the scratch waits for the last one that did.  In
-// a stream capture the events are left out (the order of a graph's launches
-// and of other calls is the caller's), and the scratch may not grow; a
-// buffer that a graph refers to is kept until the handle is destroyed.
-class Scratch {
+// Device memory that a handle's calls and the graphs captured from them share.
+// It is freed some time after the last of them has let go of it.
+class Memory {
  public:
-  // At least `bytes` of scratch, the first `zeroed` of them zero when it was
-  // allocated and left so by every kernel that uses them.
-  apk_status begin(size_t bytes, size_t zeroed, cudaStream_t stream, Err* err);
-  apk_status end(cudaStream_t stream, Err* err);
-  uint8_t* data() const { return p_; }
-  // Zeroes the first `bytes` of every buffer, those of graphs too, and waits for it.
-  apk_status clear(size_t bytes, cudaStream_t stream, Err* err);
-  void release();
+  // The first `zeroed` bytes are zero.  May be called while a stream is captured.
+  static apk_status make(int device, size_t bytes, size_t zeroed, std::shared_ptr<Memory>* out, Err* err);
+  // `graph`, and what is instantiated from it, hold m until they are destroyed.
+  static apk_status keep_for(cudaGraph_t graph, const std::shared_ptr<Memory>& m, Err* err);
+  static void free_gone();
+  Memory() = default;
+  Memory(const Memory&) = delete;
+  ~Memory();
+  uint8_t* data() const { return data_; }
+  size_t bytes() const { return bytes_; }
 
  private:
-  uint8_t* p_ = nullptr;
+  int device_ = 0;
+  uint8_t* data_ = nullptr;
   size_t bytes_ = 0;
+};
+
+// Status word and scratch of one handle.
+//
+// Calls on one handle may come from different streams: a call that uses the
+// scratch waits for the last one that did.  Nothing could order a graph's
+// launches with them, or with another graph's, so the calls of one capture get
+// scratch of their own, which lives as long as the graph does; branches of one
+// capture are ordered by an edge between their calls.  What a capture
+// allocates is bounded by what calls outside captures have needed: a larger
+// call is refused.
+class Scratch {
+ public:
+  Scratch() = default;
+  Scratch(const Scratch&) = delete;
+  ~Scratch();
+  apk_status open(int device, Err* err);  // allocates the status word
+  int* status() const { return status_ ? reinterpret_cast<int*>(status_->data()) : nullptr; }
+  // The first thing of every call that uses the status word or the scratch.
+  apk_status enter(cudaStream_t stream, Err* err);
+  // At least `bytes` of scratch, the first `zeroed` of them zero when it was
+  // allocated and left so by every kernel that uses them.
+  apk_status begin(size_t bytes, size_t zeroed, Err* err);
+  apk_status end(Err* err);
+  uint8_t* data() const { return data_; }
+  // Zeroes the first `bytes` of every buffer, those of graphs too, and waits for it.
+  apk_status clear(size_t bytes, cudaStream_t stream, Err* err);
+
+ private:
+  struct Captured {
+    unsigned long long capture = 0;
+    std::weak_ptr<Memory> memory;
+    cudaEvent_t ev = nullptr;      // the last call of the capture that used it
+    cudaStream_t last = nullptr;   // and its stream
+  };
+  int device_ = 0;
+  std::shared_ptr<Memory> status_, own_;
+  size_t most_ = 0;  // bytes that a call outside captures needed
   cudaEvent_t ev_ = nullptr;
-  bool used_ = false, capturing_ = false, captured_ = false;
-  std::vector<uint8_t*> kept_;  // earlier buffers that graphs refer to
+  bool used_ = false;
+  std::vector<Captured> captured_;
+  unsigned long long capture_ = 0;  // whose graph holds the status word
+  // of the call under way
+  cudaStream_t stream_ = nullptr;
+  cudaGraph_t graph_ = nullptr;
+  bool capturing_ = false;
+  Captured* now_ = nullptr;
+  uint8_t* data_ = nullptr;
 };
 
 // Ends the use of the scratch on every way out of a call.
 class ScratchUse {
  public:
-  ScratchUse(Scratch* s, cudaStream_t stream, Err* err) : s_(s), stream_(stream), err_(err) {}
+  ScratchUse(Scratch* s, Err* err) : s_(s), err_(err) {}
   ~ScratchUse() {
     if (begun_) {
       Err ignored;
-      s_->end(stream_, &ignored);
+      s_->end(&ignored);
     }
   }
   apk_status begin(size_t bytes, size_t zeroed) {
-    const apk_status st = s_->begin(bytes, zeroed, stream_, err_);
+    const apk_status st = s_->begin(bytes, zeroed, err_);
     begun_ = st == APK_OK;
     return st;
   }
   apk_status end() {
     if (!begun_) return APK_OK;
     begun_ = false;
-    return s_->end(stream_, err_);
+    return s_->end(err_);
   }
 
  private:
   Scratch* s_;
-  cudaStream_t stream_;
   Err* err_;
   bool begun_ = false;
 };

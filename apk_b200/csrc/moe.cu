@@ -689,7 +689,6 @@ struct apk_moe {
   apk_moe_config cfg{};
   Err err;
   int sms = 0;
-  int* status = nullptr;
   Scratch scratch;
   std::mutex mu;
 };
@@ -739,11 +738,7 @@ apk_status create(const apk_moe_config* cfg, apk_moe* h) {
   APK_TRY(cu_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, moe::moe_layer, moe::THREADS, moe::red_bytes(8)),
                     "preparing the expert kernel", &h->err));
   if (per_sm < 1) return h->err.fail(APK_EUNSUPPORTED, "the expert kernel does not fit an SM");
-  void* st = nullptr;
-  APK_TRY(cu_status(cudaMalloc(&st, 256), "cudaMalloc", &h->err));
-  h->status = static_cast<int*>(st);
-  APK_TRY(cu_status(cudaMemset(st, 0, 256), "cudaMemset", &h->err));
-  return cu_status(cudaStreamSynchronize(nullptr), "cudaStreamSynchronize", &h->err);
+  return h->scratch.open(c.device, &h->err);
 }
 
 apk_status forward(apk_moe* h, const apk_moe_io* io) {
@@ -768,7 +763,8 @@ apk_status forward(apk_moe* h, const apk_moe_io* io) {
   const size_t pairs = (size_t)io->tokens * c.top_k;
   const size_t b_log = up256((size_t)p.rsplit * io->tokens * c.experts * 4), b_hid = up256(pairs * c.d_ff * 2);
   const size_t b_out = up256(pairs * c.d_model * 4), b_choice = up256(pairs * 8);
-  ScratchUse use(&h->scratch, s, &h->err);
+  APK_TRY(h->scratch.enter(s, &h->err));
+  ScratchUse use(&h->scratch, &h->err);
   APK_TRY(use.begin(256 + b_log + b_hid + b_out + b_choice, 256));
   uint8_t* b = h->scratch.data();
   p.x = static_cast<const uint16_t*>(io->x);
@@ -790,7 +786,7 @@ apk_status forward(apk_moe* h, const apk_moe_io* io) {
   p.renorm = c.renormalize != 0;
   p.y_f32 = io->y_dtype == APK_F32;
   p.barrier = reinterpret_cast<unsigned*>(b);
-  p.status = h->status;
+  p.status = h->scratch.status();
   p.limit = c.wait_limit_ns;
   p.logits = reinterpret_cast<float*>(b + 256);
   p.hid = reinterpret_cast<uint16_t*>(b + 256 + b_log);
@@ -833,11 +829,6 @@ apk_status apk_moe_create(const apk_moe_config* cfg, apk_moe** out) {
 
 apk_status apk_moe_destroy(apk_moe* h) {
   if (!h) return APK_OK;
-  if (h->status) {
-    DeviceGuard guard(h->cfg.device);
-    h->scratch.release();
-    cudaFree(h->status);
-  }
   delete h;
   return APK_OK;
 }
@@ -845,7 +836,7 @@ apk_status apk_moe_destroy(apk_moe* h) {
 const char* apk_moe_last_error(const apk_moe* h) { return h ? h->err.text.c_str() : "NULL handle"; }
 
 apk_status apk_moe_forward(apk_moe* h, const apk_moe_io* io) {
-  if (!h || !h->status || !io) return APK_EINVAL;
+  if (!h || !h->scratch.status() || !io) return APK_EINVAL;
   try {
     std::lock_guard<std::mutex> lock(h->mu);
     return forward(h, io);
@@ -855,14 +846,14 @@ apk_status apk_moe_forward(apk_moe* h, const apk_moe_io* io) {
 }
 
 apk_status apk_moe_status(apk_moe* h, void* stream, int* device_status) {
-  if (!h || !h->status || !device_status) return APK_EINVAL;
+  if (!h || !h->scratch.status() || !device_status) return APK_EINVAL;
   try {
     std::lock_guard<std::mutex> lock(h->mu);
     DeviceGuard guard(h->cfg.device);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    APK_TRY(cu_status(cudaMemcpyAsync(device_status, h->status, sizeof(int), cudaMemcpyDeviceToHost, s), "status copy",
+    APK_TRY(cu_status(cudaMemcpyAsync(device_status, h->scratch.status(), sizeof(int), cudaMemcpyDeviceToHost, s), "status copy",
                       &h->err));
-    APK_TRY(cu_status(cudaMemsetAsync(h->status, 0, sizeof(int), s), "status clear", &h->err));
+    APK_TRY(cu_status(cudaMemsetAsync(h->scratch.status(), 0, sizeof(int), s), "status clear", &h->err));
     APK_TRY(cu_status(cudaStreamSynchronize(s), "cudaStreamSynchronize", &h->err));
     // a barrier that was given up has left its words half counted, a graph's in
     // the buffer that it was captured with

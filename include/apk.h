@@ -498,9 +498,10 @@ int apk_shard_tasks(const apk_task* tasks, int n, int world, int rank, int* idx)
  * Calls are asynchronous on `stream` (a cudaStream_t).  A handle may be used
  * from several streams: calls that need its scratch are ordered among
  * themselves.  Scratch grows on first use of a size (which allocates, and is
- * refused with APK_ESTATE inside a stream capture); a graph's launches keep
- * the scratch that they were captured with as long as the handle lives, and
- * the order of captured calls and others is the caller's.  Device waits are bounded by
+ * refused with APK_ESTATE inside a stream capture).  A captured graph has
+ * scratch of its own, for as long as it lives, the handle or not: its launches
+ * may run beside other calls and other graphs.  (Two executables instantiated
+ * from one graph share it: their order is the caller's.)  Device waits are bounded by
  * wait_limit_ns (0: 2 s); one that runs out leaves the outputs incomplete and
  * shows in apk_linear_status / apk_moe_status. */
 typedef enum apk_act {
