@@ -94,10 +94,10 @@ lin_stream(const __grid_constant__ StreamParams p) {
         if (VEC) {
           const uint4 zero = make_uint4(0, 0, 0, 0);
           const bool in = k < p.k;
-          a[u] = in ? stream::ld_weights(w0 + k) : zero;
-          b[u] = in ? stream::ld_weights(w1 + k) : zero;
+          a[u] = in ? stream::ld_late(w0 + k) : zero;
+          b[u] = in ? stream::ld_late(w1 + k) : zero;
 #pragma unroll
-          for (int i = 0; i < NT8; ++i) c[i][u] = in ? __ldg(reinterpret_cast<const uint4*>(xr[i] + k)) : zero;
+          for (int i = 0; i < NT8; ++i) c[i][u] = in ? stream::ld_rows(xr[i] + k) : zero;
         } else {
           a[u] = stream::ld8_any(w0 + k, p.k - k);
           b[u] = stream::ld8_any(w1 + k, p.k - k);
@@ -134,12 +134,12 @@ lin_stream(const __grid_constant__ StreamParams p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const bool in = k + r < p.k;
-          if (VEC) a[u][r] = in ? stream::ld_weights8(w + (long long)(k + r) * p.ldw) : make_uint2(0, 0);
+          if (VEC) a[u][r] = in ? stream::ld_late8(w + (long long)(k + r) * p.ldw) : make_uint2(0, 0);
           else a[u][r] = stream::ld4_any(w + (long long)(k + r) * p.ldw, in ? p.n - f : 0);
         }
 #pragma unroll
         for (int i = 0; i < NT8; ++i) {
-          if (VEC) c[u][i] = k < p.k ? __ldg(reinterpret_cast<const uint2*>(xr[i] + k)) : make_uint2(0, 0);
+          if (VEC) c[u][i] = k < p.k ? stream::ld_rows8(xr[i] + k) : make_uint2(0, 0);
           else c[u][i] = stream::ld4_any(xr[i] + k, p.k - k);
         }
       }

@@ -27,7 +27,8 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Weights are read once by one SM: not kept in L1.
+// Weights are read once by one SM: not kept in L1.  Through the read-only path:
+// for a kernel that starts after whatever wrote them has ended.
 __device__ __forceinline__ uint4 ld_weights(const void* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -36,9 +37,30 @@ __device__ __forceinline__ uint4 ld_weights(const void* p) {
   return v;
 }
 
-__device__ __forceinline__ uint2 ld_weights8(const void* p) {
+// The same for a kernel that may start while its predecessor still writes them
+// (pdl_wait stands between): ordinary loads, which stay behind the wait.
+__device__ __forceinline__ uint4 ld_late(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 ld_late8(const void* p) {
   uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.L2::256B.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
+// The few rows of the other operand, kept in L1.
+__device__ __forceinline__ uint4 ld_rows(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 ld_rows8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
   return v;
 }
 
