@@ -225,6 +225,9 @@ struct apk_linear {
 
 namespace {
 
+// Sizes up to here leave the kernels' 32-bit counts room to step past the end.
+constexpr int MAX_SIZE = 1 << 30;
+
 bool tma_ok(const void* p, long long ld, int outer) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld % 8 == 0 || outer == 1);
 }
@@ -268,7 +271,7 @@ apk_status forward(apk_linear* h, const apk_linear_io* io) {
   const apk_linear_config& c = h->cfg;
   const int K = c.in_features, N = c.out_features, M = io->rows;
   const cudaStream_t s = static_cast<cudaStream_t>(io->stream);
-  if (M < 0) return h->err.fail(APK_EINVAL, "rows is %d", M);
+  if (M < 0 || M > MAX_SIZE) return h->err.fail(APK_EINVAL, "rows is %d: at most 2^30", M);
   if (M == 0) return APK_OK;
   if (!io->x || !io->y) return h->err.fail(APK_EINVAL, "x or y is NULL");
   if (!valid_dtype(io->y_dtype)) return h->err.fail(APK_EINVAL, "y_dtype %d", io->y_dtype);
@@ -319,7 +322,7 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
   const cudaStream_t s = static_cast<cudaStream_t>(g->stream);
   const bool kn = c.w_layout == APK_W_KN;
   const int w_outer = kn ? K : N, w_inner = kn ? N : K;
-  if (M < 0) return h->err.fail(APK_EINVAL, "rows is %d", M);
+  if (M < 0 || M > MAX_SIZE) return h->err.fail(APK_EINVAL, "rows is %d: at most 2^30", M);
   if (!g->dx && !g->dw && !g->db) return h->err.fail(APK_EINVAL, "no gradient is asked for");
   if (g->db && !c.bias) return h->err.fail(APK_EINVAL, "db of a layer without a bias");
   if (g->dw && !valid_dtype(g->dw_dtype)) return h->err.fail(APK_EINVAL, "dw_dtype %d", g->dw_dtype);
@@ -425,8 +428,8 @@ apk_status create(const apk_linear_config* cfg, apk_linear* h) {
   if (!cfg) return h->err.fail(APK_EINVAL, "cfg is NULL");
   h->cfg = *cfg;
   const apk_linear_config& c = h->cfg;
-  if (c.in_features < 1 || c.out_features < 1)
-    return h->err.fail(APK_EINVAL, "in_features %d, out_features %d", c.in_features, c.out_features);
+  if (c.in_features < 1 || c.out_features < 1 || c.in_features > MAX_SIZE || c.out_features > MAX_SIZE)
+    return h->err.fail(APK_EINVAL, "in_features %d, out_features %d: 1 to 2^30", c.in_features, c.out_features);
   if (c.w_layout != APK_W_KN && c.w_layout != APK_W_NK) return h->err.fail(APK_EINVAL, "w_layout %d", (int)c.w_layout);
   if (c.act < APK_ACT_NONE || c.act > APK_ACT_SILU) return h->err.fail(APK_EINVAL, "act %d", (int)c.act);
   if (!c.W) return h->err.fail(APK_EINVAL, "W is NULL");

@@ -38,6 +38,7 @@ namespace moe {
 
 constexpr int WARPS = 16, THREADS = 32 * WARPS;
 constexpr int MAX_TOKENS = 64, MAX_EXPERTS = 512, MAX_TOPK = 16;
+constexpr int MAX_WIDTH = 1 << 26;  // of d_model and d_ff: a row index times one stays within 32 bits
 constexpr int LOCAL_LOGITS = 2048, LOCAL_BYTES = 96 << 10;
 constexpr int ROUND = 128;  // k of one warp's round: 8 16-byte weight loads a lane
 
@@ -714,6 +715,8 @@ apk_status create(const apk_moe_config* cfg, apk_moe* h) {
     return h->err.fail(APK_EINVAL, "top_k is %d: 1 to %d, of %d experts", c.top_k, moe::MAX_TOPK, c.experts);
   if (c.d_model < 8 || c.d_ff < 8 || c.d_model % 8 || c.d_ff % 8)
     return h->err.fail(APK_EINVAL, "d_model %d and d_ff %d have to be multiples of 8", c.d_model, c.d_ff);
+  if (c.d_model > moe::MAX_WIDTH || c.d_ff > moe::MAX_WIDTH)
+    return h->err.fail(APK_EINVAL, "d_model %d, d_ff %d: at most 2^26", c.d_model, c.d_ff);
   if (c.act < APK_ACT_NONE || c.act > APK_ACT_SILU) return h->err.fail(APK_EINVAL, "act %d", (int)c.act);
   if (!c.router || !c.w_in || !c.w_out) return h->err.fail(APK_EINVAL, "router, w_in or w_out is NULL");
   if (!aligned(c.router, 16) || !aligned(c.w_in, 16) || !aligned(c.w_out, 16))

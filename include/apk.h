@@ -518,7 +518,7 @@ typedef enum apk_w_layout { APK_W_KN = 0, APK_W_NK = 1 } apk_w_layout;
 
 typedef struct apk_linear_config {
   int device;
-  int in_features, out_features;  /* at least 1, no other limit               */
+  int in_features, out_features;  /* 1 to 2^30; a call's rows up to 2^30      */
   apk_w_layout w_layout;
   apk_act act;
   apk_dtype bias_dtype;
@@ -595,7 +595,7 @@ apk_status apk_linear_status(apk_linear* h, void* stream, int* device_status);
  *   y = the sum over the chosen experts of p * (hidden w_out^T).
  * The hidden values are rounded to bf16, everything else is fp32 until y.
  * Weights are bf16, contiguous, 16-byte aligned; d_model and d_ff are
- * multiples of 8. */
+ * multiples of 8, up to 2^26. */
 typedef struct apk_moe_config {
   int device;
   int experts, top_k;       /* up to 512; up to 16 and experts                */
