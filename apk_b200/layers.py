@@ -26,6 +26,8 @@ _ANY = tuple(_CODE)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
 _DEFAULT_WAIT_NS = 2_000_000_000
+# the native handles have the tensors' addresses
+_MOVED = "weights are in other memory than when the layer was made: make a new layer"
 
 
 def _pick(table, value, what):
@@ -133,7 +135,10 @@ class Linear(_Handle):
     weight: [in, out] for layout "kn" (the GEMM runtime's row-major B) or
     [out, in] for "nk", bf16, rows of any stride.  bias: [out] fp32 or bf16.
     act: none, relu, gelu, gelu_tanh or silu.  The layer keeps a reference to
-    the tensors, not a copy: an optimizer may update them in place."""
+    the tensors, not a copy: an optimizer may update them in place.  Other
+    tensors, or other memory for these, need another layer: a call refuses
+    weights that have moved.  Nothing is recorded for autograd: outputs carry
+    no gradient function, backward() computes the gradients."""
     _create, _destroy = "apk_linear_create", "apk_linear_destroy"
     _error, _status = "apk_linear_last_error", "apk_linear_status"
 
@@ -150,6 +155,7 @@ class Linear(_Handle):
                 raise ValueError(f"bias is {tuple(bias.shape)} with strides {bias.stride()}: "
                                  f"{self.out_features} contiguous values are wanted")
         self.weight, self.bias, self.act, self.layout = weight, bias, act, layout
+        self._w_shape, self._w_at, self._b_at = weight.shape, w, None if bias is None else bias.data_ptr()
         self.out_dtype = _pick(_TORCH, out_dtype, "out_dtype")
         self._y_code = _CODE[self.out_dtype]
         self._act = _pick(_ACT, act, "act")
@@ -164,6 +170,9 @@ class Linear(_Handle):
         x W + b in bf16, as backward() takes it.  out: the output's tensor;
         it may be the residual."""
         with self._lock:
+            b = self.bias
+            if self.weight.data_ptr() != self._w_at or (None if b is None else b.data_ptr()) != self._b_at:
+                raise ValueError(_MOVED)
             io, n = self._io, self.out_features
             io.x, io.rows, io.ldx = _rows(x, "x", self.device, self.in_features)
             shape = (io.rows, n) if len(x.shape) == 2 else (*x.shape[:-1], n)
@@ -188,7 +197,7 @@ class Linear(_Handle):
                 io.preact, io.ld_preact = z.data_ptr(), n
             else:
                 io.preact = None
-            io.y_dtype, io.stream = self._y_code, self._stream()
+            io.y_dtype, io.stream = self._y_code, _raw_stream(self._index)
             st = self._lib.apk_linear_forward(self._h, self._io_ref)
             if st:
                 self._check(st)
@@ -203,6 +212,9 @@ class Linear(_Handle):
         preact: what forward(save_preact=True) returned, for a layer with an
         activation."""
         with self._lock:
+            b = self.bias
+            if self.weight.data_ptr() != self._w_at or (None if b is None else b.data_ptr()) != self._b_at:
+                raise ValueError(_MOVED)
             g, n, k = self._grads, self.out_features, self.in_features
             g.dy, g.rows, g.ld_dy = _rows(dy, "dy", self.device, n)
             if dy.shape[:-1] != x.shape[:-1]:
@@ -221,13 +233,13 @@ class Linear(_Handle):
                 g.dx, g.ld_dx = dx.data_ptr(), k
             if need_dw:
                 dt = _pick(_TORCH, dw_dtype, "dw_dtype")
-                shape = self.weight.shape
+                shape = self._w_shape
                 dw = _like(self.weight, shape) if dt is torch.bfloat16 else self.weight.new_empty(shape, dtype=dt)
                 g.dw, g.ld_dw, g.dw_dtype = dw.data_ptr(), shape[1], _CODE[dt]
             if need_db and self.bias is not None:
                 db = torch.empty_like(self.bias)
                 g.db = db.data_ptr()
-            g.stream = self._stream()
+            g.stream = _raw_stream(self._index)
             if dw is not None or db is not None or (dx is not None and g.rows > 0):
                 st = self._lib.apk_linear_backward(self._h, self._grads_ref)
                 if st:
@@ -241,7 +253,8 @@ class MoE(_Handle):
     router [E, D], w_in [E, 2F, D] (gate rows, then up rows; [E, F, D] when
     not gated) and w_out [E, D, F], bf16 and contiguous.  Each token goes to
     its top_k experts, weighted by their softmax probabilities over all
-    experts, divided by the chosen ones' sum if renormalize."""
+    experts, divided by the chosen ones' sum if renormalize.  The weights are
+    kept by reference, as Linear keeps them; nothing is recorded for autograd."""
     _create, _destroy = "apk_moe_create", "apk_moe_destroy"
     _error, _status = "apk_moe_last_error", "apk_moe_status"
 
@@ -262,6 +275,7 @@ class MoE(_Handle):
             if not t.is_contiguous():
                 raise ValueError(f"{what} is not contiguous")
         self.router, self.w_in, self.w_out, self.top_k = router, w_in, w_out, top_k
+        self._at = (router.data_ptr(), w_in.data_ptr(), w_out.data_ptr())
         self.out_dtype = _pick(_TORCH, out_dtype, "out_dtype")
         self._y_code = _CODE[self.out_dtype]
         self._open(L.MoeConfig(self.device.index, self.experts, top_k, self.d_model, self.d_ff, _pick(_ACT, act, "act"),
@@ -274,6 +288,8 @@ class MoE(_Handle):
         """The layer's output for x [..., D]; with return_routing also the
         chosen experts (int32 [..., top_k]) and their weights (fp32)."""
         with self._lock:
+            if (self.router.data_ptr(), self.w_in.data_ptr(), self.w_out.data_ptr()) != self._at:
+                raise ValueError(_MOVED)
             io = self._io
             io.x, io.tokens, io.ldx = _rows(x, "x", self.device, self.d_model)
             y = _like(x, x.shape) if self._y_code == L.APK_BF16 else x.new_empty(x.shape, dtype=self.out_dtype)
@@ -285,7 +301,7 @@ class MoE(_Handle):
                 io.ids, io.probs = ids.data_ptr(), probs.data_ptr()
             else:
                 io.ids = io.probs = None
-            io.stream = self._stream()
+            io.stream = _raw_stream(self._index)
             st = self._lib.apk_moe_forward(self._h, self._io_ref)
             if st:
                 self._check(st)
