@@ -74,6 +74,17 @@ def _rows(t, what, device, width, dtypes=(torch.bfloat16,)):
     return v.data_ptr(), v.shape[0], (v.stride(0) if v.shape[0] > 1 else width)
 
 
+def _overlap(a, b, rows):
+    """Whether two views of `rows` rows, each (address, row pitch, row length) in
+    bytes, share memory: exact where the pitches agree, else whether their
+    extents meet."""
+    (at, pitch, length), (at2, pitch2, length2) = a, b
+    if rows == 0 or at + (rows - 1) * pitch + length <= at2 or at2 + (rows - 1) * pitch2 + length2 <= at:
+        return False
+    off = (at2 - at) % pitch
+    return pitch != pitch2 or off < length or off + length2 > pitch
+
+
 def _like(t, shape):
     """A new tensor of t's type and device; of t's own shape the cheaper way."""
     return torch.empty_like(t) if t.shape == shape and t.is_contiguous() else t.new_empty(shape)
@@ -168,7 +179,7 @@ class Linear(_Handle):
     def forward(self, x, residual=None, save_preact: bool = False, out=None):
         """act(x W + b) + residual for x [..., in]; with save_preact also
         x W + b in bf16, as backward() takes it.  out: the output's tensor;
-        it may be the residual."""
+        it may be the residual, but share no memory with x."""
         with self._lock:
             b = self.bias
             if self.weight.data_ptr() != self._w_at or (None if b is None else b.data_ptr()) != self._b_at:
@@ -191,6 +202,16 @@ class Linear(_Handle):
                     raise ValueError(f"residual is {tuple(residual.shape)}, not {shape}")
                 io.residual, _, io.ld_residual = _rows(residual, "residual", self.device, n, _ANY)
                 io.residual_dtype = _CODE[residual.dtype]
+            if out is not None:
+                es = y.element_size()
+                to = (io.y, io.ldy * es, n * es)
+                if _overlap(to, (io.x, io.ldx * 2, self.in_features * 2), io.rows):
+                    raise ValueError("out shares memory with x")
+                if residual is not None:
+                    rs = residual.element_size()
+                    of = (io.residual, io.ld_residual * rs, n * rs)
+                    if of != to and _overlap(to, of, io.rows):
+                        raise ValueError("out shares memory with residual, but is not it")
             z = None
             if save_preact:
                 z = x.new_empty(shape)
