@@ -22,7 +22,9 @@
 // by token.
 //
 // Rounding: the hidden values are rounded to bf16 once as the second
-// product's operand; logits, softmax, both products and the sum are fp32.
+// product's operand; logits, softmax, both products and the sum are fp32.  The
+// second product of an fp32 result takes 512 k at a time, as the linear layer
+// does; the first one's truncation is far below the rounding that follows it.
 #include <algorithm>
 #include <mutex>
 #include <new>
@@ -41,6 +43,7 @@ constexpr int MAX_TOKENS = 64, MAX_EXPERTS = 512, MAX_TOPK = 16;
 constexpr int MAX_WIDTH = 1 << 26;  // of d_model and d_ff: a row index times one stays within 32 bits
 constexpr int LOCAL_LOGITS = 2048, LOCAL_BYTES = 96 << 10;
 constexpr int ROUND = 128;  // k of one warp's round: 8 16-byte weight loads a lane
+constexpr int PIECE = 4;    // rounds that an accumulator of an fp32 result takes
 
 struct Params {
   const uint16_t* x;
@@ -152,11 +155,30 @@ struct Rows {
 // weights are in flight while one is multiplied, and at the end the first
 // round of the next item's rows, so that the loads do not pause between items.
 // Load reads 16 bytes of a token row.
-template <int NT8, class Load>
+// EXACT: the tensor core truncates as it adds, a bias of about 1e-9 per k of
+// the result; so every 512 k are added with rounding to a total in the shared
+// memory given.  (The accumulators of 64 tokens twice would not fit the
+// registers.)
+template <int NT8, bool EXACT = false, class Load>
 __device__ __forceinline__ void stream_rows(float (&acc)[NT8][4], Frag& f, const Rows w, const Rows next_item,
                                             const uint16_t* const (&xr)[NT8], int k, int first, int step, int t,
-                                            Load ld) {
+                                            Load ld, float* total = nullptr) {
   const int begin = first * ROUND;
+  auto flush = [&](bool back) {
+#pragma unroll
+    for (int i = 0; i < NT8; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float& sum = total[(i * 4 + c) * 32];
+        const float s = sum + acc[i][c];
+        if (back) acc[i][c] = s;
+        else sum = s, acc[i][c] = 0.f;
+      }
+  };
+  if constexpr (EXACT)
+#pragma unroll
+    for (int i = 0; i < NT8 * 4; ++i) total[i * 32] = 0.f;
+  int left = PIECE;
 #pragma unroll 1
   for (int k0 = begin; k0 < k; k0 += step * ROUND) {
     const int next = k0 + step * ROUND;
@@ -176,7 +198,12 @@ __device__ __forceinline__ void stream_rows(float (&acc)[NT8][4], Frag& f, const
     }
     if (NT8 <= 2) f = n;
     else if (next < k) load_round(f, w.w0, w.w1, next, t, k);
+    if (EXACT && --left == 0) {
+      flush(false);
+      left = PIECE;
+    }
   }
+  if constexpr (EXACT) flush(true);
   if (next_item.w0) load_round(f, next_item.w0, next_item.w1, begin, t, k);
 }
 
@@ -309,7 +336,11 @@ __device__ __forceinline__ void item_out(const Params& p, const Shared& sh, floa
 #pragma unroll
   for (int i = 0; i < NT8; ++i) xr[i] = p.hid + (long long)(base + min(8 * i + g, n - 1)) * p.f;
   float acc[NT8][4] = {};
-  stream_rows<NT8>(acc, f, w, next, xr, p.f, warp & (ws - 1), ws, t, LdWritten());
+  if (p.y_f32 && p.f > PIECE * ROUND * ws)  // (in the warp's place in the shared sums, which join_warps takes after this)
+    stream_rows<NT8, true>(acc, f, w, next, xr, p.f, warp & (ws - 1), ws, t, LdWritten(),
+                           red + warp * p.red_stride + lane);
+  else
+    stream_rows<NT8>(acc, f, w, next, xr, p.f, warp & (ws - 1), ws, t, LdWritten());
   join_warps<NT8>(acc, red, p.red_stride, ws, warp, lane);
   if (warp & (ws - 1)) return;
 #pragma unroll
