@@ -71,20 +71,22 @@ struct DzParams {
 };
 
 constexpr int DZ_COLS = 256;  // columns of a block: 8 per lane
+constexpr int DZ_BLOCKS = 4;  // of an SM
 
 // dz = dy * act'(z), rounded to bf16 (the products' operand type), and the
 // column sums of the unrounded dz.  One pass over dy and z.  A block sums its
 // rows in registers and shared memory; the last block of a column range adds
 // the row blocks' sums in their order, so db does not depend on the order of
-// arrival.  VEC: rows of 16-byte aligned 8-element chunks.  A smooth
-// activation's two hardware functions and dozen operations an element take as
-// long as its bytes: five blocks an SM (48 registers, a few spilled) overlap
-// the two best (4096 x 8192 with gelu_tanh, no dz: 39 us against 45 at four).
+// arrival.  VEC: rows of 16-byte aligned 8-element chunks.  The grid is one
+// residency of four blocks an SM (64 registers), rounded down.  4096 x 8192
+// with gelu_tanh, no dz: 34.0 us; rounded up, the 16 blocks over ran alone, 42.8;
+// five blocks an SM at 48 registers, with spills, 35.4 in one residency and
+// 40.0 with places left empty.  With dx of 256 columns behind it: 71, 84, 70, 75.
 // Blocks past the first cblocks * rblocks copy operands for the products that
 // follow (one launch for both).
 template <bool VEC>
-__global__ void __launch_bounds__(256, 5) dz_kernel(const __grid_constant__ DzParams p,
-                                                 const __grid_constant__ RepackParams copies) {
+__global__ void __launch_bounds__(256, DZ_BLOCKS) dz_kernel(const __grid_constant__ DzParams p,
+                                                         const __grid_constant__ RepackParams copies) {
   __shared__ float sum[8][DZ_COLS];
   __shared__ bool last;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -350,9 +352,9 @@ apk_status backward(apk_linear* h, const apk_linear_grads* g) {
   const bool products = g->dx || g->dw;
   const bool own_dz = products && (act || !tma_ok(g->dy, g->ld_dy, M));
   const bool px = g->dw && !tma_ok(g->x, g->ldx, M), pw = g->dx && !tma_ok(c.W, c.ldw, w_outer);
-  // blocks of the elementwise pass: about four per SM, at least 16 rows each
+  // blocks of the elementwise pass: one residency at most, at least 16 rows each
   const int cblocks = (N + lin::DZ_COLS - 1) / lin::DZ_COLS;
-  int rblocks = std::max(1, std::min((M + 15) / 16, (4 * h->sms + cblocks - 1) / cblocks));
+  int rblocks = std::max(1, std::min((M + 15) / 16, lin::DZ_BLOCKS * h->sms / cblocks));
   const int per = ((M + rblocks - 1) / rblocks + 7) / 8 * 8;
   rblocks = (M + per - 1) / per;
   const size_t zeroed = up256((size_t)cblocks * 4);
