@@ -741,6 +741,7 @@ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 struct Choice {
   const Variant* v;
   int split;
+  int slots;  // CTAs, pairs or clusters that are resident at once
   double cost;
 };
 
@@ -767,7 +768,7 @@ Choice choose(const Product* pr, int n, int sms, int dev) {
     bytes += 2.0 * ((double)pr[j].rows * pr[j].k + (double)pr[j].cols * pr[j].k + (double)pr[j].rows * pr[j].cols);
   bool exact = false;  // a long sum that is not rounded to bf16
   for (int j = 0; j < n; ++j) exact = exact || (pr[j].epi.out_f32 && pr[j].k > EXACT_KB * BK);
-  Choice best{nullptr, 1, 0};
+  Choice best{nullptr, 1, 1, 0};
   for (int i = 0; i < nv; ++i) {
     const Variant& v = vs[i];
     bool fits = v.exact == exact;
@@ -795,7 +796,7 @@ Choice choose(const Product* pr, int n, int sms, int dev) {
       double cost = 6000 + std::max(bytes / 3300, std::max(longest, sweeps));
       if (v.fm == 1) cost += v.nt * 20.0;  // the last tile's epilogue
       if (v.split) cost += 1500 + v.nt / sp * 6.0;
-      if (!best.v || cost < best.cost) best = {&v, sp, cost};
+      if (!best.v || cost < best.cost) best = {&v, sp, slots, cost};
     }
   }
   return best;
@@ -889,7 +890,7 @@ apk_status run_products(const Product* pr, int n, int sms, int dev, int* status,
     if (j == 0) p.tiles0 = p.tiles;
   }
   const int cl = v.split ? ch.split : v.cg;
-  const int groups = v.split ? p.tiles : std::min(p.tiles, std::max(1, sms / v.cg));
+  const int groups = v.split ? p.tiles : std::min(p.tiles, ch.slots);
   Launch l(dim3(groups * cl), THREADS, v.smem, stream, cl);
   void* args[] = {&p};
   const cudaError_t e = cudaLaunchKernelExC(&l.cfg, v.fn, args);
