@@ -58,9 +58,6 @@ struct Product {
   Epilogue epi;
 };
 
-// Launches one or two products, in one launch where that is faster. sms: the SMs it may
-// fill; dev: the current device.
-// `why` receives a message on failure.
 // Whether a product is faster through run_stream than through run_products.
 // Up to 8 rows [n][k] weights always are (8 x 4096 x 8192: 14.0 against 15.6
 // us).  Two MMA tiles of rows, or the narrower row pieces of [k][n], cost it
@@ -75,6 +72,8 @@ inline bool streams(int rows, long long weight_bytes, bool nk, bool tma) {
   if (!tma) return mb < 16;
   return nk ? rows <= 8 || mb < 24 : mb < (rows <= 8 ? 16 : 4);
 }
+// Launches one or two products, in one launch where that is faster.  sms: the
+// SMs it may fill; dev: the current device.  `why` receives a message on failure.
 apk_status run_products(const Product* pr, int n, int sms, int dev, int* status, long long limit, cudaStream_t stream,
                         std::string* why);
 // A product of at most 16 rows with weights [n][k] (nk) or [k][n] of any

@@ -562,7 +562,8 @@ apk_status apk_linear_forward(apk_linear* h, const apk_linear_io* io);
  * gradient is dy itself):  dz = dy * act'(preact),  dx = dz W^T,
  * dw = x^T dz in W's layout,  db = the sum of dz's rows.  An output that is
  * NULL is not computed.  dz is rounded to bf16 as the products' operand; db
- * sums it unrounded.  With rows = 0, dw and db are cleared. */
+ * sums it unrounded.  (It is a product: an infinite dy where act' is 0 gives a
+ * NaN.)  With rows = 0, dw and db are cleared. */
 typedef struct apk_linear_grads {
   const void* dy;           /* bf16 [rows][out_features]                      */
   long long ld_dy;
