@@ -58,7 +58,7 @@ struct Params {
   int red_stride;  // floats of a warp's place in the shared sums
   int rsplit;    // slices of d_model in phase 0
   int local;     // every CTA computes all logits itself
-  unsigned* barrier;  // [0] arrivals, [32] their number when this launch began
+  unsigned* barrier;  // [0] arrivals, [32] their number when this launch began, [33] whether one ran out
   int* status;
   long long limit;
   float* logits;  // [rsplit][tokens][experts]
@@ -97,13 +97,13 @@ __device__ __forceinline__ void grid_arrive(const Params& p, Shared& sh) {
     asm volatile("red.relaxed.gpu.global.add.u32 [%0], 1;" ::"l"(p.barrier) : "memory");
   }
 }
-// False: a barrier of this launch, or one before it that apk_moe_status has
-// not been asked about, ran out.  The count is of no use then, and a CTA that
+// False: a barrier of this launch, or of one before it with these words that
+// apk_moe_status has not been asked about, ran out.  The count is of no use then, and a CTA that
 // went on by it could read what others have yet to write.
 __device__ __forceinline__ bool grid_wait(const Params& p, Shared& sh) {
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && !sh.abort) {
     long long t0 = 0;
-    for (int n = 1; !sh.abort; ++n) {
+    for (int n = 1;; ++n) {
       unsigned now;
       asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(now) : "l"(p.barrier) : "memory");
       if ((int)(now - sh.target) >= 0) break;
@@ -112,6 +112,7 @@ __device__ __forceinline__ bool grid_wait(const Params& p, Shared& sh) {
         if (t0 == 0) t0 = t;
         if (t - t0 > p.limit) {
           report_status(p.status, DEV_WAIT_TIMEOUT_SPIN, nullptr);
+          *reinterpret_cast<volatile unsigned*>(p.barrier + 33) = 1;
           sh.abort = 1;
           break;
         }
@@ -518,16 +519,21 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
   extern __shared__ float red[];
   __shared__ Shared sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  if (tid == 0) {
-    sh.abort = *reinterpret_cast<volatile int*>(p.status) != 0;
-    sh.target = *reinterpret_cast<volatile unsigned*>(p.barrier + 32);
-  }
+  uint2 begun = {};
+  if (tid == 0)
+    asm volatile("ld.volatile.global.v2.u32 {%0, %1}, [%2];" : "=r"(begun.x), "=r"(begun.y) : "l"(p.barrier + 32));
+  auto begin = [&]() {  // (behind the first loads of weights, so that these do not wait for the two words)
+    if (tid != 0) return;
+    sh.target = begun.x;
+    sh.abort = begun.y != 0;
+  };
   for (int e = tid; e < p.experts; e += THREADS) sh.mask[e] = 0;
 
   // -------- 0: logits --------
   const int etiles = (p.experts + 15) / 16;
   if (p.local) {
     for (int tile = 0; tile < etiles; ++tile) item_router(p, red, tile, 0, 1, 0, sh.logits);
+    begin();
     __syncthreads();
   } else {
     const int tgroups = (p.tokens + 15) / 16;
@@ -536,6 +542,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
       item_router(p, red, it % etiles, slice, p.rsplit, it / (etiles * p.rsplit) * 16,
                   p.logits + (long long)slice * p.tokens * p.experts);
     }
+    begin();
     if (!grid_barrier(p, sh)) return;
   }
 

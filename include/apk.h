@@ -629,10 +629,10 @@ typedef struct apk_moe_io {
 } apk_moe_io;
 apk_status apk_moe_forward(apk_moe* h, const apk_moe_io* io);
 
-/* As apk_linear_status (3: a grid barrier ran out).  After an error the
- * handle's calls, graphs' launches among them, leave y as it is until this
- * has been called, which makes them usable again.  Call it with no other call
- * in flight. */
+/* As apk_linear_status (3: a grid barrier ran out).  After an error further
+ * calls (in a graph: its launches) leave y as it is until this has been
+ * called, which makes them usable again.  Call it with no other call in
+ * flight. */
 apk_status apk_moe_status(apk_moe* h, void* stream, int* device_status);
 
 /* ---- allocation-free entry point --------------------------------------- */
