@@ -21,10 +21,12 @@
 // of arrival: an expert's tokens are a bit mask, so their columns are ordered
 // by token.
 //
-// Rounding: the hidden values are rounded to bf16 once as the second
-// product's operand; logits, softmax, both products and the sum are fp32.  The
-// second product of an fp32 result takes 512 k at a time, as the linear layer
-// does; the first one's truncation is far below the rounding that follows it.
+// Rounding: logits, softmax, both products and the sum are fp32.  For a bf16
+// result the hidden values, the second product's operand, are rounded to bf16
+// once (2.3e-3 from 64 bits in the 2-norm, 1.7e-3 with the result's rounding
+// alone; 64 tokens on 4 ungated experts of 2048 x 4096 87 us).  For an fp32
+// result they are the sum of two bf16 values, 2^-17 of themselves off, and both
+// products take 512 k at a time, as the linear layer does (that case 117 us).
 #include <algorithm>
 #include <mutex>
 #include <new>
@@ -54,7 +56,7 @@ struct Params {
   int* ids;      // [tokens][top_k] or null
   float* probs;  // [tokens][top_k] or null
   long long ldx, ldy;
-  int tokens, experts, top_k, d, f, act, gated, renorm, y_f32;
+  int tokens, experts, top_k, d, f, act, gated, renorm;
   int red_stride;  // floats of a warp's place in the shared sums
   int rsplit;    // slices of d_model in phase 0
   int local;     // every CTA computes all logits itself
@@ -63,7 +65,7 @@ struct Params {
   long long limit;
   float* logits;  // [rsplit][tokens][experts]
   float2* choice; // [tokens][top_k] expert (as bits), weight
-  uint16_t* hid;  // [tokens * top_k][f], rows grouped by expert
+  uint16_t* hid;  // [tokens * top_k][f], rows grouped by expert; F32: [f / 8][2][8], both terms
   float* out;     // [tokens * top_k][d]
 };
 
@@ -155,7 +157,7 @@ struct Rows {
 // first + step, ... of k.  On entry f holds round `first`; the next round's
 // weights are in flight while one is multiplied, and at the end the first
 // round of the next item's rows, so that the loads do not pause between items.
-// Load reads 16 bytes of a token row.
+// Load reads 16 bytes of a token row, whose values have TERMS bf16 terms.
 // EXACT: the tensor core truncates as it adds, a bias of about 1e-9 per k of
 // the result; so every 512 k are added with rounding to a total in the shared
 // memory given.  (The accumulators of 64 tokens twice would not fit the
@@ -190,11 +192,15 @@ __device__ __forceinline__ void stream_rows(float (&acc)[NT8][4], Frag& f, const
       const int at = k0 + 32 * u + 8 * t;
       uint4 c[NT8];
 #pragma unroll
-      for (int i = 0; i < NT8; ++i) c[i] = at < k ? ld(xr[i] + at) : make_uint4(0, 0, 0, 0);
+      for (int v = 0; v < Load::TERMS; ++v) {
 #pragma unroll
-      for (int i = 0; i < NT8; ++i) {
-        stream::mma_bf16(acc[i], f.a[u].x, f.b[u].x, f.a[u].y, f.b[u].y, c[i].x, c[i].y);
-        stream::mma_bf16(acc[i], f.a[u].z, f.b[u].z, f.a[u].w, f.b[u].w, c[i].z, c[i].w);
+        for (int i = 0; i < NT8; ++i)
+          c[i] = at < k ? ld(xr[i] + Load::TERMS * at + 8 * v) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < NT8; ++i) {
+          stream::mma_bf16(acc[i], f.a[u].x, f.b[u].x, f.a[u].y, f.b[u].y, c[i].x, c[i].y);
+          stream::mma_bf16(acc[i], f.a[u].z, f.b[u].z, f.a[u].w, f.b[u].w, c[i].z, c[i].w);
+        }
       }
     }
     if (NT8 <= 2) f = n;
@@ -209,9 +215,12 @@ __device__ __forceinline__ void stream_rows(float (&acc)[NT8][4], Frag& f, const
 }
 
 struct LdConst {  // the layer's input: not written during the kernel
+  static constexpr int TERMS = 1;
   __device__ uint4 operator()(const uint16_t* p) const { return __ldg(reinterpret_cast<const uint4*>(p)); }
 };
+template <int N>
 struct LdWritten {  // written by other CTAs in an earlier phase: from L2
+  static constexpr int TERMS = N;
   __device__ uint4 operator()(const uint16_t* p) const { return __ldcg(reinterpret_cast<const uint4*>(p)); }
 };
 
@@ -292,7 +301,8 @@ __device__ __forceinline__ Rows rows_out(const Params& p, const Shared& sh, int 
   return {w + (long long)min(d0 + g, p.d - 1) * p.f, w + (long long)min(d0 + g + 8, p.d - 1) * p.f};
 }
 
-template <int NT8>
+// F32 of these and of the kernel: the result's type.
+template <int NT8, bool F32>
 __device__ __forceinline__ void item_in(const Params& p, const Shared& sh, float* red, Frag& f, Rows w, Rows next, int a,
                                         int tile, int n, int ws) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -301,7 +311,8 @@ __device__ __forceinline__ void item_in(const Params& p, const Shared& sh, float
 #pragma unroll
   for (int i = 0; i < NT8; ++i) xr[i] = p.x + sh.tok[base + min(8 * i + g, n - 1)] * p.ldx;
   float acc[NT8][4] = {};
-  stream_rows<NT8>(acc, f, w, next, xr, p.d, warp & (ws - 1), ws, t, LdConst());
+  // (totals in the warp's place in the shared sums, which join_warps takes after this)
+  stream_rows<NT8, F32>(acc, f, w, next, xr, p.d, warp & (ws - 1), ws, t, LdConst(), red + warp * p.red_stride + lane);
   join_warps<NT8>(acc, red, p.red_stride, ws, warp, lane);
   if (warp & (ws - 1)) return;
   with_act(p.act, [&](auto tag) {
@@ -312,11 +323,21 @@ __device__ __forceinline__ void item_in(const Params& p, const Shared& sh, float
       for (int c = 0; c < 2; ++c) {
         const int col = 8 * i + 2 * t + c;
         if (col >= n) continue;
-        uint16_t* h = p.hid + (long long)(base + col) * p.f;
+        uint16_t* h = p.hid + ((long long)(base + col) * p.f * (1 + F32));
         auto put = [&](int at, float v) {
           uint16_t r;
           asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(v));
-          if (at < p.f) h[at] = r;
+          if (at >= p.f) return;
+          if constexpr (!F32) {
+            h[at] = r;
+          } else {
+            uint16_t* const two = h + 2 * at - (at & 7);
+            two[0] = r;
+            const bool finite = (r & 0x7F80) != 0x7F80;  // (an infinity stays one)
+            const float rest = finite ? v - __uint_as_float((uint32_t)r << 16) : 0.f;
+            asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(rest));
+            two[8] = r;
+          }
         };
         if (p.gated) {
           put(f0 + g, act_f<ACT>(acc[i][c]) * acc[i][c + 2]);
@@ -328,20 +349,17 @@ __device__ __forceinline__ void item_in(const Params& p, const Shared& sh, float
   });
 }
 
-template <int NT8>
+template <int NT8, bool F32>
 __device__ __forceinline__ void item_out(const Params& p, const Shared& sh, float* red, Frag& f, Rows w, Rows next,
                                          int a, int tile, int n, int ws) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int base = sh.base[a], d0 = tile * 16;
   const uint16_t* xr[NT8];
 #pragma unroll
-  for (int i = 0; i < NT8; ++i) xr[i] = p.hid + (long long)(base + min(8 * i + g, n - 1)) * p.f;
+  for (int i = 0; i < NT8; ++i) xr[i] = p.hid + ((long long)(base + min(8 * i + g, n - 1)) * p.f * (1 + F32));
   float acc[NT8][4] = {};
-  if (p.y_f32 && p.f > PIECE * ROUND * ws)  // (in the warp's place in the shared sums, which join_warps takes after this)
-    stream_rows<NT8, true>(acc, f, w, next, xr, p.f, warp & (ws - 1), ws, t, LdWritten(),
-                           red + warp * p.red_stride + lane);
-  else
-    stream_rows<NT8>(acc, f, w, next, xr, p.f, warp & (ws - 1), ws, t, LdWritten());
+  stream_rows<NT8, F32>(acc, f, w, next, xr, p.f, warp & (ws - 1), ws, t, LdWritten<1 + F32>(),
+                        red + warp * p.red_stride + lane);
   join_warps<NT8>(acc, red, p.red_stride, ws, warp, lane);
   if (warp & (ws - 1)) return;
 #pragma unroll
@@ -378,8 +396,9 @@ __device__ __forceinline__ void item_router(const Params& p, float* red, int til
     }
 }
 
+template <bool F32>
 __device__ __forceinline__ void put_y(const Params& p, long long at, float v) {
-  if (p.y_f32) {
+  if constexpr (F32) {
     static_cast<float*>(p.y)[at] = v;
   } else {
     uint16_t r;
@@ -463,8 +482,9 @@ __device__ __forceinline__ void route_token(const Params& p, Load logit, int& my
 // One token: the output without the sum's barrier.  A CTA takes `ROWS` (8 or
 // 16) of the output's rows over all chosen experts, its warps splitting the
 // (expert, round) pairs; the probabilities are applied per expert.
-template <int ROWS>
+template <int ROWS, bool F32>
 __device__ __forceinline__ bool one_token_out(const Params& p, Shared& sh, float* red) {
+  constexpr int TERMS = 1 + F32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rounds = (p.f + ROUND - 1) / ROUND, units = p.top_k * rounds;
   auto load = [&](Frag& f, int tile, int u) {
@@ -481,7 +501,7 @@ __device__ __forceinline__ bool one_token_out(const Params& p, Shared& sh, float
     float s0 = 0.f, s1 = 0.f;
     for (int u = warp; u < units; u += WARPS) {
       const int j = u / rounds, k0 = (u - j * rounds) * ROUND;
-      const uint16_t* h = p.hid + sh.row[j] * p.f;
+      const uint16_t* h = p.hid + sh.row[j] * p.f * TERMS;
       Frag n;  // the next unit, of this tile or the next one
       if (u + WARPS < units) load(n, tile, u + WARPS);
       else if ((tile + (int)gridDim.x) * ROWS < p.d) load(n, tile + gridDim.x, warp);
@@ -489,9 +509,12 @@ __device__ __forceinline__ bool one_token_out(const Params& p, Shared& sh, float
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int at = k0 + 32 * v + 8 * t;
-        const uint4 c = at < p.f ? LdWritten()(h + at) : make_uint4(0, 0, 0, 0);
-        stream::mma_bf16(acc, f.a[v].x, f.b[v].x, f.a[v].y, f.b[v].y, c.x, c.y);
-        stream::mma_bf16(acc, f.a[v].z, f.b[v].z, f.a[v].w, f.b[v].w, c.z, c.w);
+#pragma unroll
+        for (int i = 0; i < TERMS; ++i) {
+          const uint4 c = at < p.f ? LdWritten<TERMS>()(h + TERMS * at + 8 * i) : make_uint4(0, 0, 0, 0);
+          stream::mma_bf16(acc, f.a[v].x, f.b[v].x, f.a[v].y, f.b[v].y, c.x, c.y);
+          stream::mma_bf16(acc, f.a[v].z, f.b[v].z, f.a[v].w, f.b[v].w, c.z, c.w);
+        }
       }
       s0 += sh.prob[j] * acc[0];
       s1 += sh.prob[j] * acc[2];
@@ -508,13 +531,14 @@ __device__ __forceinline__ bool one_token_out(const Params& p, Shared& sh, float
       float y = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) y += red[w * 16 + threadIdx.x];
-      put_y(p, d, y);
+      put_y<F32>(p, d, y);
     }
     __syncthreads();
   }
   return true;
 }
 
+template <bool F32>
 __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ Params p) {
   extern __shared__ float red[];
   __shared__ Shared sh;
@@ -657,7 +681,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
         const int a = it / tiles, next = it + q.step;
         const Rows wn = next < q.end ? rows_in(p, sh, next / tiles, next % tiles, g) : Rows{};
         const int n = __popcll(sh.mask[sh.active[a]]);
-        by_columns(n, [&](auto c) { item_in<decltype(c)::value>(p, sh, red, frag, w, wn, a, it % tiles, n, q.ws); });
+        by_columns(n, [&](auto c) { item_in<decltype(c)::value, F32>(p, sh, red, frag, w, wn, a, it % tiles, n, q.ws); });
         w = wn;
       }
       __syncthreads();  // the second part's groups are others
@@ -666,7 +690,8 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
 
   // -------- 2: output rows of the pairs --------
   if (p.tokens == 1) {
-    const bool ok = (p.d + 7) / 8 <= 2 * (int)gridDim.x ? one_token_out<8>(p, sh, red) : one_token_out<16>(p, sh, red);
+    const bool ok =
+        (p.d + 7) / 8 <= 2 * (int)gridDim.x ? one_token_out<8, F32>(p, sh, red) : one_token_out<16, F32>(p, sh, red);
     if (ok) grid_done(p, sh);
     return;
   }
@@ -687,7 +712,7 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
         const int a = it / tiles, next = it + q.step;
         const Rows wn = next < q.end ? rows_out(p, sh, next / tiles, next % tiles, g) : Rows{};
         const int n = __popcll(sh.mask[sh.active[a]]);
-        by_columns(n, [&](auto c) { item_out<decltype(c)::value>(p, sh, red, frag, w, wn, a, it % tiles, n, q.ws); });
+        by_columns(n, [&](auto c) { item_out<decltype(c)::value, F32>(p, sh, red, frag, w, wn, a, it % tiles, n, q.ws); });
         w = wn;
       }
       __syncthreads();
@@ -710,10 +735,10 @@ __global__ void __launch_bounds__(THREADS, 1) moe_layer(const __grid_constant__ 
       s.w += w * o.w;
     }
     const long long at = tok * p.ldy + d;
-    put_y(p, at, s.x);
-    put_y(p, at + 1, s.y);
-    put_y(p, at + 2, s.z);
-    put_y(p, at + 3, s.w);
+    put_y<F32>(p, at, s.x);
+    put_y<F32>(p, at + 1, s.y);
+    put_y<F32>(p, at + 2, s.z);
+    put_y<F32>(p, at + 3, s.w);
   }
 }
 
@@ -773,12 +798,14 @@ apk_status create(const apk_moe_config* cfg, apk_moe* h) {
   if (major != 10) return h->err.fail(APK_EUNSUPPORTED, "the kernels are built for sm_100a");
   if (c.sms < 0 || c.sms > sms) return h->err.fail(APK_EINVAL, "sms %d of %d", c.sms, sms);
   h->sms = c.sms ? c.sms : sms;
-  APK_TRY(cu_status(cudaFuncSetAttribute(moe::moe_layer, cudaFuncAttributeMaxDynamicSharedMemorySize, moe::red_bytes(8)),
-                    "preparing the expert kernel", &h->err));
-  int per_sm = 0;
-  APK_TRY(cu_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, moe::moe_layer, moe::THREADS, moe::red_bytes(8)),
-                    "preparing the expert kernel", &h->err));
-  if (per_sm < 1) return h->err.fail(APK_EUNSUPPORTED, "the expert kernel does not fit an SM");
+  for (auto kernel : {moe::moe_layer<false>, moe::moe_layer<true>}) {
+    APK_TRY(cu_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, moe::red_bytes(8)),
+                      "preparing the expert kernel", &h->err));
+    int per_sm = 0;
+    APK_TRY(cu_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, moe::THREADS, moe::red_bytes(8)),
+                      "preparing the expert kernel", &h->err));
+    if (per_sm < 1) return h->err.fail(APK_EUNSUPPORTED, "the expert kernel does not fit an SM");
+  }
   return h->scratch.open(c.device, &h->err);
 }
 
@@ -802,7 +829,7 @@ apk_status forward(apk_moe* h, const apk_moe_io* io) {
   const int etiles = (c.experts + 15) / 16;
   p.rsplit = std::max(1, std::min({h->sms / etiles, (c.d_model + moe::WARPS * moe::ROUND - 1) / (moe::WARPS * moe::ROUND), 8}));
   const size_t pairs = (size_t)io->tokens * c.top_k;
-  const size_t b_log = up256((size_t)p.rsplit * io->tokens * c.experts * 4), b_hid = up256(pairs * c.d_ff * 2);
+  const size_t b_log = up256((size_t)p.rsplit * io->tokens * c.experts * 4), b_hid = up256((pairs * c.d_ff * 2) << (io->y_dtype == APK_F32));
   const size_t b_out = up256(pairs * c.d_model * 4), b_choice = up256(pairs * 8);
   APK_TRY(h->scratch.enter(s, &h->err));
   ScratchUse use(&h->scratch, &h->err);
@@ -825,7 +852,6 @@ apk_status forward(apk_moe* h, const apk_moe_io* io) {
   p.act = c.act;
   p.gated = c.gated != 0;
   p.renorm = c.renormalize != 0;
-  p.y_f32 = io->y_dtype == APK_F32;
   p.barrier = reinterpret_cast<unsigned*>(b);
   p.status = h->scratch.status();
   p.limit = c.wait_limit_ns;
@@ -849,7 +875,8 @@ apk_status forward(apk_moe* h, const apk_moe_io* io) {
   cfg.stream = s;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  APK_TRY(cu_status(cudaLaunchKernelEx(&cfg, moe::moe_layer, p), "launching the expert kernel", &h->err));
+  APK_TRY(cu_status(cudaLaunchKernelEx(&cfg, io->y_dtype == APK_F32 ? moe::moe_layer<true> : moe::moe_layer<false>, p),
+                    "launching the expert kernel", &h->err));
   return use.end();
 }
 

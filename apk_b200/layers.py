@@ -274,7 +274,8 @@ class MoE(_Handle):
     router [E, D], w_in [E, 2F, D] (gate rows, then up rows; [E, F, D] when
     not gated) and w_out [E, D, F], bf16 and contiguous.  Each token goes to
     its top_k experts, weighted by their softmax probabilities over all
-    experts, divided by the chosen ones' sum if renormalize.  The weights are
+    experts, divided by the chosen ones' sum if renormalize.  The hidden values
+    are rounded to bf16, or with out_dtype "f32" to two bf16 terms.  Weights are
     kept by reference, as Linear keeps them; nothing is recorded for autograd."""
     _create, _destroy = "apk_moe_create", "apk_moe_destroy"
     _error, _status = "apk_moe_last_error", "apk_moe_status"

@@ -594,7 +594,8 @@ apk_status apk_linear_status(apk_linear* h, void* stream, int* device_status);
  *   divided by their sum if renormalize;
  *   hidden = act(x gate^T) * (x up^T), or act(x w_in^T) if not gated;
  *   y = the sum over the chosen experts of p * (hidden w_out^T).
- * The hidden values are rounded to bf16, everything else is fp32 until y.
+ * The hidden values are rounded to bf16 for a bf16 y, to the sum of two bf16
+ * values (2^-17 of themselves) for an fp32 y; everything else is fp32 until y.
  * Weights are bf16, contiguous, 16-byte aligned; d_model and d_ff are
  * multiples of 8, up to 2^26. */
 typedef struct apk_moe_config {

@@ -87,3 +87,49 @@ def test_experts(T, sms):
     want = w_in[0, :, :T].t().double() @ w_out[0].t().double()
     _check(moe.forward(x), want, F / 512 + 16, "y")
     assert moe.status() == 0
+
+
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("T,E,k,D,F", [(1, 8, 2, 1024, 2048), (1, 4, 3, 8192, 264), (3, 60, 4, 1032, 520), (12, 16, 2, 2048, 1408),
+                                       (30, 8, 4, 512, 4096), (64, 4, 2, 1024, 2048)])
+def test_experts_of_an_fp32_result(T, E, k, D, F, gated):
+    """The hidden values are two bf16 terms: each is off by at most 2^-17 of
+    itself, the weights by the softmax's 2^-18 or so, the sums by less; a single
+    bf16 term would be off by 2^-10 in the 2-norm."""
+    import layer_bounds as lb
+    import torch
+
+    import apk_b200
+
+    def rnd(*shape, seed, scale=1.0):
+        g = torch.Generator("cuda").manual_seed(seed)
+        return torch.empty(shape, dtype=torch.bfloat16, device="cuda").normal_(0.0, scale, generator=g)
+
+    router, w_in = rnd(E, D, seed=1, scale=D ** -0.5), rnd(E, 2 * F if gated else F, D, seed=2, scale=D ** -0.5)
+    w_out, x = rnd(E, D, F, seed=3, scale=F ** -0.5), rnd(T, D, seed=4)
+    moe = apk_b200.MoE(router, w_in, w_out, top_k=k, act="silu", gated=gated, out_dtype="f32")
+    y, ids, _ = moe.forward(x, return_routing=True)
+    want = lb.moe(x, router, w_in, w_out, ids.long(), "silu", gated, True)[0]
+    assert float((y.double() - want).norm() / want.norm()) <= 2.0 ** -16 + 2.0 ** -18
+    half = apk_b200.MoE(router, w_in, w_out, top_k=k, act="silu", gated=gated).forward(x)
+    assert float((half.double() - want).norm() / want.norm()) <= 2.0 ** -7
+
+
+@pytest.mark.parametrize("T", [1, 5, 40])
+def test_infinite_hidden_values_of_an_fp32_result(T):
+    """An infinity is one term, its rest none: it stays infinite."""
+    import torch
+
+    import apk_b200
+    w_in = torch.zeros(1, 8, 8, dtype=torch.bfloat16, device="cuda")
+    w_in[0, 0, 0] = 2.0 ** 100
+    w_out = torch.zeros(1, 8, 8, dtype=torch.bfloat16, device="cuda")
+    w_out[0, 0, 0] = 1.0
+    x = torch.zeros(T, 8, dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = 2.0 ** 100
+    for out in ("f32", "bf16"):
+        moe = apk_b200.MoE(torch.zeros(1, 8, dtype=torch.bfloat16, device="cuda"), w_in, w_out, top_k=1, act="none",
+                           gated=False, out_dtype=out)
+        y = moe.forward(x)
+        assert bool((y[:, 0] == float("inf")).all())
+        assert bool(torch.isnan(y[:, 1:]).all())      # 0 x inf
