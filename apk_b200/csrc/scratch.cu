@@ -21,13 +21,30 @@ class RelaxedCapture {
 
 // What its last user has let go of, a graph perhaps: the callback that tells
 // of a graph's end may not call CUDA.
-struct Gone {
-  std::mutex mu;
-  std::vector<std::pair<int, uint8_t*>> list;
+struct Shared {
+  std::mutex mu;  // of `gone`: held over no CUDA call, which may wait for a callback that wants it
+  std::vector<std::pair<int, uint8_t*>> gone;
+  std::mutex side_mu;
+  std::vector<std::pair<int, cudaStream_t>> side;  // per device, for clearing new memory
 };
-Gone& gone() {
-  static Gone* g = new Gone;  // never destroyed: a graph may end at the process's exit
-  return *g;
+Shared& shared() {
+  static Shared* s = new Shared;  // never destroyed: a graph may end at the process's exit
+  return *s;
+}
+
+// A stream that nothing else uses: the caller's may be captured, and the
+// legacy one is not ordered before non-blocking ones.
+apk_status side_stream(int device, cudaStream_t* out, Err* err) {
+  Shared& g = shared();
+  std::lock_guard<std::mutex> lock(g.side_mu);
+  for (const auto& s : g.side)
+    if (s.first == device) {
+      *out = s.second;
+      return APK_OK;
+    }
+  const apk_status st = cu_status(cudaStreamCreateWithFlags(out, cudaStreamNonBlocking), "cudaStreamCreate", err);
+  if (st == APK_OK) g.side.emplace_back(device, *out);
+  return st;
 }
 
 }  // namespace
@@ -39,10 +56,10 @@ apk_status cu_status(cudaError_t e, const char* what, Err* err) {
 
 Memory::~Memory() {
   if (!data_) return;
-  Gone& g = gone();
+  Shared& g = shared();
   std::lock_guard<std::mutex> lock(g.mu);
   try {
-    g.list.emplace_back(device_, data_);
+    g.gone.emplace_back(device_, data_);
   } catch (...) {  // it stays allocated
   }
 }
@@ -50,9 +67,9 @@ Memory::~Memory() {
 void Memory::free_gone() {
   std::vector<std::pair<int, uint8_t*>> list;
   {
-    Gone& g = gone();
+    Shared& g = shared();
     std::lock_guard<std::mutex> lock(g.mu);
-    list.swap(g.list);
+    list.swap(g.gone);
   }
   if (list.empty()) return;
   RelaxedCapture relaxed;
@@ -72,13 +89,10 @@ apk_status Memory::make(int device, size_t bytes, size_t zeroed, std::shared_ptr
   m->device_ = device;
   m->data_ = static_cast<uint8_t*>(q);
   m->bytes_ = bytes;
-  // on a stream of its own: the caller's may be captured, the legacy one is not ordered before non-blocking ones
   cudaStream_t side = nullptr;
-  if ((st = cu_status(cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking), "cudaStreamCreate", err)) != APK_OK)
-    return st;
-  st = cu_status(cudaMemsetAsync(q, 0, zeroed, side), "cudaMemset", err);
+  st = side_stream(device, &side, err);
+  if (st == APK_OK) st = cu_status(cudaMemsetAsync(q, 0, zeroed, side), "cudaMemset", err);
   if (st == APK_OK) st = cu_status(cudaStreamSynchronize(side), "cudaStreamSynchronize", err);
-  cudaStreamDestroy(side);
   if (st == APK_OK) *out = std::move(m);
   return st;
 }
