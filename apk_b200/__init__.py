@@ -11,12 +11,14 @@ from .runtime import (ApkError, Context, fill_normal_bf16, fill_uniform,  # noqa
                       pinned_empty, round_bf16)
 
 __all__ = ["Context", "ApkError", "fill_uniform", "fill_normal_bf16", "round_bf16", "pinned_empty",
-           "load", "LIB_PATH", "Linear", "MoE"]
+           "load", "LIB_PATH", "Linear", "MoE", "LayerNorm"]
+
+_LAYERS = {"Linear": "layers", "MoE": "layers", "LayerNorm": "layers"}
 
 
 def __getattr__(name):
     # the layer operators work on torch tensors; the rest of the package does without torch
-    if name in ("Linear", "MoE"):
-        from . import layers
-        return getattr(layers, name)
+    if name in _LAYERS:
+        import importlib
+        return getattr(importlib.import_module("." + _LAYERS[name], __name__), name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -11,8 +11,8 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libapk.so")
 
-c_int, c_uint, c_ll, c_ull, c_double, c_size_t, c_void_p, c_char_p = (
-    ctypes.c_int, ctypes.c_uint, ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_double,
+c_int, c_uint, c_ll, c_ull, c_float, c_double, c_size_t, c_void_p, c_char_p = (
+    ctypes.c_int, ctypes.c_uint, ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_float, ctypes.c_double,
     ctypes.c_size_t, ctypes.c_void_p, ctypes.c_char_p)
 
 # enums (apk.h)
@@ -117,6 +117,23 @@ class MoeIO(ctypes.Structure):
                 ("ldy", c_ll), ("ids", c_void_p), ("probs", c_void_p), ("stream", c_void_p)]
 
 
+class NormConfig(ctypes.Structure):
+    _fields_ = [("device", c_int), ("features", c_int), ("eps", c_float), ("weight_dtype", c_int),
+                ("bias_dtype", c_int), ("weight", c_void_p), ("bias", c_void_p)]
+
+
+class NormIO(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("ldx", c_ll), ("rows", c_int), ("x_dtype", c_int), ("y_dtype", c_int),
+                ("y", c_void_p), ("ldy", c_ll), ("stats", c_void_p), ("stream", c_void_p)]
+
+
+class NormGrads(ctypes.Structure):
+    _fields_ = [("dy", c_void_p), ("ld_dy", c_ll), ("x", c_void_p), ("ldx", c_ll), ("stats", c_void_p),
+                ("residual_grad", c_void_p), ("ld_residual", c_ll), ("rows", c_int), ("x_dtype", c_int),
+                ("dy_dtype", c_int), ("dx", c_void_p), ("ld_dx", c_ll), ("dw", c_void_p), ("db", c_void_p),
+                ("stream", c_void_p)]
+
+
 P = c_void_p
 # name -> (restype, argtypes); every symbol include/apk.h declares
 SIGNATURES = {
@@ -167,6 +184,11 @@ SIGNATURES = {
     "apk_moe_last_error": (c_char_p, [P]),
     "apk_moe_forward": (c_int, [P, ctypes.POINTER(MoeIO)]),
     "apk_moe_status": (c_int, [P, P, ctypes.POINTER(c_int)]),
+    "apk_norm_create": (c_int, [ctypes.POINTER(NormConfig), ctypes.POINTER(P)]),
+    "apk_norm_destroy": (c_int, [P]),
+    "apk_norm_last_error": (c_char_p, [P]),
+    "apk_norm_forward": (c_int, [P, ctypes.POINTER(NormIO)]),
+    "apk_norm_backward": (c_int, [P, ctypes.POINTER(NormGrads)]),
     "apk_sgemm_f32_noalloc": (c_int, [P, P, P, c_int, c_int, c_int, c_int, P]),
     "apk_sgemm_f32_noalloc_status": (c_int, [P, ctypes.POINTER(c_int)]),
     "apk_sgemm_f32_noalloc_selftest": (c_int, [c_ll, P]),

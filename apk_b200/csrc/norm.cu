@@ -1,0 +1,448 @@
+// Layer norm over the last axis, forward and backward (apk_norm_* of
+// include/apk.h).  No counterpart in the reference, which multiplies bare
+// matrices (src/tcyield.cu:91-356).
+//
+//   mean = sum x / D,  rstd = 1 / sqrt(sum (x - mean)^2 / D + eps)
+//   n = (x - mean) rstd,  y = n w + b
+//   g = dy w,  dx = rstd (g - mean(g) - n mean(g n)) + residual_grad
+//   dw = sum over rows of dy n,  db = sum over rows of dy
+//
+// Both passes are bound by memory: every row is read once into registers and
+// all sums over it are taken from there, in fp32 (the variance from the
+// differences, so that a mean far from zero costs no digits).
+#include <algorithm>
+
+#include "ops.cuh"
+#include "ops.h"
+
+namespace apk {
+namespace norm {
+
+constexpr int MAX_FEATURES = 16384;  // 1024 threads of two pieces
+
+struct Params {
+  const void* x;
+  const void* dy;
+  const void* w;
+  const void* b;
+  const void* r;     // residual gradient, or null
+  void* y;           // y, or dx (null: not wanted)
+  float2* stats;
+  float* part;       // [blocks][dw, db][cols rounded up to 8]
+  long long ldx, ld_dy, ld_r, ldy;
+  int rows, cols;
+  float eps;
+  int w_f32, b_f32;
+};
+
+// A row's thread t of T holds V pieces of eight columns: contiguous ones
+// where rows can be read 16 bytes at a time (VEC), else every T-th column, so
+// that a warp's loads are contiguous.
+template <bool VEC>
+__device__ __forceinline__ int column(int j, int i, int t, int T) {
+  return VEC ? (j * T + t) * 8 + i : (j * 8 + i) * T + t;
+}
+template <bool VEC, bool F32, int V>
+__device__ __forceinline__ void load_row(const void* p, long long row, ops::Raw<F32> (&raw)[V], int cols, int t, int T) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    raw[j] = {};
+    if constexpr (VEC) {
+      if ((j * T + t) * 8 < cols) ops::ld8(p, row + (j * T + t) * 8, raw[j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (column<false>(j, i, t, T) < cols) ops::set1(raw[j], i, p, row + column<false>(j, i, t, T));
+    }
+  }
+}
+template <bool VEC, bool F32>
+__device__ __forceinline__ void store_piece(void* p, long long row, const float (&v)[8], int j, int cols, int t, int T) {
+  if constexpr (VEC) {
+    ops::Raw<F32> raw;
+    ops::pack(v, raw);
+    if ((j * T + t) * 8 < cols) ops::st8(p, row + (j * T + t) * 8, raw);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (column<false>(j, i, t, T) < cols) ops::st_any(p, row + column<false>(j, i, t, T), v[i], F32);
+  }
+}
+// weight or bias, kept in L1 by its reuse from row to row
+template <bool VEC>
+__device__ __forceinline__ void load_weight(const void* p, int f32, float (&v)[8], int j, int cols, int t, int T) {
+  if (VEC && (j * T + t) * 8 < cols) {
+    if (f32) {
+      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + (j * T + t) * 8);
+      const float4 lo = q[0], hi = q[1];
+      v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+    } else {
+      ops::Raw<false> r{*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + (j * T + t) * 8)};
+      ops::unpack(r, v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = !VEC && column<false>(j, i, t, T) < cols ? ops::ld_any(p, column<false>(j, i, t, T), f32) : 0.f;
+  }
+}
+
+// Sums of a and b over the T threads of a row: a warp, or the block.  `buf`
+// alternates from call to call, so that one barrier a call is enough: who
+// writes a buffer again has passed the barrier behind its last reads.
+template <bool WARP>
+__device__ __forceinline__ float2 row_sum(float a, float b, float2 (*sh)[32], int buf, int T) {
+  a = ops::warp_sum(a);
+  b = ops::warp_sum(b);
+  if constexpr (WARP) return make_float2(a, b);
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) sh[buf][threadIdx.x >> 5] = make_float2(a, b);
+  __syncthreads();
+  const float2 v = lane < T / 32 ? sh[buf][lane] : make_float2(0.f, 0.f);
+  return make_float2(ops::warp_sum(v.x), ops::warp_sum(v.y));
+}
+
+// WARP: a row is a warp's and a block of 8 takes 8; else a row is a block's.
+template <int V, bool VEC, bool WARP, bool XF, bool YF>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) forward(const __grid_constant__ Params p) {
+  __shared__ float2 sh[2][32];
+  const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int per = WARP ? 8 : 1;
+  pdl_launch();
+  pdl_wait();
+  for (long long r = (long long)blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0); r < p.rows; r += (long long)gridDim.x * per) {
+    ops::Raw<XF> raw[V];
+    load_row<VEC, XF, V>(p.x, r * p.ldx, raw, p.cols, t, T);
+    float v[V][8], s = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      ops::unpack(raw[j], v[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[j][i];  // (zero behind the last column)
+    }
+    const float mean = row_sum<WARP>(s, 0.f, sh, 0, T).x / p.cols;
+    s = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = column<VEC>(j, i, t, T) < p.cols ? v[j][i] - mean : 0.f;
+        v[j][i] = d;
+        s = fmaf(d, d, s);
+      }
+    const float rstd = rsqrtf(row_sum<WARP>(s, 0.f, sh, 1, T).x / p.cols + p.eps);
+    if (p.stats && t == 0) p.stats[r] = make_float2(mean, rstd);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float w[8], b[8] = {};
+      load_weight<VEC>(p.w, p.w_f32, w, j, p.cols, t, T);
+      if (p.b) load_weight<VEC>(p.b, p.b_f32, b, j, p.cols, t, T);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = fmaf(v[j][i] * rstd, w[i], b[i]);
+      store_piece<VEC, YF>(p.y, r * p.ldy, w, j, p.cols, t, T);
+    }
+  }
+}
+
+// A block takes every gridDim-th row (of eight, with WARP) and keeps its
+// columns' sums of dy n and dy in registers; they are written once, for reduce().
+template <int V, bool VEC, bool WARP, bool XF, bool DF>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) backward(const __grid_constant__ Params p) {
+  __shared__ float2 sh[2][32];
+  __shared__ float join[WARP ? 8 : 1][WARP ? 256 * V : 1];
+  const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int per = WARP ? 8 : 1;
+  float dw[V][8] = {}, db[V][8] = {};
+  pdl_launch();
+  pdl_wait();
+  int buf = 0;
+  for (long long r = (long long)blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0); r < p.rows; r += (long long)gridDim.x * per) {
+    ops::Raw<XF> rx[V];
+    ops::Raw<DF> rd[V];
+    load_row<VEC, XF, V>(p.x, r * p.ldx, rx, p.cols, t, T);
+    load_row<VEC, DF, V>(p.dy, r * p.ld_dy, rd, p.cols, t, T);
+    const float2 st = p.stats[r];
+    float n[V][8], g[V][8], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float w[8];
+      load_weight<VEC>(p.w, p.w_f32, w, j, p.cols, t, T);
+      ops::unpack(rx[j], n[j]);
+      ops::unpack(rd[j], g[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        n[j][i] = (n[j][i] - st.x) * st.y;
+        dw[j][i] = fmaf(g[j][i], n[j][i], dw[j][i]);
+        db[j][i] += g[j][i];
+        g[j][i] *= w[i];  // (zero behind the last column)
+        s1 += g[j][i];
+        s2 = fmaf(g[j][i], n[j][i], s2);
+      }
+    }
+    if (!p.y) continue;
+    const float2 s = row_sum<WARP>(s1, s2, sh, buf, T);
+    buf ^= 1;
+    const float a = s.x / p.cols, b = s.y / p.cols;
+    ops::Raw<XF> rr[V];
+    if (p.r) load_row<VEC, XF, V>(p.r, r * p.ld_r, rr, p.cols, t, T);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float res[8] = {};
+      if (p.r) ops::unpack(rr[j], res);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[j][i] = fmaf(st.y, g[j][i] - a - n[j][i] * b, res[i]);
+      store_piece<VEC, XF>(p.y, r * p.ldy, g[j], j, p.cols, t, T);
+    }
+  }
+  if (!p.part) return;
+  const int ldp = (p.cols + 7) / 8 * 8;
+  float* part = p.part + (long long)blockIdx.x * 2 * ldp;
+  if constexpr (WARP) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) join[threadIdx.x >> 5][column<VEC>(j, i, t, T)] = h ? db[j][i] : dw[j][i];
+      __syncthreads();
+      for (int c = threadIdx.x; c < p.cols; c += 256) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += join[w][c];
+        part[h * ldp + c] = s;
+      }
+      __syncthreads();
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      store_piece<VEC, true>(part, 0, dw[j], j, p.cols, t, T);
+      store_piece<VEC, true>(part, ldp, db[j], j, p.cols, t, T);
+    }
+  }
+}
+
+// The blocks' sums added up, in their order: 32 columns a block, its warps
+// take every eighth partial.
+struct Reduce {
+  const float* part;
+  void* dw;
+  void* db;
+  int blocks, cols, w_f32, b_f32;
+};
+__global__ void __launch_bounds__(256) reduce(const __grid_constant__ Reduce p) {
+  __shared__ float sh[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane, ldp = (p.cols + 7) / 8 * 8;
+  void* out = blockIdx.y ? p.db : p.dw;
+  pdl_launch();
+  pdl_wait();
+  if (!out) return;
+  float s = 0.f;
+  if (c < p.cols) {
+    const float* q = p.part + blockIdx.y * ldp + c;
+#pragma unroll 8
+    for (int b = warp; b < p.blocks; b += 8) s += __ldcg(q + (long long)b * 2 * ldp);
+  }
+  sh[warp][lane] = s;
+  __syncthreads();
+  if (warp || c >= p.cols) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) s += sh[w][lane];
+  ops::st_any(out, c, s, blockIdx.y ? p.b_f32 : p.w_f32);
+}
+
+using Kernel = void (*)(Params);
+template <int V, bool VEC, bool WARP>
+Kernel fwd_of(bool xf, bool yf) {
+  return xf ? (yf ? &forward<V, VEC, WARP, true, true> : &forward<V, VEC, WARP, true, false>)
+            : (yf ? &forward<V, VEC, WARP, false, true> : &forward<V, VEC, WARP, false, false>);
+}
+template <int V, bool VEC, bool WARP>
+Kernel bwd_of(bool xf, bool df) {
+  return xf ? (df ? &backward<V, VEC, WARP, true, true> : &backward<V, VEC, WARP, true, false>)
+            : (df ? &backward<V, VEC, WARP, false, true> : &backward<V, VEC, WARP, false, false>);
+}
+
+}  // namespace norm
+}  // namespace apk
+
+using namespace apk;
+
+struct apk_norm {
+  apk_norm_config cfg{};
+  Err err;
+  int sms = 0;
+  Scratch scratch;
+  std::mutex mu;
+};
+
+namespace {
+
+apk_status create(const apk_norm_config* cfg, apk_norm* h) {
+  h->cfg = *cfg;
+  const apk_norm_config& c = h->cfg;
+  if (c.features < 1 || c.features > norm::MAX_FEATURES)
+    return h->err.fail(APK_EINVAL, "features is %d: 1 to %d", c.features, norm::MAX_FEATURES);
+  if (!(c.eps > 0.f) || !(c.eps < 1e30f)) return h->err.fail(APK_EINVAL, "eps is %g: above 0 and finite", c.eps);
+  if (!c.weight) return h->err.fail(APK_EINVAL, "weight is NULL");
+  if (!ops::valid_dtype(c.weight_dtype) || (c.bias && !ops::valid_dtype(c.bias_dtype)))
+    return h->err.fail(APK_EINVAL, "weight_dtype %d, bias_dtype %d", (int)c.weight_dtype, (int)c.bias_dtype);
+  if (!ops::aligned(c.weight, ops::esize(c.weight_dtype)) || (c.bias && !ops::aligned(c.bias, ops::esize(c.bias_dtype))))
+    return h->err.fail(APK_EINVAL, "weight or bias is not aligned to its element");
+  APK_TRY(ops::open_device(c.device, &h->sms, &h->err));
+  DeviceGuard guard(c.device);
+  return h->scratch.open(c.device, &h->err);
+}
+
+// Threads of a row, and pieces of each.
+struct Shape {
+  int V, T;
+  bool warp;
+};
+
+apk_status launch(norm::Kernel k, const norm::Params& p, int grid, int threads, cudaStream_t s, const char* what, Err* err) {
+  Launch l(dim3(grid), threads, 0, s);
+  return cu_status(cudaLaunchKernelEx(&l.cfg, k, p), what, err);
+}
+
+apk_status forward(apk_norm* h, const apk_norm_io* io) {
+  const apk_norm_config& c = h->cfg;
+  const int D = c.features, M = io->rows;
+  if (M < 0 || M > ops::MAX_SIZE) return h->err.fail(APK_EINVAL, "rows is %d: at most 2^30", M);
+  if (M == 0) return APK_OK;
+  if (!io->x || !io->y) return h->err.fail(APK_EINVAL, "x or y is NULL");
+  if (!ops::valid_dtype(io->x_dtype) || !ops::valid_dtype(io->y_dtype))
+    return h->err.fail(APK_EINVAL, "x_dtype %d, y_dtype %d", (int)io->x_dtype, (int)io->y_dtype);
+  if (io->ldx < D || io->ldy < D)
+    return h->err.fail(APK_EINVAL, "a row stride is below its row: ldx %lld, ldy %lld", io->ldx, io->ldy);
+  if (!ops::aligned(io->x, ops::esize(io->x_dtype)) || !ops::aligned(io->y, ops::esize(io->y_dtype)) || !ops::aligned(io->stats, 8))
+    return h->err.fail(APK_EINVAL, "a pointer is not aligned to its element (stats: to its pair)");
+  DeviceGuard guard(c.device);
+  norm::Params p{};
+  p.x = io->x;
+  p.ldx = io->ldx;
+  p.w = c.weight;
+  p.b = c.bias;
+  p.w_f32 = c.weight_dtype == APK_F32;
+  p.b_f32 = c.bias_dtype == APK_F32;
+  p.y = io->y;
+  p.ldy = io->ldy;
+  p.stats = reinterpret_cast<float2*>(io->stats);
+  p.rows = M;
+  p.cols = D;
+  p.eps = c.eps;
+  const bool vec = D % 8 == 0 && ops::on16(io->x, io->ldx, M, io->x_dtype) && ops::on16(io->y, io->ldy, M, io->y_dtype) &&
+                   ops::aligned(c.weight, 16) && ops::aligned(c.bias, 16);
+  const bool xf = io->x_dtype == APK_F32, yf = io->y_dtype == APK_F32;
+  norm::Kernel k;
+  int T, per = 1;
+  if (D <= 1024) {  // a warp's row
+    T = 256;
+    per = 8;
+    k = D <= 256   ? (vec ? norm::fwd_of<1, true, true>(xf, yf) : norm::fwd_of<1, false, true>(xf, yf))
+        : D <= 512 ? (vec ? norm::fwd_of<2, true, true>(xf, yf) : norm::fwd_of<2, false, true>(xf, yf))
+                   : (vec ? norm::fwd_of<4, true, true>(xf, yf) : norm::fwd_of<4, false, true>(xf, yf));
+  } else {
+    const int V = D <= 4096 ? 1 : 2;
+    T = ops::ceil_div(ops::ceil_div(D, 8 * V), 32) * 32;
+    k = V == 1 ? (vec ? norm::fwd_of<1, true, false>(xf, yf) : norm::fwd_of<1, false, false>(xf, yf))
+               : (vec ? norm::fwd_of<2, true, false>(xf, yf) : norm::fwd_of<2, false, false>(xf, yf));
+  }
+  const int grid = std::min(ops::ceil_div(M, per), h->sms * (2048 / T));
+  return launch(k, p, grid, T, static_cast<cudaStream_t>(io->stream), "launching the layer norm", &h->err);
+}
+
+apk_status backward(apk_norm* h, const apk_norm_grads* g) {
+  const apk_norm_config& c = h->cfg;
+  const int D = c.features, M = g->rows;
+  const cudaStream_t s = static_cast<cudaStream_t>(g->stream);
+  if (M < 0 || M > ops::MAX_SIZE) return h->err.fail(APK_EINVAL, "rows is %d: at most 2^30", M);
+  if (!g->dx && !g->dw && !g->db) return h->err.fail(APK_EINVAL, "no gradient is asked for");
+  if (g->db && !c.bias) return h->err.fail(APK_EINVAL, "db of a norm without a bias");
+  if (M > 0 && (!g->dy || !g->x || !g->stats)) return h->err.fail(APK_EINVAL, "dy, x or stats is NULL");
+  if (!ops::valid_dtype(g->x_dtype) || !ops::valid_dtype(g->dy_dtype))
+    return h->err.fail(APK_EINVAL, "x_dtype %d, dy_dtype %d", (int)g->x_dtype, (int)g->dy_dtype);
+  if (g->ldx < D || g->ld_dy < D || (g->dx && g->ld_dx < D) || (g->residual_grad && g->ld_residual < D))
+    return h->err.fail(APK_EINVAL, "a row stride is below its row: ldx %lld, ld_dy %lld, ld_dx %lld, ld_residual %lld", g->ldx,
+                       g->ld_dy, g->ld_dx, g->ld_residual);
+  const size_t ex = ops::esize(g->x_dtype);
+  if (!ops::aligned(g->x, ex) || !ops::aligned(g->dy, ops::esize(g->dy_dtype)) || !ops::aligned(g->dx, ex) ||
+      !ops::aligned(g->residual_grad, ex) || !ops::aligned(g->stats, 8) || !ops::aligned(g->dw, ops::esize(c.weight_dtype)) ||
+      (g->db && !ops::aligned(g->db, ops::esize(c.bias_dtype))))
+    return h->err.fail(APK_EINVAL, "a pointer is not aligned to its element (stats: to its pair)");
+  DeviceGuard guard(c.device);
+  if (M == 0) {  // sums over no rows
+    if (g->dw) APK_TRY(cu_status(cudaMemsetAsync(g->dw, 0, D * ops::esize(c.weight_dtype), s), "clearing dw", &h->err));
+    if (g->db) APK_TRY(cu_status(cudaMemsetAsync(g->db, 0, D * ops::esize(c.bias_dtype), s), "clearing db", &h->err));
+    return APK_OK;
+  }
+  norm::Params p{};
+  p.x = g->x;
+  p.dy = g->dy;
+  p.w = c.weight;
+  p.w_f32 = c.weight_dtype == APK_F32;
+  p.r = g->residual_grad;
+  p.y = g->dx;
+  p.stats = reinterpret_cast<float2*>(const_cast<float*>(g->stats));
+  p.ldx = g->ldx;
+  p.ld_dy = g->ld_dy;
+  p.ld_r = g->ld_residual;
+  p.ldy = g->ld_dx;
+  p.rows = M;
+  p.cols = D;
+  const bool vec = D % 8 == 0 && ops::on16(g->x, g->ldx, M, g->x_dtype) && ops::on16(g->dy, g->ld_dy, M, g->dy_dtype) &&
+                   (!g->dx || ops::on16(g->dx, g->ld_dx, M, g->x_dtype)) &&
+                   (!g->residual_grad || ops::on16(g->residual_grad, g->ld_residual, M, g->x_dtype)) && ops::aligned(c.weight, 16);
+  const bool xf = g->x_dtype == APK_F32, df = g->dy_dtype == APK_F32;
+  norm::Kernel k;
+  int T, per = 1;
+  if (D <= 512) {
+    T = 256;
+    per = 8;
+    k = D <= 256 ? (vec ? norm::bwd_of<1, true, true>(xf, df) : norm::bwd_of<1, false, true>(xf, df))
+                 : (vec ? norm::bwd_of<2, true, true>(xf, df) : norm::bwd_of<2, false, true>(xf, df));
+  } else {
+    const int V = D <= 2048 ? 1 : 2;
+    T = ops::ceil_div(ops::ceil_div(D, 8 * V), 32) * 32;
+    k = V == 1 ? (vec ? norm::bwd_of<1, true, false>(xf, df) : norm::bwd_of<1, false, false>(xf, df))
+               : (vec ? norm::bwd_of<2, true, false>(xf, df) : norm::bwd_of<2, false, false>(xf, df));
+  }
+  const int grid = std::min(ops::ceil_div(M, per), h->sms * std::max(1, 1024 / T));
+  const bool sums = g->dw || g->db;
+  APK_TRY(h->scratch.enter(s, &h->err));
+  ScratchUse use(&h->scratch, &h->err);
+  if (sums) {
+    APK_TRY(use.begin(ops::up256((size_t)grid * 2 * ops::ceil_div(D, 8) * 8 * 4), 0));
+    p.part = reinterpret_cast<float*>(h->scratch.data());
+  }
+  APK_TRY(launch(k, p, grid, T, s, "launching the layer norm's gradient", &h->err));
+  if (sums) {
+    const norm::Reduce q{p.part, g->dw, g->db, grid, D, c.weight_dtype == APK_F32, c.bias_dtype == APK_F32};
+    Launch l(dim3(ops::ceil_div(D, 32), 2), 256, 0, s);
+    APK_TRY(cu_status(cudaLaunchKernelEx(&l.cfg, norm::reduce, q), "launching the sum of the weight's gradient", &h->err));
+  }
+  return use.end();
+}
+
+}  // namespace
+
+extern "C" {
+
+apk_status apk_norm_create(const apk_norm_config* cfg, apk_norm** out) { return ops::make(cfg, out, create); }
+
+apk_status apk_norm_destroy(apk_norm* h) {
+  delete h;
+  return APK_OK;
+}
+
+const char* apk_norm_last_error(const apk_norm* h) { return h ? h->err.text.c_str() : "NULL handle"; }
+
+apk_status apk_norm_forward(apk_norm* h, const apk_norm_io* io) {
+  return ops::call(h, io, [&] { return forward(h, io); });
+}
+
+apk_status apk_norm_backward(apk_norm* h, const apk_norm_grads* g) {
+  return ops::call(h, g, [&] { return backward(h, g); });
+}
+
+}  // extern "C"

@@ -1,6 +1,7 @@
-"""Layer operators over torch tensors: Linear (forward, backward) and MoE.
+"""Layer operators over torch tensors: Linear and LayerNorm (forward,
+backward) and MoE.
 
-Thin classes over the C ABI's apk_linear_* and apk_moe_* (include/apk.h):
+Thin classes over the C ABI's apk_linear_*, apk_norm_* and apk_moe_* (include/apk.h):
 they check shapes, types and strides, allocate outputs with torch, and run
 on torch's current stream of the weights' device.  torch is used for memory
 and streams only; the arithmetic is libapk's.  No counterpart in the
@@ -263,6 +264,115 @@ class Linear(_Handle):
             g.stream = _raw_stream(self._index)
             if dw is not None or db is not None or (dx is not None and g.rows > 0):
                 st = self._lib.apk_linear_backward(self._h, self._grads_ref)
+                if st:
+                    self._check(st)
+            return dx, dw, db
+
+
+class LayerNorm(_Handle):
+    """y = (x - mean) rstd w + b over the last axis, and its gradients.
+
+    weight, bias: [features], fp32 or bf16, kept by reference as Linear keeps
+    them.  x may be fp32 or bf16.  Nothing is recorded for autograd."""
+    _create, _destroy, _error = "apk_norm_create", "apk_norm_destroy", "apk_norm_last_error"
+
+    def __init__(self, weight, bias=None, eps: float = 1e-5, out_dtype: str = "bf16"):
+        _tensor(weight, "weight", dtypes=_ANY, dim=1)
+        self.device, self._index = weight.device, weight.device.index
+        self.features = weight.shape[0]
+        for t, what in ((weight, "weight"), (bias, "bias")):
+            if t is None:
+                continue
+            _tensor(t, what, self.device, _ANY, 1)
+            if t.shape[0] != self.features or (t.shape[0] > 1 and t.stride(0) != 1):
+                raise ValueError(f"{what} is {tuple(t.shape)} with strides {t.stride()}: "
+                                 f"{self.features} contiguous values are wanted")
+        self.weight, self.bias, self.eps = weight, bias, eps
+        self._w_at, self._b_at = weight.data_ptr(), None if bias is None else bias.data_ptr()
+        self.out_dtype = _pick(_TORCH, out_dtype, "out_dtype")
+        self._open(L.NormConfig(self._index, self.features, eps, _CODE[weight.dtype],
+                                _CODE[bias.dtype] if bias is not None else L.APK_F32, self._w_at, self._b_at))
+        self._io, self._grads = L.NormIO(), L.NormGrads()
+        self._io.y_dtype = _CODE[self.out_dtype]
+        self._io_ref, self._grads_ref = ctypes.byref(self._io), ctypes.byref(self._grads)
+
+    def _unmoved(self):
+        b = self.bias
+        if self.weight.data_ptr() != self._w_at or (None if b is None else b.data_ptr()) != self._b_at:
+            raise ValueError(_MOVED)
+
+    def forward(self, x, save_stats: bool = False, out=None):
+        """The norm of x [..., features]; with save_stats also its rows' mean
+        and rstd, fp32 [..., 2], as backward() takes them.  out: the output's
+        tensor; it may be x, but share no memory with it otherwise."""
+        with self._lock:
+            self._unmoved()
+            io, d = self._io, self.features
+            io.x, io.rows, io.ldx = _rows(x, "x", self.device, d, _ANY)
+            io.x_dtype = _CODE[x.dtype]
+            if out is None:
+                y = _like(x, x.shape) if x.dtype is self.out_dtype else x.new_empty(x.shape, dtype=self.out_dtype)
+                io.y, io.ldy = y.data_ptr(), d
+            else:
+                y = out
+                if y.shape != x.shape:
+                    raise ValueError(f"out is {tuple(y.shape)}, not {tuple(x.shape)}")
+                io.y, _, io.ldy = _rows(y, "out", self.device, d, (self.out_dtype,))
+                ys, xs = y.element_size(), x.element_size()
+                to, of = (io.y, io.ldy * ys, d * ys), (io.x, io.ldx * xs, d * xs)
+                if to != of and _overlap(to, of, io.rows):
+                    raise ValueError("out shares memory with x, but is not it")
+            stats = None
+            if save_stats:
+                stats = x.new_empty((*x.shape[:-1], 2), dtype=torch.float32)
+                io.stats = stats.data_ptr()
+            else:
+                io.stats = None
+            io.stream = _raw_stream(self._index)
+            st = self._lib.apk_norm_forward(self._h, self._io_ref)
+            if st:
+                self._check(st)
+            return (y, stats) if save_stats else y
+
+    __call__ = forward
+
+    def backward(self, dy, x, stats, residual_grad=None, need_dx: bool = True, need_dw: bool = True,
+                 need_db: bool = True):
+        """(dx, dw, db) for the output gradient dy; None where one is not
+        needed or the norm has no bias.  stats: what forward(save_stats=True)
+        returned.  residual_grad, of x's shape and type, is added to dx."""
+        with self._lock:
+            self._unmoved()
+            g, d = self._grads, self.features
+            g.x, g.rows, g.ldx = _rows(x, "x", self.device, d, _ANY)
+            if dy.shape != x.shape:
+                raise ValueError(f"dy is {tuple(dy.shape)} and x {tuple(x.shape)}")
+            g.dy, _, g.ld_dy = _rows(dy, "dy", self.device, d, _ANY)
+            g.x_dtype, g.dy_dtype = _CODE[x.dtype], _CODE[dy.dtype]
+            _tensor(stats, "stats", self.device, (torch.float32,))
+            if stats.shape != (*x.shape[:-1], 2) or not stats.is_contiguous():
+                raise ValueError("stats: the contiguous statistics that forward(save_stats=True) returned are wanted")
+            g.stats = stats.data_ptr()
+            if residual_grad is None:
+                g.residual_grad = None
+            else:
+                if residual_grad.shape != x.shape:
+                    raise ValueError(f"residual_grad is {tuple(residual_grad.shape)}, not {tuple(x.shape)}")
+                g.residual_grad, _, g.ld_residual = _rows(residual_grad, "residual_grad", self.device, d, (x.dtype,))
+            g.dx = g.dw = g.db = None
+            dx = dw = db = None
+            if need_dx:
+                dx = _like(x, x.shape)
+                g.dx, g.ld_dx = dx.data_ptr(), d
+            if need_dw:
+                dw = _like(self.weight, self.weight.shape)
+                g.dw = dw.data_ptr()
+            if need_db and self.bias is not None:
+                db = _like(self.bias, self.bias.shape)
+                g.db = db.data_ptr()
+            g.stream = _raw_stream(self._index)
+            if dw is not None or db is not None or (dx is not None and g.rows > 0):
+                st = self._lib.apk_norm_backward(self._h, self._grads_ref)
                 if st:
                     self._check(st)
             return dx, dw, db

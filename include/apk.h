@@ -636,6 +636,69 @@ apk_status apk_moe_forward(apk_moe* h, const apk_moe_io* io);
  * flight. */
 apk_status apk_moe_status(apk_moe* h, void* stream, int* device_status);
 
+/* ---- layers: what stands around the feed-forward half --------------------- */
+
+/* The same manner as above: device pointers, strides in elements, the last
+ * axis contiguous, asynchronous on `stream`, handles that keep the caller's
+ * weight pointers, scratch that a capture does not grow.  These kernels wait
+ * for nothing, so there is no status to ask for.  A create that fails sets
+ * *out all the same (unless memory ran out), as apk_linear_create does. */
+
+/* Layer norm over the last axis:  mean and variance of each row (the variance
+ * over all of its features), rstd = 1 / sqrt(variance + eps),
+ * y = (x - mean) rstd weight + bias.  All in fp32, y rounded once. */
+typedef struct apk_norm_config {
+  int device;
+  int features;             /* 1 to 16384                                     */
+  float eps;                /* above 0                                        */
+  apk_dtype weight_dtype, bias_dtype;
+  const void* weight;       /* [features]                                     */
+  const void* bias;         /* [features] or NULL                             */
+} apk_norm_config;
+typedef struct apk_norm apk_norm;
+
+apk_status apk_norm_create(const apk_norm_config* cfg, apk_norm** out);
+apk_status apk_norm_destroy(apk_norm* h);
+const char* apk_norm_last_error(const apk_norm* h);
+
+/* rows = 0 does nothing; up to 2^30.  y may be x itself (same stride and
+ * type), else it shares no memory with x. */
+typedef struct apk_norm_io {
+  const void* x;            /* [rows][features]                               */
+  long long ldx;
+  int rows;
+  apk_dtype x_dtype, y_dtype;
+  void* y;
+  long long ldy;
+  float* stats;             /* [rows][2], mean and rstd for the backward pass, or NULL; on 8 bytes */
+  void* stream;
+} apk_norm_io;
+apk_status apk_norm_forward(apk_norm* h, const apk_norm_io* io);
+
+/* Gradients of a forward call:  n = (x - mean) rstd,  g = dy weight,
+ * dx = rstd (g - mean(g) - n mean(g n)) + residual_grad,
+ * dw = the sum over rows of dy n,  db = that of dy, in fp32 and in an order
+ * that depends on the sizes alone.  residual_grad is what reaches x past the
+ * norm (a block's residual stream).  An output that is NULL is not computed;
+ * none shares memory with an input.  With rows = 0, dw and db are cleared. */
+typedef struct apk_norm_grads {
+  const void* dy;           /* [rows][features]                               */
+  long long ld_dy;
+  const void* x;
+  long long ldx;
+  const float* stats;       /* as forward wrote it                            */
+  const void* residual_grad; /* x_dtype [rows][features] or NULL              */
+  long long ld_residual;
+  int rows;
+  apk_dtype x_dtype, dy_dtype;
+  void* dx;                 /* x_dtype [rows][features] or NULL               */
+  long long ld_dx;
+  void* dw;                 /* features of weight_dtype, or NULL              */
+  void* db;                 /* features of bias_dtype, or NULL                */
+  void* stream;
+} apk_norm_grads;
+apk_status apk_norm_backward(apk_norm* h, const apk_norm_grads* g);
+
 /* ---- allocation-free entry point --------------------------------------- */
 
 /* C = A * B (fp32, row-major, device pointers, 16-byte aligned; M and N
