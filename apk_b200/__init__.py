@@ -11,9 +11,10 @@ from .runtime import (ApkError, Context, fill_normal_bf16, fill_uniform,  # noqa
                       pinned_empty, round_bf16)
 
 __all__ = ["Context", "ApkError", "fill_uniform", "fill_normal_bf16", "round_bf16", "pinned_empty",
-           "load", "LIB_PATH", "Linear", "MoE", "LayerNorm"]
+           "load", "LIB_PATH", "Linear", "MoE", "LayerNorm",
+           "GradClip"]
 
-_LAYERS = {"Linear": "layers", "MoE": "layers", "LayerNorm": "layers"}
+_LAYERS = {"Linear": "layers", "MoE": "layers", "LayerNorm": "layers", "GradClip": "training"}
 
 
 def __getattr__(name):

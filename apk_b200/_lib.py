@@ -134,6 +134,15 @@ class NormGrads(ctypes.Structure):
                 ("stream", c_void_p)]
 
 
+class ClipConfig(ctypes.Structure):
+    _fields_ = [("device", c_int)]
+
+
+class ClipIO(ctypes.Structure):
+    _fields_ = [("count", c_int), ("in_", c_void_p), ("out", c_void_p), ("n", c_void_p), ("dtype", c_void_p),
+                ("max_norm", c_float), ("norm", c_void_p), ("stream", c_void_p)]
+
+
 P = c_void_p
 # name -> (restype, argtypes); every symbol include/apk.h declares
 SIGNATURES = {
@@ -189,6 +198,11 @@ SIGNATURES = {
     "apk_norm_last_error": (c_char_p, [P]),
     "apk_norm_forward": (c_int, [P, ctypes.POINTER(NormIO)]),
     "apk_norm_backward": (c_int, [P, ctypes.POINTER(NormGrads)]),
+    "apk_clip_create": (c_int, [ctypes.POINTER(ClipConfig), ctypes.POINTER(P)]),
+    "apk_clip_destroy": (c_int, [P]),
+    "apk_clip_last_error": (c_char_p, [P]),
+    "apk_clip_norm": (c_int, [P, ctypes.POINTER(ClipIO)]),
+    "apk_clip_scale": (c_int, [P, ctypes.POINTER(ClipIO)]),
     "apk_sgemm_f32_noalloc": (c_int, [P, P, P, c_int, c_int, c_int, c_int, P]),
     "apk_sgemm_f32_noalloc_status": (c_int, [P, ctypes.POINTER(c_int)]),
     "apk_sgemm_f32_noalloc_selftest": (c_int, [c_ll, P]),

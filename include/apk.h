@@ -699,6 +699,38 @@ typedef struct apk_norm_grads {
 } apk_norm_grads;
 apk_status apk_norm_backward(apk_norm* h, const apk_norm_grads* g);
 
+/* The global norm of many tensors, and clipping by it:
+ *   norm = sqrt(the sum of the squares of all elements of all tensors),
+ *   out = in * min(1, max_norm / (norm + 1e-6)).
+ * Squares are added in fp32 over a few values at a time and in 64 bits beyond
+ * (values whose squares leave fp32 in 64 bits throughout), in an order that
+ * depends on the sizes and addresses alone.  A norm that is infinite makes the
+ * factor 0, a NaN makes it NaN: all outputs then show it.  The host arrays are
+ * read before the call returns. */
+typedef struct apk_clip_config {
+  int device;
+} apk_clip_config;
+typedef struct apk_clip apk_clip;
+
+apk_status apk_clip_create(const apk_clip_config* cfg, apk_clip** out);
+apk_status apk_clip_destroy(apk_clip* h);
+const char* apk_clip_last_error(const apk_clip* h);
+
+typedef struct apk_clip_io {
+  int count;                /* tensors; 0 has the norm 0                      */
+  const void* const* in;    /* host array of device pointers                  */
+  void* const* out;         /* the same, of each input's type; may be in's own
+                               pointers, else no other tensor's memory; unused
+                               by apk_clip_norm                               */
+  const long long* n;       /* host array: elements of each, 0 to 2^40        */
+  const int* dtype;         /* host array of apk_dtype                        */
+  float max_norm;           /* 0 or above                                     */
+  float* norm;              /* device: receives the norm before clipping      */
+  void* stream;
+} apk_clip_io;
+apk_status apk_clip_norm(apk_clip* h, const apk_clip_io* io);
+apk_status apk_clip_scale(apk_clip* h, const apk_clip_io* io);
+
 /* ---- allocation-free entry point --------------------------------------- */
 
 /* C = A * B (fp32, row-major, device pointers, 16-byte aligned; M and N
