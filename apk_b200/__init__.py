@@ -12,9 +12,10 @@ from .runtime import (ApkError, Context, fill_normal_bf16, fill_uniform,  # noqa
 
 __all__ = ["Context", "ApkError", "fill_uniform", "fill_normal_bf16", "round_bf16", "pinned_empty",
            "load", "LIB_PATH", "Linear", "MoE", "LayerNorm",
-           "GradClip"]
+           "GradClip", "LogProbs"]
 
-_LAYERS = {"Linear": "layers", "MoE": "layers", "LayerNorm": "layers", "GradClip": "training"}
+_LAYERS = {"Linear": "layers", "MoE": "layers", "LayerNorm": "layers", "GradClip": "training",
+           "LogProbs": "training"}
 
 
 def __getattr__(name):

@@ -143,6 +143,22 @@ class ClipIO(ctypes.Structure):
                 ("max_norm", c_float), ("norm", c_void_p), ("stream", c_void_p)]
 
 
+class LogprobsConfig(ctypes.Structure):
+    _fields_ = [("device", c_int), ("top", c_int)]
+
+
+class LogprobsIO(ctypes.Structure):
+    _fields_ = [("logits", c_void_p), ("ld", c_ll), ("rows", c_int), ("vocabulary", c_int), ("dtype", c_int),
+                ("tokens_64", c_int), ("tokens", c_void_p), ("logprob", c_void_p), ("entropy", c_void_p),
+                ("top_ids", c_void_p), ("top_logprobs", c_void_p), ("stats", c_void_p), ("stream", c_void_p)]
+
+
+class LogprobsGrads(ctypes.Structure):
+    _fields_ = [("logits", c_void_p), ("ld", c_ll), ("rows", c_int), ("vocabulary", c_int), ("dtype", c_int),
+                ("tokens_64", c_int), ("tokens", c_void_p), ("dlogprob", c_void_p), ("dentropy", c_void_p),
+                ("entropy", c_void_p), ("stats", c_void_p), ("dlogits", c_void_p), ("ld_d", c_ll), ("stream", c_void_p)]
+
+
 P = c_void_p
 # name -> (restype, argtypes); every symbol include/apk.h declares
 SIGNATURES = {
@@ -203,6 +219,11 @@ SIGNATURES = {
     "apk_clip_last_error": (c_char_p, [P]),
     "apk_clip_norm": (c_int, [P, ctypes.POINTER(ClipIO)]),
     "apk_clip_scale": (c_int, [P, ctypes.POINTER(ClipIO)]),
+    "apk_logprobs_create": (c_int, [ctypes.POINTER(LogprobsConfig), ctypes.POINTER(P)]),
+    "apk_logprobs_destroy": (c_int, [P]),
+    "apk_logprobs_last_error": (c_char_p, [P]),
+    "apk_logprobs_forward": (c_int, [P, ctypes.POINTER(LogprobsIO)]),
+    "apk_logprobs_backward": (c_int, [P, ctypes.POINTER(LogprobsGrads)]),
     "apk_sgemm_f32_noalloc": (c_int, [P, P, P, c_int, c_int, c_int, c_int, P]),
     "apk_sgemm_f32_noalloc_status": (c_int, [P, ctypes.POINTER(c_int)]),
     "apk_sgemm_f32_noalloc_selftest": (c_int, [c_ll, P]),

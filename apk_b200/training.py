@@ -1,6 +1,7 @@
-"""Operators around a training step over torch tensors: GradClip.
+"""Operators around a training step over torch tensors: GradClip and
+LogProbs, which a server uses as well.
 
-Thin classes over the C ABI's apk_clip_* (include/apk.h), in the manner of
+Thin classes over the C ABI's apk_clip_* and apk_logprobs_* (include/apk.h), in the manner of
 layers.py: torch is used for memory and streams only.  No counterpart in the
 reference, which multiplies bare matrices (src/tcyield.cu:91-356).
 """
@@ -13,7 +14,7 @@ import math
 import torch
 
 from . import _lib as L
-from .layers import _ANY, _CODE, _Handle, _raw_stream, _tensor
+from .layers import _ANY, _CODE, _Handle, _like, _overlap, _raw_stream, _rows, _tensor
 
 _TYPES = set(_ANY)
 
@@ -115,3 +116,108 @@ class GradClip(_Handle):
         return self._run(grads, out, self._lib.apk_clip_scale)
 
     __call__ = clip
+
+
+class LogProbs(_Handle):
+    """Log probabilities of given tokens, entropies and the `top` largest
+    alternatives of rows of logits (fp32 or bf16), and their gradient."""
+    _create, _destroy, _error = "apk_logprobs_create", "apk_logprobs_destroy", "apk_logprobs_last_error"
+
+    def __init__(self, top: int = 0, device=None):
+        if top not in range(33):
+            raise ValueError(f"top is {top!r}: 0 to 32")
+        self.top = int(top)
+        self._index = _device_index(device)
+        self.device = torch.device("cuda", self._index)
+        self._open(L.LogprobsConfig(self._index, self.top))
+        self._io, self._grads = L.LogprobsIO(), L.LogprobsGrads()
+        self._io_ref, self._grads_ref = ctypes.byref(self._io), ctypes.byref(self._grads)
+
+    def _logits(self, logits, a):
+        if not isinstance(logits, torch.Tensor) or logits.dim() < 1 or logits.shape[-1] < max(1, self.top):
+            raise ValueError(f"logits: a tensor [..., vocabulary] of at least {max(1, self.top)} is wanted")
+        a.vocabulary = logits.shape[-1]
+        a.logits, a.rows, a.ld = _rows(logits, "logits", self.device, a.vocabulary, _ANY)
+        a.dtype = _CODE[logits.dtype]
+
+    def _per_row(self, t, what, shape, dtypes):
+        _tensor(t, what, self.device, dtypes)
+        if t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{what} is {tuple(t.shape)} with strides {t.stride()}: contiguous {tuple(shape)} is wanted")
+        return t.data_ptr()
+
+    def _tokens(self, tokens, shape, a):
+        a.tokens = self._per_row(tokens, "tokens", shape, (torch.int64, torch.int32))
+        a.tokens_64 = tokens.dtype is torch.int64
+
+    def forward(self, logits, tokens=None, save_stats: bool = False):
+        """(logprob, entropy, top_ids, top_logprobs) for logits [..., V] and
+        tokens [...]; None without tokens, or where top is 0; with save_stats
+        a fifth: what backward() takes.  A negative token is padding, with log
+        probability 0.  ids are int32, the others fp32."""
+        with self._lock:
+            io = self._io
+            self._logits(logits, io)
+            shape = logits.shape[:-1]
+            new = logits.new_empty
+            logprob = ids = tops = stats = None
+            if tokens is None:
+                io.tokens = io.logprob = None
+            else:
+                self._tokens(tokens, shape, io)
+                logprob = new(shape, dtype=torch.float32)
+                io.logprob = logprob.data_ptr()
+            entropy = new(shape, dtype=torch.float32)
+            io.entropy = entropy.data_ptr()
+            if self.top:
+                ids, tops = new((*shape, self.top), dtype=torch.int32), new((*shape, self.top), dtype=torch.float32)
+                io.top_ids, io.top_logprobs = ids.data_ptr(), tops.data_ptr()
+            if save_stats:
+                stats = new((*shape, 2), dtype=torch.float32)
+                io.stats = stats.data_ptr()
+            else:
+                io.stats = None
+            io.stream = _raw_stream(self._index)
+            st = self._lib.apk_logprobs_forward(self._h, self._io_ref)
+            if st:
+                self._check(st)
+            return (logprob, entropy, ids, tops, stats) if save_stats else (logprob, entropy, ids, tops)
+
+    __call__ = forward
+
+    def backward(self, dlogprob, logits, tokens, stats, dentropy=None, entropy=None, out=None):
+        """The logits' gradient, of their type, for the outputs' gradients
+        dlogprob and dentropy (fp32 [...]; None: not used).  stats and, with
+        dentropy, entropy: what forward(save_stats=True) returned.  out: the
+        gradient's tensor; it may be the logits, but share no memory with them
+        otherwise."""
+        with self._lock:
+            g = self._grads
+            self._logits(logits, g)
+            shape, f32 = logits.shape[:-1], (torch.float32,)
+            if dlogprob is None and dentropy is None:
+                raise ValueError("dlogprob or dentropy is wanted")
+            g.tokens = g.dlogprob = g.dentropy = g.entropy = None
+            if dlogprob is not None:
+                self._tokens(tokens, shape, g)
+                g.dlogprob = self._per_row(dlogprob, "dlogprob", shape, f32)
+            if dentropy is not None:
+                g.dentropy = self._per_row(dentropy, "dentropy", shape, f32)
+                g.entropy = self._per_row(entropy, "entropy", shape, f32)
+            g.stats = self._per_row(stats, "stats", (*shape, 2), f32)
+            if out is None:
+                out = _like(logits, logits.shape)
+                g.dlogits, g.ld_d = out.data_ptr(), g.vocabulary
+            else:
+                if not isinstance(out, torch.Tensor) or out.shape != logits.shape:
+                    raise ValueError(f"out: a tensor {tuple(logits.shape)} is wanted")
+                g.dlogits, _, g.ld_d = _rows(out, "out", self.device, g.vocabulary, (logits.dtype,))
+                es = out.element_size()
+                to, of = (g.dlogits, g.ld_d * es, g.vocabulary * es), (g.logits, g.ld * es, g.vocabulary * es)
+                if to != of and _overlap(to, of, g.rows):
+                    raise ValueError("out shares memory with logits, but is not it")
+            g.stream = _raw_stream(self._index)
+            st = self._lib.apk_logprobs_backward(self._h, self._grads_ref)
+            if st:
+                self._check(st)
+            return out

@@ -731,6 +731,63 @@ typedef struct apk_clip_io {
 apk_status apk_clip_norm(apk_clip* h, const apk_clip_io* io);
 apk_status apk_clip_scale(apk_clip* h, const apk_clip_io* io);
 
+/* Log probabilities of given tokens, the distributions' entropies and the
+ * largest alternatives.  For each row x of logits:
+ *   m = max x,  S = the sum of exp(x - m),  l = (x - m) - log S;
+ *   logprob = l[token], 0 for a negative token (padding), NaN for one that is
+ *   not in the vocabulary;  entropy = -sum exp(l) l, where a logit of -inf
+ *   adds 0;  the `top` largest logits, in order (ties to the lowest index, a
+ *   NaN counts as the largest), with their l.
+ * A row with no logit above -inf, or with a NaN or +inf, has NaNs (a negative
+ * token's logprob stays 0).  Sums are fp32. */
+typedef struct apk_logprobs_config {
+  int device;
+  int top;                  /* 0 to 32                                        */
+} apk_logprobs_config;
+typedef struct apk_logprobs apk_logprobs;
+
+apk_status apk_logprobs_create(const apk_logprobs_config* cfg, apk_logprobs** out);
+apk_status apk_logprobs_destroy(apk_logprobs* h);
+const char* apk_logprobs_last_error(const apk_logprobs* h);
+
+typedef struct apk_logprobs_io {
+  const void* logits;       /* [rows][vocabulary]                             */
+  long long ld;
+  int rows, vocabulary;     /* up to 2^30 each, top at least; rows = 0 does nothing */
+  apk_dtype dtype;
+  int tokens_64;            /* tokens are 64-bit integers, else 32-bit        */
+  const void* tokens;       /* [rows], or NULL with logprob NULL              */
+  float* logprob;           /* [rows] or NULL                                 */
+  float* entropy;           /* [rows] or NULL                                 */
+  int* top_ids;             /* [rows][top]                                    */
+  float* top_logprobs;      /* [rows][top]                                    */
+  float* stats;             /* [rows][2], m and log S for the backward pass, or NULL; on 8 bytes */
+  void* stream;
+} apk_logprobs_io;
+apk_status apk_logprobs_forward(apk_logprobs* h, const apk_logprobs_io* io);
+
+/* Gradient of a forward call by its logprob and entropy:
+ *   dlogits_j = dlogprob ([j = token] - p_j) - dentropy p_j (l_j + entropy),
+ * p = exp(l); 0 where p is.  Rows whose dlogprob (or token: padding) and
+ * dentropy are 0 get zeros, whatever their logits.  dlogits may be the logits
+ * themselves (same stride), else it shares no memory with them. */
+typedef struct apk_logprobs_grads {
+  const void* logits;
+  long long ld;
+  int rows, vocabulary;
+  apk_dtype dtype;
+  int tokens_64;
+  const void* tokens;
+  const float* dlogprob;    /* [rows] or NULL                                 */
+  const float* dentropy;    /* [rows] or NULL                                 */
+  const float* entropy;     /* [rows], as forward wrote it; with dentropy     */
+  const float* stats;       /* [rows][2], as forward wrote it                 */
+  void* dlogits;            /* dtype [rows][vocabulary]                       */
+  long long ld_d;
+  void* stream;
+} apk_logprobs_grads;
+apk_status apk_logprobs_backward(apk_logprobs* h, const apk_logprobs_grads* g);
+
 /* ---- allocation-free entry point --------------------------------------- */
 
 /* C = A * B (fp32, row-major, device pointers, 16-byte aligned; M and N
