@@ -11,11 +11,11 @@ from .runtime import (ApkError, Context, fill_normal_bf16, fill_uniform,  # noqa
                       pinned_empty, round_bf16)
 
 __all__ = ["Context", "ApkError", "fill_uniform", "fill_normal_bf16", "round_bf16", "pinned_empty",
-           "load", "LIB_PATH", "Linear", "MoE", "LayerNorm",
+           "load", "LIB_PATH", "Linear", "MoE", "Linear4", "LayerNorm",
            "GradClip", "LogProbs"]
 
-_LAYERS = {"Linear": "layers", "MoE": "layers", "LayerNorm": "layers", "GradClip": "training",
-           "LogProbs": "training"}
+_LAYERS = {"Linear": "layers", "Linear4": "layers", "MoE": "layers", "LayerNorm": "layers",
+           "GradClip": "training", "LogProbs": "training"}
 
 
 def __getattr__(name):

@@ -159,6 +159,12 @@ class LogprobsGrads(ctypes.Structure):
                 ("entropy", c_void_p), ("stats", c_void_p), ("dlogits", c_void_p), ("ld_d", c_ll), ("stream", c_void_p)]
 
 
+class Linear4Config(ctypes.Structure):
+    _fields_ = [("device", c_int), ("in_features", c_int), ("out_features", c_int), ("group", c_int), ("act", c_int),
+                ("scale_dtype", c_int), ("bias_dtype", c_int), ("W", c_void_p), ("ldw", c_ll), ("scales", c_void_p),
+                ("zeros", c_void_p), ("bias", c_void_p), ("sms", c_int), ("wait_limit_ns", c_ll)]
+
+
 P = c_void_p
 # name -> (restype, argtypes); every symbol include/apk.h declares
 SIGNATURES = {
@@ -224,6 +230,11 @@ SIGNATURES = {
     "apk_logprobs_last_error": (c_char_p, [P]),
     "apk_logprobs_forward": (c_int, [P, ctypes.POINTER(LogprobsIO)]),
     "apk_logprobs_backward": (c_int, [P, ctypes.POINTER(LogprobsGrads)]),
+    "apk_linear4_create": (c_int, [ctypes.POINTER(Linear4Config), ctypes.POINTER(P)]),
+    "apk_linear4_destroy": (c_int, [P]),
+    "apk_linear4_last_error": (c_char_p, [P]),
+    "apk_linear4_forward": (c_int, [P, ctypes.POINTER(LinearIO)]),
+    "apk_linear4_status": (c_int, [P, P, ctypes.POINTER(c_int)]),
     "apk_sgemm_f32_noalloc": (c_int, [P, P, P, c_int, c_int, c_int, c_int, P]),
     "apk_sgemm_f32_noalloc_status": (c_int, [P, ctypes.POINTER(c_int)]),
     "apk_sgemm_f32_noalloc_selftest": (c_int, [c_ll, P]),

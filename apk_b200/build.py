@@ -24,7 +24,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libapk.so")
 
 SOURCES = ["sgemm_f32.cu", "sgemm_f32_ws.cu", "gemm_bf16.cu", "gemm_bf16_pair.cu", "visibility.cu", "runtime.cu",
-           "linear_gemm.cu", "linear_stream.cu", "linear.cu", "moe.cu", "norm.cu", "clip.cu", "logprobs.cu",
+           "linear_gemm.cu", "linear_stream.cu", "linear.cu", "moe.cu", "norm.cu", "clip.cu", "logprobs.cu", "linear4.cu",
            "scratch.cu", "datagen.cpp"]
 HEADERS = ["common.cuh", "proto.h", "tcgen05.cuh", "act.cuh", "linear.h", "stream.cuh", "ops.h", "ops.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -1,7 +1,8 @@
 """Layer operators over torch tensors: Linear and LayerNorm (forward,
-backward) and MoE.
+backward), Linear4 and MoE.
 
-Thin classes over the C ABI's apk_linear_*, apk_norm_* and apk_moe_* (include/apk.h):
+Thin classes over the C ABI's apk_linear_*, apk_linear4_*, apk_norm_* and
+apk_moe_* (include/apk.h):
 they check shapes, types and strides, allocate outputs with torch, and run
 on torch's current stream of the weights' device.  torch is used for memory
 and streams only; the arithmetic is libapk's.  No counterpart in the
@@ -84,6 +85,19 @@ def _overlap(a, b, rows):
         return False
     off = (at2 - at) % pitch
     return pitch != pitch2 or off < length or off + length2 > pitch
+
+
+def _apart(io, y, residual, k, n):
+    """A linear layer's output tensor: apart from x, and the residual or apart from it."""
+    es = y.element_size()
+    to = (io.y, io.ldy * es, n * es)
+    if _overlap(to, (io.x, io.ldx * 2, k * 2), io.rows):
+        raise ValueError("out shares memory with x")
+    if residual is not None:
+        rs = residual.element_size()
+        of = (io.residual, io.ld_residual * rs, n * rs)
+        if of != to and _overlap(to, of, io.rows):
+            raise ValueError("out shares memory with residual, but is not it")
 
 
 def _like(t, shape):
@@ -204,15 +218,7 @@ class Linear(_Handle):
                 io.residual, _, io.ld_residual = _rows(residual, "residual", self.device, n, _ANY)
                 io.residual_dtype = _CODE[residual.dtype]
             if out is not None:
-                es = y.element_size()
-                to = (io.y, io.ldy * es, n * es)
-                if _overlap(to, (io.x, io.ldx * 2, self.in_features * 2), io.rows):
-                    raise ValueError("out shares memory with x")
-                if residual is not None:
-                    rs = residual.element_size()
-                    of = (io.residual, io.ld_residual * rs, n * rs)
-                    if of != to and _overlap(to, of, io.rows):
-                        raise ValueError("out shares memory with residual, but is not it")
+                _apart(io, y, residual, self.in_features, n)
             z = None
             if save_preact:
                 z = x.new_empty(shape)
@@ -267,6 +273,117 @@ class Linear(_Handle):
                 if st:
                     self._check(st)
             return dx, dw, db
+
+
+class Linear4(_Handle):
+    """y = act(x W^T + b) + r with weights of 4 bits and a scale for every
+    `group` of them along a row: W = scales (q - zeros).
+
+    weight: uint8 [out, in / 2], the even k's value in the low half of a byte;
+    in is a multiple of 32, rows start on 16 bytes.  scales: [out, groups],
+    fp32 or bf16; zeros: uint8 of that shape (0 to 15), None for 8 everywhere;
+    quantize() makes them.  bias, act and out_dtype as Linear has them; tensors
+    are kept by reference likewise.  There is no backward pass."""
+    _create, _destroy = "apk_linear4_create", "apk_linear4_destroy"
+    _error, _status = "apk_linear4_last_error", "apk_linear4_status"
+
+    def __init__(self, weight, scales, zeros=None, bias=None, group: int = 128, act: str = "none",
+                 out_dtype: str = "bf16", sms: int = 0, wait_limit_ns: int = _DEFAULT_WAIT_NS):
+        _tensor(weight, "weight", dtypes=(torch.uint8,), dim=2)
+        self.device, self._index = weight.device, weight.device.index
+        self.out_features, self.in_features = weight.shape[0], 2 * weight.shape[1]
+        self.group = int(group)
+        if self.group < 1:
+            raise ValueError(f"group is {group!r}: 32, 64 or a multiple of 128")
+        w, _, ldw = _rows(weight, "weight", self.device, weight.shape[1], (torch.uint8,))
+        shape = (self.out_features, -(-self.in_features // self.group))
+        for t, what, dtypes in ((scales, "scales", _ANY), (zeros, "zeros", (torch.uint8,))):
+            if what == "zeros" and t is None:
+                continue
+            _tensor(t, what, self.device, dtypes)
+            if t.shape != shape or not t.is_contiguous():
+                raise ValueError(f"{what} is {tuple(t.shape)} with strides {t.stride()}: contiguous {shape} is wanted")
+        if bias is not None:
+            _tensor(bias, "bias", self.device, _ANY, 1)
+            if bias.shape[0] != self.out_features or (bias.shape[0] > 1 and bias.stride(0) != 1):
+                raise ValueError(f"bias is {tuple(bias.shape)} with strides {bias.stride()}: "
+                                 f"{self.out_features} contiguous values are wanted")
+        self.weight, self.scales, self.zeros, self.bias, self.act = weight, scales, zeros, bias, act
+        self._at = self._addresses()
+        self.out_dtype = _pick(_TORCH, out_dtype, "out_dtype")
+        self._open(L.Linear4Config(self._index, self.in_features, self.out_features, self.group, _pick(_ACT, act, "act"),
+                                   _CODE[scales.dtype], _CODE[bias.dtype] if bias is not None else L.APK_F32, w, ldw,
+                                   *self._at[1:], sms, wait_limit_ns))
+        self._io = L.LinearIO()
+        self._io.y_dtype = _CODE[self.out_dtype]
+        self._io_ref = ctypes.byref(self._io)
+
+    def _addresses(self):
+        z, b = self.zeros, self.bias
+        return (self.weight.data_ptr(), self.scales.data_ptr(), None if z is None else z.data_ptr(),
+                None if b is None else b.data_ptr())
+
+    @staticmethod
+    def quantize(weight, group: int = 128, zeros: bool = False, scale_dtype: str = "bf16"):
+        """(weight, scales, zeros) in 4 bits for a floating [out, in] weight:
+        each group to the nearest of 15 steps around 0, or with zeros of 16
+        steps from its least value to its largest."""
+        n, k = weight.shape
+        dt = _pick(_TORCH, scale_dtype, "scale_dtype")
+        groups = -(-k // group)
+        w = weight.new_zeros((n, groups * group), dtype=torch.float32)
+        w[:, :k] = weight
+        w = w.view(n, groups, group)
+        if zeros:
+            low, high = w.amin(2).clamp(max=0), w.amax(2).clamp(min=0)
+            s = ((high - low) / 15).to(dt)
+            by = torch.where(s == 0, 1.0, s.float())
+            z = torch.round(-low / by).clamp(0, 15)
+        else:
+            s = (w.abs().amax(2) / 7).to(dt)
+            by = torch.where(s == 0, 1.0, s.float())
+            z = torch.full_like(by, 8.0)
+        q = torch.round(w / by[:, :, None] + z[:, :, None]).clamp(0, 15).to(torch.uint8).view(n, -1)[:, :k]
+        return q[:, 0::2] | (q[:, 1::2] << 4), s, z.to(torch.uint8) if zeros else None
+
+    def forward(self, x, residual=None, save_preact: bool = False, out=None):
+        """act(x W^T + b) + residual for x [..., in], as Linear.forward."""
+        with self._lock:
+            if self._addresses() != self._at:
+                raise ValueError(_MOVED)
+            io, n = self._io, self.out_features
+            io.x, io.rows, io.ldx = _rows(x, "x", self.device, self.in_features)
+            shape = (*x.shape[:-1], n)
+            if out is None:
+                y = x.new_empty(shape, dtype=self.out_dtype)
+                io.y, io.ldy = y.data_ptr(), n
+            else:
+                y = out
+                if y.shape != shape:
+                    raise ValueError(f"out is {tuple(y.shape)}, not {shape}")
+                io.y, _, io.ldy = _rows(y, "out", self.device, n, (self.out_dtype,))
+            if residual is None:
+                io.residual = None
+            else:
+                if residual.shape != shape:
+                    raise ValueError(f"residual is {tuple(residual.shape)}, not {shape}")
+                io.residual, _, io.ld_residual = _rows(residual, "residual", self.device, n, _ANY)
+                io.residual_dtype = _CODE[residual.dtype]
+            if out is not None:
+                _apart(io, y, residual, self.in_features, n)
+            z = None
+            if save_preact:
+                z = x.new_empty(shape)
+                io.preact, io.ld_preact = z.data_ptr(), n
+            else:
+                io.preact = None
+            io.stream = _raw_stream(self._index)
+            st = self._lib.apk_linear4_forward(self._h, self._io_ref)
+            if st:
+                self._check(st)
+            return (y, z) if save_preact else y
+
+    __call__ = forward
 
 
 class LayerNorm(_Handle):

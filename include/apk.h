@@ -640,8 +640,8 @@ apk_status apk_moe_status(apk_moe* h, void* stream, int* device_status);
 
 /* The same manner as above: device pointers, strides in elements, the last
  * axis contiguous, asynchronous on `stream`, handles that keep the caller's
- * weight pointers, scratch that a capture does not grow.  These kernels wait
- * for nothing, so there is no status to ask for.  A create that fails sets
+ * weight pointers, scratch that a capture does not grow.  Only the 4-bit
+ * layer's kernels wait, so that only it has a status to ask for.  A create that fails sets
  * *out all the same (unless memory ran out), as apk_linear_create does. */
 
 /* Layer norm over the last axis:  mean and variance of each row (the variance
@@ -787,6 +787,36 @@ typedef struct apk_logprobs_grads {
   void* stream;
 } apk_logprobs_grads;
 apk_status apk_logprobs_backward(apk_logprobs* h, const apk_logprobs_grads* g);
+
+/* A linear layer whose weights have 4 bits, for a few rows or many:
+ *   W[n][k] = scales[n][k / group] (q[n][k] - zeros[n][k / group]),
+ *   y = act(x W^T + bias) + residual, preact = x W^T + bias.
+ * A byte of W holds q of an even k in its low half and of k + 1 in its high
+ * half.  Up to 64 rows, sums and scales are fp32 throughout; more rows take
+ * products of weights that are rounded to bf16 (an fp32 y: to two bf16 terms,
+ * 2^-16 of themselves), written to scratch in every call. */
+typedef struct apk_linear4_config {
+  int device;
+  int in_features;          /* a multiple of 32, up to 2^30                   */
+  int out_features;         /* 1 to 2^30                                      */
+  int group;                /* 32, 64 or a multiple of 128 (the last group of a row may be shorter) */
+  apk_act act;
+  apk_dtype scale_dtype, bias_dtype;
+  const void* W;            /* [out_features][in_features / 2] bytes          */
+  long long ldw;            /* bytes; W and ldw are multiples of 16           */
+  const void* scales;       /* [out_features][groups], contiguous             */
+  const unsigned char* zeros; /* the same shape, the low four bits count; NULL: all 8 */
+  const void* bias;         /* out_features values, or NULL                   */
+  int sms;                  /* as in apk_linear_config                        */
+  long long wait_limit_ns;
+} apk_linear4_config;
+typedef struct apk_linear4 apk_linear4;
+
+apk_status apk_linear4_create(const apk_linear4_config* cfg, apk_linear4** out);
+apk_status apk_linear4_destroy(apk_linear4* h);
+const char* apk_linear4_last_error(const apk_linear4* h);
+apk_status apk_linear4_forward(apk_linear4* h, const apk_linear_io* io);  /* as apk_linear_forward */
+apk_status apk_linear4_status(apk_linear4* h, void* stream, int* device_status);  /* as apk_linear_status */
 
 /* ---- allocation-free entry point --------------------------------------- */
 
