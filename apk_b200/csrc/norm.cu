@@ -11,6 +11,7 @@
 // all sums over it are taken from there, in fp32 (the variance from the
 // differences, so that a mean far from zero costs no digits).
 #include <algorithm>
+#include <vector>
 
 #include "ops.cuh"
 #include "ops.h"
@@ -19,6 +20,13 @@ namespace apk {
 namespace norm {
 
 constexpr int MAX_FEATURES = 16384;  // 1024 threads of two pieces
+
+// Rows on their way, this one among them: 98 KB of shared memory (196 KB for
+// more than 512 threads, of which an SM takes one block) hold them.
+template <bool VEC, bool XF>
+constexpr int FWD_STAGES = !VEC ? 1 : XF ? 3 : 6;
+template <bool VEC, bool XF, bool DF, int T>
+constexpr int BWD_STAGES = !VEC ? 1 : 24 / ((XF ? 8 : 4) + (DF ? 4 : 2)) / (T > 512 ? 2 : 1);
 
 struct Params {
   const void* x;
@@ -31,7 +39,7 @@ struct Params {
   float* part;       // [blocks][dw, db][cols rounded up to 8]
   long long ldx, ld_dy, ld_r, ldy;
   int rows, cols;
-  float eps;
+  float eps, per_col;  // 1 / cols
   int w_f32, b_f32;
 };
 
@@ -90,7 +98,7 @@ __device__ __forceinline__ void load_weight(const void* p, int f32, float (&v)[8
 // alternates from call to call, so that one barrier a call is enough: who
 // writes a buffer again has passed the barrier behind its last reads.
 template <bool WARP>
-__device__ __forceinline__ float2 row_sum(float a, float b, float2 (*sh)[32], int buf, int T) {
+__device__ __forceinline__ float2 row_sums(float a, float b, float2 (*sh)[32], int buf, int T) {
   a = ops::warp_sum(a);
   b = ops::warp_sum(b);
   if constexpr (WARP) return make_float2(a, b);
@@ -100,18 +108,84 @@ __device__ __forceinline__ float2 row_sum(float a, float b, float2 (*sh)[32], in
   const float2 v = lane < T / 32 ? sh[buf][lane] : make_float2(0.f, 0.f);
   return make_float2(ops::warp_sum(v.x), ops::warp_sum(v.y));
 }
+template <bool WARP>
+__device__ __forceinline__ float row_sum(float a, float2 (*sh)[32], int buf, int T) {
+  a = ops::warp_sum(a);
+  if constexpr (WARP) return a;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) sh[buf][threadIdx.x >> 5].x = a;
+  __syncthreads();
+  return ops::warp_sum(lane < T / 32 ? sh[buf][lane].x : 0.f);
+}
+
+// A thread's own pieces of the rows ahead, on their way into shared memory:
+// stage, array and piece lie 16 bytes a thread apart, so that no other thread
+// reads them and no barrier is needed.  What registers could hold of the next
+// row alone left too little in flight (8192 x 4096 bf16 forward 56 us, backward
+// 68).  S stages; every row is one group of copies, an empty one behind the last.
+template <int V, bool F32, int S>
+struct Ahead {
+  uint8_t* at;  // this thread's place
+  int threads;
+  static constexpr int SLOTS = V * (F32 ? 2 : 1);
+  __device__ __forceinline__ void fetch(int stage, const void* p, long long row, int cols, int t, int T) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if ((j * T + t) * 8 < cols) {
+        const uint8_t* q = static_cast<const uint8_t*>(p) + (row + (j * T + t) * 8) * (F32 ? 4 : 2);
+#pragma unroll
+        for (int h = 0; h < (F32 ? 2 : 1); ++h)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(at + ((stage * V + j) * (F32 ? 2 : 1) + h) * threads * 16)),
+                       "l"(q + h * 16)
+                       : "memory");
+      }
+  }
+  __device__ __forceinline__ ops::Raw<F32> get(int stage, int j, int cols, int t, int T) const {
+    ops::Raw<F32> r = {};
+    if ((j * T + t) * 8 < cols) {
+      r.a = *reinterpret_cast<const uint4*>(at + (stage * V + j) * (F32 ? 2 : 1) * threads * 16);
+      if constexpr (F32) r.b = *reinterpret_cast<const uint4*>(at + ((stage * V + j) * 2 + 1) * threads * 16);
+    }
+    return r;
+  }
+};
+__device__ __forceinline__ void fetched() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int S>
+__device__ __forceinline__ void arrived() {  // the oldest of S groups
+  asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+}
 
 // WARP: a row is a warp's and a block of 8 takes 8; else a row is a block's.
-template <int V, bool VEC, bool WARP, bool XF, bool YF>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) forward(const __grid_constant__ Params p) {
+template <int V, bool VEC, bool WARP, bool XF, bool YF, int T_>
+__global__ void __launch_bounds__(T_, T_ <= 512 ? 1024 / T_ : 1) forward(const __grid_constant__ Params p) {
+  constexpr int S = FWD_STAGES<VEC, XF>;
+  extern __shared__ uint4 ring[];
   __shared__ float2 sh[2][32];
   const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
   const int per = WARP ? 8 : 1;
+  const Ahead<V, XF, S> ahead{reinterpret_cast<uint8_t*>(ring + threadIdx.x), (int)blockDim.x};
+  const long long step = (long long)gridDim.x * per;
+  long long r = (long long)blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0);
   pdl_launch();
   pdl_wait();
-  for (long long r = (long long)blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0); r < p.rows; r += (long long)gridDim.x * per) {
+  if constexpr (VEC)
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) {
+      if (r + i * step < p.rows) ahead.fetch(i, p.x, (r + i * step) * p.ldx, p.cols, t, T);
+      fetched();
+    }
+  for (int stage = 0; r < p.rows; r += step, stage = stage + 1 == S ? 0 : stage + 1) {
     ops::Raw<XF> raw[V];
-    load_row<VEC, XF, V>(p.x, r * p.ldx, raw, p.cols, t, T);
+    if constexpr (VEC) {
+      const long long next = r + (S - 1) * step;
+      if (next < p.rows) ahead.fetch(stage == 0 ? S - 1 : stage - 1, p.x, next * p.ldx, p.cols, t, T);
+      fetched();
+      arrived<S>();
+#pragma unroll
+      for (int j = 0; j < V; ++j) raw[j] = ahead.get(stage, j, p.cols, t, T);
+    } else {
+      load_row<VEC, XF, V>(p.x, r * p.ldx, raw, p.cols, t, T);
+    }
     float v[V][8], s = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -119,7 +193,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) forward(const __grid_consta
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += v[j][i];  // (zero behind the last column)
     }
-    const float mean = row_sum<WARP>(s, 0.f, sh, 0, T).x / p.cols;
+    const float mean = row_sum<WARP>(s, sh, 0, T) * p.per_col;
     s = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -129,7 +203,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) forward(const __grid_consta
         v[j][i] = d;
         s = fmaf(d, d, s);
       }
-    const float rstd = rsqrtf(row_sum<WARP>(s, 0.f, sh, 1, T).x / p.cols + p.eps);
+    const float rstd = rsqrtf(fmaf(row_sum<WARP>(s, sh, 1, T), p.per_col, p.eps));
     if (p.stats && t == 0) p.stats[r] = make_float2(mean, rstd);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -144,23 +218,52 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) forward(const __grid_consta
 }
 
 // A block takes every gridDim-th row (of eight, with WARP) and keeps its
-// columns' sums of dy n and dy in registers; they are written once, for reduce().
-template <int V, bool VEC, bool WARP, bool XF, bool DF>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) backward(const __grid_constant__ Params p) {
+// columns' sums of dy n and dy in registers; they are written once, for
+// reduce().  T_: the most threads of a block, of which an SM takes 512.
+template <int V, bool VEC, bool WARP, bool XF, bool DF, int T_>
+__global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const __grid_constant__ Params p) {
+  constexpr int S = BWD_STAGES<VEC, XF, DF, T_>;
+  extern __shared__ uint4 ring[];
   __shared__ float2 sh[2][32];
-  __shared__ float join[WARP ? 8 : 1][WARP ? 256 * V : 1];
   const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
   const int per = WARP ? 8 : 1;
+  const Ahead<V, XF, S> ax{reinterpret_cast<uint8_t*>(ring + threadIdx.x), (int)blockDim.x};
+  const Ahead<V, DF, S> ad{ax.at + S * ax.SLOTS * blockDim.x * 16, (int)blockDim.x};
+  const Ahead<V, XF, S> ar{ad.at + S * ad.SLOTS * blockDim.x * 16, (int)blockDim.x};
   float dw[V][8] = {}, db[V][8] = {};
+  const long long step = (long long)gridDim.x * per;
+  long long r = (long long)blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0);
   pdl_launch();
   pdl_wait();
+  auto fetch = [&](int stage, long long row) {
+    if (row < p.rows) {
+      ax.fetch(stage, p.x, row * p.ldx, p.cols, t, T);
+      ad.fetch(stage, p.dy, row * p.ld_dy, p.cols, t, T);
+      if (p.r) ar.fetch(stage, p.r, row * p.ld_r, p.cols, t, T);
+    }
+    fetched();
+  };
+  if constexpr (VEC)
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) fetch(i, r + i * step);
   int buf = 0;
-  for (long long r = (long long)blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0); r < p.rows; r += (long long)gridDim.x * per) {
+  float2 st = r < p.rows ? p.stats[r] : make_float2(0.f, 0.f);
+  for (int stage = 0; r < p.rows; r += step, stage = stage + 1 == S ? 0 : stage + 1) {
     ops::Raw<XF> rx[V];
     ops::Raw<DF> rd[V];
-    load_row<VEC, XF, V>(p.x, r * p.ldx, rx, p.cols, t, T);
-    load_row<VEC, DF, V>(p.dy, r * p.ld_dy, rd, p.cols, t, T);
-    const float2 st = p.stats[r];
+    if constexpr (VEC) {
+      fetch(stage == 0 ? S - 1 : stage - 1, r + (S - 1) * step);
+      arrived<S>();
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        rx[j] = ax.get(stage, j, p.cols, t, T);
+        rd[j] = ad.get(stage, j, p.cols, t, T);
+      }
+    } else {
+      load_row<VEC, XF, V>(p.x, r * p.ldx, rx, p.cols, t, T);
+      load_row<VEC, DF, V>(p.dy, r * p.ld_dy, rd, p.cols, t, T);
+    }
+    const float2 st_next = r + step < p.rows ? p.stats[r + step] : make_float2(0.f, 0.f);
     float n[V][8], g[V][8], s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -178,25 +281,32 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) backward(const __grid_const
         s2 = fmaf(g[j][i], n[j][i], s2);
       }
     }
-    if (!p.y) continue;
-    const float2 s = row_sum<WARP>(s1, s2, sh, buf, T);
-    buf ^= 1;
-    const float a = s.x / p.cols, b = s.y / p.cols;
-    ops::Raw<XF> rr[V];
-    if (p.r) load_row<VEC, XF, V>(p.r, r * p.ld_r, rr, p.cols, t, T);
+    if (p.y) {
+      const float2 s = row_sums<WARP>(s1, s2, sh, buf, T);
+      buf ^= 1;
+      const float a = s.x * p.per_col, b = s.y * p.per_col;
+      ops::Raw<XF> rr[V];
+      if (!VEC && p.r) load_row<VEC, XF, V>(p.r, r * p.ld_r, rr, p.cols, t, T);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float res[8] = {};
-      if (p.r) ops::unpack(rr[j], res);
+      for (int j = 0; j < V; ++j) {
+        float res[8] = {};
+        if (p.r) {
+          if constexpr (VEC) rr[j] = ar.get(stage, j, p.cols, t, T);
+          ops::unpack(rr[j], res);
+        }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[j][i] = fmaf(st.y, g[j][i] - a - n[j][i] * b, res[i]);
-      store_piece<VEC, XF>(p.y, r * p.ldy, g[j], j, p.cols, t, T);
+        for (int i = 0; i < 8; ++i) g[j][i] = fmaf(st.y, g[j][i] - a - n[j][i] * b, res[i]);
+        store_piece<VEC, XF>(p.y, r * p.ldy, g[j], j, p.cols, t, T);
+      }
     }
+    st = st_next;
   }
   if (!p.part) return;
   const int ldp = (p.cols + 7) / 8 * 8;
   float* part = p.part + (long long)blockIdx.x * 2 * ldp;
   if constexpr (WARP) {
+    float(*join)[256 * V] = reinterpret_cast<float(*)[256 * V]>(ring);  // (all rows have arrived)
+    __syncthreads();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -251,16 +361,60 @@ __global__ void __launch_bounds__(256) reduce(const __grid_constant__ Reduce p) 
   ops::st_any(out, c, s, blockIdx.y ? p.b_f32 : p.w_f32);
 }
 
-using Kernel = void (*)(Params);
-template <int V, bool VEC, bool WARP>
-Kernel fwd_of(bool xf, bool yf) {
-  return xf ? (yf ? &forward<V, VEC, WARP, true, true> : &forward<V, VEC, WARP, true, false>)
-            : (yf ? &forward<V, VEC, WARP, false, true> : &forward<V, VEC, WARP, false, false>);
+struct Kernel {
+  void (*fn)(Params);
+  int smem;  // of a thread
+  int threads;  // at most
+};
+template <int V, bool VEC, bool WARP, int T, bool XF, bool YF>
+Kernel fwd() {
+  return {&forward<V, VEC, WARP, XF, YF, T>, VEC ? FWD_STAGES<VEC, XF> * V * (XF ? 32 : 16) : 0, T};
 }
-template <int V, bool VEC, bool WARP>
-Kernel bwd_of(bool xf, bool df) {
-  return xf ? (df ? &backward<V, VEC, WARP, true, true> : &backward<V, VEC, WARP, true, false>)
-            : (df ? &backward<V, VEC, WARP, false, true> : &backward<V, VEC, WARP, false, false>);
+template <int V, bool VEC, bool WARP, int T, bool XF, bool DF>
+Kernel bwd() {
+  return {&backward<V, VEC, WARP, XF, DF, T>, WARP && !VEC ? 32 * V : VEC ? BWD_STAGES<VEC, XF, DF, T> * V * ((XF ? 64 : 32) + (DF ? 32 : 16)) : 0, T};
+}
+template <int V, bool WARP, int T>
+Kernel fwd_of(bool vec, bool xf, bool yf) {
+  return vec ? (xf ? (yf ? fwd<V, true, WARP, T, true, true>() : fwd<V, true, WARP, T, true, false>())
+                   : (yf ? fwd<V, true, WARP, T, false, true>() : fwd<V, true, WARP, T, false, false>()))
+             : (xf ? (yf ? fwd<V, false, WARP, T, true, true>() : fwd<V, false, WARP, T, true, false>())
+                   : (yf ? fwd<V, false, WARP, T, false, true>() : fwd<V, false, WARP, T, false, false>()));
+}
+template <int V, bool WARP, int T>
+Kernel bwd_of(bool vec, bool xf, bool df) {
+  return vec ? (xf ? (df ? bwd<V, true, WARP, T, true, true>() : bwd<V, true, WARP, T, true, false>())
+                   : (df ? bwd<V, true, WARP, T, false, true>() : bwd<V, true, WARP, T, false, false>()))
+             : (xf ? (df ? bwd<V, false, WARP, T, true, true>() : bwd<V, false, WARP, T, true, false>())
+                   : (df ? bwd<V, false, WARP, T, false, true>() : bwd<V, false, WARP, T, false, false>()));
+}
+
+// How rows are laid over threads: the kernel, threads of a block, rows of a block.
+struct Shape {
+  Kernel k;
+  int T, per;
+};
+Shape fwd_shape(int cols, bool vec, bool xf, bool yf) {
+  if (cols <= 256) return {fwd_of<1, true, 256>(vec, xf, yf), 256, 8};
+  if (cols <= 512) return {fwd_of<2, true, 256>(vec, xf, yf), 256, 8};
+  const int T = ops::ceil_div(ops::ceil_div(cols, 16), 32) * 32;
+  return {T <= 64    ? fwd_of<2, false, 64>(vec, xf, yf)
+          : T <= 128 ? fwd_of<2, false, 128>(vec, xf, yf)
+          : T <= 256 ? fwd_of<2, false, 256>(vec, xf, yf)
+          : T <= 512 ? fwd_of<2, false, 512>(vec, xf, yf)
+                     : fwd_of<2, false, 1024>(vec, xf, yf),
+          T, 1};
+}
+Shape bwd_shape(int cols, bool vec, bool xf, bool df) {
+  if (cols <= 256) return {bwd_of<1, true, 256>(vec, xf, df), 256, 8};
+  if (cols <= 512) return {bwd_of<2, true, 256>(vec, xf, df), 256, 8};
+  const int T = ops::ceil_div(ops::ceil_div(cols, 16), 32) * 32;
+  return {T <= 64    ? bwd_of<2, false, 64>(vec, xf, df)
+          : T <= 128 ? bwd_of<2, false, 128>(vec, xf, df)
+          : T <= 256 ? bwd_of<2, false, 256>(vec, xf, df)
+          : T <= 512 ? bwd_of<2, false, 512>(vec, xf, df)
+                     : bwd_of<2, false, 1024>(vec, xf, df),
+          T, 1};
 }
 
 }  // namespace norm
@@ -274,6 +428,7 @@ struct apk_norm {
   int sms = 0;
   Scratch scratch;
   std::mutex mu;
+  std::vector<const void*> ready;  // kernels that have been given their shared memory
 };
 
 namespace {
@@ -294,15 +449,16 @@ apk_status create(const apk_norm_config* cfg, apk_norm* h) {
   return h->scratch.open(c.device, &h->err);
 }
 
-// Threads of a row, and pieces of each.
-struct Shape {
-  int V, T;
-  bool warp;
-};
-
-apk_status launch(norm::Kernel k, const norm::Params& p, int grid, int threads, cudaStream_t s, const char* what, Err* err) {
-  Launch l(dim3(grid), threads, 0, s);
-  return cu_status(cudaLaunchKernelEx(&l.cfg, k, p), what, err);
+apk_status launch(apk_norm* h, const norm::Shape& sh, const norm::Params& p, int grid, cudaStream_t s, const char* what) {
+  const int smem = sh.k.smem * sh.T;
+  const void* fn = reinterpret_cast<const void*>(sh.k.fn);
+  // (a kernel's blocks differ in size: it is given what its largest need)
+  if (smem > 40 << 10 && std::find(h->ready.begin(), h->ready.end(), fn) == h->ready.end()) {
+    APK_TRY(cu_status(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, sh.k.smem * sh.k.threads), what, &h->err));
+    h->ready.push_back(fn);
+  }
+  Launch l(dim3(grid), sh.T, smem, s);
+  return cu_status(cudaLaunchKernelEx(&l.cfg, sh.k.fn, p), what, &h->err);
 }
 
 apk_status forward(apk_norm* h, const apk_norm_io* io) {
@@ -331,25 +487,13 @@ apk_status forward(apk_norm* h, const apk_norm_io* io) {
   p.rows = M;
   p.cols = D;
   p.eps = c.eps;
+  p.per_col = 1.f / D;
   const bool vec = D % 8 == 0 && ops::on16(io->x, io->ldx, M, io->x_dtype) && ops::on16(io->y, io->ldy, M, io->y_dtype) &&
                    ops::aligned(c.weight, 16) && ops::aligned(c.bias, 16);
   const bool xf = io->x_dtype == APK_F32, yf = io->y_dtype == APK_F32;
-  norm::Kernel k;
-  int T, per = 1;
-  if (D <= 1024) {  // a warp's row
-    T = 256;
-    per = 8;
-    k = D <= 256   ? (vec ? norm::fwd_of<1, true, true>(xf, yf) : norm::fwd_of<1, false, true>(xf, yf))
-        : D <= 512 ? (vec ? norm::fwd_of<2, true, true>(xf, yf) : norm::fwd_of<2, false, true>(xf, yf))
-                   : (vec ? norm::fwd_of<4, true, true>(xf, yf) : norm::fwd_of<4, false, true>(xf, yf));
-  } else {
-    const int V = D <= 4096 ? 1 : 2;
-    T = ops::ceil_div(ops::ceil_div(D, 8 * V), 32) * 32;
-    k = V == 1 ? (vec ? norm::fwd_of<1, true, false>(xf, yf) : norm::fwd_of<1, false, false>(xf, yf))
-               : (vec ? norm::fwd_of<2, true, false>(xf, yf) : norm::fwd_of<2, false, false>(xf, yf));
-  }
-  const int grid = std::min(ops::ceil_div(M, per), h->sms * (2048 / T));
-  return launch(k, p, grid, T, static_cast<cudaStream_t>(io->stream), "launching the layer norm", &h->err);
+  const norm::Shape sh = norm::fwd_shape(D, vec, xf, yf);
+  const int grid = std::min(ops::ceil_div(M, sh.per), h->sms * std::max(1, 1024 / sh.T));
+  return launch(h, sh, p, grid, static_cast<cudaStream_t>(io->stream), "launching the layer norm");
 }
 
 apk_status backward(apk_norm* h, const apk_norm_grads* g) {
@@ -390,24 +534,13 @@ apk_status backward(apk_norm* h, const apk_norm_grads* g) {
   p.ldy = g->ld_dx;
   p.rows = M;
   p.cols = D;
+  p.per_col = 1.f / D;
   const bool vec = D % 8 == 0 && ops::on16(g->x, g->ldx, M, g->x_dtype) && ops::on16(g->dy, g->ld_dy, M, g->dy_dtype) &&
                    (!g->dx || ops::on16(g->dx, g->ld_dx, M, g->x_dtype)) &&
                    (!g->residual_grad || ops::on16(g->residual_grad, g->ld_residual, M, g->x_dtype)) && ops::aligned(c.weight, 16);
   const bool xf = g->x_dtype == APK_F32, df = g->dy_dtype == APK_F32;
-  norm::Kernel k;
-  int T, per = 1;
-  if (D <= 512) {
-    T = 256;
-    per = 8;
-    k = D <= 256 ? (vec ? norm::bwd_of<1, true, true>(xf, df) : norm::bwd_of<1, false, true>(xf, df))
-                 : (vec ? norm::bwd_of<2, true, true>(xf, df) : norm::bwd_of<2, false, true>(xf, df));
-  } else {
-    const int V = D <= 2048 ? 1 : 2;
-    T = ops::ceil_div(ops::ceil_div(D, 8 * V), 32) * 32;
-    k = V == 1 ? (vec ? norm::bwd_of<1, true, false>(xf, df) : norm::bwd_of<1, false, false>(xf, df))
-               : (vec ? norm::bwd_of<2, true, false>(xf, df) : norm::bwd_of<2, false, false>(xf, df));
-  }
-  const int grid = std::min(ops::ceil_div(M, per), h->sms * std::max(1, 1024 / T));
+  const norm::Shape sh = norm::bwd_shape(D, vec, xf, df);
+  const int grid = std::min(ops::ceil_div(M, sh.per), h->sms * std::max(1, 512 / sh.T));
   const bool sums = g->dw || g->db;
   APK_TRY(h->scratch.enter(s, &h->err));
   ScratchUse use(&h->scratch, &h->err);
@@ -415,7 +548,7 @@ apk_status backward(apk_norm* h, const apk_norm_grads* g) {
     APK_TRY(use.begin(ops::up256((size_t)grid * 2 * ops::ceil_div(D, 8) * 8 * 4), 0));
     p.part = reinterpret_cast<float*>(h->scratch.data());
   }
-  APK_TRY(launch(k, p, grid, T, s, "launching the layer norm's gradient", &h->err));
+  APK_TRY(launch(h, sh, p, grid, s, "launching the layer norm's gradient"));
   if (sums) {
     const norm::Reduce q{p.part, g->dw, g->db, grid, D, c.weight_dtype == APK_F32, c.bias_dtype == APK_F32};
     Launch l(dim3(ops::ceil_div(D, 32), 2), 256, 0, s);
