@@ -8,16 +8,23 @@
 //   dx_j = dlogprob ([j = token] - p_j) - dentropy p_j (l_j + H)
 //
 // Bound by memory: the logits are read once, with a running maximum and sums
-// that are scaled where it grows.  x - m is taken before it is multiplied by
-// log2(e), so that large logits cost no digits.
+// that are scaled where it grows.  A value costs one multiply-add,
+//   t = x L - c,  c = m L rounded,  L = log2(e) rounded,
+// one 2^t and the two sums, of 2^t and of 2^t t, in pairs (f32x2).  What c's
+// and L's roundings move is taken back at the end, once a row in 64 bits: the
+// sums belong to the exact reference c / L in place of m.  Masked values (-inf)
+// are raised to -1e9, which leaves them 2^t = 0 without a 0 * inf; rows whose
+// maximum is not between -1e8 and 1e8 are taken again, step by step.
 //
 // The alternatives come out of the same pass.  The first round of 2048 values
-// gives a bound that its k-th largest value reaches; a value above the bound
-// is put into a buffer in shared memory; after 1, 2, 4, 8, ... rounds the
-// buffer is cut to its k largest, whose smallest is the new bound.  Between
-// two cuts about k values pass (the chance of the n-th value to be among the
-// k largest so far is k / n).  Rows in which far more pass, ascending ones,
-// fill the buffer up: their rounds are taken again one by one.
+// gives a bound that its k-th largest value reaches; a value that reaches the
+// bound is put into a buffer in shared memory.  As rounds go by, one warp at a
+// time raises the bound by what the buffer holds, while the others go on: any
+// bound that k values reach is right, so nobody waits for anybody.  Between n
+// and 2 n values about k pass (the n-th value is among the k largest so far
+// with chance k / n).  At the end the buffer is cut to its k largest.  Rows in
+// which far more pass, ascending ones, fill it up: they are taken again, cut
+// after every round.
 #include <algorithm>
 
 #include "act.cuh"
@@ -30,7 +37,12 @@ namespace logp {
 constexpr int THREADS = 256, ROUND = THREADS * 8;  // values of a block's round
 constexpr int MAX_TOP = 32, MAX_SPLIT = 64;
 constexpr int ROOM = ROUND + MAX_TOP;              // of the buffer: the list, and a whole round
-constexpr float NONE = -3.402823466e38f;           // the running maximum before the first value
+template <bool F32>
+constexpr int AHEAD = F32 ? 2 : 4;                 // eights of a thread on their way
+constexpr float LOWEST = -1e9f;                    // (as bf16: 0xCE6E)
+// The running maximum before the first value, and where it ends: there c is
+// rounded to steps of 16, and 2^t of the maximum itself stays below 2^8.
+constexpr float NONE = -1e8f, MOST = 1e8f;
 static_assert(MAX_SPLIT * MAX_TOP <= ROOM, "the splits' lists fit the buffer");
 
 struct Params {
@@ -42,7 +54,7 @@ struct Params {
   int* ids;
   float* tops;
   float2* stats;
-  float4* part;      // [row][split] m, S, sum e d
+  float4* part;      // [row][split] m, sum 2^t, sum 2^t t
   unsigned long long* lists;  // [row][split][top]
   unsigned* arrived; // [row], zero between launches
   int rows, vocabulary, top, split, tokens_64;
@@ -80,18 +92,26 @@ template <bool F32>
 struct Row {
   const uint8_t* base;
   int shift, n;
+  unsigned lo, whole;  // the eights that lie in the row whole: `whole` from `lo` on
   __device__ __forceinline__ Row(const uint8_t* p, int n_) : n(n_) {
     const int bytes = (int)(reinterpret_cast<uintptr_t>(p) & (F32 ? 31 : 15));
     base = p - bytes;
     shift = bytes / (F32 ? 4 : 2);
+    lo = shift ? 1 : 0;
+    const unsigned hi = (unsigned)(n + shift) / 8;
+    whole = hi > lo ? hi - lo : 0;
   }
-  __device__ __forceinline__ int eights() const { return (int)(((long long)n + shift + 7) / 8); }
-  __device__ __forceinline__ long long first(int v) const { return (long long)v * 8 - shift; }
+  __device__ __forceinline__ int eights() const { return (int)((unsigned)(n + shift + 7) / 8); }
+  __device__ __forceinline__ int first(int v) const { return v * 8 - shift; }
+  static __device__ __forceinline__ void none(ops::Raw<F32>& r) {
+    const uint32_t w = F32 ? 0xFF800000u : 0xFF80FF80u;
+    r.a = make_uint4(w, w, w, w);
+    if constexpr (F32) r.b = r.a;
+  }
   // -inf where the row does not reach
   __device__ __forceinline__ void load(int v, ops::Raw<F32>& r) const {
-    const long long e = first(v);
     const uint8_t* q = base + (long long)v * (F32 ? 32 : 16);
-    if (e >= 0 && e + 8 <= n) {
+    if ((unsigned)v - lo < whole) {
       if constexpr (F32)
         asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=r"(r.a.x), "=r"(r.a.y), "=r"(r.a.z), "=r"(r.a.w), "=r"(r.b.x), "=r"(r.b.y), "=r"(r.b.z), "=r"(r.b.w)
@@ -101,38 +121,124 @@ struct Row {
         r.a = __ldcs(reinterpret_cast<const uint4*>(q));
       return;
     }
-    const uint32_t none = F32 ? 0xFF800000u : 0xFF80FF80u;
-    r.a = make_uint4(none, none, none, none);
-    if constexpr (F32) r.b = r.a;
+    none(r);
+    const int e = first(v);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (e + i >= 0 && e + i < n) ops::set1(r, i, q, i);
   }
 };
 
+__device__ __forceinline__ unsigned long long pair2(float lo, float hi) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair2(unsigned long long v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float ex2(float t) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return e;
+}
+
+// Eight values raised to LOWEST, in pairs; the largest of them as they were (a
+// NaN stays, and is the largest).
+__device__ __forceinline__ float raised(const ops::Raw<false>& r, unsigned long long (&x)[4]) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+  uint32_t m, n;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t v;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(w[i]), "r"(0xCE6ECE6Eu));
+    x[i] = pair2(ops::bf_lo(v), ops::bf_hi(v));
+  }
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(w[0]), "r"(w[1]));
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(n) : "r"(w[2]), "r"(w[3]));
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(n));
+  return max_nan(ops::bf_lo(m), ops::bf_hi(m));
+}
+__device__ __forceinline__ float raised(const ops::Raw<true>& r, unsigned long long (&x)[4]) {
+  float v[8];
+  ops::unpack(r, v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = pair2(max_nan(v[2 * i], LOWEST), max_nan(v[2 * i + 1], LOWEST));
+  return max_nan(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])), max_nan(max_nan(v[4], v[5]), max_nan(v[6], v[7])));
+}
+
+// Sums of 2^t and 2^t t, t = x L - c, c = m L.
 struct Soft {
   float m = NONE, s = 0.f, u = 0.f;
-  // m grows to to: what was summed is scaled.  (What is more than e^1000
-  // smaller is gone, and -inf * 0 does not arise.)
+  // (never contracted into a multiply-add: what is added up goes by the rounded product)
+  static __device__ __forceinline__ float c_of(float m) { return __fmul_rn(m, LOG2E); }
   __device__ __forceinline__ void raise(float to) {
-    const float d = fmaxf(m - to, -1000.f), f = exp_of(d);
-    u = f * fmaf(s, d, u);
+    const float d = c_of(m) - c_of(to), f = ex2(d);
+    u = f * fmaf(s, fmaxf(d, -2000.f), u);  // (f is 0 there: no 0 * inf)
     s *= f;
     m = to;
   }
-  __device__ __forceinline__ void add(const float (&x)[8], float most) {
-    if (most > m) raise(most);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float d = max_nan(x[i] - m, -1000.f), e = exp_of(d);
-      s += e;
-      u = fmaf(e, d, u);
+};
+// A thread's sums, over two accumulators each.  The reference follows the
+// maximum in steps of more than STEP: with every new maximum in any lane, a
+// warp would scale in nearly every round.  (What the entropy's sum is rounded
+// by grows with the distance: 16 was as fast and cost a digit.)
+constexpr float STEP = 2.f;
+struct Sums {
+  float m = NONE, most = NONE;
+  unsigned long long s = 0, u = 0, minus_c;
+  __device__ __forceinline__ Sums() { minus_c = pair2(-Soft::c_of(NONE), -Soft::c_of(NONE)); }
+  __device__ __forceinline__ void add(const unsigned long long (&x)[4], float top) {
+    most = fmaxf(most, top);
+    if (top > m + STEP) {
+      Soft a = sums();
+      a.raise(top);
+      m = top;
+      s = pair2(a.s, 0.f);
+      u = pair2(a.u, 0.f);
+      minus_c = pair2(-Soft::c_of(m), -Soft::c_of(m));
     }
+    const unsigned long long l = pair2(LOG2E, LOG2E);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned long long t = fma2(x[i], l, minus_c);
+      float t0, t1;
+      unpair2(t, t0, t1);
+      const unsigned long long e = pair2(ex2(t0), ex2(t1));
+      s = add2(s, e);
+      u = fma2(e, t, u);
+    }
+  }
+  __device__ __forceinline__ Soft sums() const {
+    Soft a;
+    float x, y;
+    unpair2(s, x, y);
+    a.s = x + y;
+    unpair2(u, x, y);
+    a.u = x + y;
+    a.m = m;
+    return a;
+  }
+  __device__ __forceinline__ Soft soft() const {
+    Soft a = sums();
+    a.raise(most);
+    return a;
   }
 };
 
 struct Shared {
-  unsigned long long buf[ROOM];
+  unsigned long long buf[ROOM];  // 0: not written
+  unsigned long long limit;      // k values reach it
   unsigned long long group[32];
   unsigned long long list[MAX_TOP];
   float m[8], s[8], u[8];
@@ -140,7 +246,7 @@ struct Shared {
   bool last;
 };
 
-// Over the block: every thread gets the row's m, s and u.
+// Over the block: every thread gets the row's.
 __device__ __forceinline__ Soft join(Soft a, Shared& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float m = a.m;
@@ -168,6 +274,70 @@ __device__ __forceinline__ Soft join(Soft a, Shared& sh) {
   return a;
 }
 
+// A row's maximum, log of the sum of exp(x - m), and entropy.
+struct Result {
+  float m, log_s, entropy;
+};
+__device__ __forceinline__ Result result_of(const Soft& a) {
+  // sum 2^(x L - c): its reference is c / L
+  constexpr double per_l = 1.0 / (double)LOG2E;
+  const float log_s = logf(a.s);
+  return {a.m, (float)(log_s + ((double)Soft::c_of(a.m) * per_l - a.m)), log_s - a.u / a.s * (float)per_l};
+}
+// The same by the definition, for a row whose maximum is far out: x - m, and
+// exp of it, value by value.  All threads.
+template <bool F32>
+__device__ __noinline__ Result far_out(const uint8_t* x, int n, Shared& sh) {
+  float m = -INFINITY, s = 0.f, u = 0.f;
+  bool nan = false;
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const float v = ops::ld_any(x, i, F32);
+    nan |= v != v;
+    m = fmaxf(m, v);
+  }
+  auto over_all = [&](float v, auto f) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.m[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = sh.m[0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) v = f(v, sh.m[w]);
+    return v;
+  };
+  m = over_all(m, [](float a, float b) { return fmaxf(a, b); });
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const float d = max_nan(ops::ld_any(x, i, F32) - m, -1000.f), e = exp_of(d);
+    s += e;
+    u = fmaf(e, d, u);
+  }
+  s = over_all(nan ? NAN : s, [](float a, float b) { return a + b; });
+  u = over_all(u, [](float a, float b) { return a + b; });
+  const float log_s = logf(s);
+  return {m, log_s, log_s - u / s};
+}
+
+// The k-th largest of a warp's keys; 0 if fewer lanes have any.
+__device__ __forceinline__ unsigned long long kth_of(unsigned long long key, int k) {
+  const uint32_t low = (uint32_t)key;
+  uint32_t left = (uint32_t)(key >> 32), top;
+  while (true) {  // values from above, those that are equal at once
+    top = __reduce_max_sync(0xFFFFFFFFu, left);
+    if (top == 0) return 0;
+    const int n = __popc(__ballot_sync(0xFFFFFFFFu, left == top));
+    if (n >= k) break;
+    k -= n;
+    if (left == top) left = 0;
+  }
+  uint32_t tied = left == top ? low : 0, at;
+  while (true) {  // (~index: no two are equal)
+    at = __reduce_max_sync(0xFFFFFFFFu, tied);
+    if (--k == 0) break;
+    if (tied == at) tied = 0;
+  }
+  return (unsigned long long)top << 32 | at;
+}
 // The k-th largest of the bests of 32 groups of 8 threads: a bound that at
 // least k of what the threads hold reach (0 if fewer than k groups hold any).
 __device__ __forceinline__ unsigned long long bound_of(unsigned long long best, int k, Shared& sh) {
@@ -178,24 +348,59 @@ __device__ __forceinline__ unsigned long long bound_of(unsigned long long best, 
   }
   if ((threadIdx.x & 7) == 0) sh.group[threadIdx.x >> 3] = best;
   __syncthreads();
-  const unsigned long long mine = sh.group[threadIdx.x & 31];
-  int rank = 0;
-#pragma unroll 8
-  for (int i = 0; i < 32; ++i) {
-    const unsigned long long other = sh.group[i];
-    // (equal ones are 0s: any order)
-    rank += other > mine || (other == mine && i < (int)(threadIdx.x & 31));
-  }
-  const int at = __ffs(__ballot_sync(0xFFFFFFFFu, rank == k - 1)) - 1;
-  return __shfl_sync(0xFFFFFFFFu, mine, at);
+  return kth_of(sh.group[threadIdx.x & 31], k);
 }
 __device__ __forceinline__ void put(unsigned long long key, Shared& sh) {
   const int at = atomicAdd(&sh.count, 1);
   if (at < ROOM) sh.buf[at] = key;
 }
+// Those of eight values, the first of index e, that reach the bound `limit`,
+// whose value is `value`.  (One at a time: few do, and the loop that this
+// stands in has to stay short.)
+template <bool F32, class Put>
+__device__ __forceinline__ void put_from(const ops::Raw<F32>& raw, int e, int n, unsigned long long limit, float value, Put put) {
+  float x[8];
+  ops::unpack(raw, x);
+  unsigned which = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) which |= !(x[i] < value) ? 1u << i : 0u;  // (a NaN reaches it)
+#pragma unroll 1
+  for (; which; which &= which - 1) {
+    const int i = __ffs(which) - 1;
+    const float a = i & 4 ? x[4] : x[0], b = i & 4 ? x[5] : x[1], c = i & 4 ? x[6] : x[2], d = i & 4 ? x[7] : x[3];
+    const float v = i & 2 ? (i & 1 ? d : c) : i & 1 ? b : a;
+    const unsigned long long key = key_of(v, e + i);
+    if (key >= limit && e + i >= 0 && e + i < n) put(key);
+  }
+}
+template <bool F32>
+__device__ __forceinline__ unsigned long long best_of(const ops::Raw<F32>& raw, int e, int n) {
+  float x[8];
+  ops::unpack(raw, x);
+  unsigned long long best = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const unsigned long long key = e + i >= 0 && e + i < n ? key_of(x[i], e + i) : 0;
+    best = key > best ? key : best;
+  }
+  return best;
+}
+// One warp: the bound raised to the k-th largest of what its lanes see, each
+// the largest of every 32nd value in the buffer (fewer than k lanes with any: not).
+__device__ __forceinline__ void raise_limit(int k, Shared& sh) {
+  const int lane = threadIdx.x & 31;
+  const int c = min(*(volatile int*)&sh.count, ROOM);
+  unsigned long long best = 0;
+  for (int i = lane; i < c; i += 32) {
+    const unsigned long long key = *(volatile unsigned long long*)&sh.buf[i];
+    best = key > best ? key : best;
+  }
+  const unsigned long long bound = kth_of(best, k);
+  if (lane == 0 && bound) atomicMax(&sh.limit, bound);
+}
 // Cuts the buffer to its k largest, sorted; returns their smallest, or 0 if
 // there are fewer.  All threads; barriers before and behind.
-__device__ __forceinline__ unsigned long long cut(int k, Shared& sh) {
+__device__ __noinline__ unsigned long long cut(int k, Shared& sh) {
   __syncthreads();
   int c = min(sh.count, ROOM);
   if (c > 96) {  // first what the bound leaves
@@ -235,6 +440,143 @@ __device__ __forceinline__ long long token_of(const Params& p, long long row) {
   return p.tokens_64 ? static_cast<const long long*>(p.tokens)[row] : (long long)static_cast<const int*>(p.tokens)[row];
 }
 
+// One warp: a row's results.  Lane 0 has its token, lane i its i-th alternative.
+template <bool TOP>
+__device__ __forceinline__ void finish(const Params& p, long long row, long long token, float at_token, const Result& res,
+                                       unsigned long long key) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) {
+    if (p.logprob)
+      p.logprob[row] = token < 0 ? 0.f : token < p.vocabulary ? (at_token - res.m) - res.log_s : __int_as_float(0x7FC00000);
+    if (p.entropy) p.entropy[row] = res.entropy;
+    if (p.stats) p.stats[row] = make_float2(res.m, res.log_s);
+  }
+  if constexpr (TOP)
+    if (lane < p.top) {
+      p.ids[row * p.top + lane] = index_of(key);
+      p.tops[row * p.top + lane] = (value_of(key) - res.m) - res.log_s;
+    }
+}
+
+// Short rows, a warp each: all of a row is in registers.  No thread waits for
+// another warp; the alternatives' buffer is the warp's own, and where too many
+// values reach the bound (rows of equal values) the largest is taken k times.
+constexpr int SHORT = 2048, SHORT_ROOM = 192;
+template <bool F32, bool TOP, int EIGHTS>
+__global__ void __launch_bounds__(THREADS) short_rows(const __grid_constant__ Params p) {
+  __shared__ unsigned long long bufs[TOP ? 8 : 1][SHORT_ROOM], lists[TOP ? 8 : 1][MAX_TOP];
+  __shared__ int counts[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row = (long long)blockIdx.x * 8 + warp;
+  pdl_launch();
+  pdl_wait();
+  if (row >= p.rows) return;
+  const uint8_t* px = p.x + row * p.ld;
+  const Row<F32> r(px, p.vocabulary);
+  const int eights = r.eights();
+  ops::Raw<F32> raw[EIGHTS];
+#pragma unroll
+  for (int j = 0; j < EIGHTS; ++j) {
+    if (lane + 32 * j < eights) r.load(lane + 32 * j, raw[j]);
+    else Row<F32>::none(raw[j]);
+  }
+  long long token = -1;
+  float at_token = 0.f;
+  if (p.tokens && lane == 0) {
+    token = token_of(p, row);
+    if (token >= 0 && token < p.vocabulary) at_token = ops::ld_any(px, token, F32);
+  }
+  Sums sums;
+#pragma unroll
+  for (int j = 0; j < EIGHTS; ++j) {
+    unsigned long long x[4];
+    const float most = raised(raw[j], x);
+    sums.add(x, most);
+  }
+  Soft soft = sums.soft();
+  float m = soft.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  soft.raise(m);
+  soft.s = ops::warp_sum(soft.s);
+  soft.u = ops::warp_sum(soft.u);
+  Result res;
+  if (m > NONE && m < MOST) {
+    res = result_of(soft);
+  } else {  // by the definition
+    float top = -INFINITY, s = 0.f, u = 0.f;
+    bool nan = false;
+    for (int i = lane; i < p.vocabulary; i += 32) {
+      const float v = ops::ld_any(px, i, F32);
+      nan |= v != v;
+      top = fmaxf(top, v);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    for (int i = lane; i < p.vocabulary; i += 32) {
+      const float d = max_nan(ops::ld_any(px, i, F32) - top, -1000.f), e = exp_of(d);
+      s += e;
+      u = fmaf(e, d, u);
+    }
+    s = ops::warp_sum(nan ? NAN : s);
+    u = ops::warp_sum(u);
+    const float log_s = logf(s);
+    res = {top, log_s, log_s - u / s};
+  }
+  unsigned long long key = 0;
+  if constexpr (TOP) {
+    unsigned long long* buf = bufs[warp];
+    unsigned long long* list = lists[warp];
+    unsigned long long best = 0;
+#pragma unroll
+    for (int j = 0; j < EIGHTS; ++j) {
+      const unsigned long long b = best_of(raw[j], r.first(lane + 32 * j), p.vocabulary);
+      best = b > best ? b : best;
+    }
+    const unsigned long long bound = kth_of(best, p.top);
+    const float value = bound ? value_of(bound) : -INFINITY;
+    if (lane == 0) counts[warp] = 0;
+    __syncwarp();
+    if (best >= bound)
+#pragma unroll
+      for (int j = 0; j < EIGHTS; ++j)
+        put_from<F32>(raw[j], r.first(lane + 32 * j), p.vocabulary, bound, value, [&](unsigned long long k) {
+          const int to = atomicAdd(&counts[warp], 1);
+          if (to < SHORT_ROOM) buf[to] = k;
+        });
+    __syncwarp();
+    const int c = counts[warp];
+    if (c <= SHORT_ROOM) {
+      for (int i = lane; i < c; i += 32) {
+        const unsigned long long mine = buf[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < c; ++j) rank += buf[j] > mine;
+        if (rank < p.top) list[rank] = mine;
+      }
+      __syncwarp();
+      if (lane < p.top) key = list[lane];
+    } else {
+      unsigned long long last = ~0ull;
+      for (int k = 0; k < p.top; ++k) {
+        unsigned long long most = 0;
+        for (int i = lane; i < p.vocabulary; i += 32) {
+          const unsigned long long v = key_of(ops::ld_any(px, i, F32), i);
+          most = v < last && v > most ? v : most;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const unsigned long long other = __shfl_xor_sync(0xFFFFFFFFu, most, o);
+          most = other > most ? other : most;
+        }
+        last = most;
+        if (lane == k) key = most;
+      }
+    }
+  }
+  finish<TOP>(p, row, token, at_token, res, key);
+}
+
 // One row, or one of p.split parts of it, a block.
 template <bool F32, bool TOP>
 __global__ void __launch_bounds__(THREADS, 4) forward(const __grid_constant__ Params p) {
@@ -251,91 +593,86 @@ __global__ void __launch_bounds__(THREADS, 4) forward(const __grid_constant__ Pa
   const int rounds = max(0, v1 - v0 + THREADS - 1) / THREADS;
   long long token = -1;
   float at_token = 0.f;
-  if (p.tokens && tid == 0) {
+  if (p.tokens && tid == 0) {  // (its value is in flight beside the row's)
     token = token_of(p, row);
     if (token >= 0 && token < p.vocabulary) at_token = ops::ld_any(px, token, F32);
   }
-  if (TOP && tid == 0) sh.count = 0;
 
-  Soft soft;
-  float limit = 0.f;       // the k-th largest so far
-  uint32_t limit_order = 0;
+  Sums sums;
+  const int mine = v0 + tid;
   auto get = [&](int round, ops::Raw<F32>& raw) {
-    const int v = v0 + round * THREADS + tid;
-    if (round < rounds && v < v1) {
-      r.load(v, raw);
-    } else {
-      const uint32_t none = F32 ? 0xFF800000u : 0xFF80FF80u;
-      raw.a = make_uint4(none, none, none, none);
-      if constexpr (F32) raw.b = raw.a;
-    }
+    const int v = mine + round * THREADS;
+    if (v < v1) r.load(v, raw);
+    else Row<F32>::none(raw);
   };
-  auto above = [&](int round, const float (&x)[8], float most) {
-    if (!(most <= limit)) {  // (a NaN is above)
-      const int e = (int)r.first(v0 + round * THREADS + tid);
+  constexpr int N = AHEAD<F32>;
+  ops::Raw<F32> ring[N];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (order_of(x[i]) > limit_order && e + i >= 0 && e + i < p.vocabulary) put(key_of(x[i], e + i), sh);
-    }
-  };
-  auto cut_now = [&]() {
-    const unsigned long long key = cut(p.top, sh);
-    limit_order = (uint32_t)(key >> 32);
+  for (int i = 0; i < N; ++i) get(i, ring[i]);
+  unsigned long long bound = 0;  // everything reaches it
+  float limit = -INFINITY;       // its value and index
+  int limit_at = 0x7FFFFFFF;
+  auto follow = [&](unsigned long long key) {
+    if (!key) return;
+    bound = key;
     limit = value_of(key);
+    limit_at = index_of(key);
   };
-  ops::Raw<F32> now, next;
-  get(0, now);
-  get(1, next);
-  int from = 1, until = 2;  // rounds between two cuts
-  for (int round = 0; round < rounds; ++round) {
-    float x[8];
-    ops::unpack(now, x);
-    now = next;
-    get(round + 2, next);
-    const float most = max_nan(max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3])), max_nan(max_nan(x[4], x[5]), max_nan(x[6], x[7])));
-    soft.add(x, most);
+  auto put_here = [&](unsigned long long key) { put(key, sh); };
+  if constexpr (TOP) {
+    for (int i = tid; i < ROOM; i += THREADS) sh.buf[i] = 0;
+    if (tid == 0) {
+      sh.count = 0;
+      sh.limit = 0;
+    }
+    // the first round's own bound (a barrier is in it, behind the clearing)
+    const unsigned long long best = mine < v1 ? best_of(ring[0], r.first(mine), p.vocabulary) : 0;
+    follow(bound_of(best, p.top, sh));
+    if (tid == 0) atomicMax(&sh.limit, bound);
+  }
+  int until = N;  // the round at which a warp raises the bound
+  for (int round0 = 0; round0 < rounds; round0 += N) {
     if constexpr (TOP) {
-      if (round == 0) {
-        const long long e = r.first(v0 + tid);
-        const bool mine = v0 + tid < v1;
-        unsigned long long key[8], best = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          key[i] = mine && e + i >= 0 && e + i < p.vocabulary ? key_of(x[i], (int)e + i) : 0;
-          best = key[i] > best ? key[i] : best;
-        }
-        const unsigned long long bound = bound_of(best, p.top, sh);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (key[i] && key[i] >= bound) put(key[i], sh);
-        cut_now();
-      } else {
-        above(round, x, most);
-        if (round + 1 == until || round + 1 == rounds) {
-          __syncthreads();
-          if (sh.count > ROOM) {  // too many: the rounds since the last cut again, one by one
-            __syncthreads();
-            if (tid == 0) sh.count = p.top;
-            __syncthreads();
-            for (int again = from; again <= round; ++again) {
-              ops::Raw<F32> raw;
-              get(again, raw);
-              ops::unpack(raw, x);
-              float top = x[0];
-#pragma unroll
-              for (int i = 1; i < 8; ++i) top = max_nan(top, x[i]);
-              above(again, x, top);
-              cut_now();
-            }
-          } else {
-            cut_now();
-          }
-          from = until;
-          until *= 2;
-        }
+      if (round0 == until) {
+        if (tid >> 5 == (__ffs(until) & 7)) raise_limit(p.top, sh);
+        until *= 2;
       }
+      if (round0) follow(*(volatile unsigned long long*)&sh.limit);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int round = round0 + i;
+      if (round >= rounds) break;
+      unsigned long long x[4];
+      const float most = raised(ring[i], x);
+      if constexpr (TOP) {  // (equal values up to the bound's index; a NaN)
+        const int v = mine + round * THREADS, e = r.first(v);
+        if (__builtin_expect(!(most < limit) && (most != limit || e <= limit_at) && v < v1, 0))
+          put_from<F32>(ring[i], e, p.vocabulary, bound, limit, put_here);
+      }
+      get(round + N, ring[i]);
+      sums.add(x, most);
     }
   }
+  if constexpr (TOP) {
+    __syncthreads();
+    if (sh.count > ROOM) {  // too many: round by round
+      __syncthreads();
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+      bound = 0;
+      for (int round = 0; round < rounds; ++round) {
+        ops::Raw<F32> raw;
+        get(round, raw);
+        if (mine + round * THREADS < v1)
+          put_from<F32>(raw, r.first(mine + round * THREADS), p.vocabulary, bound, bound ? value_of(bound) : -INFINITY, put_here);
+        bound = cut(p.top, sh);
+      }
+    } else {
+      cut(p.top, sh);
+    }
+  }
+  Soft soft = sums.soft();
   soft = join(soft, sh);
   if (p.split > 1) {
     const long long at = row * p.split + part;
@@ -369,18 +706,12 @@ __global__ void __launch_bounds__(THREADS, 4) forward(const __grid_constant__ Pa
       cut(p.top, sh);
     }
   }
-  const float log_s = logf(soft.s);
-  if (tid == 0) {
-    if (p.logprob)
-      p.logprob[row] = token < 0 ? 0.f : token < p.vocabulary ? (at_token - soft.m) - log_s : __int_as_float(0x7FC00000);
-    if (p.entropy) p.entropy[row] = log_s - soft.u / soft.s;
-    if (p.stats) p.stats[row] = make_float2(soft.m, log_s);
-  }
-  if constexpr (TOP)
-    if (tid < p.top) {
-      p.ids[row * p.top + tid] = index_of(sh.list[tid]);
-      p.tops[row * p.top + tid] = (value_of(sh.list[tid]) - soft.m) - log_s;
-    }
+  const bool usual = soft.m > NONE && soft.m < MOST;
+  Result res = {};
+  if (!usual) res = far_out<F32>(px, p.vocabulary, sh);
+  if (tid >= 32) return;
+  if (usual) res = result_of(soft);
+  finish<TOP>(p, row, token, at_token, res, TOP && tid < p.top ? sh.list[tid] : 0);
 }
 
 struct Grads {
@@ -429,7 +760,7 @@ __global__ void __launch_bounds__(THREADS, 4) backward(const __grid_constant__ G
     for (int j = 0; j < EIGHTS; ++j) {
       const int v = v0 + j * THREADS;
       if (v >= nv) continue;
-      const long long e = r.first(v);
+      const int e = r.first(v);
       float x[8];
       ops::unpack(raw[j], x);
 #pragma unroll
@@ -437,7 +768,7 @@ __global__ void __launch_bounds__(THREADS, 4) backward(const __grid_constant__ G
       if (e >= 0 && e + 8 <= r.n) {
         ops::Raw<F32> o;
         ops::pack(x, o);
-        uint4* q = reinterpret_cast<uint4*>(out + e * (F32 ? 4 : 2));
+        uint4* q = reinterpret_cast<uint4*>(out + (long long)e * (F32 ? 4 : 2));
         __stcs(q, o.a);
         if constexpr (F32) __stcs(q + 1, o.b);
       } else {
@@ -487,6 +818,11 @@ apk_status check_logits(const void* x, long long ld, int rows, int vocabulary, i
   return APK_OK;
 }
 
+template <bool F32, bool TOP>
+auto short_of(int vocabulary) {
+  return vocabulary <= 249 ? logp::short_rows<F32, TOP, 1> : vocabulary <= 1017 ? logp::short_rows<F32, TOP, 4> : logp::short_rows<F32, TOP, 8>;
+}
+
 apk_status forward(apk_logprobs* h, const apk_logprobs_io* io) {
   const int V = io->vocabulary, M = io->rows, k = h->cfg.top;
   const cudaStream_t s = static_cast<cudaStream_t>(io->stream);
@@ -525,6 +861,12 @@ apk_status forward(apk_logprobs* h, const apk_logprobs_io* io) {
     p.lists = reinterpret_cast<unsigned long long*>(h->scratch.data() + zeroed + ops::up256(parts * 16));
   }
   const bool f = io->dtype == APK_F32;
+  if (V <= logp::SHORT - 7) {  // (and up to 7 places before the row)
+    const auto rows = k ? (f ? short_of<true, true>(V) : short_of<false, true>(V))
+                        : (f ? short_of<true, false>(V) : short_of<false, false>(V));
+    Launch l(dim3(ops::ceil_div(M, 8)), logp::THREADS, 0, s);
+    return cu_status(cudaLaunchKernelEx(&l.cfg, rows, p), "launching the log probabilities", &h->err);
+  }
   const auto kernel = k ? (f ? logp::forward<true, true> : logp::forward<false, true>)
                         : (f ? logp::forward<true, false> : logp::forward<false, false>);
   Launch l(dim3(M * p.split), logp::THREADS, 0, s);
