@@ -108,19 +108,24 @@ struct Row {
     r.a = make_uint4(w, w, w, w);
     if constexpr (F32) r.b = r.a;
   }
+  // one that lies in the row whole
+  __device__ __forceinline__ void load_whole(int v, ops::Raw<F32>& r) const {
+    const uint8_t* q = base + (long long)v * (F32 ? 32 : 16);
+    if constexpr (F32)
+      asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(r.a.x), "=r"(r.a.y), "=r"(r.a.z), "=r"(r.a.w), "=r"(r.b.x), "=r"(r.b.y), "=r"(r.b.z), "=r"(r.b.w)
+                   : "l"(q)
+                   : "memory");
+    else
+      r.a = __ldcs(reinterpret_cast<const uint4*>(q));
+  }
   // -inf where the row does not reach
   __device__ __forceinline__ void load(int v, ops::Raw<F32>& r) const {
-    const uint8_t* q = base + (long long)v * (F32 ? 32 : 16);
     if ((unsigned)v - lo < whole) {
-      if constexpr (F32)
-        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(r.a.x), "=r"(r.a.y), "=r"(r.a.z), "=r"(r.a.w), "=r"(r.b.x), "=r"(r.b.y), "=r"(r.b.z), "=r"(r.b.w)
-                     : "l"(q)
-                     : "memory");
-      else
-        r.a = __ldcs(reinterpret_cast<const uint4*>(q));
+      load_whole(v, r);
       return;
     }
+    const uint8_t* q = base + (long long)v * (F32 ? 32 : 16);
     none(r);
     const int e = first(v);
 #pragma unroll
@@ -436,6 +441,35 @@ __device__ __noinline__ unsigned long long cut(int k, Shared& sh) {
   return c >= k ? sh.list[k - 1] : 0;
 }
 
+// The same by one warp, for the end of a row: lane i gets the i-th largest.
+// (The block's way costs four barriers with all warps behind them.)
+__device__ __forceinline__ unsigned long long cut_by_warp(int k, Shared& sh) {
+  const int lane = threadIdx.x & 31, c = sh.count;
+  unsigned long long best = 0;
+  for (int i = lane; i < c; i += 32) best = sh.buf[i] > best ? sh.buf[i] : best;
+  const unsigned long long bound = kth_of(best, k);
+  int n = 0;
+  for (int i = 0; i < c; i += 32) {
+    const unsigned long long key = i + lane < c ? sh.buf[i + lane] : 0;
+    const bool in = key && key >= bound;
+    const unsigned all = __ballot_sync(0xFFFFFFFFu, in);
+    const int at = n + __popc(all & ((1u << lane) - 1));
+    __syncwarp();  // (survivors go over what has been read)
+    if (in) sh.buf[at] = key;
+    n += __popc(all);
+  }
+  __syncwarp();
+  for (int i = lane; i < n; i += 32) {
+    const unsigned long long mine = sh.buf[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) rank += sh.buf[j] > mine;
+    if (rank < k) sh.list[rank] = mine;
+  }
+  __syncwarp();
+  return lane < k ? sh.list[lane] : 0;
+}
+
 __device__ __forceinline__ long long token_of(const Params& p, long long row) {
   return p.tokens_64 ? static_cast<const long long*>(p.tokens)[row] : (long long)static_cast<const int*>(p.tokens)[row];
 }
@@ -600,9 +634,12 @@ __global__ void __launch_bounds__(THREADS, 4) forward(const __grid_constant__ Pa
 
   Sums sums;
   const int mine = v0 + tid;
+  // rounds of whole eights, but for the first, which may hold the row's first
+  const int inner = (min(v1, (int)(r.lo + r.whole)) - v0) / THREADS;
   auto get = [&](int round, ops::Raw<F32>& raw) {
     const int v = mine + round * THREADS;
-    if (v < v1) r.load(v, raw);
+    if (round > 0 && round < inner) r.load_whole(v, raw);
+    else if (v < v1) r.load(v, raw);
     else Row<F32>::none(raw);
   };
   constexpr int N = AHEAD<F32>;
@@ -646,9 +683,10 @@ __global__ void __launch_bounds__(THREADS, 4) forward(const __grid_constant__ Pa
       unsigned long long x[4];
       const float most = raised(ring[i], x);
       if constexpr (TOP) {  // (equal values up to the bound's index; a NaN)
-        const int v = mine + round * THREADS, e = r.first(v);
-        if (__builtin_expect(!(most < limit) && (most != limit || e <= limit_at) && v < v1, 0))
-          put_from<F32>(ring[i], e, p.vocabulary, bound, limit, put_here);
+        if (__builtin_expect(!(most < limit), 0)) {
+          const int v = mine + round * THREADS, e = r.first(v);
+          if ((most != limit || e <= limit_at) && v < v1) put_from<F32>(ring[i], e, p.vocabulary, bound, limit, put_here);
+        }
       }
       get(round + N, ring[i]);
       sums.add(x, most);
@@ -668,11 +706,51 @@ __global__ void __launch_bounds__(THREADS, 4) forward(const __grid_constant__ Pa
           put_from<F32>(raw, r.first(mine + round * THREADS), p.vocabulary, bound, bound ? value_of(bound) : -INFINITY, put_here);
         bound = cut(p.top, sh);
       }
-    } else {
+      __syncthreads();
+    } else if (p.split > 1) {
       cut(p.top, sh);
     }
   }
   Soft soft = sums.soft();
+  if (p.split == 1) {  // the rest is one warp's
+    float m = soft.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    soft.raise(m);
+    soft.s = ops::warp_sum(soft.s);
+    soft.u = ops::warp_sum(soft.u);
+    if ((tid & 31) == 0) {
+      sh.m[tid >> 5] = soft.m;
+      sh.s[tid >> 5] = soft.s;
+      sh.u[tid >> 5] = soft.u;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, sh.m[w]);
+    const bool usual = m > NONE && m < MOST;
+    Result res = {};
+    if (!usual) {
+      __syncthreads();  // (it uses sh.m)
+      res = far_out<F32>(px, p.vocabulary, sh);
+    }
+    if (tid >= 32) return;
+    if (usual) {
+      Soft all;
+      if (tid < 8) {
+        all.m = sh.m[tid];
+        all.s = sh.s[tid];
+        all.u = sh.u[tid];
+      }
+      all.raise(m);
+      all.s = ops::warp_sum(all.s);
+      all.u = ops::warp_sum(all.u);
+      res = result_of(all);
+    }
+    unsigned long long key = 0;
+    if constexpr (TOP) key = cut_by_warp(p.top, sh);
+    finish<TOP>(p, row, token, at_token, res, key);
+    return;
+  }
   soft = join(soft, sh);
   if (p.split > 1) {
     const long long at = row * p.split + part;
