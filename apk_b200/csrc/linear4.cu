@@ -33,19 +33,41 @@ struct Params {
   const void* s;
   const uint8_t* z;
   long long ldx, ldw;
-  int rows, n, k, group, groups, split, s_f32;
+  int rows, n, k, group, groups, s_f32;
+  int group_shift;  // log2 of the chunks of a group, or -1
+  int split;  // CTAs of a cluster that share K
+  int kw;     // warps that share a tile's K; 16 / kw tiles are worked on at once
+  int tiles;  // of 16 features
+  int slice;  // chunks of x in shared memory at once
   lin::Epilogue epi;
 };
 
-constexpr int WARPS = 8, FT = 16, CHUNK = 128;
+constexpr int WARPS = 16, FT = 16, CHUNK = 128;
+constexpr int PART_LD = 20;  // a token's 16 sums, apart by 20: no two of a warp's stores meet in a bank
+constexpr int SMEM = 226 << 10;
+constexpr int part_bytes(int tokens) { return WARPS * tokens * PART_LD * 4; }
 
+// Weights are read once.  A warp's load takes 64 bytes of eight rows; past L1
+// the two halves of a line are fetched each for itself, which costs where they
+// come out of L2 and pays where they come out of memory (1 x 4096 x 8192 out of
+// L2 9.3 us past L1 and 7.9 through it, out of memory 9.6 and 9.8; 64 rows 32.3
+// and 30.9, 32.7 and 37.7).  So: through L1 for up to 8 rows.  (KEEP)
+template <bool KEEP, class T>
+__device__ __forceinline__ T ld_w(const uint8_t* q, bool in) {
+  T v{};
+  if (!in) return v;
+  if constexpr (KEEP || sizeof(T) == 4) return *reinterpret_cast<const T*>(q);
+  else if constexpr (sizeof(T) == 16) return stream::ld_late(q);
+  else return stream::ld_late8(q);
+}
 // Eight weights less their zero point: h[i] is the pair (i, i + 4).
-__device__ __forceinline__ void dequant(uint32_t w, uint32_t zero, uint32_t (&h)[4]) {
+__device__ __forceinline__ void dequant(uint32_t w, uint32_t minus_zero, uint32_t (&h)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t v;
     asm("lop3.b32 %0, %1, 0x000F000F, 0x43004300, 0xEA;" : "=r"(v) : "r"(w >> (4 * i)));
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(h[i]) : "r"(v), "r"(zero));
+    // (v - (128 + z), as the multiply-add by one that there is an instruction for)
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(h[i]) : "r"(v), "r"(0x3F803F80u), "r"(minus_zero));
   }
 }
 // Eight values of x in the same order.
@@ -55,137 +77,210 @@ __device__ __forceinline__ void pairs(const uint4& v, uint32_t (&h)[4]) {
   h[2] = __byte_perm(v.y, v.w, 0x5410);
   h[3] = __byte_perm(v.y, v.w, 0x7632);
 }
-// 128 + z twice
-__device__ __forceinline__ uint32_t zero_pair(uint32_t z) { return 0x43004300u | (z & 15u) * 0x00010001u; }
-
 // P: groups that a chunk of 128 k has (1 for groups of 128 and more).  A
 // warp's lane (g, t) holds weights of the features g and g + 8; a group's
 // 32 / P k-values of a lane lie together.
+//
+// One CTA of 16 warps an SM (two of 8 were slower).  It lays x out in shared memory as the B fragments that its
+// warps will want, already in the nibbles' order, once for all features that
+// it takes: read from global memory, x cost more of L1 than the weights did
+// (32 rows of 4096 x 8192: 37 us).  Warps share tiles of 16 features by K;
+// a warp has AHEAD chunks of weights, 32 bytes a lane, on their way, its
+// neighbours the chunks between.
+template <int NT8>
+constexpr int AHEAD = NT8 <= 4 ? 4 : 2;
+struct Chunk {
+  uint32_t w[2][4];
+  float s[2];
+  uint32_t z;  // -(128 + zero point), of feature g in the low half
+};
 template <int NT8, int P, bool ZEROS, bool VEC>
-__global__ void __launch_bounds__(32 * WARPS, 2) stream4(const __grid_constant__ Params p) {
-  constexpr int TOK = 8 * NT8, WORDS = 4 / P;  // 32-bit words of a lane and group
-  __shared__ float part[WARPS][TOK][FT];
+__global__ void __launch_bounds__(32 * WARPS, 1) stream4(const __grid_constant__ Params p) {
+  constexpr int TOK = 8 * NT8, WORDS = 4 / P, A = AHEAD<NT8>;  // WORDS: 32-bit words of a lane and group
+  extern __shared__ uint4 xs[];  // [chunk][word][tile of tokens][lane], one tile: [chunk][word][row][t]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int rank = (int)blockIdx.x % p.split;
-  const int f0 = (int)blockIdx.x / p.split * FT, r0 = blockIdx.y * TOK;
-  const int rows = p.rows - r0;
+  const int kept = NT8 == 1 ? p.rows : TOK;  // rows in shared memory
+  float* part = reinterpret_cast<float*>(xs + p.slice * 4 * kept * 4);  // [warp][token][PART_LD]
+  const int kw = warp % p.kw, tw = warp / p.kw, at_once = WARPS / p.kw;
+  const int chunks = (p.k + CHUNK - 1) / CHUNK, per = (chunks + p.split - 1) / p.split;
+  const int c_begin = rank * per, c_end = min(c_begin + per, chunks);
+  const int sets = (p.tiles + at_once - 1) / at_once, set_step = (int)gridDim.x / p.split;
   pdl_launch();
   pdl_wait();
-  const uint16_t* xr[NT8];
+  // A lane's weights of a tile: k = chunk * 128 + h * 128 / P + t * 32 / P and
+  // what follows; and the index of the scale it loads, the chunk's t-th
+  // group's (with fewer groups: one of them), without the chunk's part.
+  const uint8_t* w_of[2];
+  long long s_of[2];
+  auto go_to = [&](int tile) {
 #pragma unroll
-  for (int i = 0; i < NT8; ++i) xr[i] = p.x + (r0 + min(8 * i + g, rows - 1)) * p.ldx;
-  const int f[2] = {min(f0 + g, p.n - 1), min(f0 + g + 8, p.n - 1)};
-  float total[NT8][4] = {};
-#pragma unroll 1
-  for (int k0 = (rank * WARPS + warp) * CHUNK; k0 < p.k; k0 += p.split * WARPS * CHUNK) {
-    uint32_t w[2][4];
-    uint4 c[NT8][4];
-    float s[2];
-    uint32_t z[2] = {8, 8};
+    for (int m = 0; m < 2; ++m) {
+      const int f = min(tile * FT + g + 8 * m, p.n - 1);
+      w_of[m] = p.w + f * p.ldw + t * (16 / P);
+      s_of[m] = (long long)f * p.groups + (t & (P - 1));
+    }
+  };
+  auto load = [&](Chunk& c, int chunk) {
+    const bool whole = (chunk + 1) * CHUNK <= p.k;  // (K ends inside the last chunk, perhaps)
 #pragma unroll
     for (int h = 0; h < P; ++h) {
-      const int k = k0 + h * (CHUNK / P) + t * (32 / P);
-      const bool in = k < p.k;
+      const bool in = whole || chunk * CHUNK + h * (CHUNK / P) + t * (32 / P) < p.k;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        const uint8_t* q = p.w + f[m] * p.ldw + k / 2;
+        const uint8_t* q = w_of[m] + (long long)chunk * (CHUNK / 2) + h * (CHUNK / 2 / P);
         if constexpr (P == 1) {
-          const uint4 v = in ? stream::ld_late(q) : make_uint4(0, 0, 0, 0);
-          w[m][0] = v.x, w[m][1] = v.y, w[m][2] = v.z, w[m][3] = v.w;
+          const uint4 v = ld_w<NT8 == 1, uint4>(q, in);
+          c.w[m][0] = v.x, c.w[m][1] = v.y, c.w[m][2] = v.z, c.w[m][3] = v.w;
         } else if constexpr (P == 2) {
-          const uint2 v = in ? stream::ld_late8(q) : make_uint2(0, 0);
-          w[m][2 * h] = v.x, w[m][2 * h + 1] = v.y;
+          const uint2 v = ld_w<NT8 == 1, uint2>(q, in);
+          c.w[m][2 * h] = v.x, c.w[m][2 * h + 1] = v.y;
         } else {
-          w[m][h] = in ? *reinterpret_cast<const uint32_t*>(q) : 0u;
+          c.w[m][h] = ld_w<NT8 == 1, uint32_t>(q, in);
         }
       }
-#pragma unroll
-      for (int j = 0; j < WORDS; ++j)
-#pragma unroll
-        for (int i = 0; i < NT8; ++i) {
-          uint4& v = c[i][h * WORDS + j];
-          if (VEC) v = in ? stream::ld_rows(xr[i] + k + 8 * j) : make_uint4(0, 0, 0, 0);
-          else v = stream::ld8_any(xr[i] + k + 8 * j, p.k - k - 8 * j);
-        }
     }
-    {  // lane t has the chunk's t-th group's scale and zero point (with fewer groups: of one of them)
-      const int k = k0 + (t & (P - 1)) * (CHUNK / P);
-      const int at = k / p.group;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const long long i = (long long)f[m] * p.groups + at;
-        s[m] = k < p.k ? ops::ld_any(p.s, i, p.s_f32) : 0.f;
-        if (ZEROS) z[m] = k < p.k ? p.z[i] : 0;
+    const bool in = whole || chunk * CHUNK + (t & (P - 1)) * (CHUNK / P) < p.k;
+    const int gr = P > 1 ? chunk * P : p.group_shift >= 0 ? chunk >> p.group_shift : chunk / (p.group / CHUNK);
+    c.s[0] = in ? ops::ld_any(p.s, s_of[0] + gr, p.s_f32) : 0.f;
+    c.s[1] = in ? ops::ld_any(p.s, s_of[1] + gr, p.s_f32) : 0.f;
+    if (ZEROS) c.z = 0xC300C300u | (in ? (uint32_t)(p.z[s_of[0] + gr] & 15) | (uint32_t)(p.z[s_of[1] + gr] & 15) << 16 : 0u);
+  };
+  // x of `n` chunks from `chunk` on; a thread's piece is eight contiguous k
+  auto stage = [&](int chunk, int n) {
+    const int rows = min(p.rows, kept);
+    for (int i = tid; i < n * 16 * kept; i += 32 * WARPS) {
+      // the 16 pieces of a row's chunk go to neighbouring threads
+      const int e = i & 15, row = (i >> 4) % kept, c = (i >> 4) / kept;
+      const int k = (chunk + c) * CHUNK + e * 8;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (row < rows) {
+        const uint16_t* q = p.x + row * p.ldx + k;
+        if (VEC) v = k < p.k ? stream::ld_rows(q) : v;
+        else v = stream::ld8_any(q, p.k - k);
       }
+      uint32_t h[4];
+      pairs(v, h);
+      // piece e is word j of group h for lane t: e = (h * 4 + t) * (4 / P) + j
+      const int j = e % WORDS, tt = e / WORDS % 4, hh = e / (WORDS * 4), word = hh * WORDS + j;
+      const int to = NT8 == 1 ? ((c * 4 + word) * kept + row) * 4 + tt : ((c * 4 + word) * kept + row) * 4 + tt;
+      xs[to] = make_uint4(h[0], h[1], h[2], h[3]);
     }
+  };
+  const int my_row = NT8 == 1 ? min(g, p.rows - 1) : g;
+  float total[NT8][4];
+  auto multiply = [&](const Chunk& c, int chunk) {  // chunk: of the slice
 #pragma unroll
     for (int h = 0; h < P; ++h) {
       float acc[NT8][4] = {};
-      float sh[2];
-      uint32_t zh[2];
+      float s[2];
+      uint32_t z[2];
+      const uint32_t zz = !ZEROS ? 0xC308C308u : P == 1 ? c.z : __shfl_sync(0xFFFFFFFFu, c.z, (lane & ~3) | h);
+      z[0] = ZEROS ? __byte_perm(zz, 0, 0x1010) : zz;
+      z[1] = ZEROS ? __byte_perm(zz, 0, 0x3232) : zz;
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        sh[m] = P == 1 ? s[m] : __shfl_sync(0xFFFFFFFFu, s[m], (lane & ~3) | h);
-        zh[m] = zero_pair(P == 1 || !ZEROS ? z[m] : __shfl_sync(0xFFFFFFFFu, z[m], (lane & ~3) | h));
-      }
+      for (int m = 0; m < 2; ++m) s[m] = P == 1 ? c.s[m] : __shfl_sync(0xFFFFFFFFu, c.s[m], (lane & ~3) | h);
 #pragma unroll
       for (int j = 0; j < WORDS; ++j) {
         uint32_t a[4], b[4];
-        dequant(w[0][h * WORDS + j], zh[0], a);
-        dequant(w[1][h * WORDS + j], zh[1], b);
+        dequant(c.w[0][h * WORDS + j], z[0], a);
+        dequant(c.w[1][h * WORDS + j], z[1], b);
+        const uint4* x = xs + ((chunk * 4 + h * WORDS + j) * kept + my_row) * 4 + t;
 #pragma unroll
         for (int i = 0; i < NT8; ++i) {
-          uint32_t x[4];
-          pairs(c[i][h * WORDS + j], x);
-          stream::mma_bf16(acc[i], a[0], b[0], a[1], b[1], x[0], x[1]);
-          stream::mma_bf16(acc[i], a[2], b[2], a[3], b[3], x[2], x[3]);
+          const uint4 v = x[i * 32];
+          stream::mma_bf16(acc[i], a[0], b[0], a[1], b[1], v.x, v.y);
+          stream::mma_bf16(acc[i], a[2], b[2], a[3], b[3], v.z, v.w);
         }
       }
 #pragma unroll
       for (int i = 0; i < NT8; ++i) {
-        total[i][0] = fmaf(sh[0], acc[i][0], total[i][0]);
-        total[i][1] = fmaf(sh[0], acc[i][1], total[i][1]);
-        total[i][2] = fmaf(sh[1], acc[i][2], total[i][2]);
-        total[i][3] = fmaf(sh[1], acc[i][3], total[i][3]);
+        total[i][0] = fmaf(s[0], acc[i][0], total[i][0]);
+        total[i][1] = fmaf(s[0], acc[i][1], total[i][1]);
+        total[i][2] = fmaf(s[1], acc[i][2], total[i][2]);
+        total[i][3] = fmaf(s[1], acc[i][3], total[i][3]);
       }
     }
-  }
+  };
+  Chunk ring[A];
+  auto prime = [&](int set, int begin) {
 #pragma unroll
-  for (int i = 0; i < NT8; ++i)
+    for (int i = 0; i < A; ++i)
+      if (set * at_once + tw < p.tiles && begin + kw + i * p.kw < min(begin + p.slice, c_end)) load(ring[i], begin + kw + i * p.kw);
+  };
+  int set = (int)blockIdx.x / p.split;
+  go_to(set * at_once + tw);
+  prime(set, c_begin);
+  const bool once = c_end - c_begin <= p.slice;  // x stays where it is
+  for (bool first = true; set < sets; set += set_step, first = false) {
+    const int tile = set * at_once + tw;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) part[warp][8 * i + 2 * t + (j & 1)][g + 8 * (j >> 1)] = total[i][j];
-  __syncthreads();
-  if (p.split > 1)
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  for (int o = rank * 32 * WARPS + tid; o < TOK * FT; o += p.split * 32 * WARPS) {
-    const int tok = o / FT, c = o % FT;
-    if (tok >= rows || f0 + c >= p.n) continue;
-    float y = 0.f;
-    if (p.split == 1) {
+    for (int i = 0; i < NT8; ++i)
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) y += part[w][tok][c];
-    } else {
-      for (int r = 0; r < p.split; ++r) {
-        uint32_t at;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&part[0][tok][c])), "r"(r));
-        float v[WARPS];
+      for (int j = 0; j < 4; ++j) total[i][j] = 0.f;
+    for (int begin = c_begin; begin < c_end; begin += p.slice) {
+      const int end = min(begin + p.slice, c_end);
+      if (!once || first) {
+        if (!once) __syncthreads();
+        stage(begin, end - begin);
+        __syncthreads();
+      }
+      if (tile < p.tiles) {
+#pragma unroll 1
+        for (int c0 = begin + kw; c0 < end; c0 += A * p.kw) {
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w)
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[w]) : "r"(at + w * (uint32_t)(TOK * FT * 4)) : "memory");
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) y += v[w];
+          for (int i = 0; i < A; ++i) {
+            const int c = c0 + i * p.kw;
+            if (c >= end) break;
+            multiply(ring[i], c - begin);
+            if (c + A * p.kw < end) load(ring[i], c + A * p.kw);
+          }
+        }
+      }
+      // the next weights travel while this tile is finished
+      if (end < c_end) {
+        prime(set, end);
+      } else {
+        go_to((set + set_step) * at_once + tw);
+        prime(set + set_step, c_begin);
       }
     }
-    const lin::Epilogue& e = p.epi;
-    const long long row = r0 + tok, col = f0 + c;
-    if (e.bias) y += ops::ld_any(e.bias, col, e.bias_f32);
-    const float res = e.res ? ops::ld_any(e.res, row * e.ld_res + col, e.res_f32) : 0.f;
-    if (e.pre) ops::st_any(e.pre, row * e.ld_pre + col, y, false);
-    with_act(e.act, [&](auto a) { ops::st_any(e.out, row * e.ld_out + col, act_f<decltype(a)::value>(y) + res, e.out_f32); });
-  }
-  if (p.split > 1) {  // no read reaches a CTA that has left
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < NT8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[(warp * TOK + 8 * i + 2 * t + (j & 1)) * PART_LD + g + 8 * (j >> 1)] = total[i][j];
+    __syncthreads();
+    if (p.split > 1)
+      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    for (int o = rank * 32 * WARPS + tid; o < at_once * TOK * FT; o += p.split * 32 * WARPS) {
+      const int c = o % FT, tok = o / FT % TOK, which = o / (FT * TOK);
+      const long long col = (long long)(set * at_once + which) * FT + c;
+      if (tok >= p.rows || col >= p.n) continue;
+      const float* from = part + (which * p.kw * TOK + tok) * PART_LD + c;
+      float y = 0.f;
+      for (int r = 0; r < p.split; ++r) {  // in the order of ranks and warps
+        if (p.split == 1) {
+          for (int w = 0; w < p.kw; ++w) y += from[w * TOK * PART_LD];
+        } else {
+          uint32_t q;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(q) : "r"(smem_u32(from)), "r"(r));
+          for (int w = 0; w < p.kw; ++w) {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(q + w * TOK * PART_LD * 4) : "memory");
+            y += v;
+          }
+        }
+      }
+      const lin::Epilogue& e = p.epi;
+      if (e.bias) y += ops::ld_any(e.bias, col, e.bias_f32);
+      const float res = e.res ? ops::ld_any(e.res, tok * e.ld_res + col, e.res_f32) : 0.f;
+      if (e.pre) ops::st_any(e.pre, tok * e.ld_pre + col, y, false);
+      with_act(e.act, [&](auto a) { ops::st_any(e.out, tok * e.ld_out + col, act_f<decltype(a)::value>(y) + res, e.out_f32); });
+    }
+    // the sums are written again, and no read reaches a CTA that has left
+    __syncthreads();
+    if (p.split > 1)
+      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
 }
 
@@ -199,36 +294,34 @@ struct Expand {
   const uint16_t* x;
   uint16_t* xx;
   long long ldw, ldx;
-  int n, k, group, groups, s_f32, low, rows;
+  int n, k, group, groups, group_log, s_f32, low, rows;
 };
 __global__ void __launch_bounds__(256) expand(const __grid_constant__ Expand p) {
   pdl_launch();
   pdl_wait();
-  const int per = p.k / 32;  // a thread's piece
+  // a block takes 2048 k of a row, a thread eight of them
+  const int per = (p.k + 2047) / 2048;
   const long long ld = p.low ? 2ll * p.k : p.k;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)p.n * per; i += (long long)gridDim.x * 256) {
-    const int f = (int)(i / per), k = (int)(i - (long long)f * per) * 32;
-    const long long at = (long long)f * p.groups + k / p.group;
+  for (long long i = blockIdx.x; i < (long long)p.n * per; i += gridDim.x) {
+    const long long f = i / per;
+    const int k = (int)(i - f * per) * 2048 + (int)threadIdx.x * 8;
+    if (k >= p.k) continue;
+    const long long at = f * p.groups + (p.group_log >= 0 ? k >> p.group_log : k / p.group);
     const float s = ops::ld_any(p.s, at, p.s_f32), z = p.z ? (float)(p.z[at] & 15) : 8.f;
-    const uint4 v = stream::ld_late(p.w + f * p.ldw + k / 2);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint4* o = reinterpret_cast<uint4*>(p.out + f * ld + k);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p.w + f * p.ldw + k / 2);
+    float q[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float q[8];
+    for (int e = 0; e < 8; ++e) q[e] = s * ((float)(w >> (4 * e) & 15u) - z);
+    ops::Raw<false> r;
+    ops::pack(q, r);
+    *reinterpret_cast<uint4*>(p.out + f * ld + k) = r.a;
+    if (p.low) {
+      float hi[8];
+      ops::unpack(r, hi);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) q[e] = s * ((float)(w[j] >> (4 * e) & 15u) - z);
-      ops::Raw<false> r;
+      for (int e = 0; e < 8; ++e) q[e] -= hi[e];
       ops::pack(q, r);
-      o[j] = r.a;
-      if (p.low) {
-        float hi[8];
-        ops::unpack(r, hi);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) q[e] -= hi[e];
-        ops::pack(q, r);
-        reinterpret_cast<uint4*>(p.out + f * ld + p.k + k)[j] = r.a;
-      }
+      *reinterpret_cast<uint4*>(p.out + f * ld + p.k + k) = r.a;
     }
   }
   if (!p.xx) return;
@@ -263,6 +356,7 @@ struct apk_linear4 {
   apk_linear4_config cfg{};
   Err err;
   int sms = 0;
+  int clusters[9] = {};  // of 2, 4 and 8 CTAs that run at once
   Scratch scratch;
   std::mutex mu;
 };
@@ -293,15 +387,29 @@ apk_status create(const apk_linear4_config* cfg, apk_linear4* h) {
   h->sms = c.sms ? c.sms : sms;
   DeviceGuard guard(c.device);
   APK_TRY(cu_status(lin::prepare(), "preparing the linear kernels", &h->err));
+  // (a layer's group and zero points leave eight kernels that it may launch)
+  for (const bool vec : {false, true}) {
+    const void* f[4] = {lin4::fn<1>(c.group, c.zeros, vec), lin4::fn<2>(c.group, c.zeros, vec), lin4::fn<4>(c.group, c.zeros, vec),
+                        lin4::fn<8>(c.group, c.zeros, vec)};
+    for (int i = 0; i < 4; ++i)
+      APK_TRY(cu_status(cudaFuncSetAttribute(f[i], cudaFuncAttributeMaxDynamicSharedMemorySize, lin4::SMEM),
+                        "preparing the 4-bit product", &h->err));
+  }
+  for (int split = 2; split <= 8; split *= 2) {
+    Launch l(dim3(split), 32 * lin4::WARPS, lin4::SMEM, nullptr, split);
+    APK_TRY(cu_status(cudaOccupancyMaxActiveClusters(&h->clusters[split], lin4::fn<1>(c.group, c.zeros, true), &l.cfg),
+                      "preparing the 4-bit product", &h->err));
+  }
   return h->scratch.open(c.device, &h->err);
 }
 
-// Rows up to here stream the weights, 16 rows at a time.
+// Rows up to here stream the weights.
 constexpr int STREAM_ROWS = 64;
 
 apk_status stream(apk_linear4* h, const apk_linear_io* io, const lin::Epilogue& epi) {
   const apk_linear4_config& c = h->cfg;
   lin4::Params p{};
+  int grid = 0;
   p.x = static_cast<const uint16_t*>(io->x);
   p.w = static_cast<const uint8_t*>(c.W);
   p.s = c.scales;
@@ -314,15 +422,41 @@ apk_status stream(apk_linear4* h, const apk_linear_io* io, const lin::Epilogue& 
   p.group = c.group;
   p.groups = ops::ceil_div(c.in_features, c.group);
   p.s_f32 = c.scale_dtype == APK_F32;
+  p.group_shift = -1;
+  for (int i = 0; i < 24; ++i)
+    if (c.group == lin4::CHUNK << i) p.group_shift = i;
   p.epi = epi;
   const bool vec = ops::on16(io->x, io->ldx, io->rows, APK_BF16);
-  const int nt = io->rows <= 8 ? 1 : 2;
-  const int tiles = ops::ceil_div(p.n, lin4::FT), blocks = ops::ceil_div(p.rows, 8 * nt);
-  // split K while every warp keeps a chunk and the blocks do not exceed two an SM
-  p.split = 1;
-  while (p.split < 8 && 2 * p.split * tiles * blocks <= 2 * h->sms && 2 * p.split * lin4::WARPS * lin4::CHUNK <= p.k) p.split *= 2;
-  const void* f = nt == 1 ? lin4::fn<1>(c.group, c.zeros, vec) : lin4::fn<2>(c.group, c.zeros, vec);
-  Launch l(dim3(tiles * p.split, blocks), 32 * lin4::WARPS, 0, static_cast<cudaStream_t>(io->stream), p.split);
+  const int nt = io->rows <= 8 ? 1 : io->rows <= 16 ? 2 : io->rows <= 32 ? 4 : 8;
+  p.tiles = ops::ceil_div(p.n, lin4::FT);
+  const int chunks = ops::ceil_div(p.k, lin4::CHUNK), kept = nt == 1 ? io->rows : 8 * nt;
+  const int room = (lin4::SMEM - lin4::part_bytes(8 * nt)) / (kept * lin4::CHUNK * 2);  // chunks of x
+  // What a launch takes, in chunks of a warp: rounds of tiles, each with its
+  // chunks and 4 for its end (of a cluster: 8), and x laid out once where it
+  // fits (half a chunk's time each), else again in every round.
+  long long best = -1;
+  for (int split = 1; split <= 8; split *= 2) {
+    if (split > 1 && (split > chunks || h->clusters[split] == 0)) break;
+    const int places = split == 1 ? h->sms : std::min(h->clusters[split], h->sms / split);
+    const int mine = ops::ceil_div(chunks, split);
+    for (int kw = 1; kw <= lin4::WARPS && places > 0; kw *= 2) {
+      const int sets = ops::ceil_div(p.tiles, lin4::WARPS / kw), rounds = ops::ceil_div(sets, places);
+      const long long x = (long long)mine * kept / 64 * (mine <= room ? 1 : rounds);
+      const long long cost = (long long)rounds * (ops::ceil_div(mine, kw) * std::max(2, nt) / 2 + (split > 1 ? 8 : 4)) + x;
+      if (best >= 0 && cost >= best) continue;
+      best = cost;
+      p.split = split;
+      p.kw = kw;
+      p.slice = std::min(mine, room);
+      grid = std::min(sets, places) * split;
+    }
+  }
+  const void* f = nt == 1   ? lin4::fn<1>(c.group, c.zeros, vec)
+                  : nt == 2 ? lin4::fn<2>(c.group, c.zeros, vec)
+                  : nt == 4 ? lin4::fn<4>(c.group, c.zeros, vec)
+                            : lin4::fn<8>(c.group, c.zeros, vec);
+  Launch l(dim3(grid), 32 * lin4::WARPS, p.slice * kept * lin4::CHUNK * 2 + lin4::part_bytes(8 * nt),
+           static_cast<cudaStream_t>(io->stream), p.split);
   void* args[] = {&p};
   return cu_status(cudaLaunchKernelExC(&l.cfg, f, args), "launching the 4-bit product", &h->err);
 }
@@ -366,12 +500,15 @@ apk_status forward(apk_linear4* h, const apk_linear_io* io) {
   e.n = N;
   e.k = K;
   e.group = c.group;
+  e.group_log = -1;
+  for (int i = 5; i < 31; ++i)
+    if (c.group == 1 << i) e.group_log = i;
   e.groups = ops::ceil_div(K, c.group);
   e.s_f32 = c.scale_dtype == APK_F32;
   e.low = low;
   e.rows = M;
-  const long long pieces = std::max<long long>((long long)N * (K / 32), copy ? (long long)M * (K / 8) : 0);
-  Launch l(dim3((unsigned)std::min<long long>(ops::ceil_div(pieces, 256ll), h->sms * 8)), 256, 0, s);
+  const long long blocks = std::max<long long>((long long)N * ops::ceil_div(K, 2048), copy ? (long long)M * (K / 8) / 256 + 1 : 0);
+  Launch l(dim3((unsigned)std::min<long long>(blocks, h->sms * 8)), 256, 0, s);
   APK_TRY(cu_status(cudaLaunchKernelEx(&l.cfg, lin4::expand, e), "launching the weights' expansion", &h->err));
   lin::Product p{};
   p.P = {e.out, ld, N, (int)ld, false};
