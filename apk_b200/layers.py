@@ -105,6 +105,15 @@ def _like(t, shape):
     return torch.empty_like(t) if t.shape == shape and t.is_contiguous() else t.new_empty(shape)
 
 
+def _new(t, shape, dtype):
+    """A new contiguous tensor on t's device (the way that costs the host least)."""
+    n, strides = 1, []
+    for size in reversed(shape):
+        strides.append(n)
+        n *= size
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=t.device)
+
+
 class _Handle:
     """Owner of one native handle; subclasses name its functions."""
     _create = _destroy = _error = _status = ""
@@ -355,7 +364,7 @@ class Linear4(_Handle):
             io.x, io.rows, io.ldx = _rows(x, "x", self.device, self.in_features)
             shape = (*x.shape[:-1], n)
             if out is None:
-                y = x.new_empty(shape, dtype=self.out_dtype)
+                y = _new(x, shape, self.out_dtype)
                 io.y, io.ldy = y.data_ptr(), n
             else:
                 y = out
@@ -428,7 +437,7 @@ class LayerNorm(_Handle):
             io.x, io.rows, io.ldx = _rows(x, "x", self.device, d, _ANY)
             io.x_dtype = _CODE[x.dtype]
             if out is None:
-                y = _like(x, x.shape) if x.dtype is self.out_dtype else x.new_empty(x.shape, dtype=self.out_dtype)
+                y = _like(x, x.shape) if x.dtype is self.out_dtype else _new(x, x.shape, self.out_dtype)
                 io.y, io.ldy = y.data_ptr(), d
             else:
                 y = out
@@ -441,7 +450,7 @@ class LayerNorm(_Handle):
                     raise ValueError("out shares memory with x, but is not it")
             stats = None
             if save_stats:
-                stats = x.new_empty((*x.shape[:-1], 2), dtype=torch.float32)
+                stats = _new(x, (*x.shape[:-1], 2), torch.float32)
                 io.stats = stats.data_ptr()
             else:
                 io.stats = None

@@ -10,13 +10,17 @@ from __future__ import annotations
 import array
 import ctypes
 import math
+import operator
 
 import torch
 
 from . import _lib as L
-from .layers import _ANY, _CODE, _Handle, _like, _overlap, _raw_stream, _rows, _tensor
+from .layers import _ANY, _CODE, _Handle, _like, _new, _overlap, _raw_stream, _rows, _tensor
 
 _TYPES = set(_ANY)
+_dtype = operator.attrgetter("dtype")
+_data_ptr, _numel, _get_device, _is_contiguous = (
+    torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous)
 
 
 def _device_index(device) -> int:
@@ -61,15 +65,17 @@ class GradClip(_Handle):
     def _check_list(self, tensors, what):
         # the usual case in few steps: there may be hundreds of them
         try:
-            if ({t.get_device() for t in tensors} <= {self._index} and {t.dtype for t in tensors} <= _TYPES
-                    and all([t.is_contiguous() for t in tensors])):
-                return
-        except (AttributeError, RuntimeError):
+            kinds = list(map(_dtype, tensors))
+            if (set(map(_get_device, tensors)) <= {self._index} and set(kinds) <= _TYPES
+                    and all(map(_is_contiguous, tensors))):
+                return kinds
+        except (AttributeError, RuntimeError, TypeError):
             pass
         for i, t in enumerate(tensors):
             _tensor(t, f"{what}[{i}]", self.device, _ANY)
             if not _dense(t):
                 raise ValueError(f"{what}[{i}], of strides {t.stride()}, is not dense in memory")
+        return list(map(_dtype, tensors))
 
     def _run(self, grads, out, function):
         grads = list(grads)
@@ -79,7 +85,7 @@ class GradClip(_Handle):
                 raise ValueError(f"{len(out)} tensors in out for {len(grads)} gradients")
             out = [o for o, t in zip(out, grads) if t is not None]
         grads = [t for t in grads if t is not None]
-        self._check_list(grads, "grads")
+        kinds = self._check_list(grads, "grads")
         if out is not None:
             self._check_list(out, "out")
             for i, (t, o) in enumerate(zip(grads, out)):
@@ -87,11 +93,11 @@ class GradClip(_Handle):
                     raise ValueError(f"out[{i}] is {o.dtype} {tuple(o.shape)}, its gradient {t.dtype} {tuple(t.shape)}")
                 if t.stride() != o.stride() and not (t.is_contiguous() and o.is_contiguous()):
                     raise ValueError(f"out[{i}] has strides {o.stride()}, its gradient {t.stride()}")
-        norm = torch.empty((), dtype=torch.float32, device=self.device)
-        at = array.array("q", [t.data_ptr() for t in grads])
-        to = at if out is None else array.array("q", [t.data_ptr() for t in out])
-        n = array.array("q", [t.numel() for t in grads])
-        kinds = array.array("i", [_CODE[t.dtype] for t in grads])
+        norm = torch.empty_strided((), (), dtype=torch.float32, device=self.device)
+        at = array.array("q", list(map(_data_ptr, grads)))
+        to = at if out is None else array.array("q", list(map(_data_ptr, out)))
+        n = array.array("q", list(map(_numel, grads)))
+        kinds = array.array("i", [_CODE[d] for d in kinds])
         with self._lock:
             io = self._io
             io.count, io.max_norm = len(grads), self.max_norm
@@ -141,6 +147,11 @@ class LogProbs(_Handle):
         a.dtype = _CODE[logits.dtype]
 
     def _per_row(self, t, what, shape, dtypes):
+        try:  # the usual case first
+            if t.shape == shape and t.dtype in dtypes and t.device == self.device and t.is_contiguous():
+                return t.data_ptr()
+        except AttributeError:
+            pass
         _tensor(t, what, self.device, dtypes)
         if t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{what} is {tuple(t.shape)} with strides {t.stride()}: contiguous {tuple(shape)} is wanted")
@@ -159,21 +170,21 @@ class LogProbs(_Handle):
             io = self._io
             self._logits(logits, io)
             shape = logits.shape[:-1]
-            new = logits.new_empty
             logprob = ids = tops = stats = None
+            entropy = _new(logits, shape, torch.float32)
             if tokens is None:
                 io.tokens = io.logprob = None
             else:
                 self._tokens(tokens, shape, io)
-                logprob = new(shape, dtype=torch.float32)
+                logprob = torch.empty_like(entropy)
                 io.logprob = logprob.data_ptr()
-            entropy = new(shape, dtype=torch.float32)
             io.entropy = entropy.data_ptr()
             if self.top:
-                ids, tops = new((*shape, self.top), dtype=torch.int32), new((*shape, self.top), dtype=torch.float32)
+                tops = _new(logits, (*shape, self.top), torch.float32)
+                ids = torch.empty_like(tops, dtype=torch.int32)
                 io.top_ids, io.top_logprobs = ids.data_ptr(), tops.data_ptr()
             if save_stats:
-                stats = new((*shape, 2), dtype=torch.float32)
+                stats = _new(logits, (*shape, 2), torch.float32)
                 io.stats = stats.data_ptr()
             else:
                 io.stats = None
