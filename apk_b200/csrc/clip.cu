@@ -18,8 +18,8 @@
 namespace apk {
 namespace clip {
 
-constexpr int THREADS = 256, VECS = 4;            // 16-byte vectors of a thread's round
-constexpr int UNIT = THREADS * VECS;              // vectors of a block's round
+constexpr int THREADS = 256, VECS = 4;            // 16-byte vectors of a thread and unit
+constexpr int UNIT = THREADS * VECS;              // vectors of a unit
 constexpr int BLOCKS = 4;                         // of an SM
 
 struct Tensor {
@@ -120,16 +120,12 @@ __device__ __forceinline__ void add_squares(const float* v, int n, float& sum, d
   }
 }
 
-// A block takes neighbouring units, of one tensor mostly: taking every
-// gridDim-th, it stepped over ten tensors' entries for each unit where there
-// are hundreds (300 tensors, 268 MB: 67 us).
-struct Range {
-  unsigned first, end;
-};
+// A block takes runs of up to 8 neighbouring units, of one tensor mostly: unit
+// by unit, it stepped over ten tensors' entries for each where there are
+// hundreds (300 tensors, 268 MB: 67 us); in one piece, blocks read far apart.
 template <int N>
-__device__ __forceinline__ Range range_of(const List<N>& list) {
-  const unsigned per = (list.units + gridDim.x - 1) / gridDim.x, first = min(blockIdx.x * per, list.units);
-  return {first, min(first + per, list.units)};
+__device__ __forceinline__ unsigned run_of(const List<N>& list) {
+  return min(max(list.units / (gridDim.x * 4), 1u), 8u);
 }
 // The last tensor that begins at unit u or before.
 template <int N>
@@ -143,7 +139,7 @@ __device__ __forceinline__ int find(const List<N>& list, unsigned u) {
   return lo;
 }
 
-// Squares are added in fp32 within a round of a thread (16 or 32 values) and
+// Squares are added in fp32 within a thread's part of a unit (16 or 32 values) and
 // in 64 bits beyond; the last block to arrive adds the blocks' sums in their
 // order.
 template <int N>
@@ -153,31 +149,45 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm(const __grid_constant__ 
   pdl_launch();
   pdl_wait();
   double total = 0.0;
-  const Range r = range_of(list);
-  int at = find(list, r.first);
-  for (unsigned u = r.first; u < r.end; ++u) {
-    while (at + 1 < list.count && u >= list.t[at + 1].first) ++at;
-    const Tensor& t = list.t[at];
-    const uint8_t* base = t.in - (reinterpret_cast<uintptr_t>(t.in) & 15);
-    uint4 raw[VECS];
+  const unsigned run = run_of(list);
+  for (unsigned first = blockIdx.x * run; first < list.units; first += gridDim.x * run) {
+    const unsigned end = min(first + run, list.units);
+    int at = find(list, first);
+    for (unsigned u = first; u < end; u += 2) {  // two units' loads at once
+      uint4 raw[2][VECS];
+      int f32[2] = {};
 #pragma unroll
-    for (int j = 0; j < VECS; ++j) {
-      const Span s = span_of(t, u, j);
-      raw[j] = s.any ? load(base, s, t.f32, false) : make_uint4(0, 0, 0, 0);
-    }
-    float sum[VECS] = {};
+      for (int k = 0; k < 2; ++k) {
+        if (u + k >= end) break;
+        while (at + 1 < list.count && u + k >= list.t[at + 1].first) ++at;
+        const Tensor& t = list.t[at];
+        const uint8_t* base = t.in - (reinterpret_cast<uintptr_t>(t.in) & 15);
+        f32[k] = t.f32;
 #pragma unroll
-    for (int j = 0; j < VECS; ++j) {
-      float v[8];
-      if (t.f32) {
-        const float q[4] = {__uint_as_float(raw[j].x), __uint_as_float(raw[j].y), __uint_as_float(raw[j].z), __uint_as_float(raw[j].w)};
-        add_squares(q, 4, sum[j], total);
-      } else {
-        ops::unpack(ops::Raw<false>{raw[j]}, v);
-        add_squares(v, 8, sum[j], total);
+        for (int j = 0; j < VECS; ++j) {
+          const Span s = span_of(t, u + k, j);
+          raw[k][j] = s.any ? load(base, s, t.f32, false) : make_uint4(0, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (u + k >= end) break;
+        float sum[VECS] = {};
+#pragma unroll
+        for (int j = 0; j < VECS; ++j) {
+          const uint4 q = raw[k][j];
+          if (f32[k]) {
+            const float v[4] = {__uint_as_float(q.x), __uint_as_float(q.y), __uint_as_float(q.z), __uint_as_float(q.w)};
+            add_squares(v, 4, sum[j], total);
+          } else {
+            float v[8];
+            ops::unpack(ops::Raw<false>{q}, v);
+            add_squares(v, 8, sum[j], total);
+          }
+        }
+        total += (double)((sum[0] + sum[1]) + (sum[2] + sum[3]));
       }
     }
-    total += (double)((sum[0] + sum[1]) + (sum[2] + sum[3]));
   }
   total = block_sum(total, sh);
   if (threadIdx.x == 0) {
@@ -199,61 +209,67 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm(const __grid_constant__ 
   }
 }
 
-// From a block's last unit to its first: what the norm read last is still in L2.
+__device__ __forceinline__ void scale_unit(const Tensor& t, unsigned u, float c) {
+      const int shift = (int)(reinterpret_cast<uintptr_t>(t.in) & 15);
+      const uint8_t* base = t.in - shift;
+      uint8_t* out = t.out - shift;
+      const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+      uint4 raw[VECS];
+      Span sp[VECS];
+  #pragma unroll
+      for (int j = 0; j < VECS; ++j) {
+        sp[j] = span_of(t, u, j);
+        if (sp[j].any) raw[j] = load(base, sp[j], t.f32, true);
+      }
+  #pragma unroll
+      for (int j = 0; j < VECS; ++j) {
+        if (!sp[j].any) continue;
+        union {
+          uint16_t h[8];
+          uint32_t w[4];
+          uint4 v;
+        } o;
+        if (t.f32) {
+          o.v = make_uint4(__float_as_uint(__uint_as_float(raw[j].x) * c), __float_as_uint(__uint_as_float(raw[j].y) * c),
+                           __float_as_uint(__uint_as_float(raw[j].z) * c), __float_as_uint(__uint_as_float(raw[j].w) * c));
+        } else {
+          float v[8];
+          ops::Raw<false> r{raw[j]};
+          ops::unpack(r, v);
+  #pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] *= c;
+          ops::pack(v, r);
+          o.v = r.a;
+        }
+        uint8_t* q = out + sp[j].vec;
+        if (sp[j].whole && same) {
+          __stcs(reinterpret_cast<uint4*>(q), o.v);
+        } else if (t.f32) {
+  #pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i >= sp[j].lo && i < sp[j].hi) reinterpret_cast<uint32_t*>(q)[i] = o.w[i];
+        } else {
+  #pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i >= sp[j].lo && i < sp[j].hi) reinterpret_cast<uint16_t*>(q)[i] = o.h[i];
+        }
+      }
+}
+
+// From the last unit to the first: what the norm read last is still in L2.
 template <int N>
 __global__ void __launch_bounds__(THREADS, BLOCKS) scale(const __grid_constant__ List<N> list, const Head* head) {
   pdl_launch();
   pdl_wait();
   const float c = head->c;
-  const Range r = range_of(list);
-  int at = r.end > r.first ? find(list, r.end - 1) : 0;
-  for (unsigned u = r.end; u-- > r.first;) {
-    while (u < list.t[at].first) --at;
-    const Tensor& t = list.t[at];
-    if (c == 1.f && t.in == t.out) continue;
-    const int shift = (int)(reinterpret_cast<uintptr_t>(t.in) & 15);
-    const uint8_t* base = t.in - shift;
-    uint8_t* out = t.out - shift;
-    const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-    uint4 raw[VECS];
-    Span sp[VECS];
-#pragma unroll
-    for (int j = 0; j < VECS; ++j) {
-      sp[j] = span_of(t, u, j);
-      if (sp[j].any) raw[j] = load(base, sp[j], t.f32, true);
-    }
-#pragma unroll
-    for (int j = 0; j < VECS; ++j) {
-      if (!sp[j].any) continue;
-      union {
-        uint16_t h[8];
-        uint32_t w[4];
-        uint4 v;
-      } o;
-      if (t.f32) {
-        o.v = make_uint4(__float_as_uint(__uint_as_float(raw[j].x) * c), __float_as_uint(__uint_as_float(raw[j].y) * c),
-                         __float_as_uint(__uint_as_float(raw[j].z) * c), __float_as_uint(__uint_as_float(raw[j].w) * c));
-      } else {
-        float v[8];
-        ops::Raw<false> r{raw[j]};
-        ops::unpack(r, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= c;
-        ops::pack(v, r);
-        o.v = r.a;
-      }
-      uint8_t* q = out + sp[j].vec;
-      if (sp[j].whole && same) {
-        __stcs(reinterpret_cast<uint4*>(q), o.v);
-      } else if (t.f32) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i >= sp[j].lo && i < sp[j].hi) reinterpret_cast<uint32_t*>(q)[i] = o.w[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i >= sp[j].lo && i < sp[j].hi) reinterpret_cast<uint16_t*>(q)[i] = o.h[i];
-      }
+  const unsigned run = run_of(list);
+  for (unsigned first = blockIdx.x * run; first < list.units; first += gridDim.x * run) {
+    int at = find(list, list.units - 1 - first);
+    for (unsigned k = first; k < min(first + run, list.units); ++k) {
+      const unsigned u = list.units - 1 - k;
+      while (u < list.t[at].first) --at;
+      const Tensor& t = list.t[at];
+      if (c != 1.f || t.in != t.out) scale_unit(t, u, c);
     }
   }
 }
