@@ -97,25 +97,58 @@ __device__ __forceinline__ void load_weight(const void* p, int f32, float (&v)[8
 // Sums of a and b over the T threads of a row: a warp, or the block.  `buf`
 // alternates from call to call, so that one barrier a call is enough: who
 // writes a buffer again has passed the barrier behind its last reads.
-template <bool WARP>
-__device__ __forceinline__ float2 row_sums(float a, float b, float2 (*sh)[32], int buf, int T) {
-  a = ops::warp_sum(a);
-  b = ops::warp_sum(b);
-  if constexpr (WARP) return make_float2(a, b);
-  const int lane = threadIdx.x & 31;
-  if (lane == 0) sh[buf][threadIdx.x >> 5] = make_float2(a, b);
+template <bool WARP, int T_>
+__device__ __forceinline__ float2 row_sums(float a, float b, float4 (*sh)[16], int buf, int T) {
+  // two sums in five exchanges: from here the lower half of the warp has a, the upper b
+  const bool upper = threadIdx.x & 16;
+  float v = upper ? b : a;
+  v += __shfl_xor_sync(0xFFFFFFFFu, upper ? a : b, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  if constexpr (WARP) {
+    const float other = __shfl_xor_sync(0xFFFFFFFFu, v, 16);
+    return upper ? make_float2(other, v) : make_float2(v, other);
+  }
+  float2* pair = reinterpret_cast<float2*>(sh[buf]);
+  if ((threadIdx.x & 15) == 0) reinterpret_cast<float*>(pair + (threadIdx.x >> 5))[upper] = v;
   __syncthreads();
-  const float2 v = lane < T / 32 ? sh[buf][lane] : make_float2(0.f, 0.f);
-  return make_float2(ops::warp_sum(v.x), ops::warp_sum(v.y));
+  if constexpr (T_ <= 256) {  // up to 8 warps: every thread adds them
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < T_ / 32; w += 2) {
+      if (w * 32 >= T) break;
+      const float4 q = sh[buf][w / 2];
+      s.x += q.x;
+      s.y += q.y;
+      if ((w + 1) * 32 < T) {
+        s.x += q.z;
+        s.y += q.w;
+      }
+    }
+    return s;
+  } else {
+    const int lane = threadIdx.x & 31;
+    const float2 q = lane < T / 32 ? pair[lane] : make_float2(0.f, 0.f);
+    return make_float2(ops::warp_sum(q.x), ops::warp_sum(q.y));
+  }
 }
-template <bool WARP>
-__device__ __forceinline__ float row_sum(float a, float2 (*sh)[32], int buf, int T) {
+template <bool WARP, int T_>
+__device__ __forceinline__ float row_sum(float a, float4 (*sh)[16], int buf, int T) {
   a = ops::warp_sum(a);
   if constexpr (WARP) return a;
+  float* one = reinterpret_cast<float*>(sh[buf]);
   const int lane = threadIdx.x & 31;
-  if (lane == 0) sh[buf][threadIdx.x >> 5].x = a;
+  if (lane == 0) one[threadIdx.x >> 5] = a;
   __syncthreads();
-  return ops::warp_sum(lane < T / 32 ? sh[buf][lane].x : 0.f);
+  if constexpr (T_ <= 256) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < T_ / 32; ++w)
+      if (w * 32 < T) s += one[w];
+    return s;
+  } else {
+    return ops::warp_sum(lane < T / 32 ? one[lane] : 0.f);
+  }
 }
 
 // A thread's own pieces of the rows ahead, on their way into shared memory:
@@ -125,30 +158,40 @@ __device__ __forceinline__ float row_sum(float a, float2 (*sh)[32], int buf, int
 // 68).  S stages; every row is one group of copies, an empty one behind the last.
 template <int V, bool F32, int S>
 struct Ahead {
-  uint8_t* at;  // this thread's place
+  uint32_t at;  // this thread's place in shared memory
   int threads;
-  static constexpr int SLOTS = V * (F32 ? 2 : 1);
-  __device__ __forceinline__ void fetch(int stage, const void* p, long long row, int cols, int t, int T) const {
+  static constexpr int HALVES = F32 ? 2 : 1, SLOTS = V * HALVES;
+  // `q`: this thread's first piece of the row; `pieces` of the V are in the row
+  __device__ __forceinline__ void fetch(int stage, const uint8_t* q, int pieces, int T) const {
+    const uint32_t to = at + stage * SLOTS * threads * 16;
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if ((j * T + t) * 8 < cols) {
-        const uint8_t* q = static_cast<const uint8_t*>(p) + (row + (j * T + t) * 8) * (F32 ? 4 : 2);
+      if (j < pieces)
 #pragma unroll
-        for (int h = 0; h < (F32 ? 2 : 1); ++h)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(at + ((stage * V + j) * (F32 ? 2 : 1) + h) * threads * 16)),
-                       "l"(q + h * 16)
+        for (int h = 0; h < HALVES; ++h)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (j * HALVES + h) * threads * 16),
+                       "l"(q + (j * T * HALVES + h) * 16ll)
                        : "memory");
-      }
   }
-  __device__ __forceinline__ ops::Raw<F32> get(int stage, int j, int cols, int t, int T) const {
+  __device__ __forceinline__ ops::Raw<F32> get(int stage, int j, int pieces) const {
     ops::Raw<F32> r = {};
-    if ((j * T + t) * 8 < cols) {
-      r.a = *reinterpret_cast<const uint4*>(at + (stage * V + j) * (F32 ? 2 : 1) * threads * 16);
-      if constexpr (F32) r.b = *reinterpret_cast<const uint4*>(at + ((stage * V + j) * 2 + 1) * threads * 16);
+    if (j < pieces) {
+      const uint32_t from = at + (stage * SLOTS + j * HALVES) * threads * 16;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.a.x), "=r"(r.a.y), "=r"(r.a.z), "=r"(r.a.w) : "r"(from) : "memory");
+      if constexpr (F32)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r.b.x), "=r"(r.b.y), "=r"(r.b.z), "=r"(r.b.w)
+                     : "r"(from + threads * 16)
+                     : "memory");
     }
     return r;
   }
 };
+// The next rows of an operand as this thread fetches them.
+template <bool F32>
+__device__ __forceinline__ const uint8_t* piece_of(const void* p, long long row, long long ld, int t) {
+  return static_cast<const uint8_t*>(p) + (row * ld + t * 8) * (F32 ? 4 : 2);
+}
 __device__ __forceinline__ void fetched() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int S>
 __device__ __forceinline__ void arrived() {  // the oldest of S groups
@@ -156,63 +199,95 @@ __device__ __forceinline__ void arrived() {  // the oldest of S groups
 }
 
 // WARP: a row is a warp's and a block of 8 takes 8; else a row is a block's.
+// Weight and bias stay in registers from row to row (read from L1 for every
+// row, they kept it busier than the rows did); T_ is the most threads of a
+// block, of which an SM takes 512.
 template <int V, bool VEC, bool WARP, bool XF, bool YF, int T_>
-__global__ void __launch_bounds__(T_, T_ <= 512 ? 1024 / T_ : 1) forward(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) forward(const __grid_constant__ Params p) {
   constexpr int S = FWD_STAGES<VEC, XF>;
+  constexpr bool HELD = T_ <= 512;
   extern __shared__ uint4 ring[];
-  __shared__ float2 sh[2][32];
+  __shared__ float4 sh[2][16];
   const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
   const int per = WARP ? 8 : 1;
-  const Ahead<V, XF, S> ahead{reinterpret_cast<uint8_t*>(ring + threadIdx.x), (int)blockDim.x};
+  const Ahead<V, XF, S> ahead{smem_u32(ring + threadIdx.x), (int)blockDim.x};
+  const int pieces = t * 8 < p.cols ? (p.cols - t * 8 - 1) / (T * 8) + 1 : 0;  // of the V, where rows go by eights
   const long long step = (long long)gridDim.x * per;
   long long r = (long long)blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0);
   pdl_launch();
   pdl_wait();
+  const uint8_t* px = piece_of<XF>(p.x, r, p.ldx, t);
+  const long long next_x = step * p.ldx * (XF ? 4 : 2);
+  int left = r < p.rows ? (int)((p.rows - r - 1) / step) + 1 : 0;  // rows to be fetched
+  auto fetch = [&](int stage) {
+    if (left > 0) {
+      ahead.fetch(stage, px, pieces, T);
+      px += next_x;
+      --left;
+    }
+    fetched();
+  };
   if constexpr (VEC)
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) {
-      if (r + i * step < p.rows) ahead.fetch(i, p.x, (r + i * step) * p.ldx, p.cols, t, T);
-      fetched();
+    for (int i = 0; i < S - 1; ++i) fetch(i);
+  ops::f32x2 w[V][4], b[V][4];
+  auto weights = [&](int j) {
+    float v[8], c[8] = {};
+    load_weight<VEC>(p.w, p.w_f32, v, j, p.cols, t, T);
+    if (p.b) load_weight<VEC>(p.b, p.b_f32, c, j, p.cols, t, T);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[j][i] = ops::pair2(v[2 * i], v[2 * i + 1]);
+      b[j][i] = ops::pair2(c[2 * i], c[2 * i + 1]);
     }
+  };
+  if constexpr (HELD)
+#pragma unroll
+    for (int j = 0; j < V; ++j) weights(j);
   for (int stage = 0; r < p.rows; r += step, stage = stage + 1 == S ? 0 : stage + 1) {
     ops::Raw<XF> raw[V];
     if constexpr (VEC) {
-      const long long next = r + (S - 1) * step;
-      if (next < p.rows) ahead.fetch(stage == 0 ? S - 1 : stage - 1, p.x, next * p.ldx, p.cols, t, T);
-      fetched();
+      fetch(stage == 0 ? S - 1 : stage - 1);
       arrived<S>();
 #pragma unroll
-      for (int j = 0; j < V; ++j) raw[j] = ahead.get(stage, j, p.cols, t, T);
+      for (int j = 0; j < V; ++j) raw[j] = ahead.get(stage, j, pieces);
     } else {
       load_row<VEC, XF, V>(p.x, r * p.ldx, raw, p.cols, t, T);
     }
-    float v[V][8], s = 0.f;
+    ops::f32x2 v[V][4], s = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      ops::unpack(raw[j], v[j]);
+      ops::unpack2(raw[j], v[j]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[j][i];  // (zero behind the last column)
+      for (int i = 0; i < 4; ++i) s = ops::add2(s, v[j][i]);  // (zero behind the last column)
     }
-    const float mean = row_sum<WARP>(s, sh, 0, T) * p.per_col;
-    s = 0.f;
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = column<VEC>(j, i, t, T) < p.cols ? v[j][i] - mean : 0.f;
-        v[j][i] = d;
-        s = fmaf(d, d, s);
-      }
-    const float rstd = rsqrtf(fmaf(row_sum<WARP>(s, sh, 1, T), p.per_col, p.eps));
-    if (p.stats && t == 0) p.stats[r] = make_float2(mean, rstd);
+    const float mean = row_sum<WARP, T_>(ops::sum2(s), sh, 0, T) * p.per_col;
+    const ops::f32x2 minus = ops::both(-mean);
+    s = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float w[8], b[8] = {};
-      load_weight<VEC>(p.w, p.w_f32, w, j, p.cols, t, T);
-      if (p.b) load_weight<VEC>(p.b, p.b_f32, b, j, p.cols, t, T);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = fmaf(v[j][i] * rstd, w[i], b[i]);
-      store_piece<VEC, YF>(p.y, r * p.ldy, w, j, p.cols, t, T);
+      for (int i = 0; i < 4; ++i) {
+        ops::f32x2 d = ops::add2(v[j][i], minus);
+        if constexpr (!VEC) {
+          float lo, hi;
+          ops::unpair2(d, lo, hi);
+          d = ops::pair2(column<false>(j, 2 * i, t, T) < p.cols ? lo : 0.f, column<false>(j, 2 * i + 1, t, T) < p.cols ? hi : 0.f);
+        }
+        v[j][i] = d;
+        if (!VEC || j < pieces) s = ops::fma2(d, d, s);
+      }
+    }
+    const float rstd = rsqrtf(fmaf(row_sum<WARP, T_>(ops::sum2(s), sh, 1, T), p.per_col, p.eps));
+    if (p.stats && t == 0) p.stats[r] = make_float2(mean, rstd);
+    const ops::f32x2 scale = ops::both(rstd);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if constexpr (!HELD) weights(j);
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ops::unpair2(ops::fma2(ops::mul2(v[j][i], scale), w[j][i], b[j][i]), y[2 * i], y[2 * i + 1]);
+      store_piece<VEC, YF>(p.y, r * p.ldy, y, j, p.cols, t, T);
     }
   }
 }
@@ -224,79 +299,91 @@ template <int V, bool VEC, bool WARP, bool XF, bool DF, int T_>
 __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const __grid_constant__ Params p) {
   constexpr int S = BWD_STAGES<VEC, XF, DF, T_>;
   extern __shared__ uint4 ring[];
-  __shared__ float2 sh[2][32];
+  __shared__ float4 sh[2][16];
   const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
   const int per = WARP ? 8 : 1;
-  const Ahead<V, XF, S> ax{reinterpret_cast<uint8_t*>(ring + threadIdx.x), (int)blockDim.x};
+  const Ahead<V, XF, S> ax{smem_u32(ring + threadIdx.x), (int)blockDim.x};
   const Ahead<V, DF, S> ad{ax.at + S * ax.SLOTS * blockDim.x * 16, (int)blockDim.x};
   const Ahead<V, XF, S> ar{ad.at + S * ad.SLOTS * blockDim.x * 16, (int)blockDim.x};
-  float dw[V][8] = {}, db[V][8] = {};
+  const int pieces = t * 8 < p.cols ? (p.cols - t * 8 - 1) / (T * 8) + 1 : 0;
+  ops::f32x2 dw[V][4] = {}, db[V][4] = {};
   const long long step = (long long)gridDim.x * per;
   long long r = (long long)blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0);
   pdl_launch();
   pdl_wait();
-  auto fetch = [&](int stage, long long row) {
-    if (row < p.rows) {
-      ax.fetch(stage, p.x, row * p.ldx, p.cols, t, T);
-      ad.fetch(stage, p.dy, row * p.ld_dy, p.cols, t, T);
-      if (p.r) ar.fetch(stage, p.r, row * p.ld_r, p.cols, t, T);
+  const uint8_t* px = piece_of<XF>(p.x, r, p.ldx, t);
+  const uint8_t* pd = piece_of<DF>(p.dy, r, p.ld_dy, t);
+  const uint8_t* pr = piece_of<XF>(p.r, r, p.ld_r, t);
+  int left = r < p.rows ? (int)((p.rows - r - 1) / step) + 1 : 0;  // rows to be fetched
+  auto fetch = [&](int stage) {
+    if (left > 0) {
+      ax.fetch(stage, px, pieces, T);
+      ad.fetch(stage, pd, pieces, T);
+      if (p.r) ar.fetch(stage, pr, pieces, T);
+      px += step * p.ldx * (XF ? 4 : 2);
+      pd += step * p.ld_dy * (DF ? 4 : 2);
+      pr += step * p.ld_r * (XF ? 4 : 2);
+      --left;
     }
     fetched();
   };
   if constexpr (VEC)
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i) fetch(i, r + i * step);
+    for (int i = 0; i < S - 1; ++i) fetch(i);
   int buf = 0;
   float2 st = r < p.rows ? p.stats[r] : make_float2(0.f, 0.f);
   for (int stage = 0; r < p.rows; r += step, stage = stage + 1 == S ? 0 : stage + 1) {
     ops::Raw<XF> rx[V];
     ops::Raw<DF> rd[V];
     if constexpr (VEC) {
-      fetch(stage == 0 ? S - 1 : stage - 1, r + (S - 1) * step);
+      fetch(stage == 0 ? S - 1 : stage - 1);
       arrived<S>();
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        rx[j] = ax.get(stage, j, p.cols, t, T);
-        rd[j] = ad.get(stage, j, p.cols, t, T);
+        rx[j] = ax.get(stage, j, pieces);
+        rd[j] = ad.get(stage, j, pieces);
       }
     } else {
       load_row<VEC, XF, V>(p.x, r * p.ldx, rx, p.cols, t, T);
       load_row<VEC, DF, V>(p.dy, r * p.ld_dy, rd, p.cols, t, T);
     }
     const float2 st_next = r + step < p.rows ? p.stats[r + step] : make_float2(0.f, 0.f);
-    float n[V][8], g[V][8], s1 = 0.f, s2 = 0.f;
+    const ops::f32x2 minus = ops::both(-st.x), rstd = ops::both(st.y);
+    ops::f32x2 n[V][4], g[V][4], s1 = 0, s2 = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float w[8];
       load_weight<VEC>(p.w, p.w_f32, w, j, p.cols, t, T);
-      ops::unpack(rx[j], n[j]);
-      ops::unpack(rd[j], g[j]);
+      ops::unpack2(rx[j], n[j]);
+      ops::unpack2(rd[j], g[j]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        n[j][i] = (n[j][i] - st.x) * st.y;
-        dw[j][i] = fmaf(g[j][i], n[j][i], dw[j][i]);
-        db[j][i] += g[j][i];
-        g[j][i] *= w[i];  // (zero behind the last column)
-        s1 += g[j][i];
-        s2 = fmaf(g[j][i], n[j][i], s2);
+      for (int i = 0; i < 4; ++i) {
+        n[j][i] = ops::mul2(ops::add2(n[j][i], minus), rstd);
+        dw[j][i] = ops::fma2(g[j][i], n[j][i], dw[j][i]);
+        db[j][i] = ops::add2(db[j][i], g[j][i]);
+        g[j][i] = ops::mul2(g[j][i], ops::pair2(w[2 * i], w[2 * i + 1]));  // (zero behind the last column)
+        s1 = ops::add2(s1, g[j][i]);
+        s2 = ops::fma2(g[j][i], n[j][i], s2);
       }
     }
     if (p.y) {
-      const float2 s = row_sums<WARP>(s1, s2, sh, buf, T);
+      const float2 s = row_sums<WARP, T_>(ops::sum2(s1), ops::sum2(s2), sh, buf, T);
       buf ^= 1;
-      const float a = s.x * p.per_col, b = s.y * p.per_col;
+      const ops::f32x2 a = ops::both(-s.x * p.per_col), b = ops::both(-s.y * p.per_col);
       ops::Raw<XF> rr[V];
       if (!VEC && p.r) load_row<VEC, XF, V>(p.r, r * p.ld_r, rr, p.cols, t, T);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float res[8] = {};
+        ops::f32x2 res[4] = {};
         if (p.r) {
-          if constexpr (VEC) rr[j] = ar.get(stage, j, p.cols, t, T);
-          ops::unpack(rr[j], res);
+          if constexpr (VEC) rr[j] = ar.get(stage, j, pieces);
+          ops::unpack2(rr[j], res);
         }
+        float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[j][i] = fmaf(st.y, g[j][i] - a - n[j][i] * b, res[i]);
-        store_piece<VEC, XF>(p.y, r * p.ldy, g[j], j, p.cols, t, T);
+        for (int i = 0; i < 4; ++i)
+          ops::unpair2(ops::fma2(rstd, ops::fma2(n[j][i], b, ops::add2(g[j][i], a)), res[i]), y[2 * i], y[2 * i + 1]);
+        store_piece<VEC, XF>(p.y, r * p.ldy, y, j, p.cols, t, T);
       }
     }
     st = st_next;
@@ -304,6 +391,14 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
   if (!p.part) return;
   const int ldp = (p.cols + 7) / 8 * 8;
   float* part = p.part + (long long)blockIdx.x * 2 * ldp;
+  float vw[V][8], vb[V][8];
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ops::unpair2(dw[j][i], vw[j][2 * i], vw[j][2 * i + 1]);
+      ops::unpair2(db[j][i], vb[j][2 * i], vb[j][2 * i + 1]);
+    }
   if constexpr (WARP) {
     float(*join)[256 * V] = reinterpret_cast<float(*)[256 * V]>(ring);  // (all rows have arrived)
     __syncthreads();
@@ -312,7 +407,7 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
 #pragma unroll
       for (int j = 0; j < V; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) join[threadIdx.x >> 5][column<VEC>(j, i, t, T)] = h ? db[j][i] : dw[j][i];
+        for (int i = 0; i < 8; ++i) join[threadIdx.x >> 5][column<VEC>(j, i, t, T)] = h ? vb[j][i] : vw[j][i];
       __syncthreads();
       for (int c = threadIdx.x; c < p.cols; c += 256) {
         float s = 0.f;
@@ -325,8 +420,8 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      store_piece<VEC, true>(part, 0, dw[j], j, p.cols, t, T);
-      store_piece<VEC, true>(part, ldp, db[j], j, p.cols, t, T);
+      store_piece<VEC, true>(part, 0, vw[j], j, p.cols, t, T);
+      store_piece<VEC, true>(part, ldp, vb[j], j, p.cols, t, T);
     }
   }
 }
@@ -492,7 +587,7 @@ apk_status forward(apk_norm* h, const apk_norm_io* io) {
                    ops::aligned(c.weight, 16) && ops::aligned(c.bias, 16);
   const bool xf = io->x_dtype == APK_F32, yf = io->y_dtype == APK_F32;
   const norm::Shape sh = norm::fwd_shape(D, vec, xf, yf);
-  const int grid = std::min(ops::ceil_div(M, sh.per), h->sms * std::max(1, 1024 / sh.T));
+  const int grid = std::min(ops::ceil_div(M, sh.per), h->sms * std::max(1, 512 / sh.T));
   return launch(h, sh, p, grid, static_cast<cudaStream_t>(io->stream), "launching the layer norm");
 }
 

@@ -87,6 +87,49 @@ __device__ __forceinline__ void set1(Raw<true>& r, int i, const void* p, long lo
   (&(i < 4 ? r.a : r.b).x)[i & 3] = static_cast<const uint32_t*>(p)[at];
 }
 
+// Pairs of fp32 values, for instructions that take two at once.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ f32x2 both(float v) { return pair2(v, v); }
+__device__ __forceinline__ void unpair2(f32x2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ float sum2(f32x2 v) {
+  float lo, hi;
+  unpair2(v, lo, hi);
+  return lo + hi;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(const Raw<false>& r, f32x2 (&v)[4]) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pair2(bf_lo(w[i]), bf_hi(w[i]));
+}
+__device__ __forceinline__ void unpack2(const Raw<true>& r, f32x2 (&v)[4]) {
+  float f[8];
+  unpack(r, f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = pair2(f[2 * i], f[2 * i + 1]);
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
