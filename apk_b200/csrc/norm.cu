@@ -205,7 +205,7 @@ __device__ __forceinline__ void arrived() {  // the oldest of S groups
 template <int V, bool VEC, bool WARP, bool XF, bool YF, int T_>
 __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) forward(const __grid_constant__ Params p) {
   constexpr int S = FWD_STAGES<VEC, XF>;
-  constexpr bool HELD = T_ <= 512;
+  constexpr bool HELD = V <= 2 && T_ <= 512;
   extern __shared__ uint4 ring[];
   __shared__ float4 sh[2][16];
   const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
@@ -298,6 +298,7 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) forward(const __
 template <int V, bool VEC, bool WARP, bool XF, bool DF, int T_>
 __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const __grid_constant__ Params p) {
   constexpr int S = BWD_STAGES<VEC, XF, DF, T_>;
+  constexpr bool HELD = VEC && T_ <= 512;  // the weight stays in registers
   extern __shared__ uint4 ring[];
   __shared__ float4 sh[2][16];
   const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
@@ -314,15 +315,16 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
   const uint8_t* px = piece_of<XF>(p.x, r, p.ldx, t);
   const uint8_t* pd = piece_of<DF>(p.dy, r, p.ld_dy, t);
   const uint8_t* pr = piece_of<XF>(p.r, r, p.ld_r, t);
+  const long long next_x = step * p.ldx * (XF ? 4 : 2), next_d = step * p.ld_dy * (DF ? 4 : 2), next_r = step * p.ld_r * (XF ? 4 : 2);
   int left = r < p.rows ? (int)((p.rows - r - 1) / step) + 1 : 0;  // rows to be fetched
   auto fetch = [&](int stage) {
     if (left > 0) {
       ax.fetch(stage, px, pieces, T);
       ad.fetch(stage, pd, pieces, T);
       if (p.r) ar.fetch(stage, pr, pieces, T);
-      px += step * p.ldx * (XF ? 4 : 2);
-      pd += step * p.ld_dy * (DF ? 4 : 2);
-      pr += step * p.ld_r * (XF ? 4 : 2);
+      px += next_x;
+      pd += next_d;
+      pr += next_r;
       --left;
     }
     fetched();
@@ -330,6 +332,16 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
   if constexpr (VEC)
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) fetch(i);
+  ops::f32x2 w[V][4];
+  auto weights = [&](int j) {
+    float v[8];
+    load_weight<VEC>(p.w, p.w_f32, v, j, p.cols, t, T);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[j][i] = ops::pair2(v[2 * i], v[2 * i + 1]);
+  };
+  if constexpr (HELD)
+#pragma unroll
+    for (int j = 0; j < V; ++j) weights(j);
   int buf = 0;
   float2 st = r < p.rows ? p.stats[r] : make_float2(0.f, 0.f);
   for (int stage = 0; r < p.rows; r += step, stage = stage + 1 == S ? 0 : stage + 1) {
@@ -352,8 +364,7 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
     ops::f32x2 n[V][4], g[V][4], s1 = 0, s2 = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float w[8];
-      load_weight<VEC>(p.w, p.w_f32, w, j, p.cols, t, T);
+      if constexpr (!HELD) weights(j);
       ops::unpack2(rx[j], n[j]);
       ops::unpack2(rd[j], g[j]);
 #pragma unroll
@@ -361,7 +372,7 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
         n[j][i] = ops::mul2(ops::add2(n[j][i], minus), rstd);
         dw[j][i] = ops::fma2(g[j][i], n[j][i], dw[j][i]);
         db[j][i] = ops::add2(db[j][i], g[j][i]);
-        g[j][i] = ops::mul2(g[j][i], ops::pair2(w[2 * i], w[2 * i + 1]));  // (zero behind the last column)
+        g[j][i] = ops::mul2(g[j][i], w[j][i]);  // (zero behind the last column)
         s1 = ops::add2(s1, g[j][i]);
         s2 = ops::fma2(g[j][i], n[j][i], s2);
       }
@@ -426,16 +437,18 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
   }
 }
 
-// The blocks' sums added up, in their order: 32 columns a block, its warps
-// take every eighth partial.
+// The blocks' sums added up, in a fixed order: 32 columns a block, its warps
+// deal the partials out.  (With 8 warps for hundreds of partials, the loads of 37 or
+// 148 partials in a row took longer than a third of the pass itself.)
 struct Reduce {
   const float* part;
   void* dw;
   void* db;
   int blocks, cols, w_f32, b_f32;
 };
-__global__ void __launch_bounds__(256) reduce(const __grid_constant__ Reduce p) {
-  __shared__ float sh[8][32];
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) reduce(const __grid_constant__ Reduce p) {
+  __shared__ float sh[WARPS][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane, ldp = (p.cols + 7) / 8 * 8;
   void* out = blockIdx.y ? p.db : p.dw;
@@ -445,15 +458,17 @@ __global__ void __launch_bounds__(256) reduce(const __grid_constant__ Reduce p) 
   float s = 0.f;
   if (c < p.cols) {
     const float* q = p.part + blockIdx.y * ldp + c;
-#pragma unroll 8
-    for (int b = warp; b < p.blocks; b += 8) s += __ldcg(q + (long long)b * 2 * ldp);
+#pragma unroll 16
+    for (int b = warp; b < p.blocks; b += WARPS) s += __ldcg(q + (long long)b * 2 * ldp);
   }
   sh[warp][lane] = s;
   __syncthreads();
-  if (warp || c >= p.cols) return;
-#pragma unroll
-  for (int w = 1; w < 8; ++w) s += sh[w][lane];
-  ops::st_any(out, c, s, blockIdx.y ? p.b_f32 : p.w_f32);
+  // a warp adds the warps' sums of its columns
+  for (int i = warp; i < 32; i += WARPS) {
+    const int mine = blockIdx.x * 32 + i;
+    s = ops::warp_sum(lane < WARPS ? sh[lane][i] : 0.f);
+    if (lane == 0 && mine < p.cols) ops::st_any(out, mine, s, blockIdx.y ? p.b_f32 : p.w_f32);
+  }
 }
 
 struct Kernel {
@@ -489,9 +504,17 @@ struct Shape {
   Kernel k;
   int T, per;
 };
-Shape fwd_shape(int cols, bool vec, bool xf, bool yf) {
+// Where there are fewer rows than blocks that run at once, a row has more
+// threads: one piece each.
+Shape fwd_shape(int cols, bool few, bool vec, bool xf, bool yf) {
   if (cols <= 256) return {fwd_of<1, true, 256>(vec, xf, yf), 256, 8};
   if (cols <= 512) return {fwd_of<2, true, 256>(vec, xf, yf), 256, 8};
+  // single elements: a warp's row needs no barrier (1537 x 1001: 4.3 us, with a block's row 5.2)
+  if (!vec && cols <= 1024 && !few)
+    return {xf ? (yf ? fwd<4, false, true, 256, true, true>() : fwd<4, false, true, 256, true, false>())
+               : (yf ? fwd<4, false, true, 256, false, true>() : fwd<4, false, true, 256, false, false>()),
+            256, 8};
+  if (few && cols <= 8192) return {fwd_of<1, false, 1024>(vec, xf, yf), ops::ceil_div(ops::ceil_div(cols, 8), 32) * 32, 1};
   const int T = ops::ceil_div(ops::ceil_div(cols, 16), 32) * 32;
   return {T <= 64    ? fwd_of<2, false, 64>(vec, xf, yf)
           : T <= 128 ? fwd_of<2, false, 128>(vec, xf, yf)
@@ -500,9 +523,10 @@ Shape fwd_shape(int cols, bool vec, bool xf, bool yf) {
                      : fwd_of<2, false, 1024>(vec, xf, yf),
           T, 1};
 }
-Shape bwd_shape(int cols, bool vec, bool xf, bool df) {
+Shape bwd_shape(int cols, bool few, bool vec, bool xf, bool df) {
   if (cols <= 256) return {bwd_of<1, true, 256>(vec, xf, df), 256, 8};
   if (cols <= 512) return {bwd_of<2, true, 256>(vec, xf, df), 256, 8};
+  if (few && cols <= 8192) return {bwd_of<1, false, 1024>(vec, xf, df), ops::ceil_div(ops::ceil_div(cols, 8), 32) * 32, 1};
   const int T = ops::ceil_div(ops::ceil_div(cols, 16), 32) * 32;
   return {T <= 64    ? bwd_of<2, false, 64>(vec, xf, df)
           : T <= 128 ? bwd_of<2, false, 128>(vec, xf, df)
@@ -586,8 +610,8 @@ apk_status forward(apk_norm* h, const apk_norm_io* io) {
   const bool vec = D % 8 == 0 && ops::on16(io->x, io->ldx, M, io->x_dtype) && ops::on16(io->y, io->ldy, M, io->y_dtype) &&
                    ops::aligned(c.weight, 16) && ops::aligned(c.bias, 16);
   const bool xf = io->x_dtype == APK_F32, yf = io->y_dtype == APK_F32;
-  const norm::Shape sh = norm::fwd_shape(D, vec, xf, yf);
-  const int grid = std::min(ops::ceil_div(M, sh.per), h->sms * std::max(1, 512 / sh.T));
+  const norm::Shape sh = norm::fwd_shape(D, M <= h->sms, vec, xf, yf);
+  const int grid = std::min(ops::ceil_div(M, sh.per), h->sms * std::max(1, (sh.k.threads > 512 ? 1024 : 512) / sh.T));
   return launch(h, sh, p, grid, static_cast<cudaStream_t>(io->stream), "launching the layer norm");
 }
 
@@ -634,8 +658,8 @@ apk_status backward(apk_norm* h, const apk_norm_grads* g) {
                    (!g->dx || ops::on16(g->dx, g->ld_dx, M, g->x_dtype)) &&
                    (!g->residual_grad || ops::on16(g->residual_grad, g->ld_residual, M, g->x_dtype)) && ops::aligned(c.weight, 16);
   const bool xf = g->x_dtype == APK_F32, df = g->dy_dtype == APK_F32;
-  const norm::Shape sh = norm::bwd_shape(D, vec, xf, df);
-  const int grid = std::min(ops::ceil_div(M, sh.per), h->sms * std::max(1, 512 / sh.T));
+  const norm::Shape sh = norm::bwd_shape(D, M <= 3 * h->sms, vec, xf, df);
+  const int grid = std::min(ops::ceil_div(M, sh.per), h->sms * std::max(1, (sh.k.threads > 512 ? 1024 : 512) / sh.T));
   const bool sums = g->dw || g->db;
   APK_TRY(h->scratch.enter(s, &h->err));
   ScratchUse use(&h->scratch, &h->err);
@@ -646,8 +670,8 @@ apk_status backward(apk_norm* h, const apk_norm_grads* g) {
   APK_TRY(launch(h, sh, p, grid, s, "launching the layer norm's gradient"));
   if (sums) {
     const norm::Reduce q{p.part, g->dw, g->db, grid, D, c.weight_dtype == APK_F32, c.bias_dtype == APK_F32};
-    Launch l(dim3(ops::ceil_div(D, 32), 2), 256, 0, s);
-    APK_TRY(cu_status(cudaLaunchKernelEx(&l.cfg, norm::reduce, q), "launching the sum of the weight's gradient", &h->err));
+    Launch l(dim3(ops::ceil_div(D, 32), 2), grid > 64 ? 1024 : 256, 0, s);
+    APK_TRY(cu_status(cudaLaunchKernelEx(&l.cfg, grid > 64 ? norm::reduce<32> : norm::reduce<8>, q), "launching the sum of the weight's gradient", &h->err));
   }
   return use.end();
 }
