@@ -38,13 +38,9 @@ struct List {
 };
 // (a launch copies its arguments: few tensors should not pay for many; 32,764 bytes is the most)
 constexpr int FEW = 60, SOME = 350, MANY = 1000;
-struct Head {  // of the scratch
-  unsigned arrived;
-  float c;
-};
 struct Sum {
-  Head* head;
-  double* part;     // one of each block of all launches
+  unsigned* arrived;  // zero between launches; null: the scaling adds the blocks' sums up
+  double* part;       // one of each block of all launches
   float* norm;
   float max_norm;
   unsigned first, blocks;  // of this launch, of all
@@ -139,9 +135,15 @@ __device__ __forceinline__ int find(const List<N>& list, unsigned u) {
   return lo;
 }
 
-// Squares are added in fp32 within a thread's part of a unit (16 or 32 values) and
-// in 64 bits beyond; the last block to arrive adds the blocks' sums in their
-// order.
+// The norm, from all blocks' sums, in their order.
+__device__ __forceinline__ double total_norm(const Sum& p, double (&sh)[8]) {
+  double total = 0.0;
+  for (unsigned i = threadIdx.x; i < p.blocks; i += THREADS) total += __ldcg(p.part + i);
+  return sqrt(block_sum(total, sh));
+}
+// Squares are added in fp32 within a thread's part of a unit (16 or 32 values)
+// and in 64 bits beyond; for the norm alone the last block to arrive adds the
+// blocks' sums.
 template <int N>
 __global__ void __launch_bounds__(THREADS, BLOCKS) norm(const __grid_constant__ List<N> list, const __grid_constant__ Sum p) {
   __shared__ double sh[8], sh2[8];
@@ -190,23 +192,21 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm(const __grid_constant__ 
     }
   }
   total = block_sum(total, sh);
+  if (!p.arrived) {
+    if (threadIdx.x == 0) p.part[p.first + blockIdx.x] = total;
+    return;
+  }
   if (threadIdx.x == 0) {
     p.part[p.first + blockIdx.x] = total;
     __threadfence();
-    last = atomicAdd(&p.head->arrived, 1u) == p.blocks - 1;
-    if (last) p.head->arrived = 0;
+    last = atomicAdd(p.arrived, 1u) == p.blocks - 1;
+    if (last) *p.arrived = 0;
   }
   __syncthreads();
   if (!last) return;
   __threadfence();
-  total = 0.0;
-  for (unsigned i = threadIdx.x; i < p.blocks; i += THREADS) total += __ldcg(p.part + i);
-  total = block_sum(total, sh2);
-  if (threadIdx.x == 0) {
-    const double n = sqrt(total), c = (double)p.max_norm / (n + 1e-6);
-    *p.norm = (float)n;
-    p.head->c = c >= 1.0 ? 1.f : (float)c;  // (a NaN stays one)
-  }
+  const double n = total_norm(p, sh2);
+  if (threadIdx.x == 0) *p.norm = (float)n;
 }
 
 __device__ __forceinline__ void scale_unit(const Tensor& t, unsigned u, float c) {
@@ -258,10 +258,15 @@ __device__ __forceinline__ void scale_unit(const Tensor& t, unsigned u, float c)
 
 // From the last unit to the first: what the norm read last is still in L2.
 template <int N>
-__global__ void __launch_bounds__(THREADS, BLOCKS) scale(const __grid_constant__ List<N> list, const Head* head) {
+__global__ void __launch_bounds__(THREADS, BLOCKS) scale(const __grid_constant__ List<N> list, const __grid_constant__ Sum p) {
+  __shared__ double sh[8];
   pdl_launch();
   pdl_wait();
-  const float c = head->c;
+  // every block adds the sums up for itself: a last block that did it for all
+  // would be 2 us behind the others
+  const double n = total_norm(p, sh), q = (double)p.max_norm / (n + 1e-6);
+  const float c = q >= 1.0 ? 1.f : (float)q;  // (a NaN stays one)
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.norm = (float)n;
   const unsigned run = run_of(list);
   for (unsigned first = blockIdx.x * run; first < list.units; first += gridDim.x * run) {
     int at = find(list, list.units - 1 - first);
@@ -358,8 +363,8 @@ apk_status run(apk_clip* h, const apk_clip_io* io, bool scales, cudaStream_t s) 
   APK_TRY(h->scratch.enter(s, &h->err));
   ScratchUse use(&h->scratch, &h->err);
   APK_TRY(use.begin(256 + ops::up256(blocks * sizeof(double)), 256));
-  clip::Sum sum{reinterpret_cast<clip::Head*>(h->scratch.data()), reinterpret_cast<double*>(h->scratch.data() + 256), io->norm,
-                io->max_norm, 0, blocks};
+  clip::Sum sum{scales ? nullptr : reinterpret_cast<unsigned*>(h->scratch.data()),
+                reinterpret_cast<double*>(h->scratch.data() + 256), io->norm, io->max_norm, 0, blocks};
   for (const auto& l : lists) {
     Launch launch(dim3(grid(l)), clip::THREADS, 0, s);
     APK_TRY(cu_status(cudaLaunchKernelEx(&launch.cfg, clip::norm<N>, l, sum), "launching the norm", &h->err));
@@ -367,9 +372,8 @@ apk_status run(apk_clip* h, const apk_clip_io* io, bool scales, cudaStream_t s) 
   }
   if (scales)
     for (size_t i = lists.size(); i-- > 0;) {
-      if (lists[i].units == 0) continue;
       Launch launch(dim3(grid(lists[i])), clip::THREADS, 0, s);
-      APK_TRY(cu_status(cudaLaunchKernelEx(&launch.cfg, clip::scale<N>, lists[i], (const clip::Head*)sum.head),
+      APK_TRY(cu_status(cudaLaunchKernelEx(&launch.cfg, clip::scale<N>, lists[i], sum),
                         "launching the scaling", &h->err));
     }
   return use.end();

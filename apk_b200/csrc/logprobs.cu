@@ -119,6 +119,21 @@ struct Row {
     else
       r.a = __ldcs(reinterpret_cast<const uint4*>(q));
   }
+  // into a row that starts at `out`, at the same place within the alignment
+  __device__ __forceinline__ void store(int v, uint8_t* out, const ops::Raw<F32>& o) const {
+    const int e = first(v);
+    uint8_t* q = out + (long long)e * (F32 ? 4 : 2);
+    if ((unsigned)v - lo < whole) {
+      __stcs(reinterpret_cast<uint4*>(q), o.a);
+      if constexpr (F32) __stcs(reinterpret_cast<uint4*>(q) + 1, o.b);
+      return;
+    }
+    float y[8];
+    ops::unpack(o, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (e + i >= 0 && e + i < n) ops::st_any(out, e + i, y[i], F32);
+  }
   // -inf where the row does not reach
   __device__ __forceinline__ void load(int v, ops::Raw<F32>& r) const {
     if ((unsigned)v - lo < whole) {
@@ -793,6 +808,10 @@ constexpr int EIGHTS = 4;  // of a thread
 
 // A block takes 8192 values of a row.  SAME: logits and gradient start at the
 // same place within 16 (32) bytes, so that both go by eights.
+//   t = ((x - m) - log S) L,  -dx = 2^t (dlogprob + dentropy (entropy + t ln 2))
+// in pairs of values; masked ones are raised to -1e9 as in the forward pass,
+// and the token's own term is added by the thread that has it.  Rows far out
+// (|m| of 1e8 and more) have x - m limited instead.
 template <bool F32, bool SAME>
 __global__ void __launch_bounds__(THREADS, 4) backward(const __grid_constant__ Grads p) {
   const long long row = blockIdx.x / p.pieces;
@@ -809,42 +828,69 @@ __global__ void __launch_bounds__(THREADS, 4) backward(const __grid_constant__ G
   const float ah = h != 0.f ? fmaf(h, p.entropy[row], a) : a;
   const Row<F32> r(p.x + row * p.ld, p.vocabulary);
   uint8_t* out = p.dx + row * p.ld_d;
-  auto grad = [&](float x, long long i) {
-    const float l = max_nan((x - st.x) - st.y, -1000.f), e = exp_of(l);
-    const float d = -e * fmaf(h, l, ah);
-    return zero ? 0.f : i == token ? d + a : d;
+  const bool usual = st.x > NONE && st.x < MOST;
+  const float s_l = st.y * LOG2E, h_l = h * 0.69314718f;
+  auto grad = [&](float x, long long i) {  // one value, by the same steps
+    float d;
+    if (usual) {
+      const float t = fmaf(max_nan(x, LOWEST) - st.x, LOG2E, -s_l);
+      d = ex2(t) * fmaf(t, -h_l, -ah);
+    } else {
+      const float l = max_nan((x - st.x) - st.y, -1000.f);
+      d = -exp_of(l) * fmaf(h, l, ah);
+    }
+    return i == token ? d + a : d;
   };
   if constexpr (SAME) {
     const int v0 = piece * EIGHTS * THREADS + (int)threadIdx.x, nv = r.eights();
+    if (zero) {
+#pragma unroll
+      for (int j = 0; j < EIGHTS; ++j) {
+        const int v = v0 + j * THREADS;
+        if (v < nv) r.store(v, out, ops::Raw<F32>{});
+      }
+      return;
+    }
     ops::Raw<F32> raw[EIGHTS];
 #pragma unroll
     for (int j = 0; j < EIGHTS; ++j)
-      if (!zero && v0 + j * THREADS < nv) r.load(v0 + j * THREADS, raw[j]);
+      if (v0 + j * THREADS < nv) r.load(v0 + j * THREADS, raw[j]);
+    const ops::f32x2 minus_m = ops::both(-st.x), l2 = ops::both(LOG2E), minus_s = ops::both(-s_l);
+    const ops::f32x2 ht = ops::both(-h_l), minus_a = ops::both(-ah);
 #pragma unroll
     for (int j = 0; j < EIGHTS; ++j) {
       const int v = v0 + j * THREADS;
       if (v >= nv) continue;
       const int e = r.first(v);
-      float x[8];
-      ops::unpack(raw[j], x);
+      float y[8];
+      if (usual) {
+        ops::f32x2 x[4];
+        raised(raw[j], x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = grad(x[i], e + i);
-      if (e >= 0 && e + 8 <= r.n) {
-        ops::Raw<F32> o;
-        ops::pack(x, o);
-        uint4* q = reinterpret_cast<uint4*>(out + (long long)e * (F32 ? 4 : 2));
-        __stcs(q, o.a);
-        if constexpr (F32) __stcs(q + 1, o.b);
+        for (int i = 0; i < 4; ++i) {
+          const ops::f32x2 t = fma2(add2(x[i], minus_m), l2, minus_s);
+          float t0, t1;
+          unpair2(t, t0, t1);
+          unpair2(ops::mul2(pair2(ex2(t0), ex2(t1)), fma2(t, ht, minus_a)), y[2 * i], y[2 * i + 1]);
+        }
+        if (token >= e && token < e + 8) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (token == e + i) y[i] += a;
+        }
       } else {
+        ops::unpack(raw[j], y);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (e + i >= 0 && e + i < r.n) ops::st_any(out, e + i, x[i], F32);
+        for (int i = 0; i < 8; ++i) y[i] = grad(y[i], e + i);
       }
+      ops::Raw<F32> o;
+      ops::pack(y, o);
+      r.store(v, out, o);
     }
   } else {
     const long long e0 = (long long)piece * EIGHTS * ROUND, e1 = min(e0 + EIGHTS * ROUND, (long long)p.vocabulary);
     for (long long e = e0 + threadIdx.x; e < e1; e += THREADS)
-      ops::st_any(out, e, grad(zero ? 0.f : ops::ld_any(p.x + row * p.ld, e, F32), e), F32);
+      ops::st_any(out, e, zero ? 0.f : grad(ops::ld_any(p.x + row * p.ld, e, F32), e), F32);
   }
 }
 

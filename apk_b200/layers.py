@@ -107,11 +107,13 @@ def _like(t, shape):
 
 def _new(t, shape, dtype):
     """A new contiguous tensor on t's device (the way that costs the host least)."""
-    n, strides = 1, []
-    for size in reversed(shape):
-        strides.append(n)
-        n *= size
-    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=t.device)
+    if len(shape) == 2:
+        strides = (shape[1], 1)
+    elif len(shape) == 1:
+        strides = (1,)
+    else:
+        return torch.empty(shape, dtype=dtype, device=t.device)
+    return torch.empty_strided(shape, strides, dtype=dtype, device=t.device)
 
 
 class _Handle:
