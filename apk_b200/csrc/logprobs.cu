@@ -16,8 +16,8 @@
 // are raised to -1e9, which leaves them 2^t = 0 without a 0 * inf; rows whose
 // maximum is not between -1e8 and 1e8 are taken again, step by step.
 //
-// The alternatives come out of the same pass.  The first round of 2048 values
-// gives a bound that its k-th largest value reaches; a value that reaches the
+// The alternatives come out of the same pass.  The first rounds of 2048 values,
+// as many as are on their way, give a bound that their k-th largest value reaches; a value that reaches the
 // bound is put into a buffer in shared memory.  As rounds go by, one warp at a
 // time raises the bound by what the buffer holds, while the others go on: any
 // bound that k values reach is right, so nobody waits for anybody.  Between n
@@ -35,7 +35,7 @@ namespace apk {
 namespace logp {
 
 constexpr int THREADS = 256, ROUND = THREADS * 8;  // values of a block's round
-constexpr int MAX_TOP = 32, MAX_SPLIT = 64;
+constexpr int MAX_TOP = 32, MAX_SPLIT = 16;
 constexpr int ROOM = ROUND + MAX_TOP;              // of the buffer: the list, and a whole round
 template <bool F32>
 constexpr int AHEAD = F32 ? 2 : 4;                 // eights of a thread on their way
@@ -43,7 +43,7 @@ constexpr float LOWEST = -1e9f;                    // (as bf16: 0xCE6E)
 // The running maximum before the first value, and where it ends: there c is
 // rounded to steps of 16, and 2^t of the maximum itself stays below 2^8.
 constexpr float NONE = -1e8f, MOST = 1e8f;
-static_assert(MAX_SPLIT * MAX_TOP <= ROOM, "the splits' lists fit the buffer");
+static_assert(MAX_SPLIT * MAX_TOP <= ROOM, "the parts' lists fit the buffer");
 
 struct Params {
   const uint8_t* x;
@@ -54,9 +54,6 @@ struct Params {
   int* ids;
   float* tops;
   float2* stats;
-  float4* part;      // [row][split] m, sum 2^t, sum 2^t t
-  unsigned long long* lists;  // [row][split][top]
-  unsigned* arrived; // [row], zero between launches
   int rows, vocabulary, top, split, tokens_64;
 };
 
@@ -249,36 +246,10 @@ struct Shared {
   unsigned long long list[MAX_TOP];
   float m[8], s[8], u[8];
   int count;
-  bool last;
+  // of a row's first block: the parts' results
+  unsigned long long lists[MAX_SPLIT * MAX_TOP];
+  float4 parts[MAX_SPLIT];
 };
-
-// Over the block: every thread gets the row's.
-__device__ __forceinline__ Soft join(Soft a, Shared& sh) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float m = a.m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  __syncthreads();  // (who reads an earlier result is done)
-  if (lane == 0) sh.m[warp] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) m = fmaxf(m, sh.m[w]);
-  a.raise(m);
-  a.s = ops::warp_sum(a.s);
-  a.u = ops::warp_sum(a.u);
-  if (lane == 0) {
-    sh.s[warp] = a.s;
-    sh.u[warp] = a.u;
-  }
-  __syncthreads();
-  a.s = a.u = 0.f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    a.s += sh.s[w];
-    a.u += sh.u[w];
-  }
-  return a;
-}
 
 // A row's maximum, log of the sum of exp(x - m), and entropy.
 struct Result {
@@ -379,17 +350,20 @@ __device__ __forceinline__ void put_from(const ops::Raw<F32>& raw, int e, int n,
     if (key >= limit && e + i >= 0 && e + i < n) put(key);
   }
 }
+// The best of eight values, the first of index e; 0 if none lies in the row.
 template <bool F32>
 __device__ __forceinline__ unsigned long long best_of(const ops::Raw<F32>& raw, int e, int n) {
   float x[8];
   ops::unpack(raw, x);
-  unsigned long long best = 0;
+  const float most =
+      max_nan(max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3])), max_nan(max_nan(x[4], x[5]), max_nan(x[6], x[7])));
+  unsigned which = 0, in = 0xFF;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const unsigned long long key = e + i >= 0 && e + i < n ? key_of(x[i], e + i) : 0;
-    best = key > best ? key : best;
-  }
-  return best;
+  for (int i = 0; i < 8; ++i) which |= x[i] == most || x[i] != x[i] ? 1u << i : 0u;  // (a NaN is the largest)
+  if (e < 0) in &= 0xFFu << -e;
+  if (e + 8 > n) in &= e < n ? 0xFFu >> (e + 8 - n) : 0u;
+  which &= in;  // (behind the row's ends are -infs: where they are the largest, all in the row are)
+  return which ? key_of(most, e + __ffs(which) - 1) : 0;
 }
 // One warp: the bound raised to the k-th largest of what its lanes see, each
 // the largest of every 32nd value in the buffer (fewer than k lanes with any: not).
@@ -442,7 +416,8 @@ __device__ __noinline__ unsigned long long cut(int k, Shared& sh) {
   return c >= k ? sh.list[k - 1] : 0;
 }
 
-// The same by one warp, for the end of a row: lane i gets the i-th largest.
+// The same by one warp, for the end of a row: lane i gets the i-th largest, or
+// 0 where there are fewer.
 // (The block's way costs four barriers with all warps behind them.)
 __device__ __forceinline__ unsigned long long cut_by_warp(int k, Shared& sh) {
   const int lane = threadIdx.x & 31, c = sh.count;
@@ -468,7 +443,7 @@ __device__ __forceinline__ unsigned long long cut_by_warp(int k, Shared& sh) {
     if (rank < k) sh.list[rank] = mine;
   }
   __syncwarp();
-  return lane < k ? sh.list[lane] : 0;
+  return lane < min(n, k) ? sh.list[lane] : 0;
 }
 
 __device__ __forceinline__ long long token_of(const Params& p, long long row) {
@@ -612,13 +587,15 @@ __global__ void __launch_bounds__(THREADS) short_rows(const __grid_constant__ Pa
   finish<TOP>(p, row, token, at_token, res, key);
 }
 
-// One row, or one of p.split parts of it, a block.
+// One row, or one of p.split parts of it, a block: few rows have a cluster each.
 template <bool F32, bool TOP>
 __global__ void __launch_bounds__(THREADS, 4) forward(const __grid_constant__ Params p) {
   __shared__ Shared sh;
   const int tid = threadIdx.x;
   const long long row = blockIdx.x / p.split;
   const int part = blockIdx.x - (int)(row * p.split);
+  // (the parts write into the first one's shared memory: it has to have begun by then)
+  if (p.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_launch();
   pdl_wait();
   const uint8_t* px = p.x + row * p.ld;
@@ -663,8 +640,14 @@ __global__ void __launch_bounds__(THREADS, 4) forward(const __grid_constant__ Pa
       sh.count = 0;
       sh.limit = 0;
     }
-    // the first round's own bound (a barrier is in it, behind the clearing)
-    const unsigned long long best = mine < v1 ? best_of(ring[0], r.first(mine), p.vocabulary) : 0;
+    // the first rounds' own bound (a barrier is in it, behind the clearing)
+    unsigned long long best = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int v = mine + i * THREADS;
+      const unsigned long long one = v < v1 ? best_of(ring[i], r.first(v), p.vocabulary) : 0;
+      best = one > best ? one : best;
+    }
     follow(bound_of(best, p.top, sh));
     if (tid == 0) atomicMax(&sh.limit, bound);
   }
@@ -708,89 +691,82 @@ __global__ void __launch_bounds__(THREADS, 4) forward(const __grid_constant__ Pa
         bound = cut(p.top, sh);
       }
       __syncthreads();
-    } else if (p.split > 1) {
-      cut(p.top, sh);
     }
   }
+  // the rest is one warp's: the block's sums and its k largest
   Soft soft = sums.soft();
-  if (p.split == 1) {  // the rest is one warp's
-    float m = soft.m;
+  float m = soft.m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    soft.raise(m);
-    soft.s = ops::warp_sum(soft.s);
-    soft.u = ops::warp_sum(soft.u);
-    if ((tid & 31) == 0) {
-      sh.m[tid >> 5] = soft.m;
-      sh.s[tid >> 5] = soft.s;
-      sh.u[tid >> 5] = soft.u;
-    }
-    __syncthreads();
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  soft.raise(m);
+  soft.s = ops::warp_sum(soft.s);
+  soft.u = ops::warp_sum(soft.u);
+  if ((tid & 31) == 0) {
+    sh.m[tid >> 5] = soft.m;
+    sh.s[tid >> 5] = soft.s;
+    sh.u[tid >> 5] = soft.u;
+  }
+  __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) m = fmaxf(m, sh.m[w]);
-    const bool usual = m > NONE && m < MOST;
-    Result res = {};
-    if (!usual) {
-      __syncthreads();  // (it uses sh.m)
-      res = far_out<F32>(px, p.vocabulary, sh);
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, sh.m[w]);
+  Soft all;
+  unsigned long long key = 0;
+  if (tid < 32) {
+    if (tid < 8) {
+      all.m = sh.m[tid];
+      all.s = sh.s[tid];
+      all.u = sh.u[tid];
     }
-    if (tid >= 32) return;
-    if (usual) {
-      Soft all;
-      if (tid < 8) {
-        all.m = sh.m[tid];
-        all.s = sh.s[tid];
-        all.u = sh.u[tid];
+    all.raise(m);
+    all.s = ops::warp_sum(all.s);
+    all.u = ops::warp_sum(all.u);
+    if constexpr (TOP) key = cut_by_warp(p.top, sh);
+  }
+  if (p.split > 1) {  // the parts meet in the first one's shared memory
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (tid < 32) {
+      uint32_t to;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&sh.parts[part])), "r"(0));
+      if (tid == 0)
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(all.m), "f"(all.s), "f"(all.u), "f"(0.f) : "memory");
+      if constexpr (TOP) {
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&sh.lists[part * p.top])), "r"(0));
+        if (tid < p.top) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + tid * 8), "l"(key) : "memory");
+      }
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (part != 0) return;
+    for (int i = 0; i < p.split; ++i) m = fmaxf(m, sh.parts[i].x);
+    if (tid < 32) {
+      all = Soft();
+      if (tid < p.split) {
+        all.m = sh.parts[tid].x;
+        all.s = sh.parts[tid].y;
+        all.u = sh.parts[tid].z;
       }
       all.raise(m);
       all.s = ops::warp_sum(all.s);
       all.u = ops::warp_sum(all.u);
-      res = result_of(all);
-    }
-    unsigned long long key = 0;
-    if constexpr (TOP) key = cut_by_warp(p.top, sh);
-    finish<TOP>(p, row, token, at_token, res, key);
-    return;
-  }
-  soft = join(soft, sh);
-  if (p.split > 1) {
-    const long long at = row * p.split + part;
-    if constexpr (TOP)
-      if (tid < p.top) p.lists[at * p.top + tid] = tid < sh.count ? sh.list[tid] : 0;
-    if (tid == 0) p.part[at] = make_float4(soft.m, soft.s, soft.u, 0.f);
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-      sh.last = atomicAdd(&p.arrived[row], 1u) == (unsigned)p.split - 1;
-      if (sh.last) p.arrived[row] = 0;
-    }
-    __syncthreads();
-    if (!sh.last) return;
-    __threadfence();
-    Soft mine;
-    if (tid < p.split) {
-      const float4 v = __ldcg(p.part + row * p.split + tid);
-      mine.m = v.x;
-      mine.s = v.y;
-      mine.u = v.z;
-    }
-    soft = join(mine, sh);
-    if constexpr (TOP) {
-      if (tid == 0) sh.count = 0;
-      __syncthreads();
-      for (int i = tid; i < p.split * p.top; i += THREADS) {
-        const unsigned long long key = __ldcg(p.lists + row * p.split * p.top + i);
-        if (key) put(key, sh);
+      if constexpr (TOP) {
+        const int n = p.split * p.top;  // (0s, of parts with fewer values, are below every bound)
+        for (int i = tid; i < n; i += 32) sh.buf[i] = sh.lists[i];
+        if (tid == 0) sh.count = n;
+        __syncwarp();
+        key = cut_by_warp(p.top, sh);
       }
-      cut(p.top, sh);
     }
   }
-  const bool usual = soft.m > NONE && soft.m < MOST;
+  const bool usual = m > NONE && m < MOST;
   Result res = {};
-  if (!usual) res = far_out<F32>(px, p.vocabulary, sh);
+  if (!usual) {
+    __syncthreads();  // (it uses sh.m)
+    res = far_out<F32>(px, p.vocabulary, sh);
+  }
   if (tid >= 32) return;
-  if (usual) res = result_of(soft);
-  finish<TOP>(p, row, token, at_token, res, TOP && tid < p.top ? sh.list[tid] : 0);
+  if (usual) res = result_of(all);
+  finish<TOP>(p, row, token, at_token, res, key);
 }
 
 struct Grads {
@@ -812,12 +788,15 @@ constexpr int EIGHTS = 4;  // of a thread
 // in pairs of values; masked ones are raised to -1e9 as in the forward pass,
 // and the token's own term is added by the thread that has it.  Rows far out
 // (|m| of 1e8 and more) have x - m limited instead.
+// p.pieces of 0: rows are short, and a warp's each.
 template <bool F32, bool SAME>
 __global__ void __launch_bounds__(THREADS, 4) backward(const __grid_constant__ Grads p) {
-  const long long row = blockIdx.x / p.pieces;
-  const int piece = blockIdx.x - (int)(row * p.pieces);
+  const int T = p.pieces ? THREADS : 32, t = threadIdx.x & (T - 1);
+  const long long row = p.pieces ? blockIdx.x / p.pieces : (long long)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+  const int piece = p.pieces ? blockIdx.x - (int)(row * p.pieces) : 0;
   pdl_launch();
   pdl_wait();
+  if (row >= p.rows) return;
   long long token = -1;
   if (p.tokens) token = p.tokens_64 ? static_cast<const long long*>(p.tokens)[row] : (long long)static_cast<const int*>(p.tokens)[row];
   float a = p.dlogprob && token >= 0 ? p.dlogprob[row] : 0.f;
@@ -842,54 +821,52 @@ __global__ void __launch_bounds__(THREADS, 4) backward(const __grid_constant__ G
     return i == token ? d + a : d;
   };
   if constexpr (SAME) {
-    const int v0 = piece * EIGHTS * THREADS + (int)threadIdx.x, nv = r.eights();
+    const int first = piece * EIGHTS * THREADS + t, end = p.pieces ? min(first + EIGHTS * THREADS, r.eights()) : r.eights();
     if (zero) {
-#pragma unroll
-      for (int j = 0; j < EIGHTS; ++j) {
-        const int v = v0 + j * THREADS;
-        if (v < nv) r.store(v, out, ops::Raw<F32>{});
-      }
+      for (int v = first; v < end; v += T) r.store(v, out, ops::Raw<F32>{});
       return;
     }
-    ops::Raw<F32> raw[EIGHTS];
-#pragma unroll
-    for (int j = 0; j < EIGHTS; ++j)
-      if (v0 + j * THREADS < nv) r.load(v0 + j * THREADS, raw[j]);
     const ops::f32x2 minus_m = ops::both(-st.x), l2 = ops::both(LOG2E), minus_s = ops::both(-s_l);
     const ops::f32x2 ht = ops::both(-h_l), minus_a = ops::both(-ah);
+    for (int v0 = first; v0 < end; v0 += EIGHTS * T) {
+      ops::Raw<F32> raw[EIGHTS];
 #pragma unroll
-    for (int j = 0; j < EIGHTS; ++j) {
-      const int v = v0 + j * THREADS;
-      if (v >= nv) continue;
-      const int e = r.first(v);
-      float y[8];
-      if (usual) {
-        ops::f32x2 x[4];
-        raised(raw[j], x);
+      for (int j = 0; j < EIGHTS; ++j)
+        if (v0 + j * T < end) r.load(v0 + j * T, raw[j]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const ops::f32x2 t = fma2(add2(x[i], minus_m), l2, minus_s);
-          float t0, t1;
-          unpair2(t, t0, t1);
-          unpair2(ops::mul2(pair2(ex2(t0), ex2(t1)), fma2(t, ht, minus_a)), y[2 * i], y[2 * i + 1]);
+      for (int j = 0; j < EIGHTS; ++j) {
+        const int v = v0 + j * T;
+        if (v >= end) continue;
+        const int e = r.first(v);
+        float y[8];
+        if (usual) {
+          ops::f32x2 x[4];
+          raised(raw[j], x);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const ops::f32x2 t2 = fma2(add2(x[i], minus_m), l2, minus_s);
+            float t0, t1;
+            unpair2(t2, t0, t1);
+            unpair2(ops::mul2(pair2(ex2(t0), ex2(t1)), fma2(t2, ht, minus_a)), y[2 * i], y[2 * i + 1]);
+          }
+          if (token >= e && token < e + 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (token == e + i) y[i] += a;
+          }
+        } else {
+          ops::unpack(raw[j], y);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = grad(y[i], e + i);
         }
-        if (token >= e && token < e + 8) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (token == e + i) y[i] += a;
-        }
-      } else {
-        ops::unpack(raw[j], y);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = grad(y[i], e + i);
+        ops::Raw<F32> o;
+        ops::pack(y, o);
+        r.store(v, out, o);
       }
-      ops::Raw<F32> o;
-      ops::pack(y, o);
-      r.store(v, out, o);
     }
   } else {
     const long long e0 = (long long)piece * EIGHTS * ROUND, e1 = min(e0 + EIGHTS * ROUND, (long long)p.vocabulary);
-    for (long long e = e0 + threadIdx.x; e < e1; e += THREADS)
+    for (long long e = e0 + t; e < e1; e += T)
       ops::st_any(out, e, zero ? 0.f : grad(ops::ld_any(p.x + row * p.ld, e, F32), e), F32);
   }
 }
@@ -902,7 +879,7 @@ using namespace apk;
 struct apk_logprobs {
   apk_logprobs_config cfg{};
   Err err;
-  int sms = 0;
+  int sms = 0, most_split = 8;
   Scratch scratch;
   std::mutex mu;
 };
@@ -915,6 +892,17 @@ apk_status create(const apk_logprobs_config* cfg, apk_logprobs* h) {
     return h->err.fail(APK_EINVAL, "top is %d: 0 to %d", h->cfg.top, logp::MAX_TOP);
   APK_TRY(ops::open_device(h->cfg.device, &h->sms, &h->err));
   DeviceGuard guard(h->cfg.device);
+  // clusters of 16, where the device has room for one
+  int fit = 1 << 20;
+  for (const void* f : {reinterpret_cast<const void*>(&logp::forward<false, false>), reinterpret_cast<const void*>(&logp::forward<false, true>),
+                        reinterpret_cast<const void*>(&logp::forward<true, false>), reinterpret_cast<const void*>(&logp::forward<true, true>)}) {
+    APK_TRY(cu_status(cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "preparing the log probabilities", &h->err));
+    Launch l(dim3(logp::MAX_SPLIT), logp::THREADS, 0, nullptr, logp::MAX_SPLIT);
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, f, &l.cfg) != cudaSuccess) cudaGetLastError();
+    fit = std::min(fit, n);
+  }
+  if (fit >= 1) h->most_split = logp::MAX_SPLIT;
   return h->scratch.open(h->cfg.device, &h->err);
 }
 
@@ -960,16 +948,8 @@ apk_status forward(apk_logprobs* h, const apk_logprobs_io* io) {
   p.vocabulary = V;
   p.top = k;
   // parts of at least a round each, while the rows alone leave places empty
-  p.split = std::max(1, std::min({logp::MAX_SPLIT, V / logp::ROUND, 2 * h->sms / M}));
-  APK_TRY(h->scratch.enter(s, &h->err));
-  ScratchUse use(&h->scratch, &h->err);
-  if (p.split > 1) {
-    const size_t zeroed = ops::up256((size_t)2 * h->sms * 4), parts = (size_t)M * p.split;
-    APK_TRY(use.begin(zeroed + ops::up256(parts * 16) + parts * k * 8, zeroed));
-    p.arrived = reinterpret_cast<unsigned*>(h->scratch.data());
-    p.part = reinterpret_cast<float4*>(h->scratch.data() + zeroed);
-    p.lists = reinterpret_cast<unsigned long long*>(h->scratch.data() + zeroed + ops::up256(parts * 16));
-  }
+  p.split = 1;
+  while (2 * p.split <= h->most_split && 2ll * p.split * M <= 2 * h->sms && 2 * p.split <= V / logp::ROUND) p.split *= 2;
   const bool f = io->dtype == APK_F32;
   if (V <= logp::SHORT - 7) {  // (and up to 7 places before the row)
     const auto rows = k ? (f ? short_of<true, true>(V) : short_of<false, true>(V))
@@ -979,9 +959,8 @@ apk_status forward(apk_logprobs* h, const apk_logprobs_io* io) {
   }
   const auto kernel = k ? (f ? logp::forward<true, true> : logp::forward<false, true>)
                         : (f ? logp::forward<true, false> : logp::forward<false, false>);
-  Launch l(dim3(M * p.split), logp::THREADS, 0, s);
-  APK_TRY(cu_status(cudaLaunchKernelEx(&l.cfg, kernel, p), "launching the log probabilities", &h->err));
-  return use.end();
+  Launch l(dim3(M * p.split), logp::THREADS, 0, s, p.split);
+  return cu_status(cudaLaunchKernelEx(&l.cfg, kernel, p), "launching the log probabilities", &h->err);
 }
 
 apk_status backward(apk_logprobs* h, const apk_logprobs_grads* g) {
@@ -1013,13 +992,15 @@ apk_status backward(apk_logprobs* h, const apk_logprobs_grads* g) {
   p.rows = M;
   p.vocabulary = V;
   p.pieces = (int)(((long long)V + 7 + logp::EIGHTS * logp::ROUND - 1) / (logp::EIGHTS * logp::ROUND));
+  const bool rows = V <= logp::SHORT;
+  if (rows) p.pieces = 0;
   if ((long long)M * p.pieces > 0x7FFFFFFFll) return h->err.fail(APK_EINVAL, "%d rows of %d are too many for a launch", M, V);
   const bool same = (reinterpret_cast<uintptr_t>(p.x) - reinterpret_cast<uintptr_t>(p.dx)) % align == 0 &&
                     (M == 1 || (p.ld - p.ld_d) % align == 0);
   const bool f = g->dtype == APK_F32;
   const auto kernel = same ? (f ? logp::backward<true, true> : logp::backward<false, true>)
                            : (f ? logp::backward<true, false> : logp::backward<false, false>);
-  Launch l(dim3(M * p.pieces), logp::THREADS, 0, static_cast<cudaStream_t>(g->stream));
+  Launch l(dim3(rows ? ops::ceil_div(M, logp::THREADS / 32) : M * p.pieces), logp::THREADS, 0, static_cast<cudaStream_t>(g->stream));
   return cu_status(cudaLaunchKernelEx(&l.cfg, kernel, p), "launching the log probabilities' gradient", &h->err);
 }
 
