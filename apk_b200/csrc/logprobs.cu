@@ -297,6 +297,16 @@ __device__ __noinline__ Result far_out(const uint8_t* x, int n, Shared& sh) {
 
 // The k-th largest of a warp's keys; 0 if fewer lanes have any.
 __device__ __forceinline__ unsigned long long kth_of(unsigned long long key, int k) {
+  if (k > 8) {  // by every lane's rank: 32 steps that do not wait for one another
+    const int lane = threadIdx.x & 31;
+    int rank = 0;
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i) {
+      const unsigned long long other = __shfl_sync(0xFFFFFFFFu, key, i);
+      rank += other > key || (other == key && i < lane);  // (equal ones are 0s)
+    }
+    return __shfl_sync(0xFFFFFFFFu, key, __ffs(__ballot_sync(0xFFFFFFFFu, rank == k - 1)) - 1);
+  }
   const uint32_t low = (uint32_t)key;
   uint32_t left = (uint32_t)(key >> 32), top;
   while (true) {  // values from above, those that are equal at once
