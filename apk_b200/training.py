@@ -18,7 +18,7 @@ from . import _lib as L
 from .layers import _ANY, _CODE, _Handle, _like, _new, _overlap, _raw_stream, _rows, _tensor
 
 _TYPES = set(_ANY)
-_dtype = operator.attrgetter("dtype")
+_dtype, _shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
 _data_ptr, _numel, _get_device, _is_contiguous = (
     torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous)
 
@@ -63,19 +63,20 @@ class GradClip(_Handle):
         self._io_ref = ctypes.byref(self._io)
 
     def _check_list(self, tensors, what):
+        """Their types, and whether all are contiguous."""
         # the usual case in few steps: there may be hundreds of them
         try:
             kinds = list(map(_dtype, tensors))
             if (set(map(_get_device, tensors)) <= {self._index} and set(kinds) <= _TYPES
                     and all(map(_is_contiguous, tensors))):
-                return kinds
+                return kinds, True
         except (AttributeError, RuntimeError, TypeError):
             pass
         for i, t in enumerate(tensors):
             _tensor(t, f"{what}[{i}]", self.device, _ANY)
             if not _dense(t):
                 raise ValueError(f"{what}[{i}], of strides {t.stride()}, is not dense in memory")
-        return list(map(_dtype, tensors))
+        return list(map(_dtype, tensors)), False
 
     def _run(self, grads, out, function):
         grads = list(grads)
@@ -85,14 +86,15 @@ class GradClip(_Handle):
                 raise ValueError(f"{len(out)} tensors in out for {len(grads)} gradients")
             out = [o for o, t in zip(out, grads) if t is not None]
         grads = [t for t in grads if t is not None]
-        kinds = self._check_list(grads, "grads")
+        kinds, plain = self._check_list(grads, "grads")
         if out is not None:
-            self._check_list(out, "out")
-            for i, (t, o) in enumerate(zip(grads, out)):
-                if t.shape != o.shape or t.dtype != o.dtype:
-                    raise ValueError(f"out[{i}] is {o.dtype} {tuple(o.shape)}, its gradient {t.dtype} {tuple(t.shape)}")
-                if t.stride() != o.stride() and not (t.is_contiguous() and o.is_contiguous()):
-                    raise ValueError(f"out[{i}] has strides {o.stride()}, its gradient {t.stride()}")
+            to, both = self._check_list(out, "out")
+            if to != kinds or not (plain and both) or list(map(_shape, out)) != list(map(_shape, grads)):
+                for i, (t, o) in enumerate(zip(grads, out)):
+                    if t.shape != o.shape or t.dtype != o.dtype:
+                        raise ValueError(f"out[{i}] is {o.dtype} {tuple(o.shape)}, its gradient {t.dtype} {tuple(t.shape)}")
+                    if t.stride() != o.stride() and not (t.is_contiguous() and o.is_contiguous()):
+                        raise ValueError(f"out[{i}] has strides {o.stride()}, its gradient {t.stride()}")
         norm = torch.empty_strided((), (), dtype=torch.float32, device=self.device)
         at = array.array("q", list(map(_data_ptr, grads)))
         to = at if out is None else array.array("q", list(map(_data_ptr, out)))
