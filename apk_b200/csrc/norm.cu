@@ -36,7 +36,10 @@ struct Params {
   const void* r;     // residual gradient, or null
   void* y;           // y, or dx (null: not wanted)
   float2* stats;
-  float* part;       // [blocks][dw, db][cols rounded up to 8]
+  float* part;       // [blocks][dw, db][cols rounded up to 8], or null
+  void* dw;          // few rows: written by blocks of their own, from row_blocks on
+  void* db;
+  int row_blocks;
   long long ldx, ld_dy, ld_r, ldy;
   int rows, cols;
   float eps, per_col;  // 1 / cols
@@ -292,7 +295,40 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) forward(const __
   }
 }
 
-// A block takes every gridDim-th row (of eight, with WARP) and keeps its
+// Few rows: eight columns of the weight's gradient a block, its threads deal the
+// rows out by eights of lanes.  The statistics are given, so that this needs
+// nothing of dx, and the whole pass is one launch without scratch.
+template <bool XF, bool DF>
+__device__ __forceinline__ void columns(const Params& p) {
+  __shared__ float sh[2][32][8];
+  const int t = threadIdx.x, c = ((int)blockIdx.x - p.row_blocks) * 8 + (t & 7), groups = blockDim.x >> 3;
+  float w = 0.f, b = 0.f;
+  if (c < p.cols)
+#pragma unroll 8
+    for (int r = t >> 3; r < p.rows; r += groups) {
+      const float2 st = p.stats[r];
+      const float d = ops::ld_any(p.dy, r * p.ld_dy + c, DF);
+      w = fmaf(d, (ops::ld_any(p.x, r * p.ldx + c, XF) - st.x) * st.y, w);
+      b += d;
+    }
+#pragma unroll
+  for (int o = 16; o >= 8; o >>= 1) {
+    w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
+    b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
+  }
+  if ((t & 31) < 8) {
+    sh[0][t >> 5][t & 7] = w;
+    sh[1][t >> 5][t & 7] = b;
+  }
+  __syncthreads();
+  if (t >= 16 || c >= p.cols) return;
+  float s = 0.f;
+  for (int i = 0; i < (int)blockDim.x / 32; ++i) s += sh[t >> 3][i][t & 7];
+  if (t < 8 && p.dw) ops::st_any(p.dw, c, s, p.w_f32);
+  if (t >= 8 && p.db) ops::st_any(p.db, c, s, p.b_f32);
+}
+
+// A block takes every row_blocks-th row (of eight, with WARP) and keeps its
 // columns' sums of dy n and dy in registers; they are written once, for
 // reduce().  T_: the most threads of a block, of which an SM takes 512.
 template <int V, bool VEC, bool WARP, bool XF, bool DF, int T_>
@@ -308,10 +344,15 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
   const Ahead<V, XF, S> ar{ad.at + S * ad.SLOTS * blockDim.x * 16, (int)blockDim.x};
   const int pieces = t * 8 < p.cols ? (p.cols - t * 8 - 1) / (T * 8) + 1 : 0;
   ops::f32x2 dw[V][4] = {}, db[V][4] = {};
-  const long long step = (long long)gridDim.x * per;
+  const long long step = (long long)p.row_blocks * per;
   long long r = (long long)blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0);
   pdl_launch();
   pdl_wait();
+  if constexpr (T_ > 512 && V == 1)
+    if ((int)blockIdx.x >= p.row_blocks) {
+      columns<XF, DF>(p);
+      return;
+    }
   const uint8_t* px = piece_of<XF>(p.x, r, p.ldx, t);
   const uint8_t* pd = piece_of<DF>(p.dy, r, p.ld_dy, t);
   const uint8_t* pr = piece_of<XF>(p.r, r, p.ld_r, t);
@@ -524,9 +565,9 @@ Shape fwd_shape(int cols, bool few, bool vec, bool xf, bool yf) {
           T, 1};
 }
 Shape bwd_shape(int cols, bool few, bool vec, bool xf, bool df) {
+  if (few) return {bwd_of<1, false, 1024>(vec, xf, df), std::max(128, ops::ceil_div(ops::ceil_div(cols, 8), 32) * 32), 1};
   if (cols <= 256) return {bwd_of<1, true, 256>(vec, xf, df), 256, 8};
   if (cols <= 512) return {bwd_of<2, true, 256>(vec, xf, df), 256, 8};
-  if (few && cols <= 8192) return {bwd_of<1, false, 1024>(vec, xf, df), ops::ceil_div(ops::ceil_div(cols, 8), 32) * 32, 1};
   const int T = ops::ceil_div(ops::ceil_div(cols, 16), 32) * 32;
   return {T <= 64    ? bwd_of<2, false, 64>(vec, xf, df)
           : T <= 128 ? bwd_of<2, false, 128>(vec, xf, df)
@@ -658,9 +699,18 @@ apk_status backward(apk_norm* h, const apk_norm_grads* g) {
                    (!g->dx || ops::on16(g->dx, g->ld_dx, M, g->x_dtype)) &&
                    (!g->residual_grad || ops::on16(g->residual_grad, g->ld_residual, M, g->x_dtype)) && ops::aligned(c.weight, 16);
   const bool xf = g->x_dtype == APK_F32, df = g->dy_dtype == APK_F32;
-  const norm::Shape sh = norm::bwd_shape(D, M <= 3 * h->sms, vec, xf, df);
+  // (64 x 8192 would take 11.6 us so, and takes 10.1; 128 x 4096 5.0 against 7.6, 333 x 1001 5.3 against 9.7)
+  const bool few = M <= 3 * h->sms && D <= 4096;
+  const norm::Shape sh = norm::bwd_shape(D, few, vec, xf, df);
   const int grid = std::min(ops::ceil_div(M, sh.per), h->sms * std::max(1, (sh.k.threads > 512 ? 1024 : 512) / sh.T));
   const bool sums = g->dw || g->db;
+  p.row_blocks = g->dx || !few ? grid : 0;
+  if (few) {
+    p.dw = g->dw;
+    p.db = g->db;
+    p.b_f32 = c.bias_dtype == APK_F32;
+    return launch(h, sh, p, p.row_blocks + (sums ? ops::ceil_div(D, 8) : 0), s, "launching the layer norm's gradient");
+  }
   APK_TRY(h->scratch.enter(s, &h->err));
   ScratchUse use(&h->scratch, &h->err);
   if (sums) {

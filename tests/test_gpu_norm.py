@@ -114,6 +114,21 @@ def test_shapes(M, D, types):
     _check_backward(norm, x, _rand(M, D, seed=D + 4, dtype=other), stats, res)
 
 
+# more rows than go by the gradient's form for few (three an SM)
+MANY = [(500, 1), (460, 7), (500, 255), (450, 256), (600, 264), (449, 512), (500, 520), (450, 1000), (446, 1024), (470, 1032),
+        (600, 2056), (446, 4096), (450, 4099), (460, 4104), (446, 8191), (500, 8192), (449, 16383), (446, 16384)]
+
+
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(map(str, t)))
+@pytest.mark.parametrize("M,D", MANY)
+def test_shapes_of_many_rows(M, D, types):
+    xt, w, other, bias = types
+    norm = _make(D, w, bias, other, seed=D)
+    x = _rand(M, D, seed=D + 3, scale=2.0, mean=0.5, dtype=xt)
+    stats = _check_forward(norm, x)
+    _check_backward(norm, x, _rand(M, D, seed=D + 4, dtype=other), stats, _rand(M, D, seed=D + 5, dtype=xt) if D % 3 else None)
+
+
 @pytest.mark.parametrize("D", [64, 1001, 2048])
 def test_many_rows(D):
     norm = _make(D)
@@ -188,10 +203,11 @@ def test_leading_axes_and_in_place():
         assert torch.equal(norm.forward(x, out=x), want)
 
 
-def test_parts_of_the_gradient_and_no_rows():
+@pytest.mark.parametrize("M,D", [(21, 96), (500, 96), (30, 1500), (600, 1500)])
+def test_parts_of_the_gradient_and_no_rows(M, D):
     import torch
-    norm = _make(96, "bf16")
-    x, dy = _rand(21, 96, seed=1), _rand(21, 96, seed=2)
+    norm = _make(D, "bf16")
+    x, dy = _rand(M, D, seed=1), _rand(M, D, seed=2)
     _, stats = norm.forward(x, save_stats=True)
     full = norm.backward(dy, x, stats)
     for i in range(8):
@@ -201,9 +217,9 @@ def test_parts_of_the_gradient_and_no_rows():
             assert (g is None) if not n else torch.equal(g, f)
     e = x[:0]
     y, st = norm.forward(e, save_stats=True)
-    assert y.shape == (0, 96) and st.shape == (0, 2)
+    assert y.shape == (0, D) and st.shape == (0, 2)
     dx, dw, db = norm.backward(e, e, st)
-    assert dx.shape == (0, 96) and not dw.any() and not db.any()
+    assert dx.shape == (0, D) and not dw.any() and not db.any()
 
 
 def test_gradient_against_differences():
