@@ -131,6 +131,34 @@ def test_strides_alignment_and_leading_axes(M):
     assert lin.forward(x[:0]).shape == (0, 3, N)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_scales_and_zeros_at_odd_addresses(group):
+    """Scales, zero points and bias behind an odd element: the same results as on their own boundaries."""
+    import torch
+
+    import apk_b200
+    K, N = 512, 70
+    lin, _ = _layer(K, N, group, zeros=True, bias=torch.float32, act="silu")
+
+    def moved(t):
+        room = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        room[1:].copy_(t.flatten())
+        return room[1:].view(t.shape)
+
+    other = apk_b200.Linear4(lin.weight, moved(lin.scales), zeros=moved(lin.zeros), bias=moved(lin.bias), group=group, act="silu")
+    for M in (1, 12, 30, 64, 90):
+        x = _rand(M, K, seed=M)
+        assert torch.equal(lin.forward(x), other.forward(x))
+
+
+def test_long_rows_in_slices():
+    """x of 64 rows that shared memory holds a part of at a time, whole chunks or not."""
+    for K, group in ((20480, 128), (9056, 32)):
+        lin, w = _layer(K, 48, group, zeros=True)
+        _check(lin, w, _rand(64, K, seed=1))
+        _check(lin, w, _rand(9, K, seed=2))
+
+
 def test_weights_in_wider_rows_and_updated_in_place():
     import torch
 

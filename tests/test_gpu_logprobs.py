@@ -167,6 +167,20 @@ def test_orders_and_ties(M, V):
             _check(x.bfloat16().contiguous(), _tokens(M, V, 1), top)
 
 
+def test_few_allowed_tokens():
+    """Rows in which fewer values than alternatives are not masked, as constrained decoding leaves them."""
+    import torch
+    for V in (300, 5000, 20000, 131072):
+        for left in (1, 2, 7):
+            x = torch.full((4, V), -math.inf, device="cuda")
+            at = torch.randperm(V, device="cuda", generator=torch.Generator("cuda").manual_seed(V))[:left]
+            x[:, at] = _rand(4, left, seed=left)
+            t = at[:1].expand(4).contiguous()
+            for top in (1, 5, 32):
+                _check(x, t, top)
+                _check(x.bfloat16(), t, top)
+
+
 def test_masked_logits():
     """-inf, and a type's lowest value, as masks: few values left, at either end, one, and many."""
     import torch

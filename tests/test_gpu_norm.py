@@ -282,6 +282,35 @@ def test_streams_devices_and_graphs():
         assert all(torch.equal(p, q) for p, q in zip(out, want[i])) and all(torch.equal(p, q) for p, q in zip(again, want[0]))
 
 
+def test_first_calls_in_a_capture():
+    """What needs no scratch may be captured before it was ever called; what does is refused, and works after one call."""
+    import torch
+
+    import apk_b200
+    w, b = torch.rand(4096, device="cuda") + 0.5, torch.rand(4096, device="cuda")
+    x, few = _rand(1000, 4096, seed=1), _rand(20, 4096, seed=2)
+    norm, graph = apk_b200.LayerNorm(w, b), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, stats = norm.forward(x, save_stats=True)
+        y2, stats2 = norm.forward(few, save_stats=True)
+        d2 = norm.backward(few, few, stats2)
+        with pytest.raises(apk_b200.ApkError, match="before the capture"):
+            norm.backward(x, x, stats)
+    graph.replay()
+    torch.cuda.synchronize()
+    other = apk_b200.LayerNorm(w, b)
+    want, ws = other.forward(x, save_stats=True)
+    assert torch.equal(y, want) and torch.equal(stats, ws) and torch.equal(y2, other.forward(few))
+    assert all(torch.equal(p, q) for p, q in zip(d2, other.backward(few, few, stats2)))
+    wd = other.backward(x, x, ws)
+    norm.backward(x, x, ws)
+    with torch.cuda.graph(graph := torch.cuda.CUDAGraph()):
+        d = norm.backward(x, x, ws)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(d, wd))
+
+
 def test_refusals():
     import torch
 
