@@ -1001,7 +1001,9 @@ apk_status backward(apk_logprobs* h, const apk_logprobs_grads* g) {
   p.stats = reinterpret_cast<const float2*>(g->stats);
   p.rows = M;
   p.vocabulary = V;
-  p.pieces = (int)(((long long)V + 7 + logp::EIGHTS * logp::ROUND - 1) / (logp::EIGHTS * logp::ROUND));
+  // (rows that start on an alignment have no places before them)
+  const bool on = reinterpret_cast<uintptr_t>(p.x) % align == 0 && (M == 1 || p.ld % align == 0);
+  p.pieces = (int)(((long long)V + (on ? 0 : 7) + logp::EIGHTS * logp::ROUND - 1) / (logp::EIGHTS * logp::ROUND));
   const bool rows = V <= logp::SHORT;
   if (rows) p.pieces = 0;
   if ((long long)M * p.pieces > 0x7FFFFFFFll) return h->err.fail(APK_EINVAL, "%d rows of %d are too many for a launch", M, V);
