@@ -676,14 +676,19 @@ __global__ void __launch_bounds__(THREADS, 4) forward(const __grid_constant__ Pa
       if (round >= rounds) break;
       unsigned long long x[4];
       const float most = raised(ring[i], x);
-      if constexpr (TOP) {  // (equal values up to the bound's index; a NaN)
-        if (__builtin_expect(!(most < limit), 0)) {
+      // (the order that the compiler makes most of: 114 and 79 us the other way
+      // for 2048 x 100003 with 5 alternatives and none, 108 and 75 this)
+      if constexpr (TOP) {
+        sums.add(x, most);
+        if (__builtin_expect(!(most < limit), 0)) {  // (equal values up to the bound's index; a NaN)
           const int v = mine + round * THREADS, e = r.first(v);
           if ((most != limit || e <= limit_at) && v < v1) put_from<F32>(ring[i], e, p.vocabulary, bound, limit, put_here);
         }
+        get(round + N, ring[i]);
+      } else {
+        get(round + N, ring[i]);
+        sums.add(x, most);
       }
-      get(round + N, ring[i]);
-      sums.add(x, most);
     }
   }
   if constexpr (TOP) {
