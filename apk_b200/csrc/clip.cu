@@ -210,50 +210,50 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) norm(const __grid_constant__ 
 }
 
 __device__ __forceinline__ void scale_unit(const Tensor& t, unsigned u, float c) {
-      const int shift = (int)(reinterpret_cast<uintptr_t>(t.in) & 15);
-      const uint8_t* base = t.in - shift;
-      uint8_t* out = t.out - shift;
-      const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-      uint4 raw[VECS];
-      Span sp[VECS];
-  #pragma unroll
-      for (int j = 0; j < VECS; ++j) {
-        sp[j] = span_of(t, u, j);
-        if (sp[j].any) raw[j] = load(base, sp[j], t.f32, true);
-      }
-  #pragma unroll
-      for (int j = 0; j < VECS; ++j) {
-        if (!sp[j].any) continue;
-        union {
-          uint16_t h[8];
-          uint32_t w[4];
-          uint4 v;
-        } o;
-        if (t.f32) {
-          o.v = make_uint4(__float_as_uint(__uint_as_float(raw[j].x) * c), __float_as_uint(__uint_as_float(raw[j].y) * c),
-                           __float_as_uint(__uint_as_float(raw[j].z) * c), __float_as_uint(__uint_as_float(raw[j].w) * c));
-        } else {
-          float v[8];
-          ops::Raw<false> r{raw[j]};
-          ops::unpack(r, v);
-  #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= c;
-          ops::pack(v, r);
-          o.v = r.a;
-        }
-        uint8_t* q = out + sp[j].vec;
-        if (sp[j].whole && same) {
-          __stcs(reinterpret_cast<uint4*>(q), o.v);
-        } else if (t.f32) {
-  #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (i >= sp[j].lo && i < sp[j].hi) reinterpret_cast<uint32_t*>(q)[i] = o.w[i];
-        } else {
-  #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i >= sp[j].lo && i < sp[j].hi) reinterpret_cast<uint16_t*>(q)[i] = o.h[i];
-        }
-      }
+  const int shift = (int)(reinterpret_cast<uintptr_t>(t.in) & 15);
+  const uint8_t* base = t.in - shift;
+  uint8_t* out = t.out - shift;
+  const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  uint4 raw[VECS];
+  Span sp[VECS];
+#pragma unroll
+  for (int j = 0; j < VECS; ++j) {
+    sp[j] = span_of(t, u, j);
+    if (sp[j].any) raw[j] = load(base, sp[j], t.f32, true);
+  }
+#pragma unroll
+  for (int j = 0; j < VECS; ++j) {
+    if (!sp[j].any) continue;
+    union {
+      uint16_t h[8];
+      uint32_t w[4];
+      uint4 v;
+    } o;
+    if (t.f32) {
+      o.v = make_uint4(__float_as_uint(__uint_as_float(raw[j].x) * c), __float_as_uint(__uint_as_float(raw[j].y) * c),
+                       __float_as_uint(__uint_as_float(raw[j].z) * c), __float_as_uint(__uint_as_float(raw[j].w) * c));
+    } else {
+      float v[8];
+      ops::Raw<false> r{raw[j]};
+      ops::unpack(r, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= c;
+      ops::pack(v, r);
+      o.v = r.a;
+    }
+    uint8_t* q = out + sp[j].vec;
+    if (sp[j].whole && same) {
+      __stcs(reinterpret_cast<uint4*>(q), o.v);
+    } else if (t.f32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i >= sp[j].lo && i < sp[j].hi) reinterpret_cast<uint32_t*>(q)[i] = o.w[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i >= sp[j].lo && i < sp[j].hi) reinterpret_cast<uint16_t*>(q)[i] = o.h[i];
+    }
+  }
 }
 
 // From the last unit to the first: what the norm read last is still in L2.
@@ -287,6 +287,7 @@ using namespace apk;
 struct apk_clip {
   apk_clip_config cfg{};
   Err err;
+  bool opened = false;
   int sms = 0;
   Scratch scratch;
   std::mutex mu;

@@ -108,7 +108,7 @@ struct Chunk<true> {
 template <int NT8, int P, bool ZEROS, bool VEC, bool WIDE>
 __global__ void __launch_bounds__(32 * WARPS, 1) stream4(const __grid_constant__ Params p) {
   constexpr int TOK = 8 * NT8, WORDS = 4 / P, A = AHEAD<NT8>;  // WORDS: 32-bit words of a lane and group
-  extern __shared__ uint4 xs[];  // [chunk][word][tile of tokens][lane], one tile: [chunk][word][row][t]
+  extern __shared__ uint4 xs[];  // [chunk][word][row][t]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int rank = (int)blockIdx.x % p.split;
   const int kept = NT8 == 1 ? p.rows : TOK;  // rows in shared memory
@@ -183,8 +183,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) stream4(const __grid_constant__
       pairs(v, h);
       // piece e is word j of group h for lane t: e = (h * 4 + t) * (4 / P) + j
       const int j = e % WORDS, tt = e / WORDS % 4, hh = e / (WORDS * 4), word = hh * WORDS + j;
-      const int to = NT8 == 1 ? ((c * 4 + word) * kept + row) * 4 + tt : ((c * 4 + word) * kept + row) * 4 + tt;
-      xs[to] = make_uint4(h[0], h[1], h[2], h[3]);
+      xs[((c * 4 + word) * kept + row) * 4 + tt] = make_uint4(h[0], h[1], h[2], h[3]);
     }
   };
   const int my_row = NT8 == 1 ? min(g, p.rows - 1) : g;
@@ -330,43 +329,45 @@ __global__ void __launch_bounds__(256) expand(const __grid_constant__ Expand p) 
   pdl_wait();
   // a block takes two rows at once, a thread eight k of 2048, and of the next 2048
   const long long ld = p.low ? 2ll * p.k : p.k;
-  for (long long f0 = blockIdx.x; f0 < p.n; f0 += 2ll * gridDim.x) for (int k0 = (int)threadIdx.x * 8; k0 < p.k; k0 += 4096) {
-    uint32_t w[4];
-    float s[4], z[4];
-    uint16_t* to[4];
+  for (long long f0 = blockIdx.x; f0 < p.n; f0 += 2ll * gridDim.x) {
+    for (int k0 = (int)threadIdx.x * 8; k0 < p.k; k0 += 4096) {
+      uint32_t w[4];
+      float s[4], z[4];
+      uint16_t* to[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const long long f = f0 + (j >> 1) * (long long)gridDim.x;
-      const int k = k0 + (j & 1) * 2048;
-      to[j] = nullptr;
-      if (f >= p.n || k >= p.k) continue;
-      const long long at = f * p.groups + (p.group_log >= 0 ? k >> p.group_log : k / p.group);
-      s[j] = ops::ld_any(p.s, at, p.s_f32);
-      z[j] = 128.f + (p.z ? (float)(p.z[at] & 15) : 8.f);
-      w[j] = *reinterpret_cast<const uint32_t*>(p.w + f * p.ldw + k / 2);
-      to[j] = p.out + f * ld + k;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (!to[j]) continue;
-      float q[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {  // 128 + q again: an integer's conversion is slower
-        uint32_t v;
-        asm("lop3.b32 %0, %1, 0x000F000F, 0x43004300, 0xEA;" : "=r"(v) : "r"(w[j] >> (4 * e)));
-        q[e] = s[j] * (ops::bf_lo(v) - z[j]);
-        q[e + 4] = s[j] * (ops::bf_hi(v) - z[j]);
+      for (int j = 0; j < 4; ++j) {
+        const long long f = f0 + (j >> 1) * (long long)gridDim.x;
+        const int k = k0 + (j & 1) * 2048;
+        to[j] = nullptr;
+        if (f >= p.n || k >= p.k) continue;
+        const long long at = f * p.groups + (p.group_log >= 0 ? k >> p.group_log : k / p.group);
+        s[j] = ops::ld_any(p.s, at, p.s_f32);
+        z[j] = 128.f + (p.z ? (float)(p.z[at] & 15) : 8.f);
+        w[j] = *reinterpret_cast<const uint32_t*>(p.w + f * p.ldw + k / 2);
+        to[j] = p.out + f * ld + k;
       }
-      ops::Raw<false> r;
-      ops::pack(q, r);
-      *reinterpret_cast<uint4*>(to[j]) = r.a;
-      if (p.low) {
-        float hi[8];
-        ops::unpack(r, hi);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q[e] -= hi[e];
+      for (int j = 0; j < 4; ++j) {
+        if (!to[j]) continue;
+        float q[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // 128 + q again: an integer's conversion is slower
+          uint32_t v;
+          asm("lop3.b32 %0, %1, 0x000F000F, 0x43004300, 0xEA;" : "=r"(v) : "r"(w[j] >> (4 * e)));
+          q[e] = s[j] * (ops::bf_lo(v) - z[j]);
+          q[e + 4] = s[j] * (ops::bf_hi(v) - z[j]);
+        }
+        ops::Raw<false> r;
         ops::pack(q, r);
-        *reinterpret_cast<uint4*>(to[j] + p.k) = r.a;
+        *reinterpret_cast<uint4*>(to[j]) = r.a;
+        if (p.low) {
+          float hi[8];
+          ops::unpack(r, hi);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q[e] -= hi[e];
+          ops::pack(q, r);
+          *reinterpret_cast<uint4*>(to[j] + p.k) = r.a;
+        }
       }
     }
   }
@@ -405,6 +406,7 @@ using namespace apk;
 struct apk_linear4 {
   apk_linear4_config cfg{};
   Err err;
+  bool opened = false;
   int sms = 0;
   int clusters[9] = {};  // of 2, 4 and 8 CTAs that run at once
   Scratch scratch;

@@ -585,6 +585,7 @@ using namespace apk;
 struct apk_norm {
   apk_norm_config cfg{};
   Err err;
+  bool opened = false;
   int sms = 0;
   Scratch scratch;
   std::mutex mu;

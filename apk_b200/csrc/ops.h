@@ -48,21 +48,24 @@ inline apk_status open_device(int device, int* sms, Err* err) {
 }
 
 // The bodies of the C entry points: no exception leaves them, and calls on one
-// handle from several host threads are taken one at a time.  H has err, mu and scratch.
+// handle from several host threads are taken one at a time.  H has err, mu and opened.
 template <class H, class Cfg, class F>
 apk_status make(const Cfg* cfg, H** out, F&& create) {
   if (!out) return APK_EINVAL;
   *out = new (std::nothrow) H;
   if (!*out) return APK_ENOMEM;
   try {
-    return cfg ? create(cfg, *out) : (*out)->err.fail(APK_EINVAL, "cfg is NULL");  // *out is set on failure too
+    if (!cfg) return (*out)->err.fail(APK_EINVAL, "cfg is NULL");  // *out is set on failure too
+    APK_TRY(create(cfg, *out));
+    (*out)->opened = true;
+    return APK_OK;
   } catch (...) {
     return APK_ENOMEM;
   }
 }
 template <class H, class F>
 apk_status call(H* h, const void* arg, F&& f) {
-  if (!h || !h->scratch.status() || !arg) return APK_EINVAL;
+  if (!h || !h->opened || !arg) return APK_EINVAL;
   try {
     std::lock_guard<std::mutex> lock(h->mu);
     return f();

@@ -247,7 +247,7 @@ def main():
     print(f"train: loss {losses[0]:.4f} -> {losses[-1]:.4f} in {a.steps} steps, {us:.0f} us a step, "
           f"{flops / us / 1e6:.0f} TFLOP/s of products")
     if a.norm:
-        losses, norms, us = train_tokens(a.steps, a.rows, a.vocabulary, a.d_model, a.d_ff, max_norm=a.max_norm or 1.0)
+        losses, norms, us = train_tokens(a.steps, a.rows, a.vocabulary, a.d_model, a.d_ff, max_norm=1.0 if a.max_norm is None else a.max_norm)
         print(f"train on tokens: loss {losses[0]:.4f} -> {losses[-1]:.4f} in {a.steps} steps, {us:.0f} us a step, "
               f"gradient norm {norms[0]:.3f} -> {norms[-1]:.3f} before clipping")
     said, us, *scores = decode(a.tokens, a.d_model, vocabulary=a.vocabulary, head_bits=a.head_bits, top=a.top)

@@ -705,7 +705,7 @@ apk_status apk_norm_backward(apk_norm* h, const apk_norm_grads* g);
  * Squares are added in fp32 over a few values at a time and in 64 bits beyond
  * (values whose squares leave fp32 in 64 bits throughout), in an order that
  * depends on the sizes and addresses alone.  A norm that is infinite makes the
- * factor 0, a NaN makes it NaN: all outputs then show it.  The host arrays are
+ * factor 0 (NaN where max_norm is infinite too), a NaN makes it NaN.  The host arrays are
  * read before the call returns. */
 typedef struct apk_clip_config {
   int device;
