@@ -23,10 +23,16 @@ constexpr int MAX_FEATURES = 16384;  // 1024 threads of two pieces
 
 // Rows on their way, this one among them: 98 KB of shared memory (196 KB for
 // more than 512 threads, of which an SM takes one block) hold them.
-template <bool VEC, bool XF>
-constexpr int FWD_STAGES = !VEC ? 1 : XF ? 3 : 6;
-template <bool VEC, bool XF, bool DF, int T>
-constexpr int BWD_STAGES = !VEC ? 1 : 24 / ((XF ? 8 : 4) + (DF ? 4 : 2)) / (T > 512 ? 2 : 1);
+template <bool XF>
+constexpr int FWD_STAGES = XF ? 3 : 6;
+template <bool XF, bool DF, int T>
+constexpr int BWD_STAGES = 24 / ((XF ? 8 : 4) + (DF ? 4 : 2)) / (T > 512 ? 2 : 1);
+// Rows that start anywhere go by their threads together through shared memory.
+// Not so the largest blocks, which have a row or few each, and short rows, a
+// warp each (forward 1537 x 1001 fp32: 4.2 us, so 5.1, 16384 x 333 bf16 9.6 and
+// 9.7; backward 500 x 111 6.0 and 7.4, 16384 x 333 23.7 and 23.4).
+template <bool VEC, bool WARP, int T>
+constexpr bool SHARED = !VEC && !WARP && T <= 512;
 
 struct Params {
   const void* x;
@@ -94,6 +100,30 @@ __device__ __forceinline__ void load_weight(const void* p, int f32, float (&v)[8
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = !VEC && column<false>(j, i, t, T) < cols ? ops::ld_any(p, column<false>(j, i, t, T), f32) : 0.f;
+  }
+}
+
+// The same of rows that go through shared memory: T is a constant, and where a
+// pair of columns lies in the row for all threads nothing is compared.
+template <bool F32>
+__device__ __forceinline__ void store_odd(void* p, long long row, const float (&v)[8], int j, int cols, int t, int T) {
+  uint8_t* q = static_cast<uint8_t*>(p) + (row + t) * (F32 ? 4 : 2);
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const int k = j * 8 + i;
+    if ((k + 2) * T <= cols) {
+      if constexpr (F32) {
+        *reinterpret_cast<float*>(q + k * T * 4) = v[i];
+        *reinterpret_cast<float*>(q + (k + 1) * T * 4) = v[i + 1];
+      } else {
+        const uint32_t two = ops::pack_bf16(v[i], v[i + 1]);
+        *reinterpret_cast<uint16_t*>(q + k * T * 2) = (uint16_t)two;
+        *reinterpret_cast<uint16_t*>(q + (k + 1) * T * 2) = (uint16_t)(two >> 16);
+      }
+    } else {
+      if (k * T + t < cols) ops::st_any(q, k * T, v[i], F32);
+      if ((k + 1) * T + t < cols) ops::st_any(q, (k + 1) * T, v[i + 1], F32);
+    }
   }
 }
 
@@ -190,6 +220,62 @@ struct Ahead {
     return r;
   }
 };
+// Rows that start anywhere: the aligned 16-byte pieces that a row touches, one
+// after the other, copied by the row's T threads and read by all of them, so
+// that a barrier stands between (`arrived`, then the barrier; behind it the
+// stage that was read last may be filled again).  T is a constant, and what lies
+// behind a row's end are zeros, so that an element costs a load and a shift:
+// with a comparison each and addresses by a running T it took 45 instructions.
+// (8192 x 4001 bf16, element by element out of global memory: 66 us forward,
+// 157 backward; so, 41 and 75.)
+template <int V, bool F32, int T>
+struct Odd {
+  static constexpr int ES = F32 ? 4 : 2, BYTES = T * V * 8 * ES + 16;  // of a stage: a piece more, for the shift
+  uint32_t at;  // the row's ring
+  int end;      // of what every row writes of a stage: its pieces wherever it starts
+  __device__ __forceinline__ Odd(uint32_t at_, int cols) : at(at_), end((cols * ES + 16 - ES + 15) / 16 * 16) {}
+  // zeros behind it, once
+  __device__ __forceinline__ void clear(int stages, int t) const {
+    for (int s = 0; s < stages; ++s)
+      for (int b = end + t * 16; b < BYTES; b += T * 16)
+        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at + s * BYTES + b), "r"(0) : "memory");
+  }
+  // `row`: its first byte, in memory that begins at `base`
+  __device__ __forceinline__ void fetch(int stage, const uint8_t* row, const void* base, int cols, int t) const {
+    const int shift = (int)(reinterpret_cast<uintptr_t>(row) & 15), bytes = shift + cols * ES;
+    const uint8_t* q = row - shift;
+    const uint32_t to = at + stage * BYTES;
+    for (int b = t * 16; b < end; b += T * 16) {
+      if (q + b < static_cast<const uint8_t*>(base)) {  // nothing in front of the first row is touched
+        for (int e = 0; e < 16; e += ES) {
+          const bool in = e >= shift && e < bytes;
+          if constexpr (F32) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + e), "r"(in ? *reinterpret_cast<const uint32_t*>(q + e) : 0u) : "memory");
+          else asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + e), "h"(in ? *reinterpret_cast<const uint16_t*>(q + e) : (uint16_t)0) : "memory");
+        }
+      } else {  // of the last pieces, what lies in the row; zeros behind it
+        const int n = max(0, min(16, bytes - b));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + b), "l"(n ? q + b : row - shift), "r"(n) : "memory");
+      }
+    }
+  }
+  // piece j of thread t, 0 behind the last column
+  __device__ __forceinline__ void get(int stage, const uint8_t* row, int j, int t, ops::f32x2 (&v)[4]) const {
+    const uint32_t from = at + stage * BYTES + (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15) + t * ES;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (F32) {
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x[i]) : "r"(from + (j * 8 + i) * T * ES) : "memory");
+      } else {
+        uint16_t h;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(from + (j * 8 + i) * T * ES) : "memory");
+        x[i] = ops::bf_lo(h);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = ops::pair2(x[2 * i], x[2 * i + 1]);
+  }
+};
 // The next rows of an operand as this thread fetches them.
 template <bool F32>
 __device__ __forceinline__ const uint8_t* piece_of(const void* p, long long row, long long ld, int t) {
@@ -207,11 +293,11 @@ __device__ __forceinline__ void arrived() {  // the oldest of S groups
 // block, of which an SM takes 512.
 template <int V, bool VEC, bool WARP, bool XF, bool YF, int T_>
 __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) forward(const __grid_constant__ Params p) {
-  constexpr int S = FWD_STAGES<VEC, XF>;
+  constexpr int S = FWD_STAGES<XF>;
   constexpr bool HELD = V <= 2 && T_ <= 512;
   extern __shared__ uint4 ring[];
   __shared__ float4 sh[2][16];
-  const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int T = WARP ? 32 : SHARED<VEC, WARP, T_> ? T_ : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
   const int per = WARP ? 8 : 1;
   const Ahead<V, XF, S> ahead{smem_u32(ring + threadIdx.x), (int)blockDim.x};
   const int pieces = t * 8 < p.cols ? (p.cols - t * 8 - 1) / (T * 8) + 1 : 0;  // of the V, where rows go by eights
@@ -219,18 +305,23 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) forward(const __
   long long r = (long long)blockIdx.x * per + (WARP ? threadIdx.x >> 5 : 0);
   pdl_launch();
   pdl_wait();
-  const uint8_t* px = piece_of<XF>(p.x, r, p.ldx, t);
+  using OddX = Odd<V, XF, T_>;
+  const OddX odd(smem_u32(ring), p.cols);
+  if constexpr (SHARED<VEC, WARP, T_>) odd.clear(S, t);
+  const uint8_t* px = piece_of<XF>(p.x, r, p.ldx, VEC ? t : 0);
+  const uint8_t* now = px;  // this row
   const long long next_x = step * p.ldx * (XF ? 4 : 2);
   int left = r < p.rows ? (int)((p.rows - r - 1) / step) + 1 : 0;  // rows to be fetched
   auto fetch = [&](int stage) {
     if (left > 0) {
-      ahead.fetch(stage, px, pieces, T);
+      if constexpr (VEC) ahead.fetch(stage, px, pieces, T);
+      else odd.fetch(stage, px, p.x, p.cols, t);
       px += next_x;
       --left;
     }
     fetched();
   };
-  if constexpr (VEC)
+  if constexpr (VEC || SHARED<VEC, WARP, T_>)
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) fetch(i);
   ops::f32x2 w[V][4], b[V][4];
@@ -248,19 +339,29 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) forward(const __
 #pragma unroll
     for (int j = 0; j < V; ++j) weights(j);
   for (int stage = 0; r < p.rows; r += step, stage = stage + 1 == S ? 0 : stage + 1) {
-    ops::Raw<XF> raw[V];
-    if constexpr (VEC) {
-      fetch(stage == 0 ? S - 1 : stage - 1);
-      arrived<S>();
-#pragma unroll
-      for (int j = 0; j < V; ++j) raw[j] = ahead.get(stage, j, pieces);
-    } else {
-      load_row<VEC, XF, V>(p.x, r * p.ldx, raw, p.cols, t, T);
-    }
     ops::f32x2 v[V][4], s = 0;
+    if constexpr (SHARED<VEC, WARP, T_>) {
+      arrived<S - 1>();
+      __syncthreads();
+      fetch(stage == 0 ? S - 1 : stage - 1);
+#pragma unroll
+      for (int j = 0; j < V; ++j) odd.get(stage, now, j, t, v[j]);
+      now += next_x;
+    } else {
+      ops::Raw<XF> raw[V];
+      if constexpr (VEC) {
+        fetch(stage == 0 ? S - 1 : stage - 1);
+        arrived<S>();
+#pragma unroll
+        for (int j = 0; j < V; ++j) raw[j] = ahead.get(stage, j, pieces);
+      } else {
+        load_row<VEC, XF, V>(p.x, r * p.ldx, raw, p.cols, t, T);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) ops::unpack2(raw[j], v[j]);
+    }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      ops::unpack2(raw[j], v[j]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s = ops::add2(s, v[j][i]);  // (zero behind the last column)
     }
@@ -272,7 +373,7 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) forward(const __
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         ops::f32x2 d = ops::add2(v[j][i], minus);
-        if constexpr (!VEC) {
+        if (!VEC && !(SHARED<VEC, WARP, T_> && (j * 8 + 2 * i + 2) * T <= p.cols)) {
           float lo, hi;
           ops::unpair2(d, lo, hi);
           d = ops::pair2(column<false>(j, 2 * i, t, T) < p.cols ? lo : 0.f, column<false>(j, 2 * i + 1, t, T) < p.cols ? hi : 0.f);
@@ -290,7 +391,8 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) forward(const __
       float y[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) ops::unpair2(ops::fma2(ops::mul2(v[j][i], scale), w[j][i], b[j][i]), y[2 * i], y[2 * i + 1]);
-      store_piece<VEC, YF>(p.y, r * p.ldy, y, j, p.cols, t, T);
+      if constexpr (SHARED<VEC, WARP, T_>) store_odd<YF>(p.y, r * p.ldy, y, j, p.cols, t, T);
+      else store_piece<VEC, YF>(p.y, r * p.ldy, y, j, p.cols, t, T);
     }
   }
 }
@@ -333,11 +435,11 @@ __device__ __forceinline__ void columns(const Params& p) {
 // reduce().  T_: the most threads of a block, of which an SM takes 512.
 template <int V, bool VEC, bool WARP, bool XF, bool DF, int T_>
 __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const __grid_constant__ Params p) {
-  constexpr int S = BWD_STAGES<VEC, XF, DF, T_>;
-  constexpr bool HELD = VEC && T_ <= 512;  // the weight stays in registers
+  constexpr int S = BWD_STAGES<XF, DF, T_>;
+  constexpr bool HELD = (VEC || !WARP) && T_ <= 512;  // the weight stays in registers
   extern __shared__ uint4 ring[];
   __shared__ float4 sh[2][16];
-  const int T = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int T = WARP ? 32 : SHARED<VEC, WARP, T_> ? T_ : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
   const int per = WARP ? 8 : 1;
   const Ahead<V, XF, S> ax{smem_u32(ring + threadIdx.x), (int)blockDim.x};
   const Ahead<V, DF, S> ad{ax.at + S * ax.SLOTS * blockDim.x * 16, (int)blockDim.x};
@@ -353,16 +455,33 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
       columns<XF, DF>(p);
       return;
     }
-  const uint8_t* px = piece_of<XF>(p.x, r, p.ldx, t);
-  const uint8_t* pd = piece_of<DF>(p.dy, r, p.ld_dy, t);
-  const uint8_t* pr = piece_of<XF>(p.r, r, p.ld_r, t);
+  using OddX = Odd<V, XF, T_>;
+  using OddD = Odd<V, DF, T_>;
+  const OddX ox(smem_u32(ring), p.cols);
+  const OddD od(ox.at + S * OddX::BYTES, p.cols);
+  const OddX orr(od.at + S * OddD::BYTES, p.cols);
+  if constexpr (SHARED<VEC, WARP, T_>) {
+    ox.clear(S, t);
+    od.clear(S, t);
+    orr.clear(S, t);
+  }
+  const uint8_t* px = piece_of<XF>(p.x, r, p.ldx, VEC ? t : 0);
+  const uint8_t* pd = piece_of<DF>(p.dy, r, p.ld_dy, VEC ? t : 0);
+  const uint8_t* pr = piece_of<XF>(p.r, r, p.ld_r, VEC ? t : 0);
+  const uint8_t *now_x = px, *now_d = pd, *now_r = pr;  // this row
   const long long next_x = step * p.ldx * (XF ? 4 : 2), next_d = step * p.ld_dy * (DF ? 4 : 2), next_r = step * p.ld_r * (XF ? 4 : 2);
   int left = r < p.rows ? (int)((p.rows - r - 1) / step) + 1 : 0;  // rows to be fetched
   auto fetch = [&](int stage) {
     if (left > 0) {
-      ax.fetch(stage, px, pieces, T);
-      ad.fetch(stage, pd, pieces, T);
-      if (p.r) ar.fetch(stage, pr, pieces, T);
+      if constexpr (VEC) {
+        ax.fetch(stage, px, pieces, T);
+        ad.fetch(stage, pd, pieces, T);
+        if (p.r) ar.fetch(stage, pr, pieces, T);
+      } else {
+        ox.fetch(stage, px, p.x, p.cols, t);
+        od.fetch(stage, pd, p.dy, p.cols, t);
+        if (p.r) orr.fetch(stage, pr, p.r, p.cols, t);
+      }
       px += next_x;
       pd += next_d;
       pr += next_r;
@@ -370,7 +489,7 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
     }
     fetched();
   };
-  if constexpr (VEC)
+  if constexpr (VEC || SHARED<VEC, WARP, T_>)
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) fetch(i);
   ops::f32x2 w[V][4];
@@ -386,28 +505,43 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
   int buf = 0;
   float2 st = r < p.rows ? p.stats[r] : make_float2(0.f, 0.f);
   for (int stage = 0; r < p.rows; r += step, stage = stage + 1 == S ? 0 : stage + 1) {
+    ops::f32x2 n[V][4], g[V][4], s1 = 0, s2 = 0;
     ops::Raw<XF> rx[V];
     ops::Raw<DF> rd[V];
-    if constexpr (VEC) {
+    if constexpr (SHARED<VEC, WARP, T_>) {
+      arrived<S - 1>();
+      __syncthreads();
       fetch(stage == 0 ? S - 1 : stage - 1);
-      arrived<S>();
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        rx[j] = ax.get(stage, j, pieces);
-        rd[j] = ad.get(stage, j, pieces);
+        ox.get(stage, now_x, j, t, n[j]);
+        od.get(stage, now_d, j, t, g[j]);
       }
+      now_x += next_x;
+      now_d += next_d;
     } else {
-      load_row<VEC, XF, V>(p.x, r * p.ldx, rx, p.cols, t, T);
-      load_row<VEC, DF, V>(p.dy, r * p.ld_dy, rd, p.cols, t, T);
+      if constexpr (VEC) {
+        fetch(stage == 0 ? S - 1 : stage - 1);
+        arrived<S>();
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          rx[j] = ax.get(stage, j, pieces);
+          rd[j] = ad.get(stage, j, pieces);
+        }
+      } else {
+        load_row<VEC, XF, V>(p.x, r * p.ldx, rx, p.cols, t, T);
+        load_row<VEC, DF, V>(p.dy, r * p.ld_dy, rd, p.cols, t, T);
+      }
     }
     const float2 st_next = r + step < p.rows ? p.stats[r + step] : make_float2(0.f, 0.f);
     const ops::f32x2 minus = ops::both(-st.x), rstd = ops::both(st.y);
-    ops::f32x2 n[V][4], g[V][4], s1 = 0, s2 = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       if constexpr (!HELD) weights(j);
-      ops::unpack2(rx[j], n[j]);
-      ops::unpack2(rd[j], g[j]);
+      if constexpr (!SHARED<VEC, WARP, T_>) {
+        ops::unpack2(rx[j], n[j]);
+        ops::unpack2(rd[j], g[j]);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         n[j][i] = ops::mul2(ops::add2(n[j][i], minus), rstd);
@@ -423,21 +557,27 @@ __global__ void __launch_bounds__(T_, T_ <= 512 ? 512 / T_ : 1) backward(const _
       buf ^= 1;
       const ops::f32x2 a = ops::both(-s.x * p.per_col), b = ops::both(-s.y * p.per_col);
       ops::Raw<XF> rr[V];
-      if (!VEC && p.r) load_row<VEC, XF, V>(p.r, r * p.ld_r, rr, p.cols, t, T);
+      if (!VEC && !SHARED<VEC, WARP, T_> && p.r) load_row<VEC, XF, V>(p.r, r * p.ld_r, rr, p.cols, t, T);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         ops::f32x2 res[4] = {};
         if (p.r) {
-          if constexpr (VEC) rr[j] = ar.get(stage, j, pieces);
-          ops::unpack2(rr[j], res);
+          if constexpr (SHARED<VEC, WARP, T_>) {
+            orr.get(stage, now_r, j, t, res);
+          } else {
+            if constexpr (VEC) rr[j] = ar.get(stage, j, pieces);
+            ops::unpack2(rr[j], res);
+          }
         }
         float y[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           ops::unpair2(ops::fma2(rstd, ops::fma2(n[j][i], b, ops::add2(g[j][i], a)), res[i]), y[2 * i], y[2 * i + 1]);
-        store_piece<VEC, XF>(p.y, r * p.ldy, y, j, p.cols, t, T);
+        if constexpr (SHARED<VEC, WARP, T_>) store_odd<XF>(p.y, r * p.ldy, y, j, p.cols, t, T);
+        else store_piece<VEC, XF>(p.y, r * p.ldy, y, j, p.cols, t, T);
       }
     }
+    now_r += next_r;
     st = st_next;
   }
   if (!p.part) return;
@@ -516,14 +656,20 @@ struct Kernel {
   void (*fn)(Params);
   int smem;  // of a thread
   int threads;  // at most
+  int more;  // shared memory besides
 };
 template <int V, bool VEC, bool WARP, int T, bool XF, bool YF>
 Kernel fwd() {
-  return {&forward<V, VEC, WARP, XF, YF, T>, VEC ? FWD_STAGES<VEC, XF> * V * (XF ? 32 : 16) : 0, T};
+  constexpr int S = FWD_STAGES<XF>;
+  return {&forward<V, VEC, WARP, XF, YF, T>, VEC || SHARED<VEC, WARP, T> ? S * V * (XF ? 32 : 16) : 0, T, SHARED<VEC, WARP, T> ? S * 16 : 0};
 }
 template <int V, bool VEC, bool WARP, int T, bool XF, bool DF>
 Kernel bwd() {
-  return {&backward<V, VEC, WARP, XF, DF, T>, WARP && !VEC ? 32 * V : VEC ? BWD_STAGES<VEC, XF, DF, T> * V * ((XF ? 64 : 32) + (DF ? 32 : 16)) : 0, T};
+  constexpr int S = BWD_STAGES<XF, DF, T>;
+  constexpr int rings = S * V * ((XF ? 64 : 32) + (DF ? 32 : 16)), join = 32 * V;  // (the join of a block's 8 warps)
+  static_assert(rings >= join, "the join lies where the rings were");
+  return {&backward<V, VEC, WARP, XF, DF, T>, VEC || SHARED<VEC, WARP, T> ? rings : WARP ? join : 0, T,
+          SHARED<VEC, WARP, T> ? S * 3 * 16 : 0};
 }
 template <int V, bool WARP, int T>
 Kernel fwd_of(bool vec, bool xf, bool yf) {
@@ -545,6 +691,11 @@ struct Shape {
   Kernel k;
   int T, per;
 };
+// Threads of two pieces each; rows through shared memory have a kernel's most.
+int threads_of(int cols, bool vec) {
+  const int T = ops::ceil_div(ops::ceil_div(cols, 16), 32) * 32;
+  return vec || T > 512 ? T : T <= 64 ? 64 : T <= 128 ? 128 : T <= 256 ? 256 : 512;
+}
 // Where there are fewer rows than blocks that run at once, a row has more
 // threads: one piece each.
 Shape fwd_shape(int cols, bool few, bool vec, bool xf, bool yf) {
@@ -556,7 +707,7 @@ Shape fwd_shape(int cols, bool few, bool vec, bool xf, bool yf) {
                : (yf ? fwd<4, false, true, 256, false, true>() : fwd<4, false, true, 256, false, false>()),
             256, 8};
   if (few && cols <= 8192) return {fwd_of<1, false, 1024>(vec, xf, yf), ops::ceil_div(ops::ceil_div(cols, 8), 32) * 32, 1};
-  const int T = ops::ceil_div(ops::ceil_div(cols, 16), 32) * 32;
+  const int T = threads_of(cols, vec);
   return {T <= 64    ? fwd_of<2, false, 64>(vec, xf, yf)
           : T <= 128 ? fwd_of<2, false, 128>(vec, xf, yf)
           : T <= 256 ? fwd_of<2, false, 256>(vec, xf, yf)
@@ -568,7 +719,7 @@ Shape bwd_shape(int cols, bool few, bool vec, bool xf, bool df) {
   if (few) return {bwd_of<1, false, 1024>(vec, xf, df), std::max(128, ops::ceil_div(ops::ceil_div(cols, 8), 32) * 32), 1};
   if (cols <= 256) return {bwd_of<1, true, 256>(vec, xf, df), 256, 8};
   if (cols <= 512) return {bwd_of<2, true, 256>(vec, xf, df), 256, 8};
-  const int T = ops::ceil_div(ops::ceil_div(cols, 16), 32) * 32;
+  const int T = threads_of(cols, vec);
   return {T <= 64    ? bwd_of<2, false, 64>(vec, xf, df)
           : T <= 128 ? bwd_of<2, false, 128>(vec, xf, df)
           : T <= 256 ? bwd_of<2, false, 256>(vec, xf, df)
@@ -611,11 +762,11 @@ apk_status create(const apk_norm_config* cfg, apk_norm* h) {
 }
 
 apk_status launch(apk_norm* h, const norm::Shape& sh, const norm::Params& p, int grid, cudaStream_t s, const char* what) {
-  const int smem = sh.k.smem * sh.T;
+  const int smem = sh.k.smem * sh.T + sh.k.more;
   const void* fn = reinterpret_cast<const void*>(sh.k.fn);
   // (a kernel's blocks differ in size: it is given what its largest need)
   if (smem > 40 << 10 && std::find(h->ready.begin(), h->ready.end(), fn) == h->ready.end()) {
-    APK_TRY(cu_status(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, sh.k.smem * sh.k.threads), what, &h->err));
+    APK_TRY(cu_status(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, sh.k.smem * sh.k.threads + sh.k.more), what, &h->err));
     h->ready.push_back(fn);
   }
   Launch l(dim3(grid), sh.T, smem, s);

@@ -356,3 +356,43 @@ def test_refusals():
         norm.forward(x)
     with pytest.raises(ValueError, match="other memory"):
         norm.backward(y, x, stats)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(map(str, t)))
+@pytest.mark.parametrize("D,ld,at", [(515, 515, 1), (1001, 1001, 0), (1003, 1010, 7), (2048, 2048, 5), (2051, 2057, 3), (4099, 4099, 6),
+                                     (8191, 8193, 1)])
+def test_rows_from_any_address(D, ld, at, types):
+    """Many rows that start anywhere, the first one too: a NaN beside a row, or in another row, does not reach it."""
+    import torch
+    xt, w, other, bias = types
+    norm = _make(D, w, bias, other, seed=D)
+    M = 500
+
+    def rows(dtype, seed):
+        room = torch.full((at + M * ld,), float("nan"), device="cuda", dtype={"bf16": torch.bfloat16, "f32": torch.float32}[dtype])
+        t = room[at:].as_strided((M, D), (ld, 1))
+        t.copy_(_rand(M, D, seed=seed, scale=2.0, mean=0.5, dtype=dtype))
+        return room, t
+
+    (_, x), (_, dy), (_, res) = rows(xt, D + 3), rows(other, D + 4), rows(xt, D + 5)
+    stats = _check_forward(norm, x)
+    _check_backward(norm, x, dy, stats, res)
+    _check_backward(norm, x, dy, stats)
+    want = norm.forward(x)
+    room, out = rows(other, D + 6)
+    kept = room.clone()
+    norm.forward(x, out=out)
+    assert torch.equal(out, want)
+    kept[at:].as_strided((M, D), (ld, 1)).copy_(want)
+    assert torch.equal(room.nan_to_num(7.0), kept.nan_to_num(7.0)), "something beside the rows was written"
+    dx = norm.backward(dy, x, stats)[0]
+    bad = torch.arange(0, M, 3, device="cuda")
+    clean = [i for i in range(M) if i % 3]
+    x[bad] = float("nan")
+    dy[bad] = float("inf")
+    assert torch.equal(norm.forward(x)[clean], want[clean]) and norm.forward(x)[bad].isnan().all()
+    assert torch.equal(norm.backward(dy, x, stats)[0][clean], dx[clean])
+    if xt == other:
+        x[bad] = 1.0
+        want = norm.forward(x)
+        assert torch.equal(norm.forward(x, out=x), want)
