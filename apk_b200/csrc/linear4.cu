@@ -105,7 +105,10 @@ struct Chunk<true> {
   uint2 s[2];
   uint32_t z[2];  // a byte each
 };
-template <int NT8, int P, bool ZEROS, bool VEC, bool WIDE>
+// XA: pieces of x that a thread has on their way while x is laid out.  (One each:
+// 32 x 4096 x 4096 14.6 us, eight 13.5; up to 8 rows, 8 x 4096 x 8192 10.1, four
+// 9.7; but the one piece of a single row 8.1 in that code and 7.9 in its own.)
+template <int NT8, int P, bool ZEROS, bool VEC, bool WIDE, int XA>
 __global__ void __launch_bounds__(32 * WARPS, 1) stream4(const __grid_constant__ Params p) {
   constexpr int TOK = 8 * NT8, WORDS = 4 / P, A = AHEAD<NT8>;  // WORDS: 32-bit words of a lane and group
   extern __shared__ uint4 xs[];  // [chunk][word][row][t]
@@ -168,22 +171,30 @@ __global__ void __launch_bounds__(32 * WARPS, 1) stream4(const __grid_constant__
   };
   // x of `n` chunks from `chunk` on; a thread's piece is eight contiguous k
   auto stage = [&](int chunk, int n) {
-    const int rows = min(p.rows, kept);
-    for (int i = tid; i < n * 16 * kept; i += 32 * WARPS) {
-      // the 16 pieces of a row's chunk go to neighbouring threads
-      const int e = i & 15, row = (i >> 4) % kept, c = (i >> 4) / kept;
-      const int k = (chunk + c) * CHUNK + e * 8;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (row < rows) {
-        const uint16_t* q = p.x + row * p.ldx + k;
-        if (VEC) v = k < p.k ? stream::ld_rows(q) : v;
-        else v = stream::ld8_any(q, p.k - k);
+    const int rows = min(p.rows, kept), all = n * 16 * kept;
+    for (int i0 = tid; i0 < all; i0 += XA * 32 * WARPS) {
+      uint4 v[XA];
+#pragma unroll
+      for (int u = 0; u < XA; ++u) {
+        // the 16 pieces of a row's chunk go to neighbouring threads
+        const int i = i0 + u * 32 * WARPS, row = (i >> 4) % kept, k = (chunk + (i >> 4) / kept) * CHUNK + (i & 15) * 8;
+        v[u] = make_uint4(0, 0, 0, 0);
+        if (i < all && row < rows) {
+          const uint16_t* q = p.x + row * p.ldx + k;
+          if (VEC) v[u] = k < p.k ? stream::ld_rows(q) : v[u];
+          else v[u] = stream::ld8_any(q, p.k - k);
+        }
       }
-      uint32_t h[4];
-      pairs(v, h);
-      // piece e is word j of group h for lane t: e = (h * 4 + t) * (4 / P) + j
-      const int j = e % WORDS, tt = e / WORDS % 4, hh = e / (WORDS * 4), word = hh * WORDS + j;
-      xs[((c * 4 + word) * kept + row) * 4 + tt] = make_uint4(h[0], h[1], h[2], h[3]);
+#pragma unroll
+      for (int u = 0; u < XA; ++u) {
+        const int i = i0 + u * 32 * WARPS, e = i & 15, row = (i >> 4) % kept, c = (i >> 4) / kept;
+        if (i >= all) break;
+        uint32_t h[4];
+        pairs(v[u], h);
+        // piece e is word j of group h for lane t: e = (h * 4 + t) * (4 / P) + j
+        const int j = e % WORDS, tt = e / WORDS % 4, hh = e / (WORDS * 4), word = hh * WORDS + j;
+        xs[((c * 4 + word) * kept + row) * 4 + tt] = make_uint4(h[0], h[1], h[2], h[3]);
+      }
     }
   };
   const int my_row = NT8 == 1 ? min(g, p.rows - 1) : g;
@@ -382,20 +393,24 @@ __global__ void __launch_bounds__(256) expand(const __grid_constant__ Expand p) 
   }
 }
 
-template <int NT8, int P, bool WIDE>
+template <int NT8, int P, bool WIDE, int XA>
 const void* fn(bool zeros, bool vec) {
-  return zeros ? (vec ? reinterpret_cast<const void*>(&stream4<NT8, P, true, true, WIDE>)
-                      : reinterpret_cast<const void*>(&stream4<NT8, P, true, false, WIDE>))
-               : (vec ? reinterpret_cast<const void*>(&stream4<NT8, P, false, true, WIDE>)
-                      : reinterpret_cast<const void*>(&stream4<NT8, P, false, false, WIDE>));
+  return zeros ? (vec ? reinterpret_cast<const void*>(&stream4<NT8, P, true, true, WIDE, XA>)
+                      : reinterpret_cast<const void*>(&stream4<NT8, P, true, false, WIDE, XA>))
+               : (vec ? reinterpret_cast<const void*>(&stream4<NT8, P, false, true, WIDE, XA>)
+                      : reinterpret_cast<const void*>(&stream4<NT8, P, false, false, WIDE, XA>));
 }
 // The kernel for a layer's group, scales and zero points, and x that is (vec) or is not on 16 bytes.
-template <int NT8>
+template <int NT8, int XA>
 const void* fn(const apk_linear4_config& c, bool vec) {
   const bool wide = c.scale_dtype == APK_BF16 && c.in_features % CHUNK == 0 && ops::aligned(c.scales, 8) && ops::aligned(c.zeros, 4);
-  return c.group == 32   ? (wide ? fn<NT8, 4, true>(c.zeros, vec) : fn<NT8, 4, false>(c.zeros, vec))
-         : c.group == 64 ? fn<NT8, 2, false>(c.zeros, vec)
-                         : fn<NT8, 1, false>(c.zeros, vec);
+  return c.group == 32   ? (wide ? fn<NT8, 4, true, XA>(c.zeros, vec) : fn<NT8, 4, false, XA>(c.zeros, vec))
+         : c.group == 64 ? fn<NT8, 2, false, XA>(c.zeros, vec)
+                         : fn<NT8, 1, false, XA>(c.zeros, vec);
+}
+// nt: tiles of 8 rows; many: more pieces of x than threads
+const void* fn(const apk_linear4_config& c, bool vec, int nt, bool many) {
+  return nt == 1 ? (many ? fn<1, 4>(c, vec) : fn<1, 1>(c, vec)) : nt == 2 ? fn<2, 8>(c, vec) : nt == 4 ? fn<4, 8>(c, vec) : fn<8, 8>(c, vec);
 }
 
 }  // namespace lin4
@@ -439,17 +454,15 @@ apk_status create(const apk_linear4_config* cfg, apk_linear4* h) {
   h->sms = c.sms ? c.sms : sms;
   DeviceGuard guard(c.device);
   APK_TRY(cu_status(lin::prepare(), "preparing the linear kernels", &h->err));
-  // (a layer's group and zero points leave eight kernels that it may launch)
-  for (const bool vec : {false, true}) {
-    const void* f[4] = {lin4::fn<1>(c, vec), lin4::fn<2>(c, vec), lin4::fn<4>(c, vec),
-                        lin4::fn<8>(c, vec)};
-    for (int i = 0; i < 4; ++i)
-      APK_TRY(cu_status(cudaFuncSetAttribute(f[i], cudaFuncAttributeMaxDynamicSharedMemorySize, lin4::SMEM),
-                        "preparing the 4-bit product", &h->err));
-  }
+  // (a layer's group and zero points leave ten kernels that it may launch)
+  for (const bool vec : {false, true})
+    for (const bool many : {false, true})
+      for (int nt = 1; nt <= (many ? 8 : 1); nt *= 2)
+        APK_TRY(cu_status(cudaFuncSetAttribute(lin4::fn(c, vec, nt, many), cudaFuncAttributeMaxDynamicSharedMemorySize, lin4::SMEM),
+                          "preparing the 4-bit product", &h->err));
   for (int split = 2; split <= 8; split *= 2) {
     Launch l(dim3(split), 32 * lin4::WARPS, lin4::SMEM, nullptr, split);
-    APK_TRY(cu_status(cudaOccupancyMaxActiveClusters(&h->clusters[split], lin4::fn<1>(c, true), &l.cfg),
+    APK_TRY(cu_status(cudaOccupancyMaxActiveClusters(&h->clusters[split], lin4::fn(c, true, 1, false), &l.cfg),
                       "preparing the 4-bit product", &h->err));
   }
   return h->scratch.open(c.device, &h->err);
@@ -484,8 +497,10 @@ apk_status stream(apk_linear4* h, const apk_linear_io* io, const lin::Epilogue& 
   const int chunks = ops::ceil_div(p.k, lin4::CHUNK), kept = nt == 1 ? io->rows : 8 * nt;
   const int room = (lin4::SMEM - lin4::part_bytes(8 * nt)) / (kept * lin4::CHUNK * 2);  // chunks of x
   // What a launch takes, in chunks of a warp: rounds of tiles, each with its
-  // chunks and 4 for its end (of a cluster: 8), and x laid out once where it
-  // fits (half a chunk's time each), else again in every round.
+  // chunks and 4 for its end (of a cluster 8, of eight CTAs 11), and x laid out once where it
+  // fits (half a chunk's time each), else again in every round.  Where warps
+  // would idle, more of them share a tile, which leaves fewer to finish
+  // (50 x 1184 x 80: 11.5 us with 8 for all clusters and few warps a tile, now 8.9).
   long long best = -1;
   for (int split = 1; split <= 8; split *= 2) {
     if (split > 1 && (split > chunks || h->clusters[split] == 0)) break;
@@ -494,8 +509,8 @@ apk_status stream(apk_linear4* h, const apk_linear_io* io, const lin::Epilogue& 
     for (int kw = 1; kw <= lin4::WARPS && places > 0; kw *= 2) {
       const int sets = ops::ceil_div(p.tiles, lin4::WARPS / kw), rounds = ops::ceil_div(sets, places);
       const long long x = (long long)mine * kept / 64 * (mine <= room ? 1 : rounds);
-      const long long cost = (long long)rounds * (ops::ceil_div(mine, kw) * std::max(2, nt) / 2 + (split > 1 ? 8 : 4)) + x;
-      if (best >= 0 && cost >= best) continue;
+      const long long cost = (long long)rounds * (ops::ceil_div(mine, kw) * std::max(2, nt) / 2 + (split == 1 ? 4 : split < 8 ? 8 : 11)) + x;
+      if (best >= 0 && (cost > best || (cost == best && split != p.split))) continue;
       best = cost;
       p.split = split;
       p.kw = kw;
@@ -503,10 +518,7 @@ apk_status stream(apk_linear4* h, const apk_linear_io* io, const lin::Epilogue& 
       grid = std::min(sets, places) * split;
     }
   }
-  const void* f = nt == 1   ? lin4::fn<1>(c, vec)
-                  : nt == 2 ? lin4::fn<2>(c, vec)
-                  : nt == 4 ? lin4::fn<4>(c, vec)
-                            : lin4::fn<8>(c, vec);
+  const void* f = lin4::fn(c, vec, nt, p.slice * 16 * kept > 32 * lin4::WARPS);
   Launch l(dim3(grid), 32 * lin4::WARPS, p.slice * kept * lin4::CHUNK * 2 + lin4::part_bytes(8 * nt),
            static_cast<cudaStream_t>(io->stream), p.split);
   void* args[] = {&p};
