@@ -577,12 +577,13 @@ __global__ void __launch_bounds__(THREADS) short_rows(const __grid_constant__ Pa
       __syncwarp();
       if (lane < p.top) key = list[lane];
     } else {
-      unsigned long long last = ~0ull;
+      unsigned long long last = 0;
       for (int k = 0; k < p.top; ++k) {
         unsigned long long most = 0;
         for (int i = lane; i < p.vocabulary; i += 32) {
           const unsigned long long v = key_of(ops::ld_any(px, i, F32), i);
-          most = v < last && v > most ? v : most;
+          // (at first nothing lies above: a NaN at index 0 has the largest key there is)
+          most = (k == 0 || v < last) && v > most ? v : most;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {

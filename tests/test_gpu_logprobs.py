@@ -384,3 +384,29 @@ def test_refusals():
                                       stats=p, dlogits=p, ld_d=64), **bad})
         assert lp._lib.apk_logprobs_backward(lp._h, ctypes.byref(a)) == L.APK_EINVAL and lp._lib.apk_logprobs_last_error(lp._h)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [33, 300, 1000, 2041, 5000])
+def test_more_equal_values_than_a_short_row_keeps(V, dtype):
+    """Rows of equal values, of NaN, and with a NaN at the first place, at the
+    last and between: NaN by index, then values by size and index."""
+    import torch
+
+    import apk_b200
+    nan = math.nan
+    x = torch.zeros(7, V, device="cuda")
+    x[1] = nan
+    x[2, 0] = nan
+    x[3, 0], x[3, V // 2], x[3, V - 1] = nan, nan, nan
+    x[4] = torch.arange(V, device="cuda") * 0.25 - 5.0
+    x[5, 1:] = nan
+    x[6] = -math.inf
+    x[6, 0] = nan
+    x = x.to({"bf16": torch.bfloat16, "f32": torch.float32}[dtype])
+    order = torch.sort(x, dim=1, descending=True, stable=True).indices  # (a NaN is the largest there too)
+    for top in (1, 5, 20, 27, 32):
+        _, entropy, ids, tops = apk_b200.LogProbs(top=top).forward(x)
+        assert torch.equal(ids, order[:, :top].int()), top
+        assert tops[[1, 2, 3, 5, 6]].isnan().all() and entropy[[1, 2, 3, 5, 6]].isnan().all()
+        _check(x[[0, 4]], _tokens(2, V, 1), top)
