@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(THREADS, 4) backward(const __grid_constant__ G
   long long token = -1;
   if (p.tokens) token = p.tokens_64 ? static_cast<const long long*>(p.tokens)[row] : (long long)static_cast<const int*>(p.tokens)[row];
   float a = p.dlogprob && token >= 0 ? p.dlogprob[row] : 0.f;
-  if (token >= p.vocabulary) a = __int_as_float(0x7FC00000);
+  if (token >= p.vocabulary && a != 0.f) a = __int_as_float(0x7FC00000);
   const float h = p.dentropy ? p.dentropy[row] : 0.f;
   const bool zero = a == 0.f && h == 0.f;  // a padded row, say: nothing is read
   const float2 st = p.stats[row];

@@ -768,7 +768,8 @@ apk_status apk_logprobs_forward(apk_logprobs* h, const apk_logprobs_io* io);
 
 /* Gradient of a forward call by its logprob and entropy:
  *   dlogits_j = dlogprob ([j = token] - p_j) - dentropy p_j (l_j + entropy),
- * p = exp(l); 0 where p is.  Rows whose dlogprob (or token: padding) and
+ * p = exp(l); 0 where p is.  A token that is not in the vocabulary makes its
+ * row NaN, unless its dlogprob is 0.  Rows whose dlogprob (or token: padding) and
  * dentropy are 0 get zeros, whatever their logits.  dlogits may be the logits
  * themselves (same stride), else it shares no memory with them. */
 typedef struct apk_logprobs_grads {

@@ -410,3 +410,27 @@ def test_more_equal_values_than_a_short_row_keeps(V, dtype):
         assert torch.equal(ids, order[:, :top].int()), top
         assert tops[[1, 2, 3, 5, 6]].isnan().all() and entropy[[1, 2, 3, 5, 6]].isnan().all()
         _check(x[[0, 4]], _tokens(2, V, 1), top)
+
+
+@pytest.mark.parametrize("V", [300, 5000, 20001])
+def test_gradient_of_tokens_outside_the_vocabulary(V):
+    """Their log probability is NaN, and so is the gradient by it; where that counts nothing, the row gets zeros, or
+    the entropy's gradient alone."""
+    import torch
+
+    import apk_b200
+    lp = apk_b200.LogProbs()
+    x = _rand(6, V, seed=1, dtype="bf16")
+    t = torch.tensor([1, V, V + 7, 3, -1, V], device="cuda")
+    logprob, entropy, _, _, stats = lp.forward(x, t, True)
+    assert logprob.isnan().tolist() == [False, True, True, False, False, True]
+    a = torch.tensor([1.0, 0.0, 2.0, 0.0, 1.0, -0.0], device="cuda")
+    none = torch.zeros(6, device="cuda")
+    for to in (None, torch.empty(6, V + 1, dtype=torch.bfloat16, device="cuda")[:, 1:]):
+        for dh in (None, none):
+            d = lp.backward(a, x, t, stats, dentropy=dh, entropy=entropy, out=to)
+            assert torch.isfinite(d[0]).all() and d[0].any() and d[2].isnan().all() and not d[[1, 3, 4, 5]].any()
+        h = _rand(6, seed=2)
+        d = lp.backward(a, x, t, stats, dentropy=h, entropy=entropy, out=to)
+        alone = lp.backward(None, x, None, stats, dentropy=h, entropy=entropy)
+        assert d[2].isnan().all() and torch.equal(d[[1, 3, 4, 5]], alone[[1, 3, 4, 5]])
