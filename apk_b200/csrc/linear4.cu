@@ -324,7 +324,9 @@ __global__ void __launch_bounds__(32 * WARPS, 1) stream4(const __grid_constant__
 }
 
 // The weights as bf16, [n][ld]; with `low` also what that rounds away, in the
-// next k columns, and x twice beside each other to go with it.
+// next k columns, and x twice beside each other to go with it.  Of a value that
+// is not finite nothing is left over, and the second x has 0 in the place of
+// its own: inf times a rest of 0 would make a NaN of an infinite sum.
 struct Expand {
   const uint8_t* w;
   const void* s;
@@ -335,6 +337,11 @@ struct Expand {
   long long ldw, ldx;
   int n, k, group, groups, group_log, s_f32, low, rows;
 };
+// Two bf16 values, 0 where one is not finite.
+__device__ __forceinline__ uint32_t finite(uint32_t v) {
+  if ((v & 0x7F80u) == 0x7F80u) v &= 0xFFFF0000u;
+  return (v & 0x7F800000u) == 0x7F800000u ? v & 0xFFFFu : v;
+}
 __global__ void __launch_bounds__(256) expand(const __grid_constant__ Expand p) {
   pdl_launch();
   pdl_wait();
@@ -375,7 +382,7 @@ __global__ void __launch_bounds__(256) expand(const __grid_constant__ Expand p) 
           float hi[8];
           ops::unpack(r, hi);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) q[e] -= hi[e];
+          for (int e = 0; e < 8; ++e) q[e] = isfinite(hi[e]) ? q[e] - hi[e] : 0.f;
           ops::pack(q, r);
           *reinterpret_cast<uint4*>(to[j] + p.k) = r.a;
         }
@@ -389,7 +396,7 @@ __global__ void __launch_bounds__(256) expand(const __grid_constant__ Expand p) 
     const int k = (int)(i - r * eights) * 8;
     const uint4 v = stream::ld8_any(p.x + r * p.ldx + k, 8);
     *reinterpret_cast<uint4*>(p.xx + r * ld + k) = v;
-    if (p.low) *reinterpret_cast<uint4*>(p.xx + r * ld + p.k + k) = v;
+    if (p.low) *reinterpret_cast<uint4*>(p.xx + r * ld + p.k + k) = make_uint4(finite(v.x), finite(v.y), finite(v.z), finite(v.w));
   }
 }
 

@@ -254,3 +254,24 @@ def test_refusals():
     with pytest.raises(ValueError, match="other memory"):
         lin.forward(x)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("M", [3, 64, 65, 130])
+def test_infinite_values_of_x(M, out):
+    """An infinite x times a weight is infinite, times 0 NaN, whatever the form that the rows take; other rows stay
+    as they are."""
+    import torch
+    lin, w = _layer(256, 72, group=32, zeros=True, out=out)
+    x = _rand(M, 256, seed=1)
+    want = lin.forward(x)
+    bad = x.clone()
+    bad[0, 5], bad[1, 200], bad[2, 31], bad[2, 64] = float("inf"), -float("inf"), float("nan"), float("inf")
+    got = lin.forward(bad)
+    rows = bad[:2].double()
+    ref = torch.where(rows.isinf(), rows, torch.zeros_like(rows)) @ w  # (0 * inf is NaN here too)
+    inf = torch.zeros(2, 72, dtype=torch.float64, device="cuda")
+    inf[0], inf[1] = float("inf") * w[5], -float("inf") * w[200]
+    assert torch.equal(ref.isnan(), inf.isnan()) and inf.isnan().any() and inf.isinf().any()
+    assert torch.equal(got[:2].isnan(), inf.isnan()) and torch.equal(got[:2].double().nan_to_num(7.0), inf.nan_to_num(7.0))
+    assert got[2].isnan().all() and torch.equal(got[3:], want[3:])
