@@ -396,3 +396,66 @@ def test_rows_from_any_address(D, ld, at, types):
         x[bad] = 1.0
         want = norm.forward(x)
         assert torch.equal(norm.forward(x, out=x), want)
+
+
+def _close_bounds(norm, x):
+    """As _forward_bounds, for a mean that is corrected by the mean of the
+    differences from it where it is larger than the deviation.  The first one is
+    within e1 = (DEPTH + 1) E mean|x|; the differences, d = x - that, are within
+    E |d|, their mean within (DEPTH + 3) E mean|d|, and |d| is up to |c| + e1.
+    The variance is mean(d^2) less the square of mean(d), which is up to e1."""
+    import torch
+    x = x.double()
+    mean = x.mean(-1, keepdim=True)
+    c = x - mean
+    e1 = (DEPTH + 1) * E * x.abs().mean(-1, keepdim=True)
+    d = c.abs() + e1
+    var, size = c.square().mean(-1, keepdim=True), d.square().mean(-1, keepdim=True)
+    em = (DEPTH + 3) * E * d.mean(-1, keepdim=True)
+    em = torch.where(mean.abs() < 1.001 * var.sqrt(), e1 + em, em)
+    ec = em + 2 * E * d
+    dv = (DEPTH + 6) * E * size + 2 * e1 * em + 3 * E * e1.square()
+    rstd = (var + norm.eps).rsqrt()
+    er = rstd * (dv / (var + norm.eps) + 6 * E)  # (the root takes half of that; rsqrtf within 2 ulp)
+    w = norm.weight.double()
+    y = c * rstd * w
+    ey = w.abs() * ((rstd + er) * ec + c.abs() * er) + 3 * E * y.abs()
+    if norm.bias is not None:
+        y = y + norm.bias.double()
+        ey = ey + E * (y.abs() + norm.bias.double().abs())
+    return (y, _round(ey, y, norm.out_dtype)), (mean, em + E * mean.abs()), (rstd, er)
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("M,D", [(12, 100), (12, 256), (12, 333), (12, 512), (12, 1000), (12, 1001), (300, 1001), (300, 1536), (12, 3000),
+                                 (300, 4099), (12, 4096), (300, 8192), (12, 8191), (12, 16384), (300, 16383)])
+def test_a_mean_far_from_zero_costs_no_digits(M, D, out):
+    """Constant rows give the bias, and rows close to one value their own norm."""
+    import layer_bounds as lb
+    import torch
+    norm = _make(D, out=out)
+    x = _rand(M, D, seed=1, dtype="f32")
+    at = torch.tensor([100.1, 5000.3, -77.7, 1.0e6 / 3, 0.1, -0.3], device="cuda")
+    for i in range(6):
+        x[i] = at[i]
+        x[6 + i] = at[i] * (1 + x[6 + i] * 1e-5)
+    x[12:] += torch.linspace(-3000, 3000, M - 12, device="cuda")[:, None]
+    y, stats = norm.forward(x, save_stats=True)
+    (want, by), (mean, bm), (rstd, br) = _close_bounds(norm, x)
+    lb.check(y, want, by, "y")
+    lb.check(stats[:, :1], mean, bm, "mean")
+    lb.check(stats[:, 1:], rstd, br, "rstd")
+    assert torch.equal(stats[:6, 0], at), "a constant row's mean"
+
+
+def test_a_mean_far_from_zero_and_almost_no_eps():
+    """The square of what the mean was off by may pass the mean of the squares: no NaN comes of it."""
+    import torch
+    for D in (200, 1001, 1536, 8191):
+        norm = _make(D, out="f32", eps=1e-30)
+        x = torch.full((64, D), 1.0, device="cuda") * torch.linspace(100.1, 9999.7, 64, device="cuda")[:, None]
+        y, stats = norm.forward(x, save_stats=True)
+        assert torch.isfinite(y).all() and torch.isfinite(stats).all()
+        x[3, 5] = float("nan")
+        y, stats = norm.forward(x, save_stats=True)
+        assert y[3].isnan().all() and stats[3].isnan().all() and torch.isfinite(y[[2, 4]]).all()
