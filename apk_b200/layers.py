@@ -140,7 +140,11 @@ class _Handle:
             raise ApkError(st, self._message())
 
     def status(self) -> int:
-        """The first device error since the last query (0: none); waits for the current stream."""
+        """The first device error since the last query (0: none); waits for the
+        current stream.  0 at once where no kernel waits on the device, so that
+        none can report an error."""
+        if not self._status:
+            return 0
         st = ctypes.c_int()
         self._check(getattr(self._lib, self._status)(self._h, self._stream(), ctypes.byref(st)))
         return st.value

@@ -45,3 +45,11 @@ def test_dense():
         assert _dense(yes)
     for no in (t[:, ::2], t[..., :7], t[:, 0], t[0, 0].expand(3, 8), t[::2]):
         assert not _dense(no)
+
+
+def test_status_of_what_has_nothing_to_report():
+    """Code that asks every layer for its status may ask these too."""
+    pytest.importorskip("torch")
+    import apk_b200
+    for kind in (apk_b200.LayerNorm, apk_b200.GradClip, apk_b200.LogProbs):
+        assert kind.__new__(kind).status() == 0
