@@ -304,12 +304,12 @@ class Linear4(_Handle):
 
     def __init__(self, weight, scales, zeros=None, bias=None, group: int = 128, act: str = "none",
                  out_dtype: str = "bf16", sms: int = 0, wait_limit_ns: int = _DEFAULT_WAIT_NS):
+        self.group = int(group)
+        if not 1 <= self.group < 1 << 31:  # (a C int: 2^32 + 128 would be 128 there)
+            raise ValueError(f"group is {group!r}: 32, 64 or a multiple of 128, below 2^31")
         _tensor(weight, "weight", dtypes=(torch.uint8,), dim=2)
         self.device, self._index = weight.device, weight.device.index
         self.out_features, self.in_features = weight.shape[0], 2 * weight.shape[1]
-        self.group = int(group)
-        if self.group < 1:
-            raise ValueError(f"group is {group!r}: 32, 64 or a multiple of 128")
         w, _, ldw = _rows(weight, "weight", self.device, weight.shape[1], (torch.uint8,))
         shape = (self.out_features, -(-self.in_features // self.group))
         for t, what, dtypes in ((scales, "scales", _ANY), (zeros, "zeros", (torch.uint8,))):

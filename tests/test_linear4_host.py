@@ -64,3 +64,12 @@ def test_quantize(k, group, zeros):
     # the zero point is rounded to half a step, and the scale by 2^-8 of up to 15 steps
     step = 0.5 + (0.5 + 15 * 2.0 ** -8 if zeros else 7 * 2.0 ** -8)
     assert bool(((got - w.double()).abs() <= step * s_k + 1e-6).all()) and not got[3].any()
+
+
+@pytest.mark.parametrize("group", [1 << 31, (1 << 32) + 128, 1 << 40, 0, -128])
+def test_groups_past_32_bits(group):
+    """(1 << 32) + 128 would reach the library as 128, whose scales are not there."""
+    torch = pytest.importorskip("torch")
+    import apk_b200
+    with pytest.raises(ValueError, match="group"):
+        apk_b200.Linear4(torch.zeros(16, 128, dtype=torch.uint8), torch.ones(16, 1), group=group)
