@@ -11,6 +11,7 @@ reference, which multiplies bare matrices (src/tcyield.cu:91-356).
 from __future__ import annotations
 
 import ctypes
+import math
 import threading
 
 import torch
@@ -27,6 +28,7 @@ _ANY = tuple(_CODE)
 # the current stream's handle; building a torch.cuda.Stream for it costs 2 us a call
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
+_INTS = 1 << 31  # the C ABI's counts are ints below this
 _DEFAULT_WAIT_NS = 2_000_000_000
 # the native handles have the tensors' addresses
 _MOVED = "weights are in other memory than when the layer was made: make a new layer"
@@ -52,21 +54,30 @@ def _tensor(t, what, device=None, dtypes=(torch.bfloat16,), dim=None):
     return t
 
 
+def _too_many(t, what):
+    return ValueError(f"{what} is {tuple(t.shape)}: rows of 2^31 elements and more, or as many rows, are not served")
+
+
 def _rows(t, what, device, width, dtypes=(torch.bfloat16,)):
     """(address, rows, row stride) of a [..., width] tensor whose last axis is
-    contiguous.  Called for every operand of every call: the usual case first."""
+    contiguous, both counts such that the library's ints hold them (ctypes would
+    cut them off).  Called for every operand of every call: the usual case first."""
     try:
         shape = t.shape
         if len(shape) == 2 and shape[1] == width and t.dtype in dtypes and t.device == device:
             s0, s1 = t.stride()
             if s1 == 1 or width == 1:
                 m = shape[0]
+                if m >= _INTS or width >= _INTS:
+                    raise _too_many(t, what)
                 return t.data_ptr(), m, (s0 if m > 1 else width)
     except (AttributeError, TypeError):
         pass
     _tensor(t, what, device, dtypes)
     if t.dim() < 1 or t.shape[-1] != width:
         raise ValueError(f"{what} is {tuple(t.shape)}: its last axis has to be {width}")
+    if width >= _INTS or math.prod(t.shape[:-1]) >= _INTS:
+        raise _too_many(t, what)
     if width > 1 and t.stride(-1) != 1:
         raise ValueError(f"{what}: its last axis has stride {t.stride(-1)}, not 1")
     try:

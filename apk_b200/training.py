@@ -144,8 +144,9 @@ class LogProbs(_Handle):
     def _logits(self, logits, a):
         if not isinstance(logits, torch.Tensor) or logits.dim() < 1 or logits.shape[-1] < max(1, self.top):
             raise ValueError(f"logits: a tensor [..., vocabulary] of at least {max(1, self.top)} is wanted")
-        a.vocabulary = logits.shape[-1]
-        a.logits, a.rows, a.ld = _rows(logits, "logits", self.device, a.vocabulary, _ANY)
+        V = logits.shape[-1]
+        a.logits, a.rows, a.ld = _rows(logits, "logits", self.device, V, _ANY)
+        a.vocabulary = V
         a.dtype = _CODE[logits.dtype]
 
     def _per_row(self, t, what, shape, dtypes):

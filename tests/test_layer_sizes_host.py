@@ -41,3 +41,30 @@ def test_rows_are_refused(libapk):
         assert lin._lib.apk_linear_backward(lin._h, ctypes.byref(g)) == L.APK_EINVAL
     torch.cuda.synchronize()
     assert lin.status() == 0
+
+
+@pytest.mark.parametrize("shape", [((1 << 32) + 5, 8), (1 << 31, 8), (2, (1 << 32) + 5), (3, 1 << 31)])
+def test_counts_past_32_bits(shape):
+    """(1 << 32) + 5 rows would reach the library as 5, and the others stay as they were."""
+    torch = pytest.importorskip("torch")
+    from apk_b200 import layers
+    t = torch.empty(shape, dtype=torch.bfloat16, device="meta")  # (without memory)
+    with pytest.raises(ValueError, match="2\\^31"):
+        layers._rows(t, "x", t.device, shape[1])
+
+
+@pytest.mark.gpu
+def test_counts_past_32_bits_in_calls(libapk):
+    """Nothing is launched: these views have one element of memory."""
+    import torch
+
+    import apk_b200
+    one = torch.zeros(1, dtype=torch.bfloat16, device="cuda")
+    many, long = one.expand((1 << 32) + 5, 64), one.expand(2, (1 << 32) + 5)
+    lin = apk_b200.Linear(torch.zeros(64, 32, dtype=torch.bfloat16, device="cuda"))
+    norm = apk_b200.LayerNorm(torch.ones(64, device="cuda"))
+    lp = apk_b200.LogProbs()
+    for call in (lambda: lin.forward(many), lambda: lin.forward(many.view(1, -1, 64)), lambda: norm.forward(many), lambda: lp.forward(many),
+                 lambda: lp.forward(long), lambda: lp.forward(long[0])):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()
