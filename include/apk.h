@@ -678,8 +678,9 @@ apk_status apk_norm_forward(apk_norm* h, const apk_norm_io* io);
 /* Gradients of a forward call:  n = (x - mean) rstd,  g = dy weight,
  * dx = rstd (g - mean(g) - n mean(g n)) + residual_grad,
  * dw = the sum over rows of dy n,  db = that of dy, in fp32 and in an order
- * that depends on the sizes alone.  residual_grad is what reaches x past the
- * norm (a block's residual stream).  An output that is NULL is not computed;
+ * that depends on the sizes, the device, and whether the weight and the rows of
+ * all operands start on 16 bytes, on nothing else.  residual_grad is what reaches
+ * x past the norm (a block's residual stream).  An output that is NULL is not computed;
  * none shares memory with an input.  With rows = 0, dw and db are cleared. */
 typedef struct apk_norm_grads {
   const void* dy;           /* [rows][features]                               */
