@@ -696,10 +696,12 @@ Kernel bwd() {
 }
 template <int V, bool WARP, int T>
 Kernel fwd_of(bool vec, bool xf, bool yf) {
-  return vec ? (xf ? (yf ? fwd<V, true, WARP, T, true, true>() : fwd<V, true, WARP, T, true, false>())
-                   : (yf ? fwd<V, true, WARP, T, false, true>() : fwd<V, true, WARP, T, false, false>()))
-             : (xf ? (yf ? fwd<V, false, WARP, T, true, true>() : fwd<V, false, WARP, T, true, false>())
-                   : (yf ? fwd<V, false, WARP, T, false, true>() : fwd<V, false, WARP, T, false, false>()));
+  if constexpr (WARP || T > 64)  // (as few single elements as 64 threads hold go by warps, or by few's form)
+    if (!vec)
+      return xf ? (yf ? fwd<V, false, WARP, T, true, true>() : fwd<V, false, WARP, T, true, false>())
+                : (yf ? fwd<V, false, WARP, T, false, true>() : fwd<V, false, WARP, T, false, false>());
+  return xf ? (yf ? fwd<V, true, WARP, T, true, true>() : fwd<V, true, WARP, T, true, false>())
+            : (yf ? fwd<V, true, WARP, T, false, true>() : fwd<V, true, WARP, T, false, false>());
 }
 template <int V, bool WARP, int T>
 Kernel bwd_of(bool vec, bool xf, bool df) {
