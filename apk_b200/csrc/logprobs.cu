@@ -804,7 +804,8 @@ constexpr int EIGHTS = 4;  // of a thread
 // in pairs of values; masked ones are raised to -1e9 as in the forward pass,
 // and the token's own term is added by the thread that has it.  Rows far out
 // (|m| of 1e8 and more) have x - m limited instead.
-// p.pieces of 0: rows are short, and a warp's each.
+// p.pieces of 0: rows are short, and a warp's each.  Not SAME: value by value
+// (2048 x 50257 bf16 in rows of 50304: 75 us, into rows of 50257 217).
 template <bool F32, bool SAME>
 __global__ void __launch_bounds__(THREADS, 4) backward(const __grid_constant__ Grads p) {
   const int T = p.pieces ? THREADS : 32, t = threadIdx.x & (T - 1);

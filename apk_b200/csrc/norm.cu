@@ -13,8 +13,9 @@
 // of large values (a row of 5000.3s, eps 1e-5, would get up to 0.3 w + b in
 // place of b): where it is larger than the deviation, mean(d) corrects it,
 //   mean = m + mean(d),  sum (x - mean)^2 = sum d^2 - mean(d) sum d.
-// Elsewhere m is off by less than roundings of d are.  (Both sums in one pass
-// for every row: 8192 x 4096 bf16 31.1 us; so 28.3, without any of it 27.6.)
+// Elsewhere the values are hardly larger than their differences, and so are the
+// sum's roundings.  (Both sums in one pass for every row: 8192 x 4096 bf16 31.1
+// us; so 28.3, without any of it 27.6.)
 #include <algorithm>
 #include <vector>
 
@@ -722,11 +723,15 @@ int threads_of(int cols, bool vec) {
   return vec || T > 512 ? T : T <= 64 ? 64 : T <= 128 ? 128 : T <= 256 ? 256 : 512;
 }
 // Where there are fewer rows than blocks that run at once, a row has more
-// threads: one piece each.
+// threads: one piece each.  (Blocks of more than 512 threads have 64 registers a
+// thread: of two pieces, the forward kernels spill 20 to 40 bytes, the gradient's
+// 210 to 280, of one piece the gradient's up to 32, where rows go by single
+// elements.  2048 x 16384 bf16 forward 45.2 us; gradients of 250 x 16384 30.8.)
 Shape fwd_shape(int cols, bool few, bool vec, bool xf, bool yf) {
   if (cols <= 256) return {fwd_of<1, true, 256>(vec, xf, yf), 256, 8};
   if (cols <= 512) return {fwd_of<2, true, 256>(vec, xf, yf), 256, 8};
-  // single elements: a warp's row needs no barrier (1537 x 1001: 4.3 us, with a block's row 5.2)
+  // single elements: a warp's row needs no barrier (1537 x 1001 fp32 4.1 us, with a block's row 4.5; bf16 both 4.4.
+  // Not so many more, or fewer: bf16 16384 x 1001 23.9 and 18.8, 4000 x 777 7.0 and 6.6, 600 x 1001 4.0 and 3.2)
   if (!vec && cols <= 1024 && !few)
     return {xf ? (yf ? fwd<4, false, true, 256, true, true>() : fwd<4, false, true, 256, true, false>())
                : (yf ? fwd<4, false, true, 256, false, true>() : fwd<4, false, true, 256, false, false>()),
@@ -876,7 +881,9 @@ apk_status backward(apk_norm* h, const apk_norm_grads* g) {
                    (!g->dx || ops::on16(g->dx, g->ld_dx, M, g->x_dtype)) &&
                    (!g->residual_grad || ops::on16(g->residual_grad, g->ld_residual, M, g->x_dtype)) && ops::aligned(c.weight, 16);
   const bool xf = g->x_dtype == APK_F32, df = g->dy_dtype == APK_F32;
-  // (64 x 8192 would take 11.6 us so, and takes 10.1; 128 x 4096 5.0 against 7.6, 333 x 1001 5.3 against 9.7)
+  // (1 x 8192 would take 9.1 us so, and takes 6.5, 64 x 8192 11.6 and 9.7; 128 x 4096 5.0 against 7.4, 333 x 1001 4.7
+  // against 8.8, 444 x 4096 9.0 against 10.4.  It would still be the faster behind the border: 600 x 1024 takes 8.3, so
+  // 5.8, 600 x 4096 10.6 and 9.7, 1184 x 1024 9.9 and 8.6)
   const bool few = M <= 3 * h->sms && D <= 4096;
   const norm::Shape sh = norm::bwd_shape(D, few, vec, xf, df);
   const int grid = std::min(ops::ceil_div(M, sh.per), h->sms * std::max(1, (sh.k.threads > 512 ? 1024 : 512) / sh.T));

@@ -309,7 +309,8 @@ class Linear4(_Handle):
     in is a multiple of 32, rows start on 16 bytes.  scales: [out, groups],
     fp32 or bf16; zeros: uint8 of that shape (0 to 15), None for 8 everywhere;
     quantize() makes them.  bias, act and out_dtype as Linear has them; tensors
-    are kept by reference likewise.  There is no backward pass."""
+    are kept by reference likewise.  Above 64 rows a bf16 result is of weights
+    rounded to bf16.  There is no backward pass."""
     _create, _destroy = "apk_linear4_create", "apk_linear4_destroy"
     _error, _status = "apk_linear4_last_error", "apk_linear4_status"
 

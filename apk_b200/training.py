@@ -117,8 +117,9 @@ class GradClip(_Handle):
     def clip(self, grads, out=None):
         """Multiplies the gradients by min(1, max_norm / (norm + 1e-6)), in
         place or into the tensors of `out`; returns the norm before that.  No
-        two of them may share memory.  An infinite norm makes the factor 0, a
-        NaN makes it NaN: look at the norm before the weights are updated."""
+        two of them may share memory.  An infinite norm makes the factor 0 (NaN
+        where max_norm is infinite too), a NaN makes it NaN: look at the norm
+        before the weights are updated."""
         if not self.max_norm >= 0.0 or math.isnan(self.max_norm):
             raise ValueError(f"max_norm is {self.max_norm}: 0 or above")
         return self._run(grads, out, self._lib.apk_clip_scale)
