@@ -130,6 +130,14 @@ def _new(t, shape, dtype):
 class _Handle:
     """Owner of one native handle; subclasses name its functions."""
     _create = _destroy = _error = _status = ""
+    # what the native handle was made with: outputs are allocated by it
+    _FIXED = frozenset(("device", "in_features", "out_features", "features", "group", "experts", "top_k", "d_model", "d_ff", "top",
+                        "act", "layout", "eps", "out_dtype"))
+
+    def __setattr__(self, name, value):
+        if name in self._FIXED and "_h" in self.__dict__:
+            raise AttributeError(f"{name} is fixed once the handle is made: make a new one")
+        object.__setattr__(self, name, value)
 
     def _open(self, cfg):
         self._lib = L.load()

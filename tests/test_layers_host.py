@@ -87,3 +87,27 @@ def test_python_refuses_host_tensors(libapk):
         apk_b200.MoE(w, w, w, top_k=1)
     with pytest.raises(AttributeError):
         apk_b200.NoSuchLayer
+
+
+@pytest.mark.parametrize("kind,name", [("LogProbs", "top"), ("LogProbs", "device"), ("LayerNorm", "features"), ("LayerNorm", "out_dtype"),
+                                       ("LayerNorm", "eps"), ("Linear", "out_features"), ("Linear", "act"), ("Linear4", "group"),
+                                       ("Linear4", "out_dtype"), ("MoE", "top_k")])
+def test_what_a_handle_was_made_with_stays(kind, name):
+    """Outputs are allocated by these, and the library writes what it was told when the handle was made."""
+    pytest.importorskip("torch")
+    import apk_b200
+    layer = getattr(apk_b200, kind).__new__(getattr(apk_b200, kind))
+    setattr(layer, name, 20)
+    layer._h = ctypes.c_void_p()
+    with pytest.raises(AttributeError, match=name):
+        setattr(layer, name, 5)
+    assert getattr(layer, name) == 20
+
+
+def test_max_norm_may_change():
+    pytest.importorskip("torch")
+    import apk_b200
+    clip = apk_b200.GradClip.__new__(apk_b200.GradClip)
+    clip._h = ctypes.c_void_p()
+    clip.max_norm = 2.0
+    assert clip.max_norm == 2.0
