@@ -216,6 +216,7 @@ class Linear(_Handle):
                                  f"{self.out_features} contiguous values are wanted")
         self.weight, self.bias, self.act, self.layout = weight, bias, act, layout
         self._w_shape, self._w_at, self._b_at = weight.shape, w, None if bias is None else bias.data_ptr()
+        self._b_dtype = None if bias is None else bias.dtype  # (another view at the same address may be shorter)
         self.out_dtype = _pick(_TORCH, out_dtype, "out_dtype")
         self._y_code = _CODE[self.out_dtype]
         self._act = _pick(_ACT, act, "act")
@@ -298,8 +299,8 @@ class Linear(_Handle):
                 shape = self._w_shape
                 dw = _like(self.weight, shape) if dt is torch.bfloat16 else self.weight.new_empty(shape, dtype=dt)
                 g.dw, g.ld_dw, g.dw_dtype = dw.data_ptr(), shape[1], _CODE[dt]
-            if need_db and self.bias is not None:
-                db = torch.empty_like(self.bias)
+            if need_db and self._b_at is not None:
+                db = _new(dy, (n,), self._b_dtype)
                 g.db = db.data_ptr()
             g.stream = _raw_stream(self._index)
             if dw is not None or db is not None or (dx is not None and g.rows > 0):
@@ -441,6 +442,8 @@ class LayerNorm(_Handle):
                                  f"{self.features} contiguous values are wanted")
         self.weight, self.bias, self.eps = weight, bias, eps
         self._w_at, self._b_at = weight.data_ptr(), None if bias is None else bias.data_ptr()
+        # (the gradients' by these: another view at the same address may be shorter)
+        self._w_dtype, self._b_dtype = weight.dtype, None if bias is None else bias.dtype
         self.out_dtype = _pick(_TORCH, out_dtype, "out_dtype")
         self._open(L.NormConfig(self._index, self.features, eps, _CODE[weight.dtype],
                                 _CODE[bias.dtype] if bias is not None else L.APK_F32, self._w_at, self._b_at))
@@ -517,10 +520,10 @@ class LayerNorm(_Handle):
                 dx = _like(x, x.shape)
                 g.dx, g.ld_dx = dx.data_ptr(), d
             if need_dw:
-                dw = _like(self.weight, self.weight.shape)
+                dw = _new(x, (d,), self._w_dtype)
                 g.dw = dw.data_ptr()
-            if need_db and self.bias is not None:
-                db = _like(self.bias, self.bias.shape)
+            if need_db and self._b_at is not None:
+                db = _new(x, (d,), self._b_dtype)
                 g.db = db.data_ptr()
             g.stream = _raw_stream(self._index)
             if dw is not None or db is not None or (dx is not None and g.rows > 0):

@@ -77,3 +77,24 @@ def test_a_weight_transposed_in_place_keeps_the_gradients_shape():
     w.t_()
     got = lin.backward(dy, x)[1]
     assert got.shape == (96, 32) and torch.equal(got, want)
+
+
+def test_shorter_views_at_the_same_address():
+    """The memory has not moved, and gradients have the size that the layer was made with."""
+    import torch
+
+    import apk_b200
+    w, b, x, dy = _rand(64, 32, seed=1), _rand(32, seed=2), _rand(500, 64, seed=3), _rand(500, 32, seed=4)
+    lin = apk_b200.Linear(w, b)
+    want = lin.backward(dy, x)
+    lin.weight, lin.bias = w[:8], b[:3]
+    assert all(torch.equal(p, q) for p, q in zip(lin.backward(dy, x), want))
+    g, c = _rand(64, seed=5), _rand(64, seed=6)
+    norm = apk_b200.LayerNorm(g, c)
+    y, stats = norm.forward(x, save_stats=True)
+    for rows in (5, 500):
+        want = norm.backward(x[:rows], x[:rows], stats[:rows])
+        norm.weight, norm.bias = g[:8], c[:3]
+        got = norm.backward(x[:rows], x[:rows], stats[:rows])
+        assert [tuple(t.shape) for t in got] == [(rows, 64), (64,), (64,)] and all(torch.equal(p, q) for p, q in zip(got, want))
+        norm.weight, norm.bias = g, c
